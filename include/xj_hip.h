@@ -425,6 +425,108 @@ int xjh_delta_chunked(int H, int S, int T, int chunk, const float *q, const floa
                       const float *v, const float *decay, const float *beta, float qscale,
                       float *state, float *out, char *err, size_t errlen);
 
+/* -------------------------------------------------------- long contexts -- */
+
+/* What a context beyond the trained one needs, no counterpart in the
+ * reference: rotary positions with scaled frequencies, a cache of keys and
+ * values in 8 bits, and attention over it with an optional sliding window.
+ *
+ * Unlike the other per-op entries these enqueue on `stream` (a hipStream_t of
+ * the current device; NULL: its default stream) and return without waiting
+ * (xjh_sync waits), never allocate and can be captured into a HIP graph. Device
+ * buffers belong to the current device, need no alignment beyond their type's
+ * (the cache and the work area: 16 bytes) and are complete when the stream
+ * reaches the call. Strides are in elements. T = 0 does nothing.
+ * Where a call takes n_past_dev (may be NULL), the tokens' position is read
+ * there on the GPU instead of n_past, which then is an upper bound for it, so
+ * that one captured graph serves every step; a value outside [0, n_past] counts
+ * as the nearer end. */
+
+/* Rotary positions. pairs: which elements of a head turn together, (i, i +
+ * n_rot/2) or (2i, 2i + 1), i < n_rot/2; the elements past n_rot do not turn.
+ * Pair i of a token at position p turns by p * f_i, f_i from base^(-2i/n_rot):
+ *   XJH_ROPE_PLAIN   f_i = base^(-2i/n_rot)
+ *   XJH_ROPE_LINEAR  that divided by factor
+ *   XJH_ROPE_YARN    with r = n_ctx_orig * base^(-2i/n_rot) / (2 pi) turns over the
+ *                    trained context and g = (r - beta_slow) / (beta_fast - beta_slow)
+ *                    clamped to [0, 1]: (g + (1 - g) / factor) of it
+ * and is multiplied by mscale (0: 0.1 ln(factor) + 1 for YARN, else 1). */
+enum { XJH_ROPE_HALF = 0, XJH_ROPE_INTERLEAVED = 1 };
+enum { XJH_ROPE_PLAIN = 0, XJH_ROPE_LINEAR = 1, XJH_ROPE_YARN = 2 };
+typedef struct {
+    int32_t pairs;
+    int32_t n_rot;               /* even, 2 .. min(D, 512) */
+    float   base;                /* > 0 */
+    int32_t scaling;
+    float   factor;              /* linear, yarn: >= 1 */
+    int32_t n_ctx_orig;          /* yarn: > 0 */
+    float   beta_fast, beta_slow;/* yarn: beta_fast > beta_slow */
+    float   mscale;
+} xjh_rope_cfg;
+/* out[t][h] = x[t][h] rotated, for T tokens of n_heads heads of D elements (x +
+ * t*x_tok + h*x_head, out likewise), token t at position pos[t] (device, may be
+ * negative) or, with pos NULL, pos0 + t. out == x with equal strides rotates
+ * in place; other overlaps are not allowed. The angles are formed in double, so far positions keep
+ * theirs (xjh_rope evaluates them in float, as the reference does). */
+int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, float *out, int64_t o_tok, int64_t o_head, int T,
+                    int n_heads, int D, const xjh_rope_cfg *cfg, const int32_t *pos, int pos0, void *stream,
+                    char *err, size_t errlen);
+
+/* A cache of the keys and values of one layer in 8 bits, one scale (float) for
+ * every `block` tokens of a kv head: a value is code * scale.
+ *   XJH_KV_I8    codes -127 .. 127; scale = largest magnitude / 127 (rounded to
+ *                float, at least 2^-126), code = nearest integer of x / scale
+ *   XJH_KV_E4M3  OCP e4m3 codes; scale = the least power of two (at least 2^-126)
+ *                with largest magnitude <= 448 scale, code = nearest e4m3 of x / scale
+ * Ties go to the even code and every code is that of the exact quotient. A block
+ * of zeros has scale 0. NaN is stored as 0 and an infinity as the largest code;
+ * neither counts for the scale, so the cache never holds them.
+ * The bytes at data, N = n_ctx rounded up to 64 positions:
+ *   keys   [Hkv][N/64][4 groups of 16 positions][D/64][4 x 16 dims][16 positions][16 dims]
+ *   values [Hkv][N/64][D/16 groups of 16 dims][4 q][16 dims][4 u][4 r], byte (q, u, r)
+ *          holding position 16 u + 4 q + r of the tile of 64
+ *   scales float [Hkv][N/block] of the keys, then of the values
+ * (the order in which the matrix cores take them: a wavefront reads 1 KB runs). */
+enum { XJH_KV_I8 = 0, XJH_KV_E4M3 = 1 };
+typedef struct {
+    int32_t  type;
+    int32_t  Hkv, D;             /* D: 64, 128 or 256 */
+    int32_t  n_ctx;
+    int32_t  block;              /* 1, 2, 4, .. 64 */
+    void    *data;               /* device, 16-byte aligned */
+    uint64_t bytes;              /* at data, at least xjh_kv8_bytes */
+} xjh_kv8;
+/* Bytes of a cache of c's type, heads, n_ctx and block; 0 when they are not supported. */
+uint64_t xjh_kv8_bytes(const xjh_kv8 *c);
+/* Quantise the rows k, v [T][Hkv*D] (token strides k_tok, v_tok) into positions
+ * n_past .. n_past+T-1. A block that positions before n_past began keeps the
+ * larger of its scale and the new rows'; where that grew, its older codes are
+ * rounded again to it. Blocks written from their first position start anew. No
+ * other byte is touched. n_past_dev: see above. */
+int xjh_kv8_store(const xjh_kv8 *c, const float *k, int64_t k_tok, const float *v, int64_t v_tok, int T, int n_past,
+                  const int32_t *n_past_dev, void *stream, char *err, size_t errlen);
+/* Read positions pos0 .. pos0+n-1 back: k, v [n][Hkv*D] (token strides k_tok, v_tok); either may be NULL. */
+int xjh_kv8_load(const xjh_kv8 *c, int pos0, int n, float *k, int64_t k_tok, float *v, int64_t v_tok, void *stream,
+                 char *err, size_t errlen);
+/* Attention of T tokens at positions n_past .. n_past+T-1, whose keys and values
+ * (and those of every earlier position that they see) are in the cache: query head h
+ * (q + t*q_tok + h*q_head, D elements) of the token at p reads kv head h / (H/Hkv)
+ * and sees the positions j <= p, with window > 0 only those with j > p - window
+ * or j < n_sink (the first tokens stay visible); out[t*o_tok + h*D ..] =
+ * softmax(scale q.K^T) V, times sigmoid(gate[t*g_tok + h*g_head ..]) when gate is
+ * not NULL. Codes are exact operands, queries and weights enter with 22 bits, sums are fp32.
+ * work: xjh_attn_kv8_work_bytes bytes, for splitting the positions over the
+ * GPU; a smaller area (or NULL) splits less. It holds nothing between calls, but
+ * calls that may run at the same time (other streams, other graphs) need one each.
+ * Positions that no row sees are not read beyond their tile of 64, whatever they
+ * hold. A query that is not finite leaves its own row not finite and no other. */
+int xjh_attn_kv8(const xjh_kv8 *c, const float *q, int64_t q_tok, int64_t q_head, const float *gate, int64_t g_tok,
+                 int64_t g_head, int T, int H, int n_past, const int32_t *n_past_dev, int window, int n_sink, float scale,
+                 float *out, int64_t o_tok, void *work, size_t work_bytes, void *stream, char *err, size_t errlen);
+/* The work area beyond which nothing is gained for these T, n_past (or any smaller
+ * n_past), window and n_sink; 0 when they are not supported. */
+size_t xjh_attn_kv8_work_bytes(const xjh_kv8 *c, int T, int H, int n_past, int window, int n_sink);
+
 #ifdef __cplusplus
 }
 #endif

@@ -357,4 +357,56 @@ void rope_table(int pos0, int n, int n_rot, float base, float2 *out);
 // first ck_n tokens (EPI_CONV's code).
 int conv_silu_launch(float *x, float *state, const float *w, int C, int K, int T, float *ck, int ck_n, hipStream_t st);
 
+// The 8-bit cache (kv8.hip), layout as xjh_kv8 in xj_hip.h: tiles of 64 positions.
+constexpr int kKvTile = 64;
+struct Kv8 {
+    uint8_t *k, *v;               // codes [Hkv][n_tiles][64 * D]
+    float *ks, *vs;               // scales [Hkv][n_tiles * 64 >> lg]
+    int32_t e4m3, Hkv, D, n_tiles, lg;
+};
+struct Kv8StoreArgs {
+    Kv8 c;
+    const float *k, *v;
+    int64_t k_tok, v_tok;
+    int32_t T, npast;
+    const int32_t *npast_dev;     // optional: the position, at most npast
+};
+int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st);
+struct Kv8LoadArgs {
+    Kv8 c;
+    float *k, *v;                 // either may be null
+    int64_t k_tok, v_tok;
+    int32_t pos0, n;
+};
+int kv8_load_launch(const Kv8LoadArgs &a, hipStream_t st);
+struct Kv8AttnArgs {
+    Kv8 c;
+    const float *q; int64_t q_tok, q_head;
+    const float *gate; int64_t g_tok, g_head;   // optional
+    float *out; int64_t o_tok;
+    int32_t T, H, npast;
+    const int32_t *npast_dev;
+    int32_t window, sinks;        // window 0: every earlier position
+    float scale;
+    float *part;                  // split partials
+    int32_t n_split, per_split;   // set by kv8_attn_launch
+};
+// part_floats: the partials' capacity (any); kv8_attn_part_floats: what the
+// launch would use with enough.
+int kv8_attn_launch(const Kv8AttnArgs &a, int64_t part_floats, hipStream_t st);
+int64_t kv8_attn_part_floats(const Kv8AttnArgs &a);
+
+// Rotary positions with given frequencies (rope.hip): pair i of a token at
+// position p turns by p * f[i] full turns, times mscale.
+constexpr int kRopeMaxPairs = 256;
+struct RopeArgs {
+    const float *x; int64_t x_tok, x_head;
+    float *out; int64_t o_tok, o_head;
+    int32_t T, n_heads, D, n_rot, interleaved, pos0;
+    const int32_t *pos;           // optional: position of each token
+    float mscale;
+    double f[kRopeMaxPairs];      // turns per position
+};
+int rope_scaled_launch(const RopeArgs &a, hipStream_t st);
+
 }  // namespace xjk

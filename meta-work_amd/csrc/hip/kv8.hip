@@ -1,0 +1,476 @@
+// A key/value cache in 8 bits with one scale per block of tokens and kv head,
+// and grouped-query attention over it (gfx950): xjh_kv8_store, xjh_kv8_load,
+// xjh_attn_kv8.
+//
+// A tile is 64 positions of a kv head, 64 D bytes of keys and as many of values, both
+// cut into 1 KB units that one wavefront reads with 16 bytes per lane and has as
+// matrix operands at once (lane l: li = l & 15, kq = l >> 4):
+//   keys    unit (u, s): lane l holds key 16 u + li, dims 64 s + 16 kq .. + 15
+//   values  unit (d): lane l holds dim 16 d + li of the keys 16 u + 4 kq + r, byte 4 u + r
+// The scores S^T = K Q^T leave lane l with the keys 16 u + 4 kq + r of query row li,
+// which are the weights that it multiplies with those values.
+#include "common.h"
+#include "kernels.h"
+
+namespace xjk {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // rows of any 4-byte alignment
+
+__device__ __forceinline__ int64_t k_at(int pos, int d, int D) {
+    const int p = pos & 63;
+    return (int64_t)(pos >> 6) * 64 * D + (p >> 4) * (16 * D) + (d >> 6) * 1024 + ((d >> 4) & 3) * 256 + (p & 15) * 16 + (d & 15);
+}
+__device__ __forceinline__ int64_t v_at(int pos, int d, int D) {
+    const int p = pos & 63;
+    return (int64_t)(pos >> 6) * 64 * D + (d >> 4) * 1024 + ((p >> 2) & 3) * 256 + (d & 15) * 16 + (p >> 4) * 4 + (p & 3);
+}
+
+__device__ __forceinline__ int clamp_past(int npast, const int32_t *dev) {
+    return dev ? min(max(*dev, 0), npast) : npast;
+}
+
+// ------------------------------------------------------------ quantising --
+
+// Largest magnitude that counts for a scale.
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;   // NaN compares false
+}
+template <bool E4>
+__device__ __forceinline__ float block_scale(float amax) {
+    if (!(amax > 0.f)) return 0.f;
+    float s;
+    if constexpr (E4) {
+        int e;
+        const float m = frexpf(amax, &e);   // 448 = 0.875 * 2^9
+        s = ldexpf(1.f, e - (m <= 0.875f ? 9 : 8));
+    } else {
+        s = (float)((double)amax / 127.0);   // 24 + 53 bits: rounded once
+    }
+    return fmaxf(s, 0x1p-126f);
+}
+// The code of x: nearest to the exact quotient x / s, ties to even.
+//   int8: rint of the product with 1 / s is at most one off; the rest x - c s
+//   is exact in one fma (it is below s and a multiple of the smaller ulp), so comparing
+//   it with s / 2 decides.
+//   e4m3: s is a power of two, the product with 1 / s is exact and converts to nearest even.
+template <bool E4>
+__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
+    if constexpr (E4) {
+        float y = x * inv;
+        y = fminf(fmaxf(y, -448.f), 448.f);
+        if (x != x || s == 0.f) y = 0.f;
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
+    } else {
+        if (x != x || s == 0.f) return 0;
+        float c = rintf(fminf(fmaxf(x * inv, -127.f), 127.f));
+        const float r2 = 2.f * fmaf(-c, s, x);
+        if (r2 > s || (r2 == s && ((int)c & 1))) c += 1.f;
+        else if (r2 < -s || (r2 == -s && ((int)c & 1))) c -= 1.f;
+        c = fminf(fmaxf(c, -127.f), 127.f);
+        return (uint32_t)(int)c & 0xFFu;
+    }
+}
+// A code of scale s_old at the larger scale s: the quotient of the code's value
+// (31 bits at most) by s in double is never on the wrong side of a border.
+template <bool E4>
+__device__ __forceinline__ uint32_t recode(uint32_t c, float s_old, float s) {
+    if constexpr (E4) {
+        const float y = __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * (s_old / s);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
+    } else {
+        return (uint32_t)(int)rint((double)(int8_t)c * (double)s_old / (double)s) & 0xFFu;
+    }
+}
+template <bool E4>
+__device__ __forceinline__ float value_of(uint32_t c, float s) {
+    if constexpr (E4) return __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * s;
+    else return (float)(int8_t)c * s;
+}
+
+// One work-group per block of tokens, kv head and keys | values: the largest magnitude of
+// the new rows, the scale (kept if the block's earlier one is larger), the codes.
+template <int D, bool E4>
+__global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs a) {
+    __shared__ float red[4];
+    const int g = blockIdx.y, tid = threadIdx.x, B = 1 << a.c.lg;
+    const bool val = blockIdx.z;
+    const int np = clamp_past(a.npast, a.npast_dev);
+    const int b = (np >> a.c.lg) + blockIdx.x, first = b << a.c.lg;
+    const int p0 = max(first, np), p1 = min(first + B, np + a.T);
+    if (p0 >= p1) return;
+    const float *x = (val ? a.v : a.k) + g * D;
+    const int64_t tok = val ? a.v_tok : a.k_tok;
+    uint8_t *codes = (val ? a.c.v : a.c.k) + (int64_t)g * a.c.n_tiles * 64 * D;
+    float *sp = (val ? a.c.vs : a.c.ks) + (((int64_t)g * a.c.n_tiles * 64) >> a.c.lg) + b;
+    float m = 0.f;
+    for (int i = tid; i < (p1 - p0) * D; i += 256) m = fmaxf(m, finite_abs(x[(p0 - np + i / D) * tok + i % D]));
+    m = xjd::block_max(m, red);
+    float s = block_scale<E4>(m);
+    if (first < np) {
+        const float old = *sp;
+        __syncthreads();   // every thread has it before it is replaced
+        s = fmaxf(s, old);
+        if (s > old)
+            for (int i = tid; i < (np - first) * D; i += 256) {
+                const int p = first + i / D, d = i % D;
+                uint8_t *c = codes + (val ? v_at(p, d, D) : k_at(p, d, D));
+                *c = (uint8_t)recode<E4>(*c, old, s);
+            }
+    }
+    if (tid == 0) *sp = s;
+    const float inv = s > 0.f ? 1.f / s : 0.f;
+    for (int i = tid; i < (p1 - p0) * D; i += 256) {
+        const int p = p0 + i / D, d = i % D;
+        codes[val ? v_at(p, d, D) : k_at(p, d, D)] = (uint8_t)code_of<E4>(x[(p - np) * tok + d], s, inv);
+    }
+}
+
+template <int D, bool E4>
+__global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs a) {
+    const int g = blockIdx.y, p = a.pos0 + blockIdx.x;
+    const bool val = a.k ? blockIdx.z : true;
+    const uint8_t *codes = (val ? a.c.v : a.c.k) + (int64_t)g * a.c.n_tiles * 64 * D;
+    const float s = (val ? a.c.vs : a.c.ks)[(((int64_t)g * a.c.n_tiles * 64) >> a.c.lg) + (p >> a.c.lg)];
+    float *y = (val ? a.v : a.k) + (int64_t)blockIdx.x * (val ? a.v_tok : a.k_tok) + g * D;
+    for (int d = threadIdx.x; d < D; d += 256) y[d] = value_of<E4>(codes[val ? v_at(p, d, D) : k_at(p, d, D)], s);
+}
+
+// ------------------------------------------------------------- attention --
+
+__device__ __forceinline__ f32x4 mfma16(hf8 a, hf8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Four codes to f16, exactly. int8: c + 128 in the low bits of 1024 is 1152 + c.
+template <bool E4>
+__device__ __forceinline__ void to_half4(uint32_t w, hf2 &x, hf2 &y) {
+    if constexpr (E4) {
+        x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false);
+        y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true);
+    } else {
+        const uint32_t b = w ^ 0x80808080u;
+        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), v = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+        hf2 p, q;
+        __builtin_memcpy(&p, &u, 4);
+        __builtin_memcpy(&q, &v, 4);
+        const hf2 off = {(_Float16)1152.f, (_Float16)1152.f};
+        x = p - off;
+        y = q - off;
+    }
+}
+__device__ __forceinline__ hf8 join8(hf2 a, hf2 b, hf2 c, hf2 d) { return hf8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
+// 16 codes as two operands of 8.
+template <bool E4>
+__device__ __forceinline__ void to_half(u32x4 w, hf8 &a, hf8 &b) {
+    hf2 h[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) to_half4<E4>(w[i], h[2 * i], h[2 * i + 1]);
+    a = join8(h[0], h[1], h[2], h[3]);
+    b = join8(h[4], h[5], h[6], h[7]);
+}
+
+// Two values as f16 planes, y = hi + lo to 22 bits. y is opaque to the compiler: as the product that it
+// comes from, it would be rounded to f16 in one step for hi and in two for lo, and where
+// the two differ (one product in 8000) lo would miss a whole step of hi.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split2(float y0, float y1, hf2 &hi, hf2 &lo) {
+    asm("" : "+v"(y0), "+v"(y1));
+    hi = __builtin_convertvector(f32x2{y0, y1}, hf2);
+    lo = __builtin_convertvector(f32x2{y0 - (float)hi.x, y1 - (float)hi.y}, hf2);   // the differences are exact
+}
+
+// The tiles that the tokens at p0 .. p1 see: the first ns (of the tokens that stay
+// visible), then those from f on; n in all.
+struct Tiles {
+    int ns, f, n;
+};
+__host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, int sinks) {
+    const int lo = window && p0 - window + 1 > 0 ? p0 - window + 1 : 0;
+    Tiles t;
+    t.f = lo >> 6;
+    const int s = window ? (int)(((int64_t)sinks + 63) >> 6) : 0;
+    t.ns = s < t.f ? s : t.f;
+    t.n = t.ns + (p1 >> 6) - t.f + 1;
+    return t;
+}
+
+// Softmax state in powers of two. With t = score + log2(value scale), the weights are
+// kept relative to a reference M that is at least max t - kGrow: w = 2^(t - M) <= 2^kGrow
+// enters as two f16 planes of w * kP (22 bits), whatever the scales' range, the total is of
+// 2^(score - M). The sums are rescaled only when max t passes M by more than kGrow.
+constexpr float kGrow = 8.f, kP = 128.f;
+
+// Split attention: 16 query rows (row = token * G + head of the kv head) per work-group,
+// a wavefront every fourth tile of its split.
+template <int D, bool E4>
+__global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
+    constexpr int NS = D / 64, ND = D / 16;
+    __shared__ __align__(16) float sc[4][3][64];
+    __shared__ float ml[4][2][16];
+    __shared__ __align__(16) float ob[4][16][D + 4];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
+    const int g = blockIdx.y, sp = blockIdx.z, G = a.H / a.c.Hkv, R = a.T * G;
+    const int np = clamp_past(a.npast, a.npast_dev);
+    const int r0 = blockIdx.x * 16, t0 = r0 / G, t1 = min(r0 + 15, R - 1) / G;
+    const Tiles tl = tiles_of(np + t0, np + t1, a.window, a.sinks);
+    const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
+    if (i0 >= tl.n) return;
+    const int row = min(r0 + li, R - 1), t = row / G, h = g * G + row % G, pos = np + t, last = np + a.T - 1;
+    // the lane's query row: dims 64 s + 16 kq + 8 e .. + 7 of step (s, e), x 2^-e = hi + lo
+    hf8 qh[2 * NS], ql[2 * NS];
+    float qsc;
+    {
+        const float *qp = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
+        f32x4 x[4 * NS];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++) {
+            x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
+#pragma unroll
+            for (int c = 0; c < 4; c++) m = fmaxf(m, fabsf(x[i][c]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        int e = 0;
+        if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
+        e = max(e, -100) - 14;
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++) {
+            hf2 hi[4], lo[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                split2(ldexpf(x[2 * i + (c >> 1)][2 * (c & 1)], -e), ldexpf(x[2 * i + (c >> 1)][2 * (c & 1) + 1], -e), hi[c], lo[c]);
+            qh[i] = join8(hi[0], hi[1], hi[2], hi[3]);
+            ql[i] = join8(lo[0], lo[1], lo[2], lo[3]);
+        }
+        qsc = ldexpf(a.scale * 1.44269504088896341f, e);
+    }
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + l * 16, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + l * 16;
+    const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
+    for (int i = i0 + w; i < i1; i += 4) {
+        const int kt = i < tl.ns ? i : tl.f + i - tl.ns, j0 = kt * 64;
+        const uint8_t *kp = kc + (int64_t)kt * 64 * D, *vp = vc + (int64_t)kt * 64 * D;
+        // the tile's scales, one position per lane; positions not written yet have none
+        {
+            const bool in = j0 + l <= last;
+            const float k1 = in ? a.c.ks[s0 + ((j0 + l) >> a.c.lg)] : 0.f, v1 = in ? a.c.vs[s0 + ((j0 + l) >> a.c.lg)] : 0.f;
+            __builtin_amdgcn_wave_barrier();
+            sc[w][0][l] = k1;
+            sc[w][1][l] = v1 * kP;
+            sc[w][2][l] = log2f(fmaxf(v1, 0x1p-100f));
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        f32x4 s[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < NS; st++) {
+                hf8 k0, k1;
+                to_half<E4>(*(const u32x4 *)(kp + u * 16 * D + st * 1024), k0, k1);
+                s[u] = mfma16(k0, ql[2 * st], s[u]);
+                s[u] = mfma16(k1, ql[2 * st + 1], s[u]);
+                s[u] = mfma16(k0, qh[2 * st], s[u]);
+                s[u] = mfma16(k1, qh[2 * st + 1], s[u]);
+            }
+        }
+        float mt = -INFINITY;
+        f32x4 vs[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const f32x4 ks = *(const f32x4 *)&sc[w][0][16 * u + 4 * kq], lv = *(const f32x4 *)&sc[w][2][16 * u + 4 * kq];
+            vs[u] = *(const f32x4 *)&sc[w][1][16 * u + 4 * kq];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int j = j0 + 16 * u + 4 * kq + r;
+                const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+                const float x = s[u][r] * (qsc * ks[r]);
+                s[u][r] = see ? x : -INFINITY;
+                mt = fmaxf(mt, s[u][r] + lv[r]);
+            }
+        }
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if (__any(mt > M + kGrow || (M == -INFINITY && mt > M))) {
+            const float mn = fmaxf(M, mt), al = mn == M ? 1.f : __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= al;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= al;
+        }
+        const float ms = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+        hf2 hi[8], lo[8];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float p = __builtin_amdgcn_exp2f(s[u][r] - ms);
+                L += p;
+                y[r] = p * vs[u][r];
+            }
+            split2(y[0], y[1], hi[2 * u], lo[2 * u]);
+            split2(y[2], y[3], hi[2 * u + 1], lo[2 * u + 1]);
+        }
+        const hf8 ph[2] = {join8(hi[0], hi[1], hi[2], hi[3]), join8(hi[4], hi[5], hi[6], hi[7])};
+        const hf8 pl[2] = {join8(lo[0], lo[1], lo[2], lo[3]), join8(lo[4], lo[5], lo[6], lo[7])};
+        // bytes of values not written yet: an e4m3 one may be a NaN, which a weight of 0 does not take out
+        u32x4 vmask = {~0u, ~0u, ~0u, ~0u};
+        if (E4 && j0 + 63 > last)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int n = last + 1 - (j0 + 16 * u + 4 * kq);
+                vmask[u] = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+            }
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            hf8 v0, v1;
+            to_half<E4>(*(const u32x4 *)(vp + d * 1024) & vmask, v0, v1);
+            o[d] = mfma16(v0, pl[0], o[d]);
+            o[d] = mfma16(v1, pl[1], o[d]);
+            o[d] = mfma16(v0, ph[0], o[d]);
+            o[d] = mfma16(v1, ph[1], o[d]);
+        }
+    }
+    // the four wavefronts' sums joined
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (kq == 0) {
+        ml[w][0][li] = M;
+        ml[w][1][li] = L;
+    }
+    __syncthreads();
+    const float m0 = fmaxf(fmaxf(ml[0][0][li], ml[1][0][li]), fmaxf(ml[2][0][li], ml[3][0][li]));
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m0);
+#pragma unroll
+    for (int d = 0; d < ND; d++) *(f32x4 *)&ob[w][li][16 * d + 4 * kq] = o[d] * f;
+    __syncthreads();
+    for (int idx = tid; idx < 16 * D; idx += 256) {
+        const int r = idx / D, d = idx % D, rr = r0 + r;
+        if (rr >= R) break;
+        float mm = -INFINITY, ll = 0.f;
+        for (int x = 0; x < 4; x++) mm = fmaxf(mm, ml[x][0][r]);
+        for (int x = 0; x < 4; x++) ll += ml[x][0][r] == -INFINITY ? 0.f : ml[x][1][r] * __builtin_amdgcn_exp2f(ml[x][0][r] - mm);
+        const float v = ob[0][r][d] + ob[1][r][d] + ob[2][r][d] + ob[3][r][d];
+        if (a.n_split > 1) {
+            float *part = a.part + (((int64_t)g * R + rr) * a.n_split + sp) * (D + 4);
+            part[4 + d] = v;
+            if (d == 0) part[0] = mm, part[1] = ll;
+        } else {
+            const int tt = rr / G, hh = g * G + rr % G;
+            float y = v * (1.f / kP) / ll;
+            if (a.gate) y *= xjd::sigm(a.gate[tt * a.g_tok + hh * a.g_head + d]);
+            a.out[tt * a.o_tok + (int64_t)hh * D + d] = y;
+        }
+    }
+}
+
+// The splits of a row joined in order.
+template <int D>
+__global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a) {
+    const int G = a.H / a.c.Hkv, R = a.T * G, rr = blockIdx.x, g = blockIdx.y, d = threadIdx.x;
+    const int np = clamp_past(a.npast, a.npast_dev), r0 = rr & ~15;
+    const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + 15, R - 1) / G, a.window, a.sinks);
+    const int ns = (tl.n + a.per_split - 1) / a.per_split;
+    const float *part = a.part + ((int64_t)g * R + rr) * a.n_split * (D + 4);
+    float M = -INFINITY;
+    for (int s = 0; s < ns; s++) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
+    float L = 0.f, y = 0.f;
+    for (int s = 0; s < ns; s++) {
+        const float m = part[(int64_t)s * (D + 4)], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        L = fmaf(f, part[(int64_t)s * (D + 4) + 1], L);
+        y = fmaf(f, part[(int64_t)s * (D + 4) + 4 + d], y);
+    }
+    y = y * (1.f / kP) / L;
+    const int t = rr / G, h = g * G + rr % G;
+    if (a.gate) y *= xjd::sigm(a.gate[t * a.g_tok + h * a.g_head + d]);
+    a.out[t * a.o_tok + (int64_t)h * D + d] = y;
+}
+
+// Tiles that the 16 rows of one work-group see at most.
+static int most_tiles(const Kv8AttnArgs &a) {
+    const int all = (a.npast + a.T - 1) / 64 + 1;
+    if (!a.window) return all;
+    const int G = a.H / a.c.Hkv, span = (16 + G - 1) / G + 1;   // tokens of 16 rows
+    const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
+    return n < all ? (int)n : all;
+}
+// Splits while the work-groups do not exceed two per CU, at least a tile per wavefront.
+static int splits_of(const Kv8AttnArgs &a) {
+    const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + 15) / 16 * a.c.Hkv;
+    const int by_tiles = (most_tiles(a) + 3) / 4;
+    int64_t n = 512 / wgs;
+    if (n > by_tiles) n = by_tiles;
+    return n < 1 ? 1 : (int)n;
+}
+int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
+    const int n = splits_of(a);
+    return n > 1 ? (int64_t)a.T * a.H * n * (a.c.D + 4) : 0;
+}
+
+template <int D, bool E4>
+static void attn_launch_d(const Kv8AttnArgs &a, hipStream_t st) {
+    const int rows = a.T * (a.H / a.c.Hkv);
+    hipLaunchKernelGGL((kv8_rows_kernel<D, E4>), dim3((rows + 15) / 16, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
+    if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a);
+}
+
+int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) {
+    Kv8AttnArgs a = in;
+    int64_t n = splits_of(a), cap = part_floats / ((int64_t)a.T * a.H * (a.c.D + 4));
+    if (n > cap) n = cap;
+    if (n < 1) n = 1;
+    const int tiles = most_tiles(a);
+    a.per_split = (int)((tiles + n - 1) / n);
+    a.n_split = (tiles + a.per_split - 1) / a.per_split;
+    switch (a.c.D) {
+    case 64: a.c.e4m3 ? attn_launch_d<64, true>(a, st) : attn_launch_d<64, false>(a, st); break;
+    case 128: a.c.e4m3 ? attn_launch_d<128, true>(a, st) : attn_launch_d<128, false>(a, st); break;
+    case 256: a.c.e4m3 ? attn_launch_d<256, true>(a, st) : attn_launch_d<256, false>(a, st); break;
+    default: return -1;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int D>
+static void store_launch_d(const Kv8StoreArgs &a, hipStream_t st) {
+    // blocks of T rows from any position
+    const dim3 grid((unsigned)(((int64_t)a.T + (1 << a.c.lg) - 2) >> a.c.lg) + 1, a.c.Hkv, 2);
+    if (a.c.e4m3) hipLaunchKernelGGL((kv8_store_kernel<D, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_store_kernel<D, false>), grid, dim3(256), 0, st, a);
+}
+int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st) {
+    switch (a.c.D) {
+    case 64: store_launch_d<64>(a, st); break;
+    case 128: store_launch_d<128>(a, st); break;
+    case 256: store_launch_d<256>(a, st); break;
+    default: return -1;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int D>
+static void load_launch_d(const Kv8LoadArgs &a, hipStream_t st) {
+    const dim3 grid(a.n, a.c.Hkv, a.k && a.v ? 2 : 1);
+    if (a.c.e4m3) hipLaunchKernelGGL((kv8_load_kernel<D, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_load_kernel<D, false>), grid, dim3(256), 0, st, a);
+}
+int kv8_load_launch(const Kv8LoadArgs &a, hipStream_t st) {
+    switch (a.c.D) {
+    case 64: load_launch_d<64>(a, st); break;
+    case 128: load_launch_d<128>(a, st); break;
+    case 256: load_launch_d<256>(a, st); break;
+    default: return -1;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace xjk

@@ -96,6 +96,20 @@ class XjsConfig(C.Structure):
                 ("eot_id", C.c_int32)]
 
 
+KV_I8, KV_E4M3 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
+
+
+class XjhRopeCfg(C.Structure):
+    _fields_ = [("pairs", C.c_int32), ("n_rot", C.c_int32), ("base", C.c_float), ("scaling", C.c_int32), ("factor", C.c_float),
+                ("n_ctx_orig", C.c_int32), ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("mscale", C.c_float)]
+
+
+class XjhKv8(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "Hkv", "D", "n_ctx", "block")] + [("data", C.c_void_p), ("bytes", C.c_uint64)]
+
+
 # -------------------------------------------------------------- library --
 
 _lib = None
@@ -185,6 +199,13 @@ def lib():
     _sig(L, "xjh_rope", I, P, I, I, I64, I64, I, I, F, CP, S)
     _sig(L, "xjh_conv_silu", I, P, P, P, I, I, I, P, I, CP, S)
     _sig(L, "xjh_attn_decode", I, I, I, I, I, I, F, F, I, I, P, P, P, P, P, P, P, P, CP, S)
+    PK = C.POINTER(XjhKv8)
+    _sig(L, "xjh_rope_scaled", I, P, I64, I64, P, I64, I64, I, I, I, C.POINTER(XjhRopeCfg), P, I, P, CP, S)
+    _sig(L, "xjh_kv8_bytes", U64, PK)
+    _sig(L, "xjh_kv8_store", I, PK, P, I64, P, I64, I, I, P, P, CP, S)
+    _sig(L, "xjh_kv8_load", I, PK, I, I, P, I64, P, I64, P, CP, S)
+    _sig(L, "xjh_attn_kv8", I, PK, P, I64, I64, P, I64, I64, I, I, I, P, I, I, F, P, I64, P, S, P, CP, S)
+    _sig(L, "xjh_attn_kv8_work_bytes", S, PK, I, I, I, I, I)
     _lib = L
     return L
 
@@ -782,6 +803,75 @@ def delta_step(qkv, k_off, v_off, beta_raw, alpha_raw, dt, A, Hk, Hv, S, eps, qs
                                 qscale, ds.ptr, do.ptr, dck.ptr if ck_n else None, ck_n, err, ERR), err, "delta_step")
     return (do.get(np.float32, (T, Hv * S)), ds.get(np.float32, (Hv, S, S)),
             dck.get(np.float32, (ck_n, Hv, S, S)) if ck_n else None)
+
+
+# ---------------------------------------------------------- long contexts --
+
+def rope_scaled(x, n_rot, base, pos, pairs=ROPE_HALF, in_place=False, **scaling):
+    """Rotary positions on the GPU of x [T][heads][D]; pos: the first token's position, or an
+    int32 array of every token's. scaling: the other fields of XjhRopeCfg."""
+    x = np.ascontiguousarray(x, np.float32)
+    T, H, D = x.shape
+    cfg = XjhRopeCfg(pairs=pairs, n_rot=n_rot, base=base, **scaling)
+    dx = Dev(x)
+    do = dx if in_place else Dev(nbytes=max(x.nbytes, 1))
+    dp = None if np.isscalar(pos) else Dev(np.ascontiguousarray(pos, np.int32))
+    err = _err()
+    _check(lib().xjh_rope_scaled(dx.ptr, H * D, D, do.ptr, H * D, D, T, H, D, C.byref(cfg), dp.ptr if dp else None,
+                                 0 if dp else int(pos), None, err, ERR), err, "rope_scaled")
+    lib().xjh_sync()
+    return do.get(np.float32, x.shape)
+
+
+class Kv8:
+    """An 8-bit key/value cache on the GPU (xjh_kv8); arrays in and out are numpy, every call waits."""
+
+    def __init__(self, Hkv, D, n_ctx, block=32, type=KV_I8):
+        self.c = XjhKv8(type=type, Hkv=Hkv, D=D, n_ctx=n_ctx, block=block)
+        n = lib().xjh_kv8_bytes(C.byref(self.c))
+        if not n:
+            raise XjError(f"unsupported cache (Hkv={Hkv}, D={D}, n_ctx={n_ctx}, block={block}, type={type})")
+        self.buf = Dev(np.zeros(n, np.uint8))
+        self.c.data, self.c.bytes = self.buf.ptr, n
+
+    def bytes(self):
+        return self.buf.get(np.uint8, self.c.bytes)
+
+    def put_bytes(self, b):
+        self.buf.put(b)
+
+    def store(self, k, v, n_past):
+        """k, v [T][Hkv][D] into positions n_past .."""
+        k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
+        dk, dv, row, err = Dev(k), Dev(v), self.c.Hkv * self.c.D, _err()
+        _check(lib().xjh_kv8_store(C.byref(self.c), dk.ptr, row, dv.ptr, row, k.shape[0], n_past, None, None, err, ERR), err,
+               "kv8_store")
+        lib().xjh_sync()
+
+    def load(self, pos0, n):
+        """(k, v) [n][Hkv][D] of the positions pos0 .. pos0 + n - 1."""
+        row, err = self.c.Hkv * self.c.D, _err()
+        dk, dv = Dev(nbytes=max(1, n * row * 4)), Dev(nbytes=max(1, n * row * 4))
+        _check(lib().xjh_kv8_load(C.byref(self.c), pos0, n, dk.ptr, row, dv.ptr, row, None, err, ERR), err, "kv8_load")
+        lib().xjh_sync()
+        shape = (n, self.c.Hkv, self.c.D)
+        return dk.get(np.float32, shape), dv.get(np.float32, shape)
+
+    def attend(self, q, n_past, gate=None, window=0, n_sink=0, scale=None, work_bytes=None):
+        """Attention of q [T][H][D] at positions n_past .. over the cache, [T][H*D]. work_bytes: the
+        work area (default: what the library asks for)."""
+        q = np.ascontiguousarray(q, np.float32)
+        T, H, D = q.shape
+        dq, do, err = Dev(q), Dev(nbytes=max(1, q.nbytes)), _err()
+        dg = Dev(np.ascontiguousarray(gate, np.float32)) if gate is not None else None
+        if work_bytes is None:
+            work_bytes = lib().xjh_attn_kv8_work_bytes(C.byref(self.c), T, H, n_past, window, n_sink)
+        dw = Dev(nbytes=work_bytes) if work_bytes else None
+        _check(lib().xjh_attn_kv8(C.byref(self.c), dq.ptr, H * D, D, dg.ptr if dg else None, H * D, D, T, H, n_past, None, window,
+                                  n_sink, D ** -0.5 if scale is None else scale, do.ptr, H * D, dw.ptr if dw else None, work_bytes,
+                                  None, err, ERR), err, "attn_kv8")
+        lib().xjh_sync()
+        return do.get(np.float32, (T, H * D))
 
 
 def device_name():
