@@ -203,35 +203,84 @@ __host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, i
 // 2^(score - M). The sums are rescaled only when max t passes M by more than kGrow.
 constexpr float kGrow = 8.f, kP = 128.f;
 
-// Split attention: 16 query rows (row = token * G + head of the kv head) per work-group,
-// a wavefront every fourth tile of its split.
-template <int D, bool E4>
-__global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
-    constexpr int NS = D / 64, ND = D / 16;
-    __shared__ __align__(16) float sc[4][3][64];
-    __shared__ float ml[4][2][16];
-    __shared__ __align__(16) float ob[4][16][D + 4];
+constexpr int kMaxSplit = 512;
+
+// Work-group barrier ordering LDS accesses only (global loads in flight stay in flight).
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// The sum over the lanes l and l ^ 8 (a row of 16 turned by half).
+__device__ __forceinline__ float add_ror8(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
+}
+
+// N units of 1 KB from p (uniform): a scalar base per 4 KB and one lane offset, so the addresses take no registers.
+template <int N>
+__device__ __forceinline__ void load_units(const uint8_t *p, uint32_t lane, u32x4 (&r)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+        auto b = (const __attribute__((address_space(1))) uint8_t *)(p + c * 1024);
+        asm("" : "+s"(b));
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[c + i] = *(const __attribute__((address_space(1))) u32x4 *)(b + lane + i * 1024);
+    }
+}
+
+// Attention of few rows (row = token * G + head of the kv head): a work-group takes R of them and a split of
+// the tiles, a wavefront every fourth tile of it, straight from the cache into registers. With R = 8 an
+// operand's 16 columns are both planes of the 8 rows, so a product costs one instruction; with R = 16 the planes
+// follow one another. The queries lie in LDS as operands (8 reads of 16 bytes per tile and lane; in
+// registers they would leave no room for the tiles in flight). A tile's values are requested before its scores are
+// formed and the next tile's keys right after, so 16 KB per wavefront are always in flight.
+template <int D, bool E4, int R>
+__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
+    constexpr int NS = D / 64, ND = D / 16, NW = 4;
+    constexpr bool ST = R == 8;
+    __shared__ __align__(16) float sc[NW][3][64];
+    __shared__ float ml[NW][2][R];
+    constexpr int kQ = (ST ? 1 : 2) * 2 * NS * 1024, kO = NW * R * (D + 4) * 4;
+    __shared__ __align__(16) uint8_t mem[kQ > kO ? kQ : kO];   // the queries, then the wavefronts' sums
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
-    const int g = blockIdx.y, sp = blockIdx.z, G = a.H / a.c.Hkv, R = a.T * G;
+    const int g = blockIdx.y, sp = blockIdx.z, G = a.H / a.c.Hkv, rows = a.T * G;
     const int np = clamp_past(a.npast, a.npast_dev);
-    const int r0 = blockIdx.x * 16, t0 = r0 / G, t1 = min(r0 + 15, R - 1) / G;
+    const int r0 = blockIdx.x * R, t0 = r0 / G, t1 = min(r0 + R - 1, rows - 1) / G;
     const Tiles tl = tiles_of(np + t0, np + t1, a.window, a.sinks);
     const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
     if (i0 >= tl.n) return;
-    const int row = min(r0 + li, R - 1), t = row / G, h = g * G + row % G, pos = np + t, last = np + a.T - 1;
+    const int row = min(r0 + (li & (R - 1)), rows - 1), t = row / G, h = g * G + row % G, pos = np + t, last = np + a.T - 1;
+    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D;
+    const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
+    u32x4 kr[4 * NS], vr[ND];
+    float k1 = 0.f, v1 = 0.f;
+    auto tile = [&](int i) { return i < tl.ns ? i : tl.f + i - tl.ns; };
+    auto load_k = [&](int kt) {   // and the tile's scales, one position per lane; positions not written yet have none
+        load_units<4 * NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
+        const int j = kt * 64 + l;
+        const bool in = j <= last;
+        k1 = in ? a.c.ks[s0 + (j >> a.c.lg)] : 0.f;
+        v1 = in ? a.c.vs[s0 + (j >> a.c.lg)] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load_v = [&](int kt) {
+        load_units<ND>(vc + (int64_t)kt * 64 * D, l * 16, vr);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int i = i0 + w;
+    if (i < i1) load_k(tile(i));
     // the lane's query row: dims 64 s + 16 kq + 8 e .. + 7 of step (s, e), x 2^-e = hi + lo
-    hf8 qh[2 * NS], ql[2 * NS];
     float qsc;
     {
         const float *qp = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
         f32x4 x[4 * NS];
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * NS; i++) {
-            x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
+        for (int i = 0; i < 4 * NS; i++) x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) m = fmaxf(m, fabsf(x[i][c]));
-        }
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         int e = 0;
@@ -243,8 +292,14 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; c++)
                 split2(ldexpf(x[2 * i + (c >> 1)][2 * (c & 1)], -e), ldexpf(x[2 * i + (c >> 1)][2 * (c & 1) + 1], -e), hi[c], lo[c]);
-            qh[i] = join8(hi[0], hi[1], hi[2], hi[3]);
-            ql[i] = join8(lo[0], lo[1], lo[2], lo[3]);
+            if (i % NW != w) continue;
+            const hf8 vh = join8(hi[0], hi[1], hi[2], hi[3]), vl = join8(lo[0], lo[1], lo[2], lo[3]);
+            if constexpr (ST) {
+                *(hf8 *)(mem + i * 1024 + l * 16) = li < 8 ? vh : vl;
+            } else {
+                *(hf8 *)(mem + 2 * i * 1024 + l * 16) = vh;
+                *(hf8 *)(mem + (2 * i + 1) * 1024 + l * 16) = vl;
+            }
         }
         qsc = ldexpf(a.scale * 1.44269504088896341f, e);
     }
@@ -252,50 +307,62 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
-    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + l * 16, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + l * 16;
-    const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
-    for (int i = i0 + w; i < i1; i += 4) {
-        const int kt = i < tl.ns ? i : tl.f + i - tl.ns, j0 = kt * 64;
-        const uint8_t *kp = kc + (int64_t)kt * 64 * D, *vp = vc + (int64_t)kt * 64 * D;
-        // the tile's scales, one position per lane; positions not written yet have none
-        {
-            const bool in = j0 + l <= last;
-            const float k1 = in ? a.c.ks[s0 + ((j0 + l) >> a.c.lg)] : 0.f, v1 = in ? a.c.vs[s0 + ((j0 + l) >> a.c.lg)] : 0.f;
-            __builtin_amdgcn_wave_barrier();
-            sc[w][0][l] = k1;
-            sc[w][1][l] = v1 * kP;
-            sc[w][2][l] = log2f(fmaxf(v1, 0x1p-100f));
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
+    lds_barrier();
+    for (; i < i1; i += NW) {
+        const int kt = tile(i), j0 = kt * 64;
+        load_v(kt);
+        __builtin_amdgcn_wave_barrier();
+        sc[w][0][l] = k1;
+        sc[w][1][l] = v1 * kP;
+        sc[w][2][l] = log2f(fmaxf(v1, 0x1p-100f));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         f32x4 s[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int st = 0; st < NS; st++) {
-                hf8 k0, k1;
-                to_half<E4>(*(const u32x4 *)(kp + u * 16 * D + st * 1024), k0, k1);
-                s[u] = mfma16(k0, ql[2 * st], s[u]);
-                s[u] = mfma16(k1, ql[2 * st + 1], s[u]);
-                s[u] = mfma16(k0, qh[2 * st], s[u]);
-                s[u] = mfma16(k1, qh[2 * st + 1], s[u]);
+        for (int st = 0; st < NS; st++) {
+            hf8 qa[ST ? 2 : 4];   // step 2 st and 2 st + 1 (R = 16: both planes of each)
+#pragma unroll
+            for (int c = 0; c < (ST ? 2 : 4); c++) qa[c] = *(const hf8 *)(mem + (st * (ST ? 2 : 4) + c) * 1024 + l * 16);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                hf8 ka, kb;
+                to_half<E4>(kr[u * NS + st], ka, kb);
+                if constexpr (ST) {
+                    s[u] = mfma16(ka, qa[0], s[u]);
+                    s[u] = mfma16(kb, qa[1], s[u]);
+                } else {
+                    s[u] = mfma16(ka, qa[1], s[u]);
+                    s[u] = mfma16(kb, qa[3], s[u]);
+                    s[u] = mfma16(ka, qa[0], s[u]);
+                    s[u] = mfma16(kb, qa[2], s[u]);
+                }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + NW < i1) load_k(tile(i + NW));
         float mt = -INFINITY;
-        f32x4 vs[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const f32x4 ks = *(const f32x4 *)&sc[w][0][16 * u + 4 * kq], lv = *(const f32x4 *)&sc[w][2][16 * u + 4 * kq];
-            vs[u] = *(const f32x4 *)&sc[w][1][16 * u + 4 * kq];
+            const f32x4 ks = *(const f32x4 *)&sc[w][0][16 * u + 4 * kq];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int j = j0 + 16 * u + 4 * kq + r;
-                const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-                const float x = s[u][r] * (qsc * ks[r]);
-                s[u][r] = see ? x : -INFINITY;
-                mt = fmaxf(mt, s[u][r] + lv[r]);
-            }
+            for (int r = 0; r < 4; r++) s[u][r] = (ST ? add_ror8(s[u][r]) : s[u][r]) * (qsc * ks[r]);
+        }
+        // a tile that some row does not see whole
+        if (j0 + 63 > np + t0 || (a.window && j0 <= np + t1 - a.window && j0 + 63 >= a.sinks))
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = j0 + 16 * u + 4 * kq + r;
+                    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
+                }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const f32x4 lv = *(const f32x4 *)&sc[w][2][16 * u + 4 * kq];
+#pragma unroll
+            for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
         }
         mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
@@ -310,58 +377,78 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
         hf2 hi[8], lo[8];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
+            const f32x4 vs = *(const f32x4 *)&sc[w][1][16 * u + 4 * kq];
             float y[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float p = __builtin_amdgcn_exp2f(s[u][r] - ms);
                 L += p;
-                y[r] = p * vs[u][r];
+                y[r] = p * vs[r];
             }
             split2(y[0], y[1], hi[2 * u], lo[2 * u]);
             split2(y[2], y[3], hi[2 * u + 1], lo[2 * u + 1]);
         }
-        const hf8 ph[2] = {join8(hi[0], hi[1], hi[2], hi[3]), join8(hi[4], hi[5], hi[6], hi[7])};
-        const hf8 pl[2] = {join8(lo[0], lo[1], lo[2], lo[3]), join8(lo[4], lo[5], lo[6], lo[7])};
+        hf8 ph[2] = {join8(hi[0], hi[1], hi[2], hi[3]), join8(hi[4], hi[5], hi[6], hi[7])};
+        hf8 pl[2] = {join8(lo[0], lo[1], lo[2], lo[3]), join8(lo[4], lo[5], lo[6], lo[7])};
+        if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
+            if (li >= 8) ph[0] = pl[0], ph[1] = pl[1];
+        }
         // bytes of values not written yet: an e4m3 one may be a NaN, which a weight of 0 does not take out
-        u32x4 vmask = {~0u, ~0u, ~0u, ~0u};
-        if (E4 && j0 + 63 > last)
+        if (E4 && j0 + 63 > last) {
+            u32x4 vmask;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const int n = last + 1 - (j0 + 16 * u + 4 * kq);
                 vmask[u] = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
             }
 #pragma unroll
+            for (int d = 0; d < ND; d++) vr[d] &= vmask;
+        }
+#pragma unroll
         for (int d = 0; d < ND; d++) {
-            hf8 v0, v1;
-            to_half<E4>(*(const u32x4 *)(vp + d * 1024) & vmask, v0, v1);
-            o[d] = mfma16(v0, pl[0], o[d]);
-            o[d] = mfma16(v1, pl[1], o[d]);
-            o[d] = mfma16(v0, ph[0], o[d]);
-            o[d] = mfma16(v1, ph[1], o[d]);
+            hf8 va, vb;
+            to_half<E4>(vr[d], va, vb);
+            if constexpr (!ST) {
+                o[d] = mfma16(va, pl[0], o[d]);
+                o[d] = mfma16(vb, pl[1], o[d]);
+            }
+            o[d] = mfma16(va, ph[0], o[d]);
+            o[d] = mfma16(vb, ph[1], o[d]);
         }
     }
-    // the four wavefronts' sums joined
+    // the wavefronts' sums joined
     L += __shfl_xor(L, 16, 64);
     L += __shfl_xor(L, 32, 64);
-    if (kq == 0) {
-        ml[w][0][li] = M;
-        ml[w][1][li] = L;
+    if (l < R) {
+        ml[w][0][l] = M;
+        ml[w][1][l] = L;
     }
-    __syncthreads();
-    const float m0 = fmaxf(fmaxf(ml[0][0][li], ml[1][0][li]), fmaxf(ml[2][0][li], ml[3][0][li]));
-    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m0);
+    lds_barrier();   // every wavefront is done with the queries, too
+    float m0 = ml[0][0][li & (R - 1)];
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(f32x4 *)&ob[w][li][16 * d + 4 * kq] = o[d] * f;
-    __syncthreads();
-    for (int idx = tid; idx < 16 * D; idx += 256) {
+    for (int x = 1; x < NW; x++) m0 = fmaxf(m0, ml[x][0][li & (R - 1)]);
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m0);
+    float(*ob)[R][D + 4] = (float(*)[R][D + 4])mem;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+        f32x4 v = o[d] * f;
+        if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
+        if (li < R) *(f32x4 *)&ob[w][li][16 * d + 4 * kq] = v;
+    }
+    lds_barrier();
+    for (int idx = tid; idx < R * D; idx += 256) {
         const int r = idx / D, d = idx % D, rr = r0 + r;
-        if (rr >= R) break;
-        float mm = -INFINITY, ll = 0.f;
-        for (int x = 0; x < 4; x++) mm = fmaxf(mm, ml[x][0][r]);
-        for (int x = 0; x < 4; x++) ll += ml[x][0][r] == -INFINITY ? 0.f : ml[x][1][r] * __builtin_amdgcn_exp2f(ml[x][0][r] - mm);
-        const float v = ob[0][r][d] + ob[1][r][d] + ob[2][r][d] + ob[3][r][d];
+        if (rr >= rows) break;
+        float mm = ml[0][0][r], ll = 0.f, v = 0.f;
+#pragma unroll
+        for (int x = 1; x < NW; x++) mm = fmaxf(mm, ml[x][0][r]);
+#pragma unroll
+        for (int x = 0; x < NW; x++) {
+            ll += ml[x][0][r] == -INFINITY ? 0.f : ml[x][1][r] * __builtin_amdgcn_exp2f(ml[x][0][r] - mm);
+            v += ob[x][r][d];
+        }
         if (a.n_split > 1) {
-            float *part = a.part + (((int64_t)g * R + rr) * a.n_split + sp) * (D + 4);
+            float *part = a.part + (((int64_t)g * rows + rr) * a.n_split + sp) * (D + 4);
             part[4 + d] = v;
             if (d == 0) part[0] = mm, part[1] = ll;
         } else {
@@ -373,40 +460,55 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(const Kv8AttnArgs a) {
     }
 }
 
-// The splits of a row joined in order.
+// The splits of a row joined in order: the first wavefront forms every split's factor, a thread per dim sums.
 template <int D>
-__global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a) {
-    const int G = a.H / a.c.Hkv, R = a.T * G, rr = blockIdx.x, g = blockIdx.y, d = threadIdx.x;
-    const int np = clamp_past(a.npast, a.npast_dev), r0 = rr & ~15;
-    const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + 15, R - 1) / G, a.window, a.sinks);
+__global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a, int R) {
+    __shared__ float fac[kMaxSplit];
+    __shared__ float total;
+    const int G = a.H / a.c.Hkv, rows = a.T * G, rr = blockIdx.x, g = blockIdx.y, d = threadIdx.x;
+    const int np = clamp_past(a.npast, a.npast_dev), r0 = rr / R * R;
+    const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + R - 1, rows - 1) / G, a.window, a.sinks);
     const int ns = (tl.n + a.per_split - 1) / a.per_split;
-    const float *part = a.part + ((int64_t)g * R + rr) * a.n_split * (D + 4);
-    float M = -INFINITY;
-    for (int s = 0; s < ns; s++) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
-    float L = 0.f, y = 0.f;
-    for (int s = 0; s < ns; s++) {
-        const float m = part[(int64_t)s * (D + 4)], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-        L = fmaf(f, part[(int64_t)s * (D + 4) + 1], L);
-        y = fmaf(f, part[(int64_t)s * (D + 4) + 4 + d], y);
+    const float *part = a.part + ((int64_t)g * rows + rr) * a.n_split * (D + 4);
+    if (d < 64) {
+        float M = -INFINITY, L = 0.f;
+        for (int s = d; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
+        M = xjd::wave_max(M);
+        for (int s = d; s < ns; s += 64) {
+            const float m = part[(int64_t)s * (D + 4)], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+            fac[s] = f;
+            L = fmaf(f, part[(int64_t)s * (D + 4) + 1], L);
+        }
+        L = xjd::row16_sum(L);
+        L += __shfl_xor(L, 16, 64);
+        L += __shfl_xor(L, 32, 64);
+        if (d == 0) total = L;
     }
-    y = y * (1.f / kP) / L;
+    __syncthreads();
+    float y = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < ns; s++) y = fmaf(fac[s], part[(int64_t)s * (D + 4) + 4 + d], y);
+    y = y * (1.f / kP) / total;
     const int t = rr / G, h = g * G + rr % G;
     if (a.gate) y *= xjd::sigm(a.gate[t * a.g_tok + h * a.g_head + d]);
     a.out[t * a.o_tok + (int64_t)h * D + d] = y;
 }
 
-// Tiles that the 16 rows of one work-group see at most.
-static int most_tiles(const Kv8AttnArgs &a) {
+// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions).
+static int rows_of(const Kv8AttnArgs &a) { return (int64_t)a.T * (a.H / a.c.Hkv) <= 8 ? 8 : 16; }
+// Tiles that R rows see at most.
+static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int all = (a.npast + a.T - 1) / 64 + 1;
     if (!a.window) return all;
-    const int G = a.H / a.c.Hkv, span = (16 + G - 1) / G + 1;   // tokens of 16 rows
+    const int G = a.H / a.c.Hkv, span = (R + G - 1) / G + 1;   // tokens of R rows
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
 // Splits while the work-groups do not exceed two per CU, at least a tile per wavefront.
 static int splits_of(const Kv8AttnArgs &a) {
-    const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + 15) / 16 * a.c.Hkv;
-    const int by_tiles = (most_tiles(a) + 3) / 4;
+    const int R = rows_of(a);
+    const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
+    const int by_tiles = (most_tiles(a, R) + 3) / 4;
     int64_t n = 512 / wgs;
     if (n > by_tiles) n = by_tiles;
     return n < 1 ? 1 : (int)n;
@@ -417,10 +519,12 @@ int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
 }
 
 template <int D, bool E4>
-static void attn_launch_d(const Kv8AttnArgs &a, hipStream_t st) {
+static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     const int rows = a.T * (a.H / a.c.Hkv);
-    hipLaunchKernelGGL((kv8_rows_kernel<D, E4>), dim3((rows + 15) / 16, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
-    if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a);
+    const dim3 grid((rows + R - 1) / R, a.c.Hkv, a.n_split);
+    if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
+    if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a, R);
 }
 
 int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) {
@@ -428,13 +532,13 @@ int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) 
     int64_t n = splits_of(a), cap = part_floats / ((int64_t)a.T * a.H * (a.c.D + 4));
     if (n > cap) n = cap;
     if (n < 1) n = 1;
-    const int tiles = most_tiles(a);
+    const int R = rows_of(a), tiles = most_tiles(a, R);
     a.per_split = (int)((tiles + n - 1) / n);
     a.n_split = (tiles + a.per_split - 1) / a.per_split;
     switch (a.c.D) {
-    case 64: a.c.e4m3 ? attn_launch_d<64, true>(a, st) : attn_launch_d<64, false>(a, st); break;
-    case 128: a.c.e4m3 ? attn_launch_d<128, true>(a, st) : attn_launch_d<128, false>(a, st); break;
-    case 256: a.c.e4m3 ? attn_launch_d<256, true>(a, st) : attn_launch_d<256, false>(a, st); break;
+    case 64: a.c.e4m3 ? attn_launch_d<64, true>(a, R, st) : attn_launch_d<64, false>(a, R, st); break;
+    case 128: a.c.e4m3 ? attn_launch_d<128, true>(a, R, st) : attn_launch_d<128, false>(a, R, st); break;
+    case 256: a.c.e4m3 ? attn_launch_d<256, true>(a, R, st) : attn_launch_d<256, false>(a, R, st); break;
     default: return -1;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
