@@ -20,15 +20,6 @@ typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // rows of any 4-byte alignment
 
-__device__ __forceinline__ int64_t k_at(int pos, int d, int D) {
-    const int p = pos & 63;
-    return (int64_t)(pos >> 6) * 64 * D + (p >> 4) * (16 * D) + (d >> 6) * 1024 + ((d >> 4) & 3) * 256 + (p & 15) * 16 + (d & 15);
-}
-__device__ __forceinline__ int64_t v_at(int pos, int d, int D) {
-    const int p = pos & 63;
-    return (int64_t)(pos >> 6) * 64 * D + (d >> 4) * 1024 + ((p >> 2) & 3) * 256 + (d & 15) * 16 + (p >> 4) * 4 + (p & 3);
-}
-
 __device__ __forceinline__ int clamp_past(int npast, const int32_t *dev) {
     return dev ? min(max(*dev, 0), npast) : npast;
 }
@@ -92,52 +83,154 @@ __device__ __forceinline__ float value_of(uint32_t c, float s) {
     else return (float)(int8_t)c * s;
 }
 
-// One work-group per block of tokens, kv head and keys | values: the largest magnitude of
-// the new rows, the scale (kept if the block's earlier one is larger), the codes.
-template <int D, bool E4>
-__global__ __launch_bounds__(256) void kv8_store_kernel(const Kv8StoreArgs a) {
-    __shared__ float red[4];
-    const int g = blockIdx.y, tid = threadIdx.x, B = 1 << a.c.lg;
-    const bool val = blockIdx.z;
-    const int np = clamp_past(a.npast, a.npast_dev);
-    const int b = (np >> a.c.lg) + blockIdx.x, first = b << a.c.lg;
-    const int p0 = max(first, np), p1 = min(first + B, np + a.T);
-    if (p0 >= p1) return;
-    const float *x = (val ? a.v : a.k) + g * D;
-    const int64_t tok = val ? a.v_tok : a.k_tok;
-    uint8_t *codes = (val ? a.c.v : a.c.k) + (int64_t)g * a.c.n_tiles * 64 * D;
-    float *sp = (val ? a.c.vs : a.c.ks) + (((int64_t)g * a.c.n_tiles * 64) >> a.c.lg) + b;
-    float m = 0.f;
-    for (int i = tid; i < (p1 - p0) * D; i += 256) m = fmaxf(m, finite_abs(x[(p0 - np + i / D) * tok + i % D]));
-    m = xjd::block_max(m, red);
-    float s = block_scale<E4>(m);
-    if (first < np) {
-        const float old = *sp;
-        __syncthreads();   // every thread has it before it is replaced
-        s = fmaxf(s, old);
-        if (s > old)
-            for (int i = tid; i < (np - first) * D; i += 256) {
-                const int p = first + i / D, d = i % D;
-                uint8_t *c = codes + (val ? v_at(p, d, D) : k_at(p, d, D));
-                *c = (uint8_t)recode<E4>(*c, old, s);
-            }
-    }
-    if (tid == 0) *sp = s;
-    const float inv = s > 0.f ? 1.f / s : 0.f;
-    for (int i = tid; i < (p1 - p0) * D; i += 256) {
-        const int p = p0 + i / D, d = i % D;
-        codes[val ? v_at(p, d, D) : k_at(p, d, D)] = (uint8_t)code_of<E4>(x[(p - np) * tok + d], s, inv);
+// Store and load move a tile in groups of 16 positions by D / 4 lanes, a lane 4 dims, so that the float rows
+// (four times the codes' bytes) go 16 bytes per lane and whole rows per instruction. Group q of the
+// keys is the 16 positions of one unit row; of the values the positions 16 u + 4 q + r, whose codes of a dim
+// are 16 bytes.
+template <bool VAL>
+__device__ __forceinline__ int group_pos(int q, int i) { return VAL ? 16 * (i >> 2) + 4 * q + (i & 3) : 16 * q + i; }
+
+// The lane's codes: w[i] byte c = dim d0 + c of the group's position i.
+template <int D, bool VAL>
+__device__ __forceinline__ void get_codes(const uint8_t *tile, int q, int d0, uint32_t (&w)[16]) {
+    if constexpr (VAL) {
+        const uint8_t *p = tile + (d0 >> 4) * 1024 + q * 256 + (d0 & 15) * 16;
+        u32x4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = *(const u32x4 *)(p + 16 * c);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {   // 4 dims x 4 positions turned
+            const uint32_t a = __builtin_amdgcn_perm(v[1][u], v[0][u], 0x05010400u), b = __builtin_amdgcn_perm(v[1][u], v[0][u], 0x07030602u);
+            const uint32_t c = __builtin_amdgcn_perm(v[3][u], v[2][u], 0x05010400u), d = __builtin_amdgcn_perm(v[3][u], v[2][u], 0x07030602u);
+            w[4 * u] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+            w[4 * u + 1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+            w[4 * u + 2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+            w[4 * u + 3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+        }
+    } else {
+        const uint8_t *p = tile + q * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (d0 & 15);
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = *(const uint32_t *)(p + 16 * i);
     }
 }
+template <int D, bool VAL>
+__device__ __forceinline__ void put_codes(uint8_t *tile, int q, int d0, const uint32_t (&w)[16]) {
+    if constexpr (VAL) {
+        uint8_t *p = tile + (d0 >> 4) * 1024 + q * 256 + (d0 & 15) * 16;
+        u32x4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint32_t a = __builtin_amdgcn_perm(w[4 * u + 1], w[4 * u], 0x05010400u), b = __builtin_amdgcn_perm(w[4 * u + 1], w[4 * u], 0x07030602u);
+            const uint32_t c = __builtin_amdgcn_perm(w[4 * u + 3], w[4 * u + 2], 0x05010400u), d = __builtin_amdgcn_perm(w[4 * u + 3], w[4 * u + 2], 0x07030602u);
+            v[0][u] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+            v[1][u] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+            v[2][u] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+            v[3][u] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) *(u32x4 *)(p + 16 * c) = v[c];
+    } else {
+        uint8_t *p = tile + q * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (d0 & 15);
+#pragma unroll
+        for (int i = 0; i < 16; i++) *(uint32_t *)(p + 16 * i) = w[i];
+    }
+}
+// The largest of D / 4 consecutive lanes, in each of them.
+template <int D>
+__device__ __forceinline__ float row_max(float v) {
+    v = xjd::row16_max(v);
+    if (D >= 128) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    if (D >= 256) v = fmaxf(v, __shfl_xor(v, 32, 64));
+    return v;
+}
 
+// A work-group stores one tile of a kv head's keys or values (D threads, a group each D / 4): the
+// rows' largest magnitudes, joined over every block in LDS, the scales, the codes. In a
+// tile that is not new from end to end the codes of the other positions are read
+// and written back as they are, those of a begun block at its new scale if that grew.
+template <int D, bool E4, bool VAL>
+__device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64]) {
+    const int g = blockIdx.y, tid = threadIdx.x, q = tid / (D / 4), d0 = tid % (D / 4) * 4, B = 1 << a.c.lg;
+    const int np = clamp_past(a.npast, a.npast_dev), kt = (np >> 6) + blockIdx.x, j0 = kt * 64, end = np + a.T;
+    if (j0 >= end) return;
+    const float *x = (VAL ? a.v : a.k) + g * D + d0;
+    const int64_t tok = VAL ? a.v_tok : a.k_tok;
+    uint8_t *tile = (VAL ? a.c.v : a.c.k) + ((int64_t)g * a.c.n_tiles + kt) * 64 * D;
+    float *sp = (VAL ? a.c.vs : a.c.ks) + ((((int64_t)g * a.c.n_tiles + kt) * 64) >> a.c.lg);
+    const bool whole = j0 >= np && j0 + 64 <= end;
+    uint32_t w[16];
+    if (!whole) get_codes<D, VAL>(tile, q, d0, w);
+    f32x4 y[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int p = j0 + group_pos<VAL>(q, i);
+        y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p >= np && p < end) y[i] = *(const f32x4_u *)(x + (int64_t)(p - np) * tok);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float m = row_max<D>(fmaxf(fmaxf(finite_abs(y[i].x), finite_abs(y[i].y)), fmaxf(finite_abs(y[i].z), finite_abs(y[i].w))));
+        if (d0 == 0) sm[0][group_pos<VAL>(q, i)] = m;
+    }
+    __syncthreads();
+    if (tid < 64) {   // position j0 + tid: sm[0] its block's scale, sm[1] the block's earlier scale if it is begun
+        float m = sm[0][tid];
+        for (int o = 1; o < B; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const int first = (j0 + tid) & -B;
+        float s = block_scale<E4>(m), old = 0.f;
+        if (first < np && first + B > np) {
+            old = sp[tid >> a.c.lg];
+            s = fmaxf(s, old);
+        }
+        sm[0][tid] = s;
+        sm[1][tid] = old;
+        if ((tid & (B - 1)) == 0 && first < end && first + B > np) sp[tid >> a.c.lg] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int pl = group_pos<VAL>(q, i), p = j0 + pl;
+        const float s = sm[0][pl], inv = s > 0.f ? 1.f / s : 0.f;
+        if (whole || (p >= np && p < end)) {
+            w[i] = code_of<E4>(y[i].x, s, inv) | code_of<E4>(y[i].y, s, inv) << 8 | code_of<E4>(y[i].z, s, inv) << 16 | code_of<E4>(y[i].w, s, inv) << 24;
+        } else if (p < np && (p | (B - 1)) >= np) {
+            const float old = sm[1][pl];
+            if (s > old)
+                w[i] = recode<E4>(w[i] & 0xFFu, old, s) | recode<E4>(w[i] >> 8 & 0xFFu, old, s) << 8 |
+                       recode<E4>(w[i] >> 16 & 0xFFu, old, s) << 16 | recode<E4>(w[i] >> 24, old, s) << 24;
+        }
+    }
+    put_codes<D, VAL>(tile, q, d0, w);
+}
 template <int D, bool E4>
-__global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8LoadArgs a) {
-    const int g = blockIdx.y, p = a.pos0 + blockIdx.x;
-    const bool val = a.k ? blockIdx.z : true;
-    const uint8_t *codes = (val ? a.c.v : a.c.k) + (int64_t)g * a.c.n_tiles * 64 * D;
-    const float s = (val ? a.c.vs : a.c.ks)[(((int64_t)g * a.c.n_tiles * 64) >> a.c.lg) + (p >> a.c.lg)];
-    float *y = (val ? a.v : a.k) + (int64_t)blockIdx.x * (val ? a.v_tok : a.k_tok) + g * D;
-    for (int d = threadIdx.x; d < D; d += 256) y[d] = value_of<E4>(codes[val ? v_at(p, d, D) : k_at(p, d, D)], s);
+__global__ __launch_bounds__(D) void kv8_store_kernel(const Kv8StoreArgs a) {
+    __shared__ float sm[2][64];
+    if (blockIdx.z) store_tile<D, E4, true>(a, sm);
+    else store_tile<D, E4, false>(a, sm);
+}
+
+template <int D, bool E4, bool VAL>
+__device__ __forceinline__ void load_tile(const Kv8LoadArgs &a) {
+    const int g = blockIdx.y, tid = threadIdx.x, q = tid / (D / 4), d0 = tid % (D / 4) * 4;
+    const int kt = (a.pos0 >> 6) + blockIdx.x, j0 = kt * 64;
+    const float *sp = (VAL ? a.c.vs : a.c.ks) + ((((int64_t)g * a.c.n_tiles + kt) * 64) >> a.c.lg);
+    uint32_t w[16];
+    get_codes<D, VAL>((VAL ? a.c.v : a.c.k) + ((int64_t)g * a.c.n_tiles + kt) * 64 * D, q, d0, w);
+    float *y = (VAL ? a.v : a.k) + g * D + d0;
+    const int64_t tok = VAL ? a.v_tok : a.k_tok;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int pl = group_pos<VAL>(q, i), t = j0 + pl - a.pos0;
+        if (t < 0 || t >= a.n) continue;
+        const float s = sp[pl >> a.c.lg];
+        *(f32x4_u *)(y + t * tok) = f32x4{value_of<E4>(w[i] & 0xFFu, s), value_of<E4>(w[i] >> 8 & 0xFFu, s), value_of<E4>(w[i] >> 16 & 0xFFu, s),
+                                          value_of<E4>(w[i] >> 24, s)};
+    }
+}
+template <int D, bool E4>
+__global__ __launch_bounds__(D) void kv8_load_kernel(const Kv8LoadArgs a) {
+    if (a.k && !(a.v && blockIdx.z)) load_tile<D, E4, false>(a);
+    else load_tile<D, E4, true>(a);
 }
 
 // ------------------------------------------------------------- attention --
@@ -546,10 +639,9 @@ int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) 
 
 template <int D>
 static void store_launch_d(const Kv8StoreArgs &a, hipStream_t st) {
-    // blocks of T rows from any position
-    const dim3 grid((unsigned)(((int64_t)a.T + (1 << a.c.lg) - 2) >> a.c.lg) + 1, a.c.Hkv, 2);
-    if (a.c.e4m3) hipLaunchKernelGGL((kv8_store_kernel<D, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_store_kernel<D, false>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(((int64_t)a.T + 62) >> 6) + 1, a.c.Hkv, 2);   // tiles of T rows from any position
+    if (a.c.e4m3) hipLaunchKernelGGL((kv8_store_kernel<D, true>), grid, dim3(D), 0, st, a);
+    else hipLaunchKernelGGL((kv8_store_kernel<D, false>), grid, dim3(D), 0, st, a);
 }
 int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st) {
     switch (a.c.D) {
@@ -563,9 +655,9 @@ int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st) {
 
 template <int D>
 static void load_launch_d(const Kv8LoadArgs &a, hipStream_t st) {
-    const dim3 grid(a.n, a.c.Hkv, a.k && a.v ? 2 : 1);
-    if (a.c.e4m3) hipLaunchKernelGGL((kv8_load_kernel<D, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_load_kernel<D, false>), grid, dim3(256), 0, st, a);
+    const dim3 grid(((a.pos0 + a.n - 1) >> 6) - (a.pos0 >> 6) + 1, a.c.Hkv, a.k && a.v ? 2 : 1);
+    if (a.c.e4m3) hipLaunchKernelGGL((kv8_load_kernel<D, true>), grid, dim3(D), 0, st, a);
+    else hipLaunchKernelGGL((kv8_load_kernel<D, false>), grid, dim3(D), 0, st, a);
 }
 int kv8_load_launch(const Kv8LoadArgs &a, hipStream_t st) {
     switch (a.c.D) {
