@@ -309,6 +309,109 @@ __device__ __forceinline__ float add_ror8(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
 }
 
+// A lane's part of its query row as operands, step (s, e) the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo. Returns what
+// a product of them is multiplied with: the row's 2^e, the scale and log2 e.
+template <int D>
+__device__ __forceinline__ float split_query(const float *q, float scale, hf8 (&qh)[D / 32], hf8 (&ql)[D / 32]) {
+    f32x4 x[D / 16];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) x[i] = *(const f32x4_u *)(q + 64 * (i >> 2) + 4 * (i & 3));
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) m = fmaxf(m, fabsf(x[i][c]));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    int e = 0;
+    if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
+    e = max(e, -100) - 14;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        hf2 hi[4], lo[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            split2(ldexpf(x[2 * i + (c >> 1)][2 * (c & 1)], -e), ldexpf(x[2 * i + (c >> 1)][2 * (c & 1) + 1], -e), hi[c], lo[c]);
+        qh[i] = join8(hi[0], hi[1], hi[2], hi[3]);
+        ql[i] = join8(lo[0], lo[1], lo[2], lo[3]);
+    }
+    return ldexpf(scale * 1.44269504088896341f, e);
+}
+
+// The softmax of a tile's scores: s (products so far) becomes the weights' planes. sc: the tile's scales (keys, values times
+// kP, log2 of the values'); edge: some row does not see the whole tile.
+template <bool ST, int ND>
+__device__ __forceinline__ void tile_weights(const Kv8AttnArgs &a, f32x4 (&s)[4], const float (*sc)[64], float qsc, int j0, int pos, bool edge,
+                                             float &M, float &L, f32x4 (&o)[ND], hf8 (&ph)[2], hf8 (&pl)[2]) {
+    const int kq = (threadIdx.x & 63) >> 4;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const f32x4 ks = *(const f32x4 *)&sc[0][16 * u + 4 * kq];
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[u][r] = (ST ? add_ror8(s[u][r]) : s[u][r]) * (qsc * ks[r]);
+    }
+    if (edge)
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int j = j0 + 16 * u + 4 * kq + r;
+                if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
+            }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const f32x4 lv = *(const f32x4 *)&sc[2][16 * u + 4 * kq];
+#pragma unroll
+        for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
+    }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    if (__any(mt > M + kGrow || (M == -INFINITY && mt > M))) {
+        const float mn = fmaxf(M, mt), al = mn == M ? 1.f : __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        L *= al;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= al;
+    }
+    const float ms = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+    hf2 hi[8], lo[8];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const f32x4 vs = *(const f32x4 *)&sc[1][16 * u + 4 * kq];
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float p = __builtin_amdgcn_exp2f(s[u][r] - ms);
+            L += p;
+            y[r] = p * vs[r];
+        }
+        split2(y[0], y[1], hi[2 * u], lo[2 * u]);
+        split2(y[2], y[3], hi[2 * u + 1], lo[2 * u + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        ph[i] = join8(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+        pl[i] = join8(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+    }
+}
+// Some row at the positions p0 .. p1 does not see the whole tile at j0.
+__device__ __forceinline__ bool tile_edge(const Kv8AttnArgs &a, int j0, int p0, int p1) {
+    return j0 + 63 > p0 || (a.window && j0 <= p1 - a.window && j0 + 63 >= a.sinks);
+}
+// The lane's bytes of a values unit at j0 that positions after `last` do not hold: an e4m3 code not written yet may be a NaN,
+// which a weight of 0 does not take out.
+__device__ __forceinline__ u32x4 written(int j0, int last) {
+    const int kq = (threadIdx.x & 63) >> 4;
+    u32x4 m;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int n = last + 1 - (j0 + 16 * u + 4 * kq);
+        m[u] = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+    }
+    return m;
+}
+
 // N units of 1 KB from p (uniform): a scalar base per 4 KB and one lane offset, so the addresses take no registers.
 template <int N>
 __device__ __forceinline__ void load_units(const uint8_t *p, uint32_t lane, u32x4 (&r)[N]) {
@@ -362,39 +465,17 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
     };
     int i = i0 + w;
     if (i < i1) load_k(tile(i));
-    // the lane's query row: dims 64 s + 16 kq + 8 e .. + 7 of step (s, e), x 2^-e = hi + lo
-    float qsc;
-    {
-        const float *qp = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
-        f32x4 x[4 * NS];
-        float m = 0.f;
+    hf8 qh[2 * NS], ql[2 * NS];
+    const float qsc = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
 #pragma unroll
-        for (int i = 0; i < 4 * NS; i++) x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
-#pragma unroll
-        for (int i = 0; i < 4 * NS; i++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) m = fmaxf(m, fabsf(x[i][c]));
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        int e = 0;
-        if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-        e = max(e, -100) - 14;
-#pragma unroll
-        for (int i = 0; i < 2 * NS; i++) {
-            hf2 hi[4], lo[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-                split2(ldexpf(x[2 * i + (c >> 1)][2 * (c & 1)], -e), ldexpf(x[2 * i + (c >> 1)][2 * (c & 1) + 1], -e), hi[c], lo[c]);
-            if (i % NW != w) continue;
-            const hf8 vh = join8(hi[0], hi[1], hi[2], hi[3]), vl = join8(lo[0], lo[1], lo[2], lo[3]);
-            if constexpr (ST) {
-                *(hf8 *)(mem + i * 1024 + l * 16) = li < 8 ? vh : vl;
-            } else {
-                *(hf8 *)(mem + 2 * i * 1024 + l * 16) = vh;
-                *(hf8 *)(mem + (2 * i + 1) * 1024 + l * 16) = vl;
-            }
+    for (int i = 0; i < 2 * NS; i++) {
+        if (i % NW != w) continue;
+        if constexpr (ST) {
+            *(hf8 *)(mem + i * 1024 + l * 16) = li < 8 ? qh[i] : ql[i];
+        } else {
+            *(hf8 *)(mem + 2 * i * 1024 + l * 16) = qh[i];
+            *(hf8 *)(mem + (2 * i + 1) * 1024 + l * 16) = ql[i];
         }
-        qsc = ldexpf(a.scale * 1.44269504088896341f, e);
     }
     f32x4 o[ND];
 #pragma unroll
@@ -435,67 +516,15 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
         if (i + NW < i1) load_k(tile(i + NW));
-        float mt = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const f32x4 ks = *(const f32x4 *)&sc[w][0][16 * u + 4 * kq];
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[u][r] = (ST ? add_ror8(s[u][r]) : s[u][r]) * (qsc * ks[r]);
-        }
-        // a tile that some row does not see whole
-        if (j0 + 63 > np + t0 || (a.window && j0 <= np + t1 - a.window && j0 + 63 >= a.sinks))
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int j = j0 + 16 * u + 4 * kq + r;
-                    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
-                }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const f32x4 lv = *(const f32x4 *)&sc[w][2][16 * u + 4 * kq];
-#pragma unroll
-            for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
-        }
-        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-        if (__any(mt > M + kGrow || (M == -INFINITY && mt > M))) {
-            const float mn = fmaxf(M, mt), al = mn == M ? 1.f : __builtin_amdgcn_exp2f(M - mn);
-            M = mn;
-            L *= al;
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[d] *= al;
-        }
-        const float ms = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
-        hf2 hi[8], lo[8];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const f32x4 vs = *(const f32x4 *)&sc[w][1][16 * u + 4 * kq];
-            float y[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float p = __builtin_amdgcn_exp2f(s[u][r] - ms);
-                L += p;
-                y[r] = p * vs[r];
-            }
-            split2(y[0], y[1], hi[2 * u], lo[2 * u]);
-            split2(y[2], y[3], hi[2 * u + 1], lo[2 * u + 1]);
-        }
-        hf8 ph[2] = {join8(hi[0], hi[1], hi[2], hi[3]), join8(hi[4], hi[5], hi[6], hi[7])};
-        hf8 pl[2] = {join8(lo[0], lo[1], lo[2], lo[3]), join8(lo[4], lo[5], lo[6], lo[7])};
+        hf8 ph[2], pl[2];
+        tile_weights<ST>(a, s, sc[w], qsc, j0, pos, tile_edge(a, j0, np + t0, np + t1), M, L, o, ph, pl);
         if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
             if (li >= 8) ph[0] = pl[0], ph[1] = pl[1];
         }
-        // bytes of values not written yet: an e4m3 one may be a NaN, which a weight of 0 does not take out
         if (E4 && j0 + 63 > last) {
-            u32x4 vmask;
+            const u32x4 m = written(j0, last);
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int n = last + 1 - (j0 + 16 * u + 4 * kq);
-                vmask[u] = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-            }
-#pragma unroll
-            for (int d = 0; d < ND; d++) vr[d] &= vmask;
+            for (int d = 0; d < ND; d++) vr[d] &= m;
         }
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -553,6 +582,127 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
     }
 }
 
+// Attention of many rows: a work-group takes 64 query rows, a wavefront 16, and walks the tiles together. A tile's codes
+// become f16 operands in LDS once for all of them (64 KB at D = 256, in operand order: every access is 64 consecutive
+// 16-byte pieces), the next tile's codes are in flight meanwhile. Two work-groups share a CU, so one's softmax
+// runs beside the other's products.
+template <int D, bool E4>
+__global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a, int fold) {
+    constexpr int NS = D / 64, ND = D / 16, NU = D / 64;   // units of keys (and of values) per wavefront: 4 NS / 4 = ND / 4
+    __shared__ __align__(16) uint8_t Ks[64 * D * 2], Vs[64 * D * 2];
+    __shared__ __align__(16) float sc[3][64];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
+    const int G = a.H / a.c.Hkv, rows = a.T * G, N = gridDim.x;
+    // the row blocks with the most tiles first; where two rounds of work-groups cover all, the second in rising order, so that
+    // a CU's two have equal sums
+    const int b = blockIdx.x, srt = fold && b >= N / 2 ? N - 1 - (b - N / 2) : b;
+    const int g = srt % a.c.Hkv, sp = blockIdx.y, r0 = (N / a.c.Hkv - 1 - srt / a.c.Hkv) * 64;
+    const int np = clamp_past(a.npast, a.npast_dev), last = np + a.T - 1;
+    const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + 63, rows - 1) / G, a.window, a.sinks);
+    const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
+    if (i0 >= tl.n) return;
+    const int rw = r0 + 16 * w, row = min(rw + li, rows - 1), t = row / G, h = g * G + row % G, pos = np + t;
+    const int p0 = np + min(rw, rows - 1) / G, p1 = np + min(rw + 15, rows - 1) / G;   // the wavefront's rows
+    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D;
+    const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
+    u32x4 kr[NU], vr[NU];
+    float k1 = 0.f, v1 = 0.f;
+    auto load = [&](int i) {
+        const int kt = i < tl.ns ? i : tl.f + i - tl.ns, j = kt * 64 + l;
+        const uint8_t *kp = kc + (int64_t)kt * 64 * D + w * NU * 1024 + l * 16, *vp = vc + (int64_t)kt * 64 * D + w * NU * 1024 + l * 16;
+#pragma unroll
+        for (int c = 0; c < NU; c++) kr[c] = *(const u32x4 *)(kp + c * 1024);
+#pragma unroll
+        for (int c = 0; c < NU; c++) vr[c] = *(const u32x4 *)(vp + c * 1024);
+        if (w == 0) {
+            const bool in = j <= last;
+            k1 = in ? a.c.ks[s0 + (j >> a.c.lg)] : 0.f;
+            v1 = in ? a.c.vs[s0 + (j >> a.c.lg)] : 0.f;
+        }
+    };
+    load(i0);
+    hf8 qh[2 * NS], ql[2 * NS];
+    const float qsc = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    for (int i = i0; i < i1; i++) {
+        const int j0 = (i < tl.ns ? i : tl.f + i - tl.ns) * 64;
+        lds_barrier();   // the tile before is used
+        if (E4 && j0 + 63 > last) {
+            const u32x4 m = written(j0, last);
+#pragma unroll
+            for (int c = 0; c < NU; c++) vr[c] &= m;
+        }
+#pragma unroll
+        for (int c = 0; c < NU; c++) {
+            hf8 x, y;
+            uint8_t *kd = Ks + (w * NU + c) * 2048 + l * 16, *vd = Vs + (w * NU + c) * 2048 + l * 16;
+            to_half<E4>(kr[c], x, y);
+            *(hf8 *)kd = x;
+            *(hf8 *)(kd + 1024) = y;
+            to_half<E4>(vr[c], x, y);
+            *(hf8 *)vd = x;
+            *(hf8 *)(vd + 1024) = y;
+        }
+        if (w == 0) {
+            sc[0][l] = k1;
+            sc[1][l] = v1 * kP;
+            sc[2][l] = log2f(fmaxf(v1, 0x1p-100f));
+        }
+        lds_barrier();
+        if (i + 1 < i1) load(i + 1);
+        if (j0 > p1 || (a.window && j0 + 63 <= p0 - a.window && j0 >= a.sinks)) continue;   // nothing of it is seen (uniform)
+        f32x4 s[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < 2 * NS; st++) {
+            hf8 ka[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) ka[u] = *(const hf8 *)(Ks + (u * 2 * NS + st) * 1024 + l * 16);
+#pragma unroll
+            for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], ql[st], s[u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], qh[st], s[u]);
+        }
+        hf8 ph[2], pl[2];
+        tile_weights<false>(a, s, sc, qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const hf8 va = *(const hf8 *)(Vs + d * 2048 + l * 16), vb = *(const hf8 *)(Vs + d * 2048 + 1024 + l * 16);
+            o[d] = mfma16(va, pl[0], o[d]);
+            o[d] = mfma16(vb, pl[1], o[d]);
+            o[d] = mfma16(va, ph[0], o[d]);
+            o[d] = mfma16(vb, ph[1], o[d]);
+        }
+    }
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (rw + li >= rows) return;
+    if (a.n_split > 1) {   // register r of o[d]: dim 16 d + 4 kq + r
+        float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
+#pragma unroll
+        for (int d = 0; d < ND; d++) *(f32x4 *)(part + 4 + 16 * d + 4 * kq) = o[d];
+        if (kq == 0) part[0] = M, part[1] = L;
+        return;
+    }
+    const float inv = (1.f / kP) / L;
+    float *op = a.out + t * a.o_tok + (int64_t)h * D + 4 * kq;
+    const float *gp = a.gate + t * a.g_tok + h * a.g_head + 4 * kq;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+        f32x4 v = o[d] * inv;
+        if (a.gate) {
+            const f32x4 x = *(const f32x4_u *)(gp + 16 * d);
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] *= xjd::sigm(x[r]);
+        }
+        *(f32x4_u *)(op + 16 * d) = v;
+    }
+}
+
 // The splits of a row joined in order: the first wavefront forms every split's factor, a thread per dim sums.
 template <int D>
 __global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a, int R) {
@@ -587,8 +737,12 @@ __global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a, int R
     a.out[t * a.o_tok + (int64_t)h * D + d] = y;
 }
 
-// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions).
-static int rows_of(const Kv8AttnArgs &a) { return (int64_t)a.T * (a.H / a.c.Hkv) <= 8 ? 8 : 16; }
+// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions), up to 32
+// take the kernel without LDS tiles.
+static int rows_of(const Kv8AttnArgs &a) {
+    const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
+    return n <= 8 ? 8 : n <= 32 ? 16 : 64;
+}
 // Tiles that R rows see at most.
 static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int all = (a.npast + a.T - 1) / 64 + 1;
@@ -602,7 +756,7 @@ static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
     const int by_tiles = (most_tiles(a, R) + 3) / 4;
-    int64_t n = 512 / wgs;
+    int64_t n = (R == 64 ? 256 : 512) / wgs;
     if (n > by_tiles) n = by_tiles;
     return n < 1 ? 1 : (int)n;
 }
@@ -613,10 +767,10 @@ int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
 
 template <int D, bool E4>
 static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
-    const int rows = a.T * (a.H / a.c.Hkv);
-    const dim3 grid((rows + R - 1) / R, a.c.Hkv, a.n_split);
-    if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
+    const int rows = a.T * (a.H / a.c.Hkv), nb = (rows + R - 1) / R;
+    if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
+    else if (R == 16) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), dim3(nb * a.c.Hkv, a.n_split), dim3(256), 0, st, a, nb * a.c.Hkv <= 512);
     if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a, R);
 }
 
