@@ -416,11 +416,11 @@ __device__ __forceinline__ u32x4 written(int j0, int last) {
 template <int N>
 __device__ __forceinline__ void load_units(const uint8_t *p, uint32_t lane, u32x4 (&r)[N]) {
 #pragma unroll
-    for (int c = 0; c < N; c += 4) {
+    for (int c = 0; c < N; c += 4) {   // (N a power of two)
         auto b = (const __attribute__((address_space(1))) uint8_t *)(p + c * 1024);
         asm("" : "+s"(b));
 #pragma unroll
-        for (int i = 0; i < 4; i++) r[c + i] = *(const __attribute__((address_space(1))) u32x4 *)(b + lane + i * 1024);
+        for (int i = 0; i < (N < 4 ? N : 4); i++) r[c + i] = *(const __attribute__((address_space(1))) u32x4 *)(b + lane + i * 1024);
     }
 }
 
@@ -582,122 +582,163 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
     }
 }
 
-// Attention of many rows: a work-group takes 64 query rows, a wavefront 16, and walks the tiles together. A tile's codes
-// become f16 operands in LDS once for all of them (64 KB at D = 256, in operand order: every access is 64 consecutive
-// 16-byte pieces), the next tile's codes are in flight meanwhile. Two work-groups share a CU, so one's softmax
-// runs beside the other's products.
+// sigmoid by the exponential and reciprocal instructions (1 ulp each).
+__device__ __forceinline__ float sigm_fast(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
+
+// Attention of many rows: a work-group takes 64 query rows of a kv head, its two groups of four wavefronts (16 rows each)
+// every other tile. A tile's codes become f16 operands in LDS once for the four wavefronts (64 KB at D = 256, in operand
+// order: every access is 64 consecutive 16-byte pieces). Per tile a group has a step on the vector units (the softmax of the
+// tile's scores; its values and the next tile's keys turned into operands) and one on the matrix cores (its values'
+// products, then the next tile's scores); the groups take them in turn, one a step behind the other,
+// so that on every SIMD one wavefront keeps the matrix core busy while the other has the vector unit.
 template <int D, bool E4>
-__global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a, int fold) {
+__global__ __launch_bounds__(512, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) {
     constexpr int NS = D / 64, ND = D / 16, NU = D / 64;   // units of keys (and of values) per wavefront: 4 NS / 4 = ND / 4
-    __shared__ __align__(16) uint8_t Ks[64 * D * 2], Vs[64 * D * 2];
-    __shared__ __align__(16) float sc[3][64];
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
-    const int G = a.H / a.c.Hkv, rows = a.T * G, N = gridDim.x;
-    // the row blocks with the most tiles first; where two rounds of work-groups cover all, the second in rising order, so that
-    // a CU's two have equal sums
-    const int b = blockIdx.x, srt = fold && b >= N / 2 ? N - 1 - (b - N / 2) : b;
-    const int g = srt % a.c.Hkv, sp = blockIdx.y, r0 = (N / a.c.Hkv - 1 - srt / a.c.Hkv) * 64;
+    __shared__ __align__(16) uint8_t Ks[2][64 * D * 2], Vs[2][64 * D * 2];
+    __shared__ __align__(16) float sc[2][2][3][64];   // [group][tile parity]
+    __shared__ float ml[2][2][64];
+    const int tid = threadIdx.x, l = tid & 63, li = l & 15, kq = l >> 4;
+    const int grp = __builtin_amdgcn_readfirstlane(tid >> 8), w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+    const int G = a.H / a.c.Hkv, rows = a.T * G, b = blockIdx.x;
+    const int g = b % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - b / a.c.Hkv) * 64;   // the most tiles first
     const int np = clamp_past(a.npast, a.npast_dev), last = np + a.T - 1;
     const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + 63, rows - 1) / G, a.window, a.sinks);
-    const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
-    if (i0 >= tl.n) return;
+    const int i0 = sp * a.per_split, nt = min(a.per_split, tl.n - i0);
+    if (nt <= 0) return;
     const int rw = r0 + 16 * w, row = min(rw + li, rows - 1), t = row / G, h = g * G + row % G, pos = np + t;
     const int p0 = np + min(rw, rows - 1) / G, p1 = np + min(rw + 15, rows - 1) / G;   // the wavefront's rows
     const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D;
     const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
+    const int n = (nt + 1 - grp) / 2;   // the group's tiles
+    auto tile = [&](int j) {
+        const int i = i0 + grp + 2 * j;
+        return i < tl.ns ? i : tl.f + i - tl.ns;
+    };
     u32x4 kr[NU], vr[NU];
     float k1 = 0.f, v1 = 0.f;
-    auto load = [&](int i) {
-        const int kt = i < tl.ns ? i : tl.f + i - tl.ns, j = kt * 64 + l;
-        const uint8_t *kp = kc + (int64_t)kt * 64 * D + w * NU * 1024 + l * 16, *vp = vc + (int64_t)kt * 64 * D + w * NU * 1024 + l * 16;
-#pragma unroll
-        for (int c = 0; c < NU; c++) kr[c] = *(const u32x4 *)(kp + c * 1024);
-#pragma unroll
-        for (int c = 0; c < NU; c++) vr[c] = *(const u32x4 *)(vp + c * 1024);
+    auto load_k = [&](int j) {
+        const int kt = tile(j), p = kt * 64 + l;
+        load_units<NU>(kc + (int64_t)kt * 64 * D + w * NU * 1024, l * 16, kr);
         if (w == 0) {
-            const bool in = j <= last;
-            k1 = in ? a.c.ks[s0 + (j >> a.c.lg)] : 0.f;
-            v1 = in ? a.c.vs[s0 + (j >> a.c.lg)] : 0.f;
+            const bool in = p <= last;
+            k1 = in ? a.c.ks[s0 + (p >> a.c.lg)] : 0.f;
+            v1 = in ? a.c.vs[s0 + (p >> a.c.lg)] : 0.f;
         }
     };
-    load(i0);
+    if (n > 0) load_k(0);
     hf8 qh[2 * NS], ql[2 * NS];
     const float qsc = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
-    f32x4 o[ND];
+    f32x4 o[ND], s[4];
+    hf8 ph[2], pl[2];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
-    for (int i = i0; i < i1; i++) {
-        const int j0 = (i < tl.ns ? i : tl.f + i - tl.ns) * 64;
-        lds_barrier();   // the tile before is used
-        if (E4 && j0 + 63 > last) {
-            const u32x4 m = written(j0, last);
+    for (int x = 0; x < nt + 3; x++) {   // 2 n + 2 steps of either group, the second's one later
+        const int step = x - grp, j = step >> 1;
+        if (step >= 0 && !(step & 1) && j <= n) {
+            if (j > 0) {   // tile j - 1: softmax, values
+                const int j0 = tile(j - 1) * 64;
+                tile_weights<false>(a, s, sc[grp][(j - 1) & 1], qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
+                if (E4 && j0 + 63 > last) {
+                    const u32x4 m = written(j0, last);
 #pragma unroll
-            for (int c = 0; c < NU; c++) vr[c] &= m;
-        }
+                    for (int c = 0; c < NU; c++) vr[c] &= m;
+                }
 #pragma unroll
-        for (int c = 0; c < NU; c++) {
-            hf8 x, y;
-            uint8_t *kd = Ks + (w * NU + c) * 2048 + l * 16, *vd = Vs + (w * NU + c) * 2048 + l * 16;
-            to_half<E4>(kr[c], x, y);
-            *(hf8 *)kd = x;
-            *(hf8 *)(kd + 1024) = y;
-            to_half<E4>(vr[c], x, y);
-            *(hf8 *)vd = x;
-            *(hf8 *)(vd + 1024) = y;
+                for (int c = 0; c < NU; c++) {
+                    hf8 x, y;
+                    to_half<E4>(vr[c], x, y);
+                    *(hf8 *)(Vs[grp] + (w * NU + c) * 2048 + l * 16) = x;
+                    *(hf8 *)(Vs[grp] + (w * NU + c) * 2048 + 1024 + l * 16) = y;
+                }
+            }
+            if (j < n) {   // the keys of tile j
+#pragma unroll
+                for (int c = 0; c < NU; c++) {
+                    hf8 x, y;
+                    to_half<E4>(kr[c], x, y);
+                    *(hf8 *)(Ks[grp] + (w * NU + c) * 2048 + l * 16) = x;
+                    *(hf8 *)(Ks[grp] + (w * NU + c) * 2048 + 1024 + l * 16) = y;
+                }
+                if (w == 0) {
+                    sc[grp][j & 1][0][l] = k1;
+                    sc[grp][j & 1][1][l] = v1 * kP;
+                    sc[grp][j & 1][2][l] = log2f(fmaxf(v1, 0x1p-100f));
+                }
+            }
         }
-        if (w == 0) {
-            sc[0][l] = k1;
-            sc[1][l] = v1 * kP;
-            sc[2][l] = log2f(fmaxf(v1, 0x1p-100f));
+        if (step >= 0 && (step & 1) && j <= n) {
+            if (j < n) load_units<NU>(vc + (int64_t)tile(j) * 64 * D + w * NU * 1024, l * 16, vr);
+            if (j + 1 < n) load_k(j + 1);
+            if (j > 0)
+#pragma unroll
+                for (int d = 0; d < ND; d += 2) {
+                    hf8 v[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[c] = *(const hf8 *)(Vs[grp] + d * 2048 + c * 1024 + l * 16);
+                    o[d] = mfma16(v[0], pl[0], o[d]);
+                    o[d + 1] = mfma16(v[2], pl[0], o[d + 1]);
+                    o[d] = mfma16(v[1], pl[1], o[d]);
+                    o[d + 1] = mfma16(v[3], pl[1], o[d + 1]);
+                    o[d] = mfma16(v[0], ph[0], o[d]);
+                    o[d + 1] = mfma16(v[2], ph[0], o[d + 1]);
+                    o[d] = mfma16(v[1], ph[1], o[d]);
+                    o[d + 1] = mfma16(v[3], ph[1], o[d + 1]);
+                }
+            if (j < n) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < 2 * NS; st++) {
+                    hf8 ka[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) ka[u] = *(const hf8 *)(Ks[grp] + (u * 2 * NS + st) * 1024 + l * 16);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], ql[st], s[u]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], qh[st], s[u]);
+                }
+            }
         }
         lds_barrier();
-        if (i + 1 < i1) load(i + 1);
-        if (j0 > p1 || (a.window && j0 + 63 <= p0 - a.window && j0 >= a.sinks)) continue;   // nothing of it is seen (uniform)
-        f32x4 s[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < 2 * NS; st++) {
-            hf8 ka[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) ka[u] = *(const hf8 *)(Ks + (u * 2 * NS + st) * 1024 + l * 16);
-#pragma unroll
-            for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], ql[st], s[u]);
-#pragma unroll
-            for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], qh[st], s[u]);
-        }
-        hf8 ph[2], pl[2];
-        tile_weights<false>(a, s, sc, qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const hf8 va = *(const hf8 *)(Vs + d * 2048 + l * 16), vb = *(const hf8 *)(Vs + d * 2048 + 1024 + l * 16);
-            o[d] = mfma16(va, pl[0], o[d]);
-            o[d] = mfma16(vb, pl[1], o[d]);
-            o[d] = mfma16(va, ph[0], o[d]);
-            o[d] = mfma16(vb, ph[1], o[d]);
-        }
     }
+    // the groups' sums joined: each hands the other half of its dims over and finishes the rest
     L += __shfl_xor(L, 16, 64);
     L += __shfl_xor(L, 32, 64);
-    if (rw + li >= rows) return;
-    if (a.n_split > 1) {   // register r of o[d]: dim 16 d + 4 kq + r
-        float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
-#pragma unroll
-        for (int d = 0; d < ND; d++) *(f32x4 *)(part + 4 + 16 * d + 4 * kq) = o[d];
-        if (kq == 0) part[0] = M, part[1] = L;
-        return;
+    if (kq == 0) {
+        ml[grp][0][16 * w + li] = M;
+        ml[grp][1][16 * w + li] = L;
     }
-    const float inv = (1.f / kP) / L;
-    float *op = a.out + t * a.o_tok + (int64_t)h * D + 4 * kq;
-    const float *gp = a.gate + t * a.g_tok + h * a.g_head + 4 * kq;
+    lds_barrier();
+    const float m2 = ml[grp ^ 1][0][16 * w + li], l2 = ml[grp ^ 1][1][16 * w + li], mm = fmaxf(M, m2);
+    const float f1 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mm), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mm);
+    const float ll = grp ? l2 * f2 + L * f1 : L * f1 + l2 * f2;   // (the same sum in both)
+    f32x4 *xo = (f32x4 *)Ks;   // [receiving group][wavefront][ND / 2][64]
 #pragma unroll
     for (int d = 0; d < ND; d++) {
-        f32x4 v = o[d] * inv;
-        if (a.gate) {
+        o[d] *= f1;
+        if ((d >= ND / 2) != grp) xo[(((grp ^ 1) * 4 + w) * (ND / 2) + d % (ND / 2)) * 64 + l] = o[d];
+    }
+    lds_barrier();
+    if (rw + li >= rows) return;
+    float *op = a.out + t * a.o_tok + (int64_t)h * D + 4 * kq;
+    const float *gp = a.gate ? a.gate + t * a.g_tok + h * a.g_head + 4 * kq : nullptr;
+    float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
+    const float inv = __builtin_amdgcn_rcpf(ll) * (1.f / kP);
+    if (a.n_split > 1 && kq == 0 && grp == 0) part[0] = mm, part[1] = ll;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {   // register r of o[d]: dim 16 d + 4 kq + r
+        if ((d >= ND / 2) != grp) continue;
+        f32x4 v = o[d] + xo[((grp * 4 + w) * (ND / 2) + d % (ND / 2)) * 64 + l];
+        if (a.n_split > 1) {
+            *(f32x4 *)(part + 4 + 16 * d + 4 * kq) = v;
+            continue;
+        }
+        v *= inv;
+        if (gp) {
             const f32x4 x = *(const f32x4_u *)(gp + 16 * d);
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[r] *= xjd::sigm(x[r]);
+            for (int r = 0; r < 4; r++) v[r] *= sigm_fast(x[r]);
         }
         *(f32x4_u *)(op + 16 * d) = v;
     }
@@ -770,7 +811,7 @@ static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     const int rows = a.T * (a.H / a.c.Hkv), nb = (rows + R - 1) / R;
     if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
     else if (R == 16) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), dim3(nb * a.c.Hkv, a.n_split), dim3(256), 0, st, a, nb * a.c.Hkv <= 512);
+    else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), dim3(nb * a.c.Hkv, a.n_split), dim3(512), 0, st, a);
     if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a, R);
 }
 
