@@ -296,8 +296,6 @@ __host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, i
 // 2^(score - M). The sums are rescaled only when max t passes M by more than kGrow.
 constexpr float kGrow = 8.f, kP = 128.f;
 
-constexpr int kMaxSplit = 512;
-
 // Work-group barrier ordering LDS accesses only (global loads in flight stay in flight).
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -340,7 +338,7 @@ __device__ __forceinline__ float split_query(const float *q, float scale, hf8 (&
 
 // The softmax of a tile's scores: s (products so far) becomes the weights' planes. sc: the tile's scales (keys, values times
 // kP, log2 of the values'); edge: some row does not see the whole tile.
-template <bool ST, int ND>
+template <int ND>
 __device__ __forceinline__ void tile_weights(const Kv8AttnArgs &a, f32x4 (&s)[4], const float (*sc)[64], float qsc, int j0, int pos, bool edge,
                                              float &M, float &L, f32x4 (&o)[ND], hf8 (&ph)[2], hf8 (&pl)[2]) {
     const int kq = (threadIdx.x & 63) >> 4;
@@ -349,7 +347,7 @@ __device__ __forceinline__ void tile_weights(const Kv8AttnArgs &a, f32x4 (&s)[4]
     for (int u = 0; u < 4; u++) {
         const f32x4 ks = *(const f32x4 *)&sc[0][16 * u + 4 * kq];
 #pragma unroll
-        for (int r = 0; r < 4; r++) s[u][r] = (ST ? add_ror8(s[u][r]) : s[u][r]) * (qsc * ks[r]);
+        for (int r = 0; r < 4; r++) s[u][r] *= qsc * ks[r];
     }
     if (edge)
 #pragma unroll
@@ -424,20 +422,41 @@ __device__ __forceinline__ void load_units(const uint8_t *p, uint32_t lane, u32x
     }
 }
 
-// Attention of few rows (row = token * G + head of the kv head): a work-group takes R of them and a split of
-// the tiles, a wavefront every fourth tile of it, straight from the cache into registers. With R = 8 an
-// operand's 16 columns are both planes of the 8 rows, so a product costs one instruction; with R = 16 the planes
-// follow one another. The queries lie in LDS as operands (8 reads of 16 bytes per tile and lane; in
-// registers they would leave no room for the tiles in flight). A tile's values are requested before its scores are
-// formed and the next tile's keys right after, so 16 KB per wavefront are always in flight.
+// sigmoid by the exponential and reciprocal instructions (1 ulp each).
+__device__ __forceinline__ float sigm_fast(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
+
+// N groups of 4 sums, 16 dims apart from dim d0 of the token's head: over the total, gated, into the output row at hd.
+template <int N>
+__device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int t, int h, int64_t hd, int d0, float total, const f32x4 *o) {
+    const float inv = (1.f / kP) / total;
+    float *op = a.out + t * a.o_tok + hd + d0;
+    f32x4 x[N];
+    if (a.gate)
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = *(const f32x4_u *)(a.gate + t * a.g_tok + h * a.g_head + d0 + 16 * i);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        f32x4 v = o[i] * inv;
+        if (a.gate)
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] *= sigm_fast(x[i][r]);
+        *(f32x4_u *)(op + 16 * i) = v;
+    }
+}
+
+// Attention of few rows (row = token * G + head of the kv head): a work-group takes R of them and a split of the tiles. Its
+// four wavefronts share every tile: each forms the scores of 16 keys, all of them (through LDS) the weights of
+// all 64, each the sums of a quarter of the dims, so that a short context's one tile takes a quarter of the time and a wavefront
+// needs few registers (four on a SIMD hide the loads). Every wavefront always has its part of the next
+// tile in flight, 8 KB at D = 256. With R = 8 an operand's 16 columns are both planes of the 8 rows, so a product costs
+// one instruction; with R = 16 the planes follow one another, with R = 32 there are two sets of columns.
 template <int D, bool E4, int R>
-__global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
-    constexpr int NS = D / 64, ND = D / 16, NW = 4;
+__global__ __launch_bounds__(256, R == 32 ? 2 : 3) void kv8_rows_kernel(const Kv8AttnArgs a) {
+    constexpr int NS = D / 64, NV = D / 64, CT = R == 32 ? 2 : 1;   // a wavefront's units of keys and of values; column sets
     constexpr bool ST = R == 8;
-    __shared__ __align__(16) float sc[NW][3][64];
-    __shared__ float ml[NW][2][R];
-    constexpr int kQ = (ST ? 1 : 2) * 2 * NS * 1024, kO = NW * R * (D + 4) * 4;
-    __shared__ __align__(16) uint8_t mem[kQ > kO ? kQ : kO];   // the queries, then the wavefronts' sums
+    __shared__ __align__(16) float sc[2][3][64];
+    __shared__ __align__(16) f32x4 sb[2][CT][4][64];   // [tile parity][columns][16 keys][lane]
+    __shared__ __align__(16) hf8 qs[ST ? 1 : CT][ST ? 1 : 2 * NS][2][64];   // the queries' planes, if not in registers
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int g = blockIdx.y, sp = blockIdx.z, G = a.H / a.c.Hkv, rows = a.T * G;
     const int np = clamp_past(a.npast, a.npast_dev);
@@ -445,145 +464,134 @@ __global__ __launch_bounds__(256, 2) void kv8_rows_kernel(const Kv8AttnArgs a) {
     const Tiles tl = tiles_of(np + t0, np + t1, a.window, a.sinks);
     const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
     if (i0 >= tl.n) return;
-    const int row = min(r0 + (li & (R - 1)), rows - 1), t = row / G, h = g * G + row % G, pos = np + t, last = np + a.T - 1;
-    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D;
+    const int last = np + a.T - 1;
+    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + w * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
     const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
-    u32x4 kr[4 * NS], vr[ND];
-    float k1 = 0.f, v1 = 0.f;
+    u32x4 kr[NS], vr[NV];
+    float s1 = 0.f;   // wavefront 0: the keys' scale of position l; 1: the values'
     auto tile = [&](int i) { return i < tl.ns ? i : tl.f + i - tl.ns; };
-    auto load_k = [&](int kt) {   // and the tile's scales, one position per lane; positions not written yet have none
-        load_units<4 * NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
+    auto load_k = [&](int kt) {   // positions not written yet have no scale
+        load_units<NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
         const int j = kt * 64 + l;
-        const bool in = j <= last;
-        k1 = in ? a.c.ks[s0 + (j >> a.c.lg)] : 0.f;
-        v1 = in ? a.c.vs[s0 + (j >> a.c.lg)] : 0.f;
-        __builtin_amdgcn_sched_barrier(0);
+        if (w < 2) s1 = j <= last ? (w ? a.c.vs : a.c.ks)[s0 + (j >> a.c.lg)] : 0.f;
     };
-    auto load_v = [&](int kt) {
-        load_units<ND>(vc + (int64_t)kt * 64 * D, l * 16, vr);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    int i = i0 + w;
-    if (i < i1) load_k(tile(i));
-    hf8 qh[2 * NS], ql[2 * NS];
-    const float qsc = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
+    auto load_v = [&](int kt) { load_units<NV>(vc + (int64_t)kt * 64 * D, l * 16, vr); };
+    load_k(tile(i0));
+    load_v(tile(i0));
+    __builtin_amdgcn_sched_barrier(0);
+    hf8 q8[2 * NS];   // R = 8: the lane's plane
+    float qsc[CT], M[CT], L[CT];
+    int row[CT], pos[CT];
+    f32x4 o[CT][NV];
 #pragma unroll
-    for (int i = 0; i < 2 * NS; i++) {
-        if (i % NW != w) continue;
-        if constexpr (ST) {
-            *(hf8 *)(mem + i * 1024 + l * 16) = li < 8 ? qh[i] : ql[i];
-        } else {
-            *(hf8 *)(mem + 2 * i * 1024 + l * 16) = qh[i];
-            *(hf8 *)(mem + (2 * i + 1) * 1024 + l * 16) = ql[i];
+    for (int c = 0; c < CT; c++) {
+        row[c] = r0 + 16 * c + (li & (R - 1));
+        const int rr = min(row[c], rows - 1), t = rr / G, h = g * G + rr % G;
+        pos[c] = np + t;
+        hf8 qh[2 * NS], ql[2 * NS];
+        qsc[c] = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++) {
+            if constexpr (ST) q8[i] = li < 8 ? qh[i] : ql[i];
+            else if (i % 4 == w) qs[c][i][0][l] = qh[i], qs[c][i][1][l] = ql[i];
         }
+        M[c] = -INFINITY;
+        L[c] = 0.f;
+#pragma unroll
+        for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    f32x4 o[ND];
+    if (!ST) lds_barrier();
+    for (int i = i0; i < i1; i++) {
+        const int kt = tile(i), j0 = kt * 64, par = i & 1;
+        const bool more = i + 1 < i1;
+        f32x4 x[CT];
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, L = 0.f;
-    lds_barrier();
-    for (; i < i1; i += NW) {
-        const int kt = tile(i), j0 = kt * 64;
-        load_v(kt);
-        __builtin_amdgcn_wave_barrier();
-        sc[w][0][l] = k1;
-        sc[w][1][l] = v1 * kP;
-        sc[w][2][l] = log2f(fmaxf(v1, 0x1p-100f));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        f32x4 s[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < CT; c++) x[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < NS; st++) {
-            hf8 qa[ST ? 2 : 4];   // step 2 st and 2 st + 1 (R = 16: both planes of each)
+            hf8 ka, kb;
+            to_half<E4>(kr[st], ka, kb);
 #pragma unroll
-            for (int c = 0; c < (ST ? 2 : 4); c++) qa[c] = *(const hf8 *)(mem + (st * (ST ? 2 : 4) + c) * 1024 + l * 16);
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                hf8 ka, kb;
-                to_half<E4>(kr[u * NS + st], ka, kb);
+            for (int c = 0; c < CT; c++) {
                 if constexpr (ST) {
-                    s[u] = mfma16(ka, qa[0], s[u]);
-                    s[u] = mfma16(kb, qa[1], s[u]);
+                    x[c] = mfma16(ka, q8[2 * st], x[c]);
+                    x[c] = mfma16(kb, q8[2 * st + 1], x[c]);
                 } else {
-                    s[u] = mfma16(ka, qa[1], s[u]);
-                    s[u] = mfma16(kb, qa[3], s[u]);
-                    s[u] = mfma16(ka, qa[0], s[u]);
-                    s[u] = mfma16(kb, qa[2], s[u]);
+                    x[c] = mfma16(ka, qs[c][2 * st][1][l], x[c]);
+                    x[c] = mfma16(kb, qs[c][2 * st + 1][1][l], x[c]);
+                    x[c] = mfma16(ka, qs[c][2 * st][0][l], x[c]);
+                    x[c] = mfma16(kb, qs[c][2 * st + 1][0][l], x[c]);
                 }
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (i + NW < i1) load_k(tile(i + NW));
-        hf8 ph[2], pl[2];
-        tile_weights<ST>(a, s, sc[w], qsc, j0, pos, tile_edge(a, j0, np + t0, np + t1), M, L, o, ph, pl);
-        if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
-            if (li >= 8) ph[0] = pl[0], ph[1] = pl[1];
+        if (w < 2) {
+            sc[par][w][l] = w ? s1 * kP : s1;
+            if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-100f));
+        }
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            if constexpr (ST)
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[c][r] = add_ror8(x[c][r]);
+            sb[par][c][w][l] = x[c];
+        }
+        if (more) load_k(tile(i + 1));
+        lds_barrier();   // (the other parity: one barrier a tile)
+        hf8 ph[CT][2], pl[CT][2];
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            f32x4 s[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) s[u] = sb[par][c][u][l];
+            tile_weights(a, s, sc[par], qsc[c], j0, pos[c], tile_edge(a, j0, np + t0, np + t1), M[c], L[c], o[c], ph[c], pl[c]);
+            if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
+                if (li >= 8) ph[c][0] = pl[c][0], ph[c][1] = pl[c][1];
+            }
         }
         if (E4 && j0 + 63 > last) {
             const u32x4 m = written(j0, last);
 #pragma unroll
-            for (int d = 0; d < ND; d++) vr[d] &= m;
+            for (int d = 0; d < NV; d++) vr[d] &= m;
         }
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
+        for (int d = 0; d < NV; d++) {
             hf8 va, vb;
             to_half<E4>(vr[d], va, vb);
-            if constexpr (!ST) {
-                o[d] = mfma16(va, pl[0], o[d]);
-                o[d] = mfma16(vb, pl[1], o[d]);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                if constexpr (!ST) {
+                    o[c][d] = mfma16(va, pl[c][0], o[c][d]);
+                    o[c][d] = mfma16(vb, pl[c][1], o[c][d]);
+                }
+                o[c][d] = mfma16(va, ph[c][0], o[c][d]);
+                o[c][d] = mfma16(vb, ph[c][1], o[c][d]);
             }
-            o[d] = mfma16(va, ph[0], o[d]);
-            o[d] = mfma16(vb, ph[1], o[d]);
         }
+        if (more) load_v(tile(i + 1));
     }
-    // the wavefronts' sums joined
-    L += __shfl_xor(L, 16, 64);
-    L += __shfl_xor(L, 32, 64);
-    if (l < R) {
-        ml[w][0][l] = M;
-        ml[w][1][l] = L;
-    }
-    lds_barrier();   // every wavefront is done with the queries, too
-    float m0 = ml[0][0][li & (R - 1)];
 #pragma unroll
-    for (int x = 1; x < NW; x++) m0 = fmaxf(m0, ml[x][0][li & (R - 1)]);
-    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m0);
-    float(*ob)[R][D + 4] = (float(*)[R][D + 4])mem;
+    for (int c = 0; c < CT; c++) {
+        L[c] += __shfl_xor(L[c], 16, 64);
+        L[c] += __shfl_xor(L[c], 32, 64);
+        if constexpr (ST)
 #pragma unroll
-    for (int d = 0; d < ND; d++) {
-        f32x4 v = o[d] * f;
-        if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
-        if (li < R) *(f32x4 *)&ob[w][li][16 * d + 4 * kq] = v;
-    }
-    lds_barrier();
-    for (int idx = tid; idx < R * D; idx += 256) {
-        const int r = idx / D, d = idx % D, rr = r0 + r;
-        if (rr >= rows) break;
-        float mm = ml[0][0][r], ll = 0.f, v = 0.f;
+            for (int d = 0; d < NV; d++)
 #pragma unroll
-        for (int x = 1; x < NW; x++) mm = fmaxf(mm, ml[x][0][r]);
-#pragma unroll
-        for (int x = 0; x < NW; x++) {
-            ll += ml[x][0][r] == -INFINITY ? 0.f : ml[x][1][r] * __builtin_amdgcn_exp2f(ml[x][0][r] - mm);
-            v += ob[x][r][d];
-        }
+                for (int r = 0; r < 4; r++) o[c][d][r] = add_ror8(o[c][d][r]);
+        if (row[c] >= rows || li >= R) continue;
+        // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
+        const int d0 = 16 * w * NV + 4 * kq;
         if (a.n_split > 1) {
-            float *part = a.part + (((int64_t)g * rows + rr) * a.n_split + sp) * (D + 4);
-            part[4 + d] = v;
-            if (d == 0) part[0] = mm, part[1] = ll;
+            float *part = a.part + (((int64_t)g * rows + row[c]) * a.n_split + sp) * (D + 4);
+            if (w == 0 && kq == 0) part[0] = M[c], part[1] = L[c];
+#pragma unroll
+            for (int d = 0; d < NV; d++) *(f32x4 *)(part + 4 + d0 + 16 * d) = o[c][d];
         } else {
-            const int tt = rr / G, hh = g * G + rr % G;
-            float y = v * (1.f / kP) / ll;
-            if (a.gate) y *= xjd::sigm(a.gate[tt * a.g_tok + hh * a.g_head + d]);
-            a.out[tt * a.o_tok + (int64_t)hh * D + d] = y;
+            const int t = row[c] / G, h = g * G + row[c] % G;
+            finish_row<NV>(a, t, h, h * D, d0, L[c], o[c]);
         }
     }
 }
-
-// sigmoid by the exponential and reciprocal instructions (1 ulp each).
-__device__ __forceinline__ float sigm_fast(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
 
 // Attention of many rows: a work-group takes 64 query rows of a kv head, its two groups of four wavefronts (16 rows each)
 // every other tile. A tile's codes become f16 operands in LDS once for the four wavefronts (64 KB at D = 256, in operand
@@ -638,7 +646,7 @@ __global__ __launch_bounds__(512, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
         if (step >= 0 && !(step & 1) && j <= n) {
             if (j > 0) {   // tile j - 1: softmax, values
                 const int j0 = tile(j - 1) * 64;
-                tile_weights<false>(a, s, sc[grp][(j - 1) & 1], qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
+                tile_weights(a, s, sc[grp][(j - 1) & 1], qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
                 if (E4 && j0 + 63 > last) {
                     const u32x4 m = written(j0, last);
 #pragma unroll
@@ -721,68 +729,90 @@ __global__ __launch_bounds__(512, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     }
     lds_barrier();
     if (rw + li >= rows) return;
-    float *op = a.out + t * a.o_tok + (int64_t)h * D + 4 * kq;
-    const float *gp = a.gate ? a.gate + t * a.g_tok + h * a.g_head + 4 * kq : nullptr;
     float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
-    const float inv = __builtin_amdgcn_rcpf(ll) * (1.f / kP);
     if (a.n_split > 1 && kq == 0 && grp == 0) part[0] = mm, part[1] = ll;
+    auto give = [&](int d1, const f32x4 *half) {   // register r of o[d]: dim 16 d + 4 kq + r
+        f32x4 v[ND / 2];
 #pragma unroll
-    for (int d = 0; d < ND; d++) {   // register r of o[d]: dim 16 d + 4 kq + r
-        if ((d >= ND / 2) != grp) continue;
-        f32x4 v = o[d] + xo[((grp * 4 + w) * (ND / 2) + d % (ND / 2)) * 64 + l];
-        if (a.n_split > 1) {
-            *(f32x4 *)(part + 4 + 16 * d + 4 * kq) = v;
-            continue;
+        for (int d = 0; d < ND / 2; d++) {
+            v[d] = half[d] + xo[((grp * 4 + w) * (ND / 2) + d) * 64 + l];
+            if (a.n_split > 1) *(f32x4 *)(part + 4 + 16 * (d1 + d) + 4 * kq) = v[d];
         }
-        v *= inv;
-        if (gp) {
-            const f32x4 x = *(const f32x4_u *)(gp + 16 * d);
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] *= sigm_fast(x[r]);
-        }
-        *(f32x4_u *)(op + 16 * d) = v;
-    }
+        if (a.n_split == 1) finish_row<ND / 2>(a, t, h, (int64_t)h * D, 16 * d1 + 4 * kq, ll, v);
+    };
+    if (grp == 0) give(0, o);
+    else give(ND / 2, o + ND / 2);
 }
 
-// The splits of a row joined in order: the first wavefront forms every split's factor, a thread per dim sums.
-template <int D>
-__global__ __launch_bounds__(D) void kv8_merge_kernel(const Kv8AttnArgs a, int R) {
-    __shared__ float fac[kMaxSplit];
-    __shared__ float total;
-    const int G = a.H / a.c.Hkv, rows = a.T * G, rr = blockIdx.x, g = blockIdx.y, d = threadIdx.x;
+// The splits of a row joined in order: W wavefronts take every W-th split each (a lane D / 64 dims), their sums are added in
+// order. W = 1: four rows per work-group.
+template <int D, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const Kv8AttnArgs a, int R) {
+    constexpr int V = D / 64;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    __shared__ float red[W][V][64], rl[W];
+    const int tid = threadIdx.x, l = tid & 63, w = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int G = a.H / a.c.Hkv, rows = a.T * G, rr = W == 1 ? (int)blockIdx.x * 4 + (tid >> 6) : (int)blockIdx.x, g = blockIdx.y;
+    if (rr >= rows) return;
     const int np = clamp_past(a.npast, a.npast_dev), r0 = rr / R * R;
     const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + R - 1, rows - 1) / G, a.window, a.sinks);
     const int ns = (tl.n + a.per_split - 1) / a.per_split;
     const float *part = a.part + ((int64_t)g * rows + rr) * a.n_split * (D + 4);
-    if (d < 64) {
-        float M = -INFINITY, L = 0.f;
-        for (int s = d; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
-        M = xjd::wave_max(M);
-        for (int s = d; s < ns; s += 64) {
-            const float m = part[(int64_t)s * (D + 4)], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            fac[s] = f;
-            L = fmaf(f, part[(int64_t)s * (D + 4) + 1], L);
-        }
-        L = xjd::row16_sum(L);
-        L += __shfl_xor(L, 16, 64);
-        L += __shfl_xor(L, 32, 64);
-        if (d == 0) total = L;
-    }
-    __syncthreads();
-    float y = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < ns; s++) y = fmaf(fac[s], part[(int64_t)s * (D + 4) + 4 + d], y);
-    y = y * (1.f / kP) / total;
     const int t = rr / G, h = g * G + rr % G;
-    if (a.gate) y *= xjd::sigm(a.gate[t * a.g_tok + h * a.g_head + d]);
-    a.out[t * a.o_tok + (int64_t)h * D + d] = y;
+    float M = -INFINITY;
+    for (int s = l; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
+    M = xjd::wave_max(M);
+    vec y = 0.f;
+    float L = 0.f;
+    constexpr int U = 8;
+    for (int s = w; s < ns; s += U * W) {
+        vec v[U];
+        float m[U], c[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {   // (past the end: the last one again, with weight 0)
+            const float *p = part + (int64_t)min(s + i * W, ns - 1) * (D + 4);
+            m[i] = p[0];
+            c[i] = p[1];
+            __builtin_memcpy(&v[i], p + 4 + V * l, sizeof(vec));
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const float f = s + i * W >= ns || m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
+            L = fmaf(f, c[i], L);
+            if (f > 0.f) y += v[i] * f;
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int i = 0; i < V; i++) red[w][i][l] = V == 1 ? ((float *)&y)[0] : ((float *)&y)[i];
+        if (l == 0) rl[w] = L;
+        __syncthreads();
+        if (w) return;
+        L = 0.f;
+        y = 0.f;
+#pragma unroll
+        for (int x = 0; x < W; x++) {
+            L += rl[x];
+#pragma unroll
+            for (int i = 0; i < V; i++) ((float *)&y)[i] += red[x][i][l];
+        }
+    }
+    y *= (1.f / kP) / L;
+    float *op = a.out + t * a.o_tok + (int64_t)h * D + V * l;
+    if (a.gate) {
+        const float *gp = a.gate + t * a.g_tok + h * a.g_head + V * l;
+#pragma unroll
+        for (int i = 0; i < V; i++) ((float *)&y)[i] *= sigm_fast(gp[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
 
 // Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions), up to 32
-// take the kernel without LDS tiles.
+// take the kernel without operand tiles in LDS.
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
-    return n <= 8 ? 8 : n <= 32 ? 16 : 64;
+    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64;
 }
 // Tiles that R rows see at most.
 static int most_tiles(const Kv8AttnArgs &a, int R) {
@@ -792,12 +822,13 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
-// Splits while the work-groups do not exceed two per CU, at least a tile per wavefront.
+// Splits of the tiles: work-groups for every CU to hold (64 rows: one, of up to 8 wavefronts; fewer: three or four), and four
+// tiles for each of 64 rows, whose partial sums cost as much as a tile.
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
-    const int by_tiles = (most_tiles(a, R) + 3) / 4;
-    int64_t n = (R == 64 ? 256 : 512) / wgs;
+    const int by_tiles = R == 64 ? (most_tiles(a, R) + 3) / 4 : most_tiles(a, R);
+    int64_t n = (R == 64 ? 256 : R == 32 ? 512 : 768) / wgs;
     if (n > by_tiles) n = by_tiles;
     return n < 1 ? 1 : (int)n;
 }
@@ -811,8 +842,11 @@ static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     const int rows = a.T * (a.H / a.c.Hkv), nb = (rows + R - 1) / R;
     if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
     else if (R == 16) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
+    else if (R == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 32>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), dim3(nb * a.c.Hkv, a.n_split), dim3(512), 0, st, a);
-    if (a.n_split > 1) hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3(rows, a.c.Hkv), dim3(D), 0, st, a, R);
+    if (a.n_split == 1) return;
+    if (a.n_split <= 16 || rows * a.c.Hkv > 1024) hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((rows + 3) / 4, a.c.Hkv), dim3(256), 0, st, a, R);
+    else hipLaunchKernelGGL((kv8_merge_kernel<D, 8>), dim3(rows, a.c.Hkv), dim3(512), 0, st, a, R);
 }
 
 int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) {
