@@ -255,14 +255,13 @@ __device__ __forceinline__ void to_half4(uint32_t w, hf2 &x, hf2 &y) {
     }
 }
 __device__ __forceinline__ hf8 join8(hf2 a, hf2 b, hf2 c, hf2 d) { return hf8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
-// 16 codes as two operands of 8.
+// 8 codes as an operand.
 template <bool E4>
-__device__ __forceinline__ void to_half(u32x4 w, hf8 &a, hf8 &b) {
-    hf2 h[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) to_half4<E4>(w[i], h[2 * i], h[2 * i + 1]);
-    a = join8(h[0], h[1], h[2], h[3]);
-    b = join8(h[4], h[5], h[6], h[7]);
+__device__ __forceinline__ hf8 to_half(uint32_t w0, uint32_t w1) {
+    hf2 h[4];
+    to_half4<E4>(w0, h[0], h[1]);
+    to_half4<E4>(w1, h[2], h[3]);
+    return join8(h[0], h[1], h[2], h[3]);
 }
 
 // Two values as f16 planes, y = hi + lo to 22 bits. y is opaque to the compiler: as the product that it
@@ -307,92 +306,6 @@ __device__ __forceinline__ float add_ror8(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
 }
 
-// A lane's part of its query row as operands, step (s, e) the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo. Returns what
-// a product of them is multiplied with: the row's 2^e, the scale and log2 e.
-template <int D>
-__device__ __forceinline__ float split_query(const float *q, float scale, hf8 (&qh)[D / 32], hf8 (&ql)[D / 32]) {
-    f32x4 x[D / 16];
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 16; i++) x[i] = *(const f32x4_u *)(q + 64 * (i >> 2) + 4 * (i & 3));
-#pragma unroll
-    for (int i = 0; i < D / 16; i++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) m = fmaxf(m, fabsf(x[i][c]));
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    int e = 0;
-    if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-    e = max(e, -100) - 14;
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-        hf2 hi[4], lo[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-            split2(ldexpf(x[2 * i + (c >> 1)][2 * (c & 1)], -e), ldexpf(x[2 * i + (c >> 1)][2 * (c & 1) + 1], -e), hi[c], lo[c]);
-        qh[i] = join8(hi[0], hi[1], hi[2], hi[3]);
-        ql[i] = join8(lo[0], lo[1], lo[2], lo[3]);
-    }
-    return ldexpf(scale * 1.44269504088896341f, e);
-}
-
-// The softmax of a tile's scores: s (products so far) becomes the weights' planes. sc: the tile's scales (keys, values times
-// kP, log2 of the values'); edge: some row does not see the whole tile.
-template <int ND>
-__device__ __forceinline__ void tile_weights(const Kv8AttnArgs &a, f32x4 (&s)[4], const float (*sc)[64], float qsc, int j0, int pos, bool edge,
-                                             float &M, float &L, f32x4 (&o)[ND], hf8 (&ph)[2], hf8 (&pl)[2]) {
-    const int kq = (threadIdx.x & 63) >> 4;
-    float mt = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const f32x4 ks = *(const f32x4 *)&sc[0][16 * u + 4 * kq];
-#pragma unroll
-        for (int r = 0; r < 4; r++) s[u][r] *= qsc * ks[r];
-    }
-    if (edge)
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int j = j0 + 16 * u + 4 * kq + r;
-                if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
-            }
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const f32x4 lv = *(const f32x4 *)&sc[2][16 * u + 4 * kq];
-#pragma unroll
-        for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
-    }
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    if (__any(mt > M + kGrow || (M == -INFINITY && mt > M))) {
-        const float mn = fmaxf(M, mt), al = mn == M ? 1.f : __builtin_amdgcn_exp2f(M - mn);
-        M = mn;
-        L *= al;
-#pragma unroll
-        for (int d = 0; d < ND; d++) o[d] *= al;
-    }
-    const float ms = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
-    hf2 hi[8], lo[8];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const f32x4 vs = *(const f32x4 *)&sc[1][16 * u + 4 * kq];
-        float y[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float p = __builtin_amdgcn_exp2f(s[u][r] - ms);
-            L += p;
-            y[r] = p * vs[r];
-        }
-        split2(y[0], y[1], hi[2 * u], lo[2 * u]);
-        split2(y[2], y[3], hi[2 * u + 1], lo[2 * u + 1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        ph[i] = join8(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-        pl[i] = join8(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-    }
-}
 // Some row at the positions p0 .. p1 does not see the whole tile at j0.
 __device__ __forceinline__ bool tile_edge(const Kv8AttnArgs &a, int j0, int p0, int p1) {
     return j0 + 63 > p0 || (a.window && j0 <= p1 - a.window && j0 + 63 >= a.sinks);
@@ -444,27 +357,35 @@ __device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int t, int h, i
     }
 }
 
-// Attention of few rows (row = token * G + head of the kv head): a work-group takes R of them and a split of the tiles. Its
-// four wavefronts share every tile: each forms the scores of 16 keys, all of them (through LDS) the weights of
-// all 64, each the sums of a quarter of the dims, so that a short context's one tile takes a quarter of the time and a wavefront
-// needs few registers (four on a SIMD hide the loads). Every wavefront always has its part of the next
-// tile in flight, 8 KB at D = 256. With R = 8 an operand's 16 columns are both planes of the 8 rows, so a product costs
-// one instruction; with R = 16 the planes follow one another, with R = 32 there are two sets of columns.
+// Attention: a work-group takes R query rows (row = token * G + head of the kv head) and a split of the tiles. Its four
+// wavefronts share every tile, each a part of every step, so nothing is converted or summed twice:
+//   scores   16 keys each, for all rows: K units from the cache to registers, the queries stay in registers
+//   weights  a quarter of the (row, key) pairs each: scores and weights pass through LDS (a few KB a tile)
+//   sums     a quarter of the dims each, for all rows
+// A wavefront's part of the next tile (8 KB at D = 256) is always in flight. Two to four work-groups share a CU: one's
+// vector instructions (conversions, softmax) run beside another's products, which they outweigh (D = 256, R = 32: 260
+// against 64 products of 16 cycles a tile).
+// An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; more: 16 rows, the planes one
+// after the other, R / 16 sets of columns.
 template <int D, bool E4, int R>
-__global__ __launch_bounds__(256, R == 32 ? 2 : 3) void kv8_rows_kernel(const Kv8AttnArgs a) {
-    constexpr int NS = D / 64, NV = D / 64, CT = R == 32 ? 2 : 1;   // a wavefront's units of keys and of values; column sets
+__global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
+    constexpr int NS = D / 64, NV = D / 64, NQ = 2 * NS;   // a wavefront's units of keys and of values; 32-dim steps of a score
     constexpr bool ST = R == 8;
-    __shared__ __align__(16) float sc[2][3][64];
-    __shared__ __align__(16) f32x4 sb[2][CT][4][64];   // [tile parity][columns][16 keys][lane]
-    __shared__ __align__(16) hf8 qs[ST ? 1 : CT][ST ? 1 : 2 * NS][2][64];   // the queries' planes, if not in registers
+    constexpr int CT = ST ? 1 : R / 16, NP = ST ? 1 : 2;   // sets of columns, operands per set
+    constexpr int QW = NQ >= 4 ? NQ / 4 : 1;               // steps whose queries a wavefront prepares
+    __shared__ __align__(16) hf8 qs[CT][NQ][NP][64];
+    __shared__ __align__(16) f32x4 sb[CT][4][64];          // scores [columns][16 keys][lane]
+    __shared__ __align__(16) uint8_t pb[CT][2][NP][1024];  // weights as operands [columns][32 keys][plane][lane]
+    __shared__ __align__(16) float sc[2][3][64];           // [tile parity] scales of the keys, of the values times kP, their log2
+    __shared__ float alb[CT][16], mx[CT][4][16], ms[CT][16];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
-    const int g = blockIdx.y, sp = blockIdx.z, G = a.H / a.c.Hkv, rows = a.T * G;
-    const int np = clamp_past(a.npast, a.npast_dev);
-    const int r0 = blockIdx.x * R, t0 = r0 / G, t1 = min(r0 + R - 1, rows - 1) / G;
-    const Tiles tl = tiles_of(np + t0, np + t1, a.window, a.sinks);
+    const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
+    // the rows with the most tiles first
+    const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - (int)blockIdx.x / a.c.Hkv) * R;
+    const int p0 = np + r0 / G, p1 = np + min(r0 + R - 1, rows - 1) / G, last = np + a.T - 1;
+    const Tiles tl = tiles_of(p0, p1, a.window, a.sinks);
     const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
     if (i0 >= tl.n) return;
-    const int last = np + a.T - 1;
     const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + w * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
     const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
     u32x4 kr[NS], vr[NV];
@@ -479,269 +400,231 @@ __global__ __launch_bounds__(256, R == 32 ? 2 : 3) void kv8_rows_kernel(const Kv
     load_k(tile(i0));
     load_v(tile(i0));
     __builtin_amdgcn_sched_barrier(0);
-    hf8 q8[2 * NS];   // R = 8: the lane's plane
-    float qsc[CT], M[CT], L[CT];
-    int row[CT], pos[CT];
+    auto query = [&](int c, int &t, int &h) {   // the lane's row in a set of columns
+        const int rr = min(r0 + 16 * c + (li & (R - 1)), rows - 1);
+        t = rr / G;
+        h = g * G + rr % G;
+    };
+    // the queries as operands, step i = 2 s + e the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo, e per row
+    {
+        f32x4 x[CT][QW][2];
+        const bool mine = w * QW < NQ;
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            int t, h;
+            query(c, t, h);
+            const float *q = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < QW; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int st = mine ? w * QW + i : 0;
+                    x[c][i][e] = *(const f32x4_u *)(q + 64 * (st >> 1) + 8 * (st & 1) + 4 * e);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[c][i][e][r]));
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (l < 16) mx[c][w][l] = m;
+        }
+        lds_barrier();
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const float m = fmaxf(fmaxf(mx[c][0][li], mx[c][1][li]), fmaxf(mx[c][2][li], mx[c][3][li]));
+            int e = 0;
+            if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
+            e = max(e, -100) - 14;
+            if (l < 16 && w == 0) ms[c][l] = ldexpf(a.scale * 1.44269504088896341f, e);   // what a product is multiplied with
+#pragma unroll
+            for (int i = 0; i < QW; i++) {
+                hf2 hi[4], lo[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    split2(ldexpf(x[c][i][r >> 1][2 * (r & 1)], -e), ldexpf(x[c][i][r >> 1][2 * (r & 1) + 1], -e), hi[r], lo[r]);
+                const hf8 qh = join8(hi[0], hi[1], hi[2], hi[3]), ql = join8(lo[0], lo[1], lo[2], lo[3]);
+                if (!mine) continue;
+                if constexpr (ST) qs[c][w * QW + i][0][l] = li < 8 ? qh : ql;
+                else qs[c][w * QW + i][0][l] = qh, qs[c][w * QW + i][NP - 1][l] = ql;
+            }
+        }
+        lds_barrier();
+    }
+    hf8 q[CT][NQ][NP];
     f32x4 o[CT][NV];
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        row[c] = r0 + 16 * c + (li & (R - 1));
-        const int rr = min(row[c], rows - 1), t = rr / G, h = g * G + rr % G;
-        pos[c] = np + t;
-        hf8 qh[2 * NS], ql[2 * NS];
-        qsc[c] = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
 #pragma unroll
-        for (int i = 0; i < 2 * NS; i++) {
-            if constexpr (ST) q8[i] = li < 8 ? qh[i] : ql[i];
-            else if (i % 4 == w) qs[c][i][0][l] = qh[i], qs[c][i][1][l] = ql[i];
-        }
-        M[c] = -INFINITY;
-        L[c] = 0.f;
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int p = 0; p < NP; p++) q[c][i][p] = qs[c][i][p][l];
 #pragma unroll
         for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (!ST) lds_barrier();
+    // the wavefront's part of the weights: CT of the four sets of 16 keys, from u0, of the columns cw
+    const int cw = (w * CT) >> 2, u0 = (w * CT) & 3;
+    const float qsc = ms[cw][li];
+    int tw, hw;
+    query(cw, tw, hw);
+    const int pos = np + tw;
+    float M = -INFINITY, L = 0.f;
     for (int i = i0; i < i1; i++) {
         const int kt = tile(i), j0 = kt * 64, par = i & 1;
         const bool more = i + 1 < i1;
-        f32x4 x[CT];
+        {   // scores
+            f32x4 x[CT];
 #pragma unroll
-        for (int c = 0; c < CT; c++) x[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < CT; c++) x[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int st = 0; st < NS; st++) {
-            hf8 ka, kb;
-            to_half<E4>(kr[st], ka, kb);
+            for (int st = 0; st < NQ; st++) {
+                const hf8 k = to_half<E4>(kr[st >> 1][2 * (st & 1)], kr[st >> 1][2 * (st & 1) + 1]);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int c = 0; c < CT; c++) x[c] = mfma16(k, q[c][st][p], x[c]);
+            }
+            if (w < 2) {
+                sc[par][w][l] = w ? s1 * kP : s1;
+                if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-100f));
+            }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                if constexpr (ST) {
-                    x[c] = mfma16(ka, q8[2 * st], x[c]);
-                    x[c] = mfma16(kb, q8[2 * st + 1], x[c]);
-                } else {
-                    x[c] = mfma16(ka, qs[c][2 * st][1][l], x[c]);
-                    x[c] = mfma16(kb, qs[c][2 * st + 1][1][l], x[c]);
-                    x[c] = mfma16(ka, qs[c][2 * st][0][l], x[c]);
-                    x[c] = mfma16(kb, qs[c][2 * st + 1][0][l], x[c]);
-                }
+                f32x4 v = x[c];
+                if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
+                sb[c][w][l] = v;
             }
-        }
-        if (w < 2) {
-            sc[par][w][l] = w ? s1 * kP : s1;
-            if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-100f));
-        }
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            if constexpr (ST)
-#pragma unroll
-                for (int r = 0; r < 4; r++) x[c][r] = add_ror8(x[c][r]);
-            sb[par][c][w][l] = x[c];
         }
         if (more) load_k(tile(i + 1));
-        lds_barrier();   // (the other parity: one barrier a tile)
-        hf8 ph[CT][2], pl[CT][2];
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
+        lds_barrier();
+        {   // weights
             f32x4 s[4];
+            float mt = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 4; u++) s[u] = sb[par][c][u][l];
-            tile_weights(a, s, sc[par], qsc[c], j0, pos[c], tile_edge(a, j0, np + t0, np + t1), M[c], L[c], o[c], ph[c], pl[c]);
-            if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
-                if (li >= 8) ph[c][0] = pl[c][0], ph[c][1] = pl[c][1];
+            for (int u = 0; u < 4; u++) {
+                const f32x4 ks = *(const f32x4 *)&sc[par][0][16 * u + 4 * kq];
+                s[u] = sb[cw][u][l];
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[u][r] *= qsc * ks[r];
+            }
+            if (tile_edge(a, j0, p0, p1))
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int j = j0 + 16 * u + 4 * kq + r;
+                        if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
+                    }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const f32x4 lv = *(const f32x4 *)&sc[par][2][16 * u + 4 * kq];
+#pragma unroll
+                for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
+            }
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            float al = 1.f;
+            if (mt > M + kGrow || (M == -INFINITY && mt > M)) {   // (the wavefronts of the same columns agree)
+                const float mn = fmaxf(M, mt);
+                al = __builtin_amdgcn_exp2f(M - mn);
+                M = mn;
+                L *= al;
+            }
+            if (u0 == 0 && kq == 0) alb[cw][li] = al;
+            const float ref = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+#pragma unroll
+            for (int v = 0; v < CT; v++) {
+                const int u = u0 + v;
+                f32x4 x = s[v];
+                if (CT < 4)   // s[u0 + v] without a register index that varies
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (y == u) x = s[y];
+                const f32x4 vs = *(const f32x4 *)&sc[par][1][16 * u + 4 * kq];
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = __builtin_amdgcn_exp2f(x[r] - ref);
+                    L += p;
+                    y[r] = p * vs[r];
+                }
+                hf2 h0, h1, l0, l1;
+                split2(y[0], y[1], h0, l0);
+                split2(y[2], y[3], h1, l1);
+                typedef _Float16 hf4 __attribute__((ext_vector_type(4)));
+                const hf4 hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
+                const int at = l * 16 + 8 * (u & 1);
+                if constexpr (ST) {
+                    *(hf4 *)(pb[cw][u >> 1][0] + at) = li < 8 ? hi : lo;
+                } else {
+                    *(hf4 *)(pb[cw][u >> 1][0] + at) = hi;
+                    *(hf4 *)(pb[cw][u >> 1][NP - 1] + at) = lo;
+                }
             }
         }
-        if (E4 && j0 + 63 > last) {
-            const u32x4 m = written(j0, last);
-#pragma unroll
-            for (int d = 0; d < NV; d++) vr[d] &= m;
-        }
-#pragma unroll
-        for (int d = 0; d < NV; d++) {
-            hf8 va, vb;
-            to_half<E4>(vr[d], va, vb);
+        lds_barrier();
+        {   // sums
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                if constexpr (!ST) {
-                    o[c][d] = mfma16(va, pl[c][0], o[c][d]);
-                    o[c][d] = mfma16(vb, pl[c][1], o[c][d]);
-                }
-                o[c][d] = mfma16(va, ph[c][0], o[c][d]);
-                o[c][d] = mfma16(vb, ph[c][1], o[c][d]);
+                const float al = alb[c][li];
+                if (__any(al != 1.f))
+#pragma unroll
+                    for (int d = 0; d < NV; d++) o[c][d] *= al;
             }
+            if (E4 && j0 + 63 > last) {
+                const u32x4 m = written(j0, last);
+#pragma unroll
+                for (int d = 0; d < NV; d++) vr[d] &= m;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                hf8 p[CT][NP];
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int x = 0; x < NP; x++) p[c][x] = *(const hf8 *)(pb[c][h][x] + l * 16);
+#pragma unroll
+                for (int d = 0; d < NV; d++) {
+                    const hf8 v = to_half<E4>(vr[d][2 * h], vr[d][2 * h + 1]);
+#pragma unroll
+                    for (int x = NP - 1; x >= 0; x--)
+#pragma unroll
+                        for (int c = 0; c < CT; c++) o[c][d] = mfma16(v, p[c][x], o[c][d]);
+                }
+            }
+            if (more) load_v(tile(i + 1));
         }
-        if (more) load_v(tile(i + 1));
     }
+    // the rows' totals
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (l < 16) {
+        mx[cw][CT == 4 ? 0 : w % (4 / CT)][l] = L;
+        if (u0 == 0) ms[cw][l] = M;
+    }
+    lds_barrier();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        L[c] += __shfl_xor(L[c], 16, 64);
-        L[c] += __shfl_xor(L[c], 32, 64);
         if constexpr (ST)
 #pragma unroll
             for (int d = 0; d < NV; d++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) o[c][d][r] = add_ror8(o[c][d][r]);
-        if (row[c] >= rows || li >= R) continue;
-        // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
-        const int d0 = 16 * w * NV + 4 * kq;
+        const int row = r0 + 16 * c + li;
+        if (row >= rows || li >= R) continue;
+        float total = mx[c][0][li];
+#pragma unroll
+        for (int x = 1; x < 4 / CT; x++) total += mx[c][x][li];
+        const int d0 = 16 * w * NV + 4 * kq;   // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
         if (a.n_split > 1) {
-            float *part = a.part + (((int64_t)g * rows + row[c]) * a.n_split + sp) * (D + 4);
-            if (w == 0 && kq == 0) part[0] = M[c], part[1] = L[c];
+            float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
+            if (w == 0 && kq == 0) part[0] = ms[c][li], part[1] = total;
 #pragma unroll
             for (int d = 0; d < NV; d++) *(f32x4 *)(part + 4 + d0 + 16 * d) = o[c][d];
         } else {
-            const int t = row[c] / G, h = g * G + row[c] % G;
-            finish_row<NV>(a, t, h, h * D, d0, L[c], o[c]);
+            const int h = g * G + row % G;
+            finish_row<NV>(a, row / G, h, h * D, d0, total, o[c]);
         }
     }
-}
-
-// Attention of many rows: a work-group takes 64 query rows of a kv head, its two groups of four wavefronts (16 rows each)
-// every other tile. A tile's codes become f16 operands in LDS once for the four wavefronts (64 KB at D = 256, in operand
-// order: every access is 64 consecutive 16-byte pieces). Per tile a group has a step on the vector units (the softmax of the
-// tile's scores; its values and the next tile's keys turned into operands) and one on the matrix cores (its values'
-// products, then the next tile's scores); the groups take them in turn, one a step behind the other,
-// so that on every SIMD one wavefront keeps the matrix core busy while the other has the vector unit.
-template <int D, bool E4>
-__global__ __launch_bounds__(512, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) {
-    constexpr int NS = D / 64, ND = D / 16, NU = D / 64;   // units of keys (and of values) per wavefront: 4 NS / 4 = ND / 4
-    __shared__ __align__(16) uint8_t Ks[2][64 * D * 2], Vs[2][64 * D * 2];
-    __shared__ __align__(16) float sc[2][2][3][64];   // [group][tile parity]
-    __shared__ float ml[2][2][64];
-    const int tid = threadIdx.x, l = tid & 63, li = l & 15, kq = l >> 4;
-    const int grp = __builtin_amdgcn_readfirstlane(tid >> 8), w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
-    const int G = a.H / a.c.Hkv, rows = a.T * G, b = blockIdx.x;
-    const int g = b % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - b / a.c.Hkv) * 64;   // the most tiles first
-    const int np = clamp_past(a.npast, a.npast_dev), last = np + a.T - 1;
-    const Tiles tl = tiles_of(np + r0 / G, np + min(r0 + 63, rows - 1) / G, a.window, a.sinks);
-    const int i0 = sp * a.per_split, nt = min(a.per_split, tl.n - i0);
-    if (nt <= 0) return;
-    const int rw = r0 + 16 * w, row = min(rw + li, rows - 1), t = row / G, h = g * G + row % G, pos = np + t;
-    const int p0 = np + min(rw, rows - 1) / G, p1 = np + min(rw + 15, rows - 1) / G;   // the wavefront's rows
-    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D;
-    const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
-    const int n = (nt + 1 - grp) / 2;   // the group's tiles
-    auto tile = [&](int j) {
-        const int i = i0 + grp + 2 * j;
-        return i < tl.ns ? i : tl.f + i - tl.ns;
-    };
-    u32x4 kr[NU], vr[NU];
-    float k1 = 0.f, v1 = 0.f;
-    auto load_k = [&](int j) {
-        const int kt = tile(j), p = kt * 64 + l;
-        load_units<NU>(kc + (int64_t)kt * 64 * D + w * NU * 1024, l * 16, kr);
-        if (w == 0) {
-            const bool in = p <= last;
-            k1 = in ? a.c.ks[s0 + (p >> a.c.lg)] : 0.f;
-            v1 = in ? a.c.vs[s0 + (p >> a.c.lg)] : 0.f;
-        }
-    };
-    if (n > 0) load_k(0);
-    hf8 qh[2 * NS], ql[2 * NS];
-    const float qsc = split_query<D>(a.q + t * a.q_tok + h * a.q_head + 16 * kq, a.scale, qh, ql);
-    f32x4 o[ND], s[4];
-    hf8 ph[2], pl[2];
-#pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, L = 0.f;
-    for (int x = 0; x < nt + 3; x++) {   // 2 n + 2 steps of either group, the second's one later
-        const int step = x - grp, j = step >> 1;
-        if (step >= 0 && !(step & 1) && j <= n) {
-            if (j > 0) {   // tile j - 1: softmax, values
-                const int j0 = tile(j - 1) * 64;
-                tile_weights(a, s, sc[grp][(j - 1) & 1], qsc, j0, pos, tile_edge(a, j0, p0, p1), M, L, o, ph, pl);
-                if (E4 && j0 + 63 > last) {
-                    const u32x4 m = written(j0, last);
-#pragma unroll
-                    for (int c = 0; c < NU; c++) vr[c] &= m;
-                }
-#pragma unroll
-                for (int c = 0; c < NU; c++) {
-                    hf8 x, y;
-                    to_half<E4>(vr[c], x, y);
-                    *(hf8 *)(Vs[grp] + (w * NU + c) * 2048 + l * 16) = x;
-                    *(hf8 *)(Vs[grp] + (w * NU + c) * 2048 + 1024 + l * 16) = y;
-                }
-            }
-            if (j < n) {   // the keys of tile j
-#pragma unroll
-                for (int c = 0; c < NU; c++) {
-                    hf8 x, y;
-                    to_half<E4>(kr[c], x, y);
-                    *(hf8 *)(Ks[grp] + (w * NU + c) * 2048 + l * 16) = x;
-                    *(hf8 *)(Ks[grp] + (w * NU + c) * 2048 + 1024 + l * 16) = y;
-                }
-                if (w == 0) {
-                    sc[grp][j & 1][0][l] = k1;
-                    sc[grp][j & 1][1][l] = v1 * kP;
-                    sc[grp][j & 1][2][l] = log2f(fmaxf(v1, 0x1p-100f));
-                }
-            }
-        }
-        if (step >= 0 && (step & 1) && j <= n) {
-            if (j < n) load_units<NU>(vc + (int64_t)tile(j) * 64 * D + w * NU * 1024, l * 16, vr);
-            if (j + 1 < n) load_k(j + 1);
-            if (j > 0)
-#pragma unroll
-                for (int d = 0; d < ND; d += 2) {
-                    hf8 v[4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) v[c] = *(const hf8 *)(Vs[grp] + d * 2048 + c * 1024 + l * 16);
-                    o[d] = mfma16(v[0], pl[0], o[d]);
-                    o[d + 1] = mfma16(v[2], pl[0], o[d + 1]);
-                    o[d] = mfma16(v[1], pl[1], o[d]);
-                    o[d + 1] = mfma16(v[3], pl[1], o[d + 1]);
-                    o[d] = mfma16(v[0], ph[0], o[d]);
-                    o[d + 1] = mfma16(v[2], ph[0], o[d + 1]);
-                    o[d] = mfma16(v[1], ph[1], o[d]);
-                    o[d + 1] = mfma16(v[3], ph[1], o[d + 1]);
-                }
-            if (j < n) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < 2 * NS; st++) {
-                    hf8 ka[4];
-#pragma unroll
-                    for (int u = 0; u < 4; u++) ka[u] = *(const hf8 *)(Ks[grp] + (u * 2 * NS + st) * 1024 + l * 16);
-#pragma unroll
-                    for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], ql[st], s[u]);
-#pragma unroll
-                    for (int u = 0; u < 4; u++) s[u] = mfma16(ka[u], qh[st], s[u]);
-                }
-            }
-        }
-        lds_barrier();
-    }
-    // the groups' sums joined: each hands the other half of its dims over and finishes the rest
-    L += __shfl_xor(L, 16, 64);
-    L += __shfl_xor(L, 32, 64);
-    if (kq == 0) {
-        ml[grp][0][16 * w + li] = M;
-        ml[grp][1][16 * w + li] = L;
-    }
-    lds_barrier();
-    const float m2 = ml[grp ^ 1][0][16 * w + li], l2 = ml[grp ^ 1][1][16 * w + li], mm = fmaxf(M, m2);
-    const float f1 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mm), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mm);
-    const float ll = grp ? l2 * f2 + L * f1 : L * f1 + l2 * f2;   // (the same sum in both)
-    f32x4 *xo = (f32x4 *)Ks;   // [receiving group][wavefront][ND / 2][64]
-#pragma unroll
-    for (int d = 0; d < ND; d++) {
-        o[d] *= f1;
-        if ((d >= ND / 2) != grp) xo[(((grp ^ 1) * 4 + w) * (ND / 2) + d % (ND / 2)) * 64 + l] = o[d];
-    }
-    lds_barrier();
-    if (rw + li >= rows) return;
-    float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
-    if (a.n_split > 1 && kq == 0 && grp == 0) part[0] = mm, part[1] = ll;
-    auto give = [&](int d1, const f32x4 *half) {   // register r of o[d]: dim 16 d + 4 kq + r
-        f32x4 v[ND / 2];
-#pragma unroll
-        for (int d = 0; d < ND / 2; d++) {
-            v[d] = half[d] + xo[((grp * 4 + w) * (ND / 2) + d) * 64 + l];
-            if (a.n_split > 1) *(f32x4 *)(part + 4 + 16 * (d1 + d) + 4 * kq) = v[d];
-        }
-        if (a.n_split == 1) finish_row<ND / 2>(a, t, h, (int64_t)h * D, 16 * d1 + 4 * kq, ll, v);
-    };
-    if (grp == 0) give(0, o);
-    else give(ND / 2, o + ND / 2);
 }
 
 // The splits of a row joined in order: W wavefronts take every W-th split each (a lane D / 64 dims), their sums are added in
@@ -808,11 +691,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
 
-// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions), up to 32
-// take the kernel without operand tiles in LDS.
+// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions); as many as
+// there are, up to what the queries' registers allow (32 of 256 dims, 64 of fewer).
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
-    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64;
+    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 || a.c.D == 256 ? 32 : 64;
 }
 // Tiles that R rows see at most.
 static int most_tiles(const Kv8AttnArgs &a, int R) {
@@ -822,14 +705,12 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
-// Splits of the tiles: work-groups for every CU to hold (64 rows: one, of up to 8 wavefronts; fewer: three or four), and four
-// tiles for each of 64 rows, whose partial sums cost as much as a tile.
+// Splits of the tiles while the work-groups do not exceed what the CUs hold.
 static int splits_of(const Kv8AttnArgs &a) {
-    const int R = rows_of(a);
+    const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
-    const int by_tiles = R == 64 ? (most_tiles(a, R) + 3) / 4 : most_tiles(a, R);
-    int64_t n = (R == 64 ? 256 : R == 32 ? 512 : 768) / wgs;
-    if (n > by_tiles) n = by_tiles;
+    int64_t n = (R >= 32 ? 512 : 768) / wgs;
+    if (n > tiles) n = tiles;
     return n < 1 ? 1 : (int)n;
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
@@ -840,10 +721,11 @@ int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
 template <int D, bool E4>
 static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     const int rows = a.T * (a.H / a.c.Hkv), nb = (rows + R - 1) / R;
-    if (R == 8) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 8>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
-    else if (R == 16) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 16>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
-    else if (R == 32) hipLaunchKernelGGL((kv8_rows_kernel<D, E4, 32>), dim3(nb, a.c.Hkv, a.n_split), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), dim3(nb * a.c.Hkv, a.n_split), dim3(512), 0, st, a);
+    const dim3 grid(nb * a.c.Hkv, a.n_split);
+    if (R == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 8>), grid, dim3(256), 0, st, a);
+    else if (R == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
+    else if (R == 32) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 32>), grid, dim3(256), 0, st, a);
+    else if constexpr (D < 256) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 64>), grid, dim3(256), 0, st, a);
     if (a.n_split == 1) return;
     if (a.n_split <= 16 || rows * a.c.Hkv > 1024) hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((rows + 3) / 4, a.c.Hkv), dim3(256), 0, st, a, R);
     else hipLaunchKernelGGL((kv8_merge_kernel<D, 8>), dim3(rows, a.c.Hkv), dim3(512), 0, st, a, R);
