@@ -16,6 +16,7 @@ namespace xjk {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hf2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hf4 __attribute__((ext_vector_type(4)));
 typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));   // rows of any 4-byte alignment
@@ -44,26 +45,44 @@ __device__ __forceinline__ float block_scale(float amax) {
     }
     return fmaxf(s, 0x1p-126f);
 }
-// The code of x: nearest to the exact quotient x / s, ties to even.
-//   int8: rint of the product with 1 / s is at most one off; the rest x - c s
-//   is exact in one fma (it is below s and a multiple of the smaller ulp), so comparing
-//   it with s / 2 decides.
+// The codes of four values: nearest to the exact quotients x / s, ties to even (inv = 1 / s, 0 for s = 0).
 //   e4m3: s is a power of two, the product with 1 / s is exact and converts to nearest even.
+//   int8: the product, rounded by adding 1.5 * 2^23 (the sum's low byte is the code), is off by less than 2^-14. Where one lies
+//   nearer than that to a border (one value in 8000), the rests decide: x - c s is exact in one fma (it is below s
+//   and a multiple of the smaller ulp), and compared with s / 2.
 template <bool E4>
-__device__ __forceinline__ uint32_t code_of(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t codes_of(const f32x4 x, float s, float inv) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        y[i] = x[i] * inv;
+        y[i] = y[i] != y[i] ? 0.f : y[i];   // NaN, and an infinity in a block of scale 0
+        y[i] = __builtin_amdgcn_fmed3f(y[i], E4 ? -448.f : -127.f, E4 ? 448.f : 127.f);
+    }
     if constexpr (E4) {
-        float y = x * inv;
-        y = fminf(fmaxf(y, -448.f), 448.f);
-        if (x != x || s == 0.f) y = 0.f;
-        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xFFu;
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     } else {
-        if (x != x || s == 0.f) return 0;
-        float c = rintf(fminf(fmaxf(x * inv, -127.f), 127.f));
-        const float r2 = 2.f * fmaf(-c, s, x);
-        if (r2 > s || (r2 == s && ((int)c & 1))) c += 1.f;
-        else if (r2 < -s || (r2 == -s && ((int)c & 1))) c -= 1.f;
-        c = fminf(fmaxf(c, -127.f), 127.f);
-        return (uint32_t)(int)c & 0xFFu;
+        constexpr float kMagic = 12582912.f;
+        float r[4], far = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r[i] = y[i] + kMagic;
+            far = fmaxf(far, fabsf(y[i] - (r[i] - kMagic)));
+        }
+        if (__any(far > 0.5f - 0x1p-14f)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float c = r[i] - kMagic;
+                const float rest = fmaf(-c, s, x[i]), half = 0.5f * s;
+                const bool odd = (int)c & 1;
+                if (rest > half || (rest == half && odd)) c += 1.f;
+                else if (rest < -half || (rest == -half && odd)) c -= 1.f;
+                r[i] = fminf(fmaxf(c, -127.f), 127.f) + kMagic;   // (an infinity's rest is one)
+            }
+        }
+        const uint32_t u = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x0c0c0400u);
+        return __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x04000c0cu) | u;
     }
 }
 // A code of scale s_old at the larger scale s: the quotient of the code's value
@@ -135,12 +154,21 @@ __device__ __forceinline__ void put_codes(uint8_t *tile, int q, int d0, const ui
         for (int i = 0; i < 16; i++) *(uint32_t *)(p + 16 * i) = w[i];
     }
 }
+// The larger of a lane's value and that of lane l ^ 16, l ^ 32.
+__device__ __forceinline__ float max_x16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // The largest of D / 4 consecutive lanes, in each of them.
 template <int D>
 __device__ __forceinline__ float row_max(float v) {
     v = xjd::row16_max(v);
-    if (D >= 128) v = fmaxf(v, __shfl_xor(v, 16, 64));
-    if (D >= 256) v = fmaxf(v, __shfl_xor(v, 32, 64));
+    if (D >= 128) v = max_x16(v);
+    if (D >= 256) v = max_x32(v);
     return v;
 }
 
@@ -159,6 +187,7 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
     float *sp = (VAL ? a.c.vs : a.c.ks) + ((((int64_t)g * a.c.n_tiles + kt) * 64) >> a.c.lg);
     const bool whole = j0 >= np && j0 + 64 <= end;
     uint32_t w[16];
+    const float old_s = !whole && tid < 64 ? sp[tid >> a.c.lg] : 0.f;
     if (!whole) get_codes<D, VAL>(tile, q, d0, w);
     f32x4 y[16];
 #pragma unroll
@@ -169,8 +198,11 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        const float m = row_max<D>(fmaxf(fmaxf(finite_abs(y[i].x), finite_abs(y[i].y)), fmaxf(finite_abs(y[i].z), finite_abs(y[i].w))));
-        if (d0 == 0) sm[0][group_pos<VAL>(q, i)] = m;
+        const int pl = group_pos<VAL>(q, i), p = j0 + pl;
+        float m = 0.f;
+        if (whole || (p >= np && p < end))   // (uniform among the row's lanes)
+            m = row_max<D>(fmaxf(fmaxf(finite_abs(y[i].x), finite_abs(y[i].y)), fmaxf(finite_abs(y[i].z), finite_abs(y[i].w))));
+        if (d0 == 0) sm[0][pl] = m;
     }
     __syncthreads();
     if (tid < 64) {   // position j0 + tid: sm[0] its block's scale, sm[1] the block's earlier scale if it is begun
@@ -179,7 +211,7 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
         const int first = (j0 + tid) & -B;
         float s = block_scale<E4>(m), old = 0.f;
         if (first < np && first + B > np) {
-            old = sp[tid >> a.c.lg];
+            old = old_s;
             s = fmaxf(s, old);
         }
         sm[0][tid] = s;
@@ -192,7 +224,7 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
         const int pl = group_pos<VAL>(q, i), p = j0 + pl;
         const float s = sm[0][pl], inv = s > 0.f ? 1.f / s : 0.f;
         if (whole || (p >= np && p < end)) {
-            w[i] = code_of<E4>(y[i].x, s, inv) | code_of<E4>(y[i].y, s, inv) << 8 | code_of<E4>(y[i].z, s, inv) << 16 | code_of<E4>(y[i].w, s, inv) << 24;
+            w[i] = codes_of<E4>(y[i], s, inv);
         } else if (p < np && (p | (B - 1)) >= np) {
             const float old = sm[1][pl];
             if (s > old)
@@ -271,7 +303,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split2(float y0, float y1, hf2 &hi, hf2 &lo) {
     asm("" : "+v"(y0), "+v"(y1));
     hi = __builtin_convertvector(f32x2{y0, y1}, hf2);
-    lo = __builtin_convertvector(f32x2{y0 - (float)hi.x, y1 - (float)hi.y}, hf2);   // the differences are exact
+    lo = __builtin_convertvector(f32x2{fmaf((float)hi.x, -1.f, y0), fmaf((float)hi.y, -1.f, y1)}, hf2);   // (exact differences, one mixed fma each)
 }
 
 // The tiles that the tokens at p0 .. p1 see: the first ns (of the tokens that stay
@@ -338,11 +370,21 @@ __device__ __forceinline__ void load_units(const uint8_t *p, uint32_t lane, u32x
 // sigmoid by the exponential and reciprocal instructions (1 ulp each).
 __device__ __forceinline__ float sigm_fast(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
 
-// N groups of 4 sums, 16 dims apart from dim d0 of the token's head: over the total, gated, into the output row at hd.
-template <int N>
-__device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int t, int h, int64_t hd, int d0, float total, const f32x4 *o) {
+// N groups of 4 sums, 16 dims apart from dim d0, of a row with reference M and total: the split's partial sums [row][split][M,
+// total, -, -, D sums], or, unsplit, over the total and gated into the output row.
+template <int N, int D = 64 * N>
+__device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int sp, int d0, float M, float total, const f32x4 *o) {
+    const int G = a.H / a.c.Hkv;
+    if (a.n_split > 1) {
+        float *part = a.part + (((int64_t)g * a.T * G + row) * a.n_split + sp) * (D + 4);
+        if (d0 == 0) part[0] = M, part[1] = total;
+#pragma unroll
+        for (int i = 0; i < N; i++) *(f32x4 *)(part + 4 + d0 + 16 * i) = o[i];
+        return;
+    }
+    const int t = row / G, h = g * G + row % G;
     const float inv = (1.f / kP) / total;
-    float *op = a.out + t * a.o_tok + hd + d0;
+    float *op = a.out + t * a.o_tok + (int64_t)h * D + d0;
     f32x4 x[N];
     if (a.gate)
 #pragma unroll
@@ -357,31 +399,30 @@ __device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int t, int h, i
     }
 }
 
-// Attention: a work-group takes R query rows (row = token * G + head of the kv head) and a split of the tiles. Its four
-// wavefronts share every tile, each a part of every step, so nothing is converted or summed twice:
-//   scores   16 keys each, for all rows: K units from the cache to registers, the queries stay in registers
+// Attention of up to 16 rows (row = token * G + head of the kv head): a work-group takes R of them and a split of the tiles. Its
+// four wavefronts share every tile, each a part of every step, so nothing is converted or summed twice and one tile (a
+// short context's) takes a quarter of the time:
+//   scores   16 keys each: K units from the cache to registers, the queries stay in registers
 //   weights  a quarter of the (row, key) pairs each: scores and weights pass through LDS (a few KB a tile)
-//   sums     a quarter of the dims each, for all rows
-// A wavefront's part of the next tile (8 KB at D = 256) is always in flight. Two to four work-groups share a CU: one's
-// vector instructions (conversions, softmax) run beside another's products, which they outweigh (D = 256, R = 32: 260
-// against 64 products of 16 cycles a tile).
-// An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; more: 16 rows, the planes one
-// after the other, R / 16 sets of columns.
+//   sums     a quarter of the dims each
+// A wavefront's part of the next tile (8 KB at D = 256) is always in flight, three or four work-groups share a CU: a long
+// cache streams (one token at 131000 positions of the 4B shape: 268 MB in 49.4 us, 5.4 TB/s; a 1 GiB copy reaches 5.15).
+// An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; R = 16: one plane after the
+// other.
 template <int D, bool E4, int R>
 __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     constexpr int NS = D / 64, NV = D / 64, NQ = 2 * NS;   // a wavefront's units of keys and of values; 32-dim steps of a score
     constexpr bool ST = R == 8;
-    constexpr int CT = ST ? 1 : R / 16, NP = ST ? 1 : 2;   // sets of columns, operands per set
+    constexpr int NP = ST ? 1 : 2;                         // operands a step
     constexpr int QW = NQ >= 4 ? NQ / 4 : 1;               // steps whose queries a wavefront prepares
-    __shared__ __align__(16) hf8 qs[CT][NQ][NP][64];
-    __shared__ __align__(16) f32x4 sb[CT][4][64];          // scores [columns][16 keys][lane]
-    __shared__ __align__(16) uint8_t pb[CT][2][NP][1024];  // weights as operands [columns][32 keys][plane][lane]
-    __shared__ __align__(16) float sc[2][3][64];           // [tile parity] scales of the keys, of the values times kP, their log2
-    __shared__ float alb[CT][16], mx[CT][4][16], ms[CT][16];
+    __shared__ __align__(16) hf8 qs[NQ][NP][64];
+    __shared__ __align__(16) f32x4 sb[4][64];          // scores [16 keys][lane]
+    __shared__ __align__(16) uint8_t pb[2][NP][1024];  // weights as operands [32 keys][plane][lane]
+    __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys, of the values times kP, their log2
+    __shared__ float alb[16], mx[4][16];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
-    // the rows with the most tiles first
-    const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - (int)blockIdx.x / a.c.Hkv) * R;
+    const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = (int)blockIdx.x / a.c.Hkv * R;
     const int p0 = np + r0 / G, p1 = np + min(r0 + R - 1, rows - 1) / G, last = np + a.T - 1;
     const Tiles tl = tiles_of(p0, p1, a.window, a.sinks);
     const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
@@ -400,230 +441,426 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     load_k(tile(i0));
     load_v(tile(i0));
     __builtin_amdgcn_sched_barrier(0);
-    auto query = [&](int c, int &t, int &h) {   // the lane's row in a set of columns
-        const int rr = min(r0 + 16 * c + (li & (R - 1)), rows - 1);
-        t = rr / G;
-        h = g * G + rr % G;
-    };
+    const int row = r0 + (li & (R - 1)), rq = min(row, rows - 1), t = rq / G, h = g * G + rq % G, pos = np + t;
     // the queries as operands, step i = 2 s + e the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo, e per row
+    float qsc;
     {
-        f32x4 x[CT][QW][2];
         const bool mine = w * QW < NQ;
+        const float *qp = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
+        f32x4 x[QW][2];
+        float m = 0.f;
 #pragma unroll
-        for (int c = 0; c < CT; c++) {
-            int t, h;
-            query(c, t, h);
-            const float *q = a.q + t * a.q_tok + h * a.q_head + 16 * kq;
-            float m = 0.f;
+        for (int i = 0; i < QW; i++)
 #pragma unroll
-            for (int i = 0; i < QW; i++)
+            for (int e = 0; e < 2; e++) {
+                const int st = mine ? w * QW + i : 0;
+                x[i][e] = *(const f32x4_u *)(qp + 64 * (st >> 1) + 8 * (st & 1) + 4 * e);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int st = mine ? w * QW + i : 0;
-                    x[c][i][e] = *(const f32x4_u *)(q + 64 * (st >> 1) + 8 * (st & 1) + 4 * e);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[c][i][e][r]));
-                }
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            if (l < 16) mx[c][w][l] = m;
-        }
-        lds_barrier();
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            const float m = fmaxf(fmaxf(mx[c][0][li], mx[c][1][li]), fmaxf(mx[c][2][li], mx[c][3][li]));
-            int e = 0;
-            if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-            e = max(e, -100) - 14;
-            if (l < 16 && w == 0) ms[c][l] = ldexpf(a.scale * 1.44269504088896341f, e);   // what a product is multiplied with
-#pragma unroll
-            for (int i = 0; i < QW; i++) {
-                hf2 hi[4], lo[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    split2(ldexpf(x[c][i][r >> 1][2 * (r & 1)], -e), ldexpf(x[c][i][r >> 1][2 * (r & 1) + 1], -e), hi[r], lo[r]);
-                const hf8 qh = join8(hi[0], hi[1], hi[2], hi[3]), ql = join8(lo[0], lo[1], lo[2], lo[3]);
-                if (!mine) continue;
-                if constexpr (ST) qs[c][w * QW + i][0][l] = li < 8 ? qh : ql;
-                else qs[c][w * QW + i][0][l] = qh, qs[c][w * QW + i][NP - 1][l] = ql;
+                for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[i][e][r]));
             }
+        m = max_x16(max_x32(m));
+        if (l < 16) mx[w][l] = m;
+        lds_barrier();
+        m = fmaxf(fmaxf(mx[0][li], mx[1][li]), fmaxf(mx[2][li], mx[3][li]));
+        int e = 0;
+        if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
+        e = max(e, -100) - 14;
+        qsc = ldexpf(a.scale * 1.44269504088896341f, e);   // what a product is multiplied with
+#pragma unroll
+        for (int i = 0; i < QW; i++) {
+            hf2 hi[4], lo[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) split2(ldexpf(x[i][r >> 1][2 * (r & 1)], -e), ldexpf(x[i][r >> 1][2 * (r & 1) + 1], -e), hi[r], lo[r]);
+            const hf8 qh = join8(hi[0], hi[1], hi[2], hi[3]), ql = join8(lo[0], lo[1], lo[2], lo[3]);
+            if (!mine) continue;
+            if constexpr (ST) qs[w * QW + i][0][l] = li < 8 ? qh : ql;
+            else qs[w * QW + i][0][l] = qh, qs[w * QW + i][NP - 1][l] = ql;
         }
         lds_barrier();
     }
-    hf8 q[CT][NQ][NP];
-    f32x4 o[CT][NV];
+    hf8 q[NQ][NP];
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
+    for (int i = 0; i < NQ; i++)
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
+        for (int p = 0; p < NP; p++) q[i][p] = qs[i][p][l];
+    f32x4 o[NV];
 #pragma unroll
-            for (int p = 0; p < NP; p++) q[c][i][p] = qs[c][i][p][l];
-#pragma unroll
-        for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    // the wavefront's part of the weights: CT of the four sets of 16 keys, from u0, of the columns cw
-    const int cw = (w * CT) >> 2, u0 = (w * CT) & 3;
-    const float qsc = ms[cw][li];
-    int tw, hw;
-    query(cw, tw, hw);
-    const int pos = np + tw;
+    for (int d = 0; d < NV; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
     for (int i = i0; i < i1; i++) {
         const int kt = tile(i), j0 = kt * 64, par = i & 1;
         const bool more = i + 1 < i1;
         {   // scores
-            f32x4 x[CT];
-#pragma unroll
-            for (int c = 0; c < CT; c++) x[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 x[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int st = 0; st < NQ; st++) {
                 const hf8 k = to_half<E4>(kr[st >> 1][2 * (st & 1)], kr[st >> 1][2 * (st & 1) + 1]);
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int c = 0; c < CT; c++) x[c] = mfma16(k, q[c][st][p], x[c]);
+                for (int p = NP - 1; p >= 0; p--) x[st & 1] = mfma16(k, q[st][p], x[st & 1]);
             }
             if (w < 2) {
                 sc[par][w][l] = w ? s1 * kP : s1;
                 if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-100f));
             }
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                f32x4 v = x[c];
-                if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
-                sb[c][w][l] = v;
-            }
+            f32x4 v = x[0] + x[1];
+            if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
+            sb[w][l] = v;
         }
         if (more) load_k(tile(i + 1));
         lds_barrier();
-        {   // weights
-            f32x4 s[4];
-            float mt = -INFINITY;
+        {   // weights: the maximum over all keys, the terms of the wavefront's 16
+            f32x4 s[4];   // of the sets of 16 keys from w on, around
+            float mt = -INFINITY, qe = qsc;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const f32x4 ks = *(const f32x4 *)&sc[par][0][16 * u + 4 * kq];
-                s[u] = sb[cw][u][l];
-#pragma unroll
-                for (int r = 0; r < 4; r++) s[u][r] *= qsc * ks[r];
+            for (int v = 0; v < 4; v++) {
+                const int u = (w + v) & 3;
+                s[v] = sb[u][l] * *(const f32x4 *)&sc[par][0][16 * u + 4 * kq];
             }
-            if (tile_edge(a, j0, p0, p1))
+            if (tile_edge(a, j0, p0, p1)) {
+                qe = 1.f;
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+                for (int v = 0; v < 4; v++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int j = j0 + 16 * u + 4 * kq + r;
-                        if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) s[u][r] = -INFINITY;
+                        const int j = j0 + 16 * ((w + v) & 3) + 4 * kq + r;
+                        const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+                        s[v][r] = see ? s[v][r] * qsc : -INFINITY;
                     }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const f32x4 lv = *(const f32x4 *)&sc[par][2][16 * u + 4 * kq];
-#pragma unroll
-                for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[u][r] + lv[r]);
             }
-            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const f32x4 lv = *(const f32x4 *)&sc[par][2][16 * ((w + v) & 3) + 4 * kq];
+#pragma unroll
+                for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[v][r], qe, lv[r]));
+            }
+            mt = max_x16(max_x32(mt));
             float al = 1.f;
-            if (mt > M + kGrow || (M == -INFINITY && mt > M)) {   // (the wavefronts of the same columns agree)
+            if (mt > M + kGrow || (M == -INFINITY && mt > M)) {   // (the wavefronts agree)
                 const float mn = fmaxf(M, mt);
                 al = __builtin_amdgcn_exp2f(M - mn);
                 M = mn;
                 L *= al;
             }
-            if (u0 == 0 && kq == 0) alb[cw][li] = al;
+            if (w == 0 && kq == 0) alb[li] = al;
             const float ref = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+            const f32x4 vs = *(const f32x4 *)&sc[par][1][16 * w + 4 * kq];
+            float y[4];
 #pragma unroll
-            for (int v = 0; v < CT; v++) {
-                const int u = u0 + v;
-                f32x4 x = s[v];
-                if (CT < 4)   // s[u0 + v] without a register index that varies
-#pragma unroll
-                    for (int y = 0; y < 4; y++)
-                        if (y == u) x = s[y];
-                const f32x4 vs = *(const f32x4 *)&sc[par][1][16 * u + 4 * kq];
-                float y[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float p = __builtin_amdgcn_exp2f(x[r] - ref);
-                    L += p;
-                    y[r] = p * vs[r];
-                }
-                hf2 h0, h1, l0, l1;
-                split2(y[0], y[1], h0, l0);
-                split2(y[2], y[3], h1, l1);
-                typedef _Float16 hf4 __attribute__((ext_vector_type(4)));
-                const hf4 hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
-                const int at = l * 16 + 8 * (u & 1);
-                if constexpr (ST) {
-                    *(hf4 *)(pb[cw][u >> 1][0] + at) = li < 8 ? hi : lo;
-                } else {
-                    *(hf4 *)(pb[cw][u >> 1][0] + at) = hi;
-                    *(hf4 *)(pb[cw][u >> 1][NP - 1] + at) = lo;
-                }
+            for (int r = 0; r < 4; r++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[0][r], qe, -ref));
+                L += p;
+                y[r] = p * vs[r];
+            }
+            hf2 h0, h1, l0, l1;
+            split2(y[0], y[1], h0, l0);
+            split2(y[2], y[3], h1, l1);
+            const hf4 hi = {h0.x, h0.y, h1.x, h1.y}, lo = {l0.x, l0.y, l1.x, l1.y};
+            const int at = l * 16 + 8 * (w & 1);
+            if constexpr (ST) {   // both column halves hold the row's weights: one keeps each plane
+                *(hf4 *)(pb[w >> 1][0] + at) = li < 8 ? hi : lo;
+            } else {
+                *(hf4 *)(pb[w >> 1][0] + at) = hi;
+                *(hf4 *)(pb[w >> 1][NP - 1] + at) = lo;
             }
         }
         lds_barrier();
-        {   // sums
+        // sums
+        const float al = alb[li];
+        if (__any(al != 1.f))
 #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                const float al = alb[c][li];
-                if (__any(al != 1.f))
+            for (int d = 0; d < NV; d++) o[d] *= al;
+        if (E4 && j0 + 63 > last) {
+            const u32x4 m = written(j0, last);
 #pragma unroll
-                    for (int d = 0; d < NV; d++) o[c][d] *= al;
+            for (int d = 0; d < NV; d++) vr[d] &= m;
+        }
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            hf8 p[NP];
+#pragma unroll
+            for (int x = 0; x < NP; x++) p[x] = *(const hf8 *)(pb[y][x] + l * 16);
+#pragma unroll
+            for (int d = 0; d < NV; d++) {
+                const hf8 v = to_half<E4>(vr[d][2 * y], vr[d][2 * y + 1]);
+#pragma unroll
+                for (int x = NP - 1; x >= 0; x--) o[d] = mfma16(v, p[x], o[d]);
             }
-            if (E4 && j0 + 63 > last) {
-                const u32x4 m = written(j0, last);
+        }
+        if (more) load_v(tile(i + 1));
+    }
+    // the rows' totals
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (l < 16) mx[w][l] = L;
+    lds_barrier();
+    if constexpr (ST)
 #pragma unroll
-                for (int d = 0; d < NV; d++) vr[d] &= m;
+        for (int d = 0; d < NV; d++) o[d] = f32x4{add_ror8(o[d].x), add_ror8(o[d].y), add_ror8(o[d].z), add_ror8(o[d].w)};
+    if (row >= rows || li >= R) return;
+    const float total = (mx[0][li] + mx[1][li]) + (mx[2][li] + mx[3][li]);
+    finish<NV>(a, g, row, sp, 16 * w * NV + 4 * kq, M, total, o);   // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
+}
+
+// Attention of more rows: 32 by four wavefronts, in a pipeline of three tiles with one barrier a tile: while tile i's scores
+// are formed, the weights of tile i - 1 and the sums of tile i - 2 are, all of it independent.
+//   scores, weights  16 rows (w >> 1) by 32 keys (w & 1): the rows' queries and the scores stay in registers, the two
+//                    wavefronts of the rows exchange their maxima and all of them the weights through LDS
+//   sums             a quarter of the dims for all rows
+// int8 keys are matrix operands as they are: the queries are 24-bit integers per row in three signed digits of 8 bits
+// (x = X 2^e, |X| <= 2^22), every product and sum is exact until the digits' sums are joined in fp32.
+// Bound by the two units of a SIMD, whose times add up here: of 64 rows' tile of 64 keys at D = 256 (3750 cycles) the products are
+// 1792 and the vector instructions (conversions, softmax, two planes) 1600. Measured the same with the operands of 64 rows shared
+// through LDS, with its two groups of wavefronts in opposite steps, and with vector instructions placed among the products.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <int D, bool E4>
+__global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) {
+    constexpr int NS = D / 64, NQ = E4 ? 2 * NS : NS, NP = E4 ? 2 : 3;
+    constexpr int CT = 2, NV = D / 64;   // columns; a wavefront's units of values
+    __shared__ __align__(16) uint8_t pb[2][CT][2][2][1024];   // weights [tile parity][columns][32 keys][plane][lane]
+    __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP, their log2 (and unused)
+    __shared__ float alb[2][CT][16], mx[2][CT][2][16], ms[CT][16];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
+    const int cw = w >> 1, u0 = 2 * (w & 1);
+    const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
+    const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - (int)blockIdx.x / a.c.Hkv) * 32;
+    const int p0 = np + r0 / G, p1 = np + min(r0 + 31, rows - 1) / G, last = np + a.T - 1;
+    const Tiles tl = tiles_of(p0, p1, a.window, a.sinks);
+    const int i0 = sp * a.per_split, nt = min(a.per_split, tl.n - i0);
+    if (nt <= 0) return;
+    const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + u0 * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
+    const float *scp = (w & 1 ? a.c.vs : a.c.ks) + (((int64_t)g * a.c.n_tiles * 64) >> a.c.lg);
+    u32x4 kr[2 * NS], vr[NV];
+    float s1;   // even wavefronts: the keys' scale of a tile's position l; odd: the values'
+    auto tile = [&](int i) { return i0 + i < tl.ns ? i0 + i : tl.f + i0 + i - tl.ns; };
+    auto load_k = [&](int i) { load_units<2 * NS>(kc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, kr); };
+    auto load_v = [&](int i) { load_units<NV>(vc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, vr); };
+    auto load_s = [&](int i) { s1 = scp[min(tile(min(i, nt - 1)) * 64 + l, last) >> a.c.lg]; };
+    auto put_s = [&](int i) {   // positions not written yet have no scale (every pair of wavefronts the same)
+        const float x = tile(min(i, nt - 1)) * 64 + l <= last ? s1 : 0.f;
+        sc[i & 3][w & 1][l] = w & 1 ? x * kP : x;
+        sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-100f));
+    };
+    load_s(0);
+    load_k(0);
+    load_v(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // the wavefront's queries as operands, an exponent per row; the two wavefronts of the rows prepare them both
+    const int rq = min(r0 + 16 * cw + li, rows - 1), tq = rq / G, pos = np + tq;
+    u32x4 q[NQ][NP];
+    float qsc;
+    {
+        const float *qp = a.q + tq * a.q_tok + (g * G + rq % G) * a.q_head + 16 * kq;
+        f32x4 x[4 * NS];
+        float m = 0.f;
+        bool fin = true;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; i++) {
+            x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
+#pragma unroll
+            for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[i][r])), fin &= fabsf(x[i][r]) < INFINITY;
+        }
+        m = max_x16(max_x32(m));
+        const uint64_t bad = ~__ballot(fin);   // a NaN or infinity, which integers do not hold, is put into the row's factor
+        fin = !((bad >> li | bad >> (li + 16) | bad >> (li + 32) | bad >> (li + 48)) & 1);
+        int e = 0;
+        if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
+        e = max(e, -100) - (E4 ? 14 : 22);
+        qsc = fin ? ldexpf(a.scale * 1.44269504088896341f, e) : NAN;   // what a product is multiplied with
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            if constexpr (E4) {
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    hf2 hi[4], lo[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        split2(ldexpf(x[4 * s + 2 * y + (r >> 1)][2 * (r & 1)], -e), ldexpf(x[4 * s + 2 * y + (r >> 1)][2 * (r & 1) + 1], -e), hi[r], lo[r]);
+                    const hf8 qh = join8(hi[0], hi[1], hi[2], hi[3]), ql = join8(lo[0], lo[1], lo[2], lo[3]);
+                    __builtin_memcpy(&q[2 * s + y][0], &qh, 16);
+                    __builtin_memcpy(&q[2 * s + y][1], &ql, 16);
+                }
+            } else {
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    uint32_t X[4];   // the bytes of X + 0x808080, each less 128, are its signed digits
+#pragma unroll
+                    for (int r = 0; r < 4; r++) X[r] = ((uint32_t)(int)rintf(ldexpf(x[4 * s + y][r], -e)) + 0x808080u) ^ 0x808080u;
+#pragma unroll
+                    for (int p = 0; p < 3; p++) {
+                        const uint32_t sel = (uint32_t)p | (uint32_t)(4 + p) << 8 | 0x0c0c0000u;
+                        q[s][p][y] = __builtin_amdgcn_perm(X[1], X[0], sel) | __builtin_amdgcn_perm(X[3], X[2], sel) << 16;
+                    }
+                }
             }
+        }
+    }
+    f32x4 o[CT][NV], s[2];   // sums; products of the tile before with its keys' scales
+    float qe = 1.f;           // what makes them powers of two
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                hf8 p[CT][NP];
+    for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f, mt = -INFINITY;
+    put_s(0);
+    load_s(1);
+    lds_barrier();
+
+    // steps of the pipeline: the scores of tile i (S), the weights of tile i - 1 (W), the sums of tile i - 2 (P)
+    for (int i = 0; i < nt + 2; i++) {
+        const bool S = i < nt, W = i >= 1 && i <= nt, P = i >= 2;
+        const int par = i & 1, pw = par ^ 1;   // tile i and i - 2; tile i - 1
+        hf8 pf[2][CT];   // weights of half y >> 1, plane 1 - (y & 1): two groups of columns ahead
+        auto get_p = [&](int y) {
+#pragma unroll
+            for (int c = 0; c < CT; c++) pf[y & 1][c] = *(const hf8 *)(pb[par][c][y >> 1][1 - (y & 1)] + l * 16);
+        };
+        if (P) {
+            float al[CT];
+#pragma unroll
+            for (int c = 0; c < CT; c++) al[c] = alb[par][c][li];
+            get_p(0);
+            get_p(1);
+            bool any = false;
+#pragma unroll
+            for (int c = 0; c < CT; c++) any |= al[c] != 1.f;
+            if (__any(any))
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
-                    for (int x = 0; x < NP; x++) p[c][x] = *(const hf8 *)(pb[c][h][x] + l * 16);
+                    for (int d = 0; d < NV; d++) o[c][d] *= al[c];
+            if (E4) {
+                const int j0 = tile(i - 2) * 64;
+                if (j0 + 63 > last) {
+                    const u32x4 m = written(j0, last);
 #pragma unroll
-                for (int d = 0; d < NV; d++) {
-                    const hf8 v = to_half<E4>(vr[d][2 * h], vr[d][2 * h + 1]);
-#pragma unroll
-                    for (int x = NP - 1; x >= 0; x--)
-#pragma unroll
-                        for (int c = 0; c < CT; c++) o[c][d] = mfma16(v, p[c][x], o[c][d]);
+                    for (int d = 0; d < NV; d++) vr[d] &= m;
                 }
             }
-            if (more) load_v(tile(i + 1));
         }
+        f32x4 y[2];
+        if (S) {
+            if constexpr (E4) {
+                f32x4 x[2][2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) x[u][0] = x[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < NQ; st++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const u32x4 &k4 = kr[u * NS + (st >> 1)];
+                        const hf8 k = to_half<E4>(k4[2 * (st & 1)], k4[2 * (st & 1) + 1]);
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            hf8 qq;
+                            __builtin_memcpy(&qq, &q[st][p], 16);
+                            x[u][p] = mfma16(k, qq, x[u][p]);
+                        }
+                    }
+#pragma unroll
+                for (int u = 0; u < 2; u++) y[u] = x[u][0] + x[u][1];
+            } else {
+                i32x4 x[2][3];
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int p = 0; p < 3; p++) x[u][p] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+#pragma unroll
+                    for (int p = 0; p < 3; p++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+                            x[u][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)kr[u * NS + st], (i32x4)q[st][p], x[u][p], 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < 2; u++)   // a digit's sum is below 2^23
+#pragma unroll
+                    for (int r = 0; r < 4; r++) y[u][r] = fmaf((float)x[u][2][r], 65536.f, (float)((x[u][1][r] << 8) + x[u][0][r]));
+            }
+            load_k(i + 1);
+        }
+        if (W) {
+            const float mm = fmaxf(mt, mx[pw][cw][1 - (w & 1)][li]);
+            // (the two wavefronts of the rows agree)
+            const float mn = mm > M + kGrow || M == -INFINITY ? fmaxf(M, mm) : M;
+            const float al = mn == M ? 1.f : __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= al;
+            alb[pw][cw][li] = al;
+            const float ref = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+            hf2 hi[4], lo[4];
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const f32x4 vs = *(const f32x4 *)&sc[(i - 1) & 3][1][16 * (u0 + v) + 4 * kq];
+                float z[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[v][r], qe, -ref));
+                    L += p;
+                    z[r] = p * vs[r];
+                }
+                split2(z[0], z[1], hi[2 * v], lo[2 * v]);
+                split2(z[2], z[3], hi[2 * v + 1], lo[2 * v + 1]);
+            }
+            *(hf8 *)(pb[pw][cw][w & 1][0] + l * 16) = join8(hi[0], hi[1], hi[2], hi[3]);
+            *(hf8 *)(pb[pw][cw][w & 1][1] + l * 16) = join8(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (S) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
+            const int j0 = tile(i) * 64;
+            qe = qsc;
+            if (tile_edge(a, j0, p0, p1)) {
+                qe = 1.f;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
+                        const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+                        s[u][r] = see ? s[u][r] * qsc : -INFINITY;
+                    }
+            }
+            mt = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
+#pragma unroll
+                for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
+            }
+            mt = max_x16(max_x32(mt));
+            mx[par][cw][w & 1][li] = mt;
+            put_s(i + 1);
+            load_s(i + 2);
+        }
+        if (P) {
+            hf8 v[NV];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                if (!(x & 1))
+#pragma unroll
+                    for (int d = 0; d < NV; d++) v[d] = to_half<E4>(vr[d][x], vr[d][x + 1]);
+#pragma unroll
+                for (int d = 0; d < NV; d++)
+#pragma unroll
+                    for (int c = 0; c < CT; c++) o[c][d] = mfma16(v[d], pf[x & 1][c], o[c][d]);
+                if (x < 2) get_p(x + 2);
+            }
+            load_v(i - 1);
+        }
+        lds_barrier();
     }
     // the rows' totals
     L += __shfl_xor(L, 16, 64);
     L += __shfl_xor(L, 32, 64);
     if (l < 16) {
-        mx[cw][CT == 4 ? 0 : w % (4 / CT)][l] = L;
+        mx[0][cw][w & 1][l] = L;
         if (u0 == 0) ms[cw][l] = M;
     }
     lds_barrier();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-        if constexpr (ST)
-#pragma unroll
-            for (int d = 0; d < NV; d++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) o[c][d][r] = add_ror8(o[c][d][r]);
-        const int row = r0 + 16 * c + li;
-        if (row >= rows || li >= R) continue;
-        float total = mx[c][0][li];
-#pragma unroll
-        for (int x = 1; x < 4 / CT; x++) total += mx[c][x][li];
-        const int d0 = 16 * w * NV + 4 * kq;   // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
-        if (a.n_split > 1) {
-            float *part = a.part + (((int64_t)g * rows + row) * a.n_split + sp) * (D + 4);
-            if (w == 0 && kq == 0) part[0] = ms[c][li], part[1] = total;
-#pragma unroll
-            for (int d = 0; d < NV; d++) *(f32x4 *)(part + 4 + d0 + 16 * d) = o[c][d];
-        } else {
-            const int h = g * G + row % G;
-            finish_row<NV>(a, row / G, h, h * D, d0, total, o[c]);
-        }
+        const int row = r0 + 16 * c + li;   // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
+        if (row < rows) finish<NV>(a, g, row, sp, 16 * w * NV + 4 * kq, ms[c][li], mx[0][c][0][li] + mx[0][c][1][li], o[c]);
     }
 }
 
@@ -691,11 +928,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
 
-// Rows of a work-group: up to 8 rows share every product between their planes (half the matrix instructions); as many as
-// there are, up to what the queries' registers allow (32 of 256 dims, 64 of fewer).
+// Rows of a work-group: up to 8 share every product between their planes (half the matrix instructions), up to 16 have the kernel
+// with the shorter way through one tile (one token at 4000 positions: 5.9 us, 13 in the other one).
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
-    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 || a.c.D == 256 ? 32 : 64;
+    return n <= 8 ? 8 : n <= 16 ? 16 : 32;
 }
 // Tiles that R rows see at most.
 static int most_tiles(const Kv8AttnArgs &a, int R) {
@@ -705,13 +942,14 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
-// Splits of the tiles while the work-groups do not exceed what the CUs hold.
+// Splits of the tiles. Up to 16 rows: three work-groups per CU, a tile each if there are no more (one token at 4000 positions in 16,
+// 32, 63 splits: 15.9, 14.7, 11.2 us; at 131000 in 64, 128, 256: 63, 55, 60). More rows: one per CU, two tiles each at least (333 tokens
+// with a window of 1024 in 2, 3, 6 splits: 28, 25, 26 us; 5 tokens with a window of 4096 in 16, 32, 65: 18, 15, 17).
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
-    int64_t n = (R >= 32 ? 512 : 768) / wgs;
-    if (n > tiles) n = tiles;
-    return n < 1 ? 1 : (int)n;
+    const int64_t n = (R == 32 ? 256 : 768) / wgs, most = R == 32 ? (tiles + 1) / 2 : tiles;
+    return n < 1 ? 1 : (int)(n < most ? n : most);
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
     const int n = splits_of(a);
@@ -720,13 +958,13 @@ int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
 
 template <int D, bool E4>
 static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
-    const int rows = a.T * (a.H / a.c.Hkv), nb = (rows + R - 1) / R;
-    const dim3 grid(nb * a.c.Hkv, a.n_split);
+    const int rows = a.T * (a.H / a.c.Hkv);
+    const dim3 grid((rows + R - 1) / R * a.c.Hkv, a.n_split);
     if (R == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 8>), grid, dim3(256), 0, st, a);
     else if (R == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
-    else if (R == 32) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 32>), grid, dim3(256), 0, st, a);
-    else if constexpr (D < 256) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 64>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), grid, dim3(256), 0, st, a);
     if (a.n_split == 1) return;
+    // eight wavefronts a row while the rows do not fill the GPU by themselves
     if (a.n_split <= 16 || rows * a.c.Hkv > 1024) hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((rows + 3) / 4, a.c.Hkv), dim3(256), 0, st, a, R);
     else hipLaunchKernelGGL((kv8_merge_kernel<D, 8>), dim3(rows, a.c.Hkv), dim3(512), 0, st, a, R);
 }
