@@ -5,6 +5,7 @@
 // turns are dropped exactly, and sine and cosine of the rest are taken in float:
 // an angle keeps 2^-24 of a turn at any position (a float product p f_i loses it at
 // once: 2^-8 of a radian at 100000).
+// Bound by the rows' bytes (4096 tokens of 16 heads of 256: 134 MB).
 #include "common.h"
 #include "kernels.h"
 
@@ -12,37 +13,62 @@ namespace xjk {
 
 // One work-group per token: the token's cosines and sines once in LDS, then every
 // head's pairs and, when the result goes elsewhere, the elements that do not turn.
+// V: elements per access, 4 where every run of them (a half of n_rot, n_rot, the
+// rest of the head) is a multiple of 4.
+template <int V>
 __global__ __launch_bounds__(256) void rope_scaled_kernel(const RopeArgs a) {
-    __shared__ float2 cs[kRopeMaxPairs];
+    typedef float vec __attribute__((ext_vector_type(V)));
+    typedef float vec_u __attribute__((ext_vector_type(V), aligned(4)));
+    __shared__ __align__(16) float cs[2][kRopeMaxPairs];
     const int t = blockIdx.x, tid = threadIdx.x, half = a.n_rot / 2;
     const double p = a.pos ? a.pos[t] : (double)a.pos0 + t;
     if (tid < half) {
         const double w = p * a.f[tid];
         float s, c;
         sincospif((float)(2.0 * (w - rint(w))), &s, &c);
-        cs[tid] = float2{c * a.mscale, s * a.mscale};
+        cs[0][tid] = c * a.mscale;
+        cs[1][tid] = s * a.mscale;
     }
     __syncthreads();
     const float *xt = a.x + t * a.x_tok;
     float *ot = a.out + t * a.o_tok;
-    for (int i = tid; i < a.n_heads * half; i += 256) {
-        const int h = i / half, j = i % half;
-        const int e0 = a.interleaved ? 2 * j : j, e1 = a.interleaved ? 2 * j + 1 : j + half;
-        const float u = xt[h * a.x_head + e0], v = xt[h * a.x_head + e1];
-        ot[h * a.o_head + e0] = u * cs[j].x - v * cs[j].y;
-        ot[h * a.o_head + e1] = u * cs[j].y + v * cs[j].x;
+    if (a.interleaved) {   // V pairs are 2 V elements
+        for (int i = tid; i < a.n_heads * (half / V); i += 256) {
+            const int h = i / (half / V), j = i % (half / V) * V;
+            const vec x0 = *(const vec_u *)(xt + h * a.x_head + 2 * j), x1 = *(const vec_u *)(xt + h * a.x_head + 2 * j + V);
+            vec y[2];
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                const float u = V == 1 ? x0[0] : k < V / 2 ? x0[2 * k % V] : x1[2 * k % V], v = V == 1 ? x1[0] : k < V / 2 ? x0[(2 * k + 1) % V] : x1[(2 * k + 1) % V];
+                const float c = cs[0][j + k], s = cs[1][j + k];
+                y[2 * k / V][2 * k % V] = u * c - v * s;
+                y[(2 * k + 1) / V][(2 * k + 1) % V] = u * s + v * c;
+            }
+            *(vec_u *)(ot + h * a.o_head + 2 * j) = y[0];
+            *(vec_u *)(ot + h * a.o_head + 2 * j + V) = y[1];
+        }
+    } else {
+        for (int i = tid; i < a.n_heads * (half / V); i += 256) {
+            const int h = i / (half / V), j = i % (half / V) * V;
+            const vec u = *(const vec_u *)(xt + h * a.x_head + j), v = *(const vec_u *)(xt + h * a.x_head + j + half);
+            const vec c = *(const vec *)&cs[0][j], s = *(const vec *)&cs[1][j];
+            *(vec_u *)(ot + h * a.o_head + j) = u * c - v * s;
+            *(vec_u *)(ot + h * a.o_head + j + half) = u * s + v * c;
+        }
     }
-    if (a.out == a.x) return;
-    const int rest = a.D - a.n_rot;
+    const int rest = (a.D - a.n_rot) / V;
+    if (a.out == a.x || !rest) return;
     for (int i = tid; i < a.n_heads * rest; i += 256) {
-        const int h = i / rest, j = a.n_rot + i % rest;
-        ot[h * a.o_head + j] = xt[h * a.x_head + j];
+        const int h = i / rest, j = a.n_rot + i % rest * V;
+        *(vec_u *)(ot + h * a.o_head + j) = *(const vec_u *)(xt + h * a.x_head + j);
     }
 }
 
 int rope_scaled_launch(const RopeArgs &a, hipStream_t st) {
     if (a.T < 1 || a.n_heads < 1 || a.n_rot < 2 || a.n_rot % 2 || a.n_rot / 2 > kRopeMaxPairs || a.n_rot > a.D) return -1;
-    hipLaunchKernelGGL(rope_scaled_kernel, dim3(a.T), dim3(256), 0, st, a);
+    const bool v4 = a.n_rot % 8 == 0 && (a.out == a.x || (a.D - a.n_rot) % 4 == 0);
+    if (v4) hipLaunchKernelGGL(rope_scaled_kernel<4>, dim3(a.T), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(rope_scaled_kernel<1>, dim3(a.T), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
