@@ -102,56 +102,55 @@ __device__ __forceinline__ float value_of(uint32_t c, float s) {
     else return (float)(int8_t)c * s;
 }
 
-// Store and load move a tile in groups of 16 positions by D / 4 lanes, a lane 4 dims, so that the float rows
-// (four times the codes' bytes) go 16 bytes per lane and whole rows per instruction. Group q of the
-// keys is the 16 positions of one unit row; of the values the positions 16 u + 4 q + r, whose codes of a dim
-// are 16 bytes.
+// Store and load move a tile in 8 groups of 8 positions by D / 4 lanes, a lane 4 dims, so that the float rows
+// (four times the codes' bytes) go 16 bytes per lane and whole rows per instruction. Group q of the keys is 8
+// positions in a row; of the values the positions 16 u + 4 (q / 2) + r with u / 2 = q % 2, whose codes of a dim are 8 bytes.
 template <bool VAL>
-__device__ __forceinline__ int group_pos(int q, int i) { return VAL ? 16 * (i >> 2) + 4 * q + (i & 3) : 16 * q + i; }
+__device__ __forceinline__ int group_pos(int q, int i) { return VAL ? 16 * (2 * (q & 1) + (i >> 2)) + 4 * (q >> 1) + (i & 3) : 8 * q + i; }
 
+// 4 x 4 bytes turned: byte c of w[r] becomes byte r of the result's c.
+__device__ __forceinline__ void turn4(const uint32_t (&w)[4], uint32_t (&v)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    v[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    v[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    v[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    v[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
 // The lane's codes: w[i] byte c = dim d0 + c of the group's position i.
 template <int D, bool VAL>
-__device__ __forceinline__ void get_codes(const uint8_t *tile, int q, int d0, uint32_t (&w)[16]) {
+__device__ __forceinline__ void get_codes(const uint8_t *tile, int q, int d0, uint32_t (&w)[8]) {
     if constexpr (VAL) {
-        const uint8_t *p = tile + (d0 >> 4) * 1024 + q * 256 + (d0 & 15) * 16;
-        u32x4 v[4];
+        const uint8_t *p = tile + (d0 >> 4) * 1024 + (q >> 1) * 256 + (d0 & 15) * 16 + 8 * (q & 1);
+        uint2 v[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) v[c] = *(const u32x4 *)(p + 16 * c);
+        for (int c = 0; c < 4; c++) v[c] = *(const uint2 *)(p + 16 * c);
+        const uint32_t x[4] = {v[0].x, v[1].x, v[2].x, v[3].x}, y[4] = {v[0].y, v[1].y, v[2].y, v[3].y};
+        uint32_t lo[4], hi[4];
+        turn4(x, lo);
+        turn4(y, hi);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {   // 4 dims x 4 positions turned
-            const uint32_t a = __builtin_amdgcn_perm(v[1][u], v[0][u], 0x05010400u), b = __builtin_amdgcn_perm(v[1][u], v[0][u], 0x07030602u);
-            const uint32_t c = __builtin_amdgcn_perm(v[3][u], v[2][u], 0x05010400u), d = __builtin_amdgcn_perm(v[3][u], v[2][u], 0x07030602u);
-            w[4 * u] = __builtin_amdgcn_perm(c, a, 0x05040100u);
-            w[4 * u + 1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
-            w[4 * u + 2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
-            w[4 * u + 3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
-        }
+        for (int r = 0; r < 4; r++) w[r] = lo[r], w[4 + r] = hi[r];
     } else {
-        const uint8_t *p = tile + q * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (d0 & 15);
+        const uint8_t *p = tile + (q >> 1) * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (q & 1) * 128 + (d0 & 15);
 #pragma unroll
-        for (int i = 0; i < 16; i++) w[i] = *(const uint32_t *)(p + 16 * i);
+        for (int i = 0; i < 8; i++) w[i] = *(const uint32_t *)(p + 16 * i);
     }
 }
 template <int D, bool VAL>
-__device__ __forceinline__ void put_codes(uint8_t *tile, int q, int d0, const uint32_t (&w)[16]) {
+__device__ __forceinline__ void put_codes(uint8_t *tile, int q, int d0, const uint32_t (&w)[8]) {
     if constexpr (VAL) {
-        uint8_t *p = tile + (d0 >> 4) * 1024 + q * 256 + (d0 & 15) * 16;
-        u32x4 v[4];
+        uint8_t *p = tile + (d0 >> 4) * 1024 + (q >> 1) * 256 + (d0 & 15) * 16 + 8 * (q & 1);
+        const uint32_t x[4] = {w[0], w[1], w[2], w[3]}, y[4] = {w[4], w[5], w[6], w[7]};
+        uint32_t lo[4], hi[4];
+        turn4(x, lo);
+        turn4(y, hi);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const uint32_t a = __builtin_amdgcn_perm(w[4 * u + 1], w[4 * u], 0x05010400u), b = __builtin_amdgcn_perm(w[4 * u + 1], w[4 * u], 0x07030602u);
-            const uint32_t c = __builtin_amdgcn_perm(w[4 * u + 3], w[4 * u + 2], 0x05010400u), d = __builtin_amdgcn_perm(w[4 * u + 3], w[4 * u + 2], 0x07030602u);
-            v[0][u] = __builtin_amdgcn_perm(c, a, 0x05040100u);
-            v[1][u] = __builtin_amdgcn_perm(c, a, 0x07060302u);
-            v[2][u] = __builtin_amdgcn_perm(d, b, 0x05040100u);
-            v[3][u] = __builtin_amdgcn_perm(d, b, 0x07060302u);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) *(u32x4 *)(p + 16 * c) = v[c];
+        for (int c = 0; c < 4; c++) *(uint2 *)(p + 16 * c) = uint2{lo[c], hi[c]};
     } else {
-        uint8_t *p = tile + q * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (d0 & 15);
+        uint8_t *p = tile + (q >> 1) * (16 * D) + (d0 >> 6) * 1024 + ((d0 >> 4) & 3) * 256 + (q & 1) * 128 + (d0 & 15);
 #pragma unroll
-        for (int i = 0; i < 16; i++) *(uint32_t *)(p + 16 * i) = w[i];
+        for (int i = 0; i < 8; i++) *(uint32_t *)(p + 16 * i) = w[i];
     }
 }
 // The larger of a lane's value and that of lane l ^ 16, l ^ 32.
@@ -172,7 +171,7 @@ __device__ __forceinline__ float row_max(float v) {
     return v;
 }
 
-// A work-group stores one tile of a kv head's keys or values (D threads, a group each D / 4): the
+// A work-group stores one tile of a kv head's keys or values (2 D threads, a group each D / 4): the
 // rows' largest magnitudes, joined over every block in LDS, the scales, the codes. In a
 // tile that is not new from end to end the codes of the other positions are read
 // and written back as they are, those of a begun block at its new scale if that grew.
@@ -186,18 +185,18 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
     uint8_t *tile = (VAL ? a.c.v : a.c.k) + ((int64_t)g * a.c.n_tiles + kt) * 64 * D;
     float *sp = (VAL ? a.c.vs : a.c.ks) + ((((int64_t)g * a.c.n_tiles + kt) * 64) >> a.c.lg);
     const bool whole = j0 >= np && j0 + 64 <= end;
-    uint32_t w[16];
+    uint32_t w[8];
     const float old_s = !whole && tid < 64 ? sp[tid >> a.c.lg] : 0.f;
     if (!whole) get_codes<D, VAL>(tile, q, d0, w);
-    f32x4 y[16];
+    f32x4 y[8];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < 8; i++) {
         const int p = j0 + group_pos<VAL>(q, i);
         y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (p >= np && p < end) y[i] = *(const f32x4_u *)(x + (int64_t)(p - np) * tok);
     }
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < 8; i++) {
         const int pl = group_pos<VAL>(q, i), p = j0 + pl;
         float m = 0.f;
         if (whole || (p >= np && p < end))   // (uniform among the row's lanes)
@@ -220,7 +219,7 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < 8; i++) {
         const int pl = group_pos<VAL>(q, i), p = j0 + pl;
         const float s = sm[0][pl], inv = s > 0.f ? 1.f / s : 0.f;
         if (whole || (p >= np && p < end)) {
@@ -235,34 +234,39 @@ __device__ __forceinline__ void store_tile(const Kv8StoreArgs &a, float (*sm)[64
     put_codes<D, VAL>(tile, q, d0, w);
 }
 template <int D, bool E4>
-__global__ __launch_bounds__(D) void kv8_store_kernel(const Kv8StoreArgs a) {
+__global__ __launch_bounds__(2 * D) void kv8_store_kernel(const Kv8StoreArgs a) {
     __shared__ float sm[2][64];
     if (blockIdx.z) store_tile<D, E4, true>(a, sm);
     else store_tile<D, E4, false>(a, sm);
 }
 
-template <int D, bool E4, bool VAL>
+// Read back, Y groups a thread.
+template <int D, bool E4, bool VAL, int Y>
 __device__ __forceinline__ void load_tile(const Kv8LoadArgs &a) {
-    const int g = blockIdx.y, tid = threadIdx.x, q = tid / (D / 4), d0 = tid % (D / 4) * 4;
+    const int g = blockIdx.y, tid = threadIdx.x, q = Y * (tid / (D / 4)), d0 = tid % (D / 4) * 4;
     const int kt = (a.pos0 >> 6) + blockIdx.x, j0 = kt * 64;
     const float *sp = (VAL ? a.c.vs : a.c.ks) + ((((int64_t)g * a.c.n_tiles + kt) * 64) >> a.c.lg);
-    uint32_t w[16];
-    get_codes<D, VAL>((VAL ? a.c.v : a.c.k) + ((int64_t)g * a.c.n_tiles + kt) * 64 * D, q, d0, w);
-    float *y = (VAL ? a.v : a.k) + g * D + d0;
+    const uint8_t *tile = (VAL ? a.c.v : a.c.k) + ((int64_t)g * a.c.n_tiles + kt) * 64 * D;
+    uint32_t w[Y][8];
+#pragma unroll
+    for (int y = 0; y < Y; y++) get_codes<D, VAL>(tile, q + y, d0, w[y]);
+    float *out = (VAL ? a.v : a.k) + g * D + d0;
     const int64_t tok = VAL ? a.v_tok : a.k_tok;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int pl = group_pos<VAL>(q, i), t = j0 + pl - a.pos0;
-        if (t < 0 || t >= a.n) continue;
-        const float s = sp[pl >> a.c.lg];
-        *(f32x4_u *)(y + t * tok) = f32x4{value_of<E4>(w[i] & 0xFFu, s), value_of<E4>(w[i] >> 8 & 0xFFu, s), value_of<E4>(w[i] >> 16 & 0xFFu, s),
-                                          value_of<E4>(w[i] >> 24, s)};
-    }
+    for (int y = 0; y < Y; y++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int pl = group_pos<VAL>(q + y, i), t = j0 + pl - a.pos0;
+            if (t < 0 || t >= a.n) continue;
+            const float s = sp[pl >> a.c.lg];
+            *(f32x4_u *)(out + t * tok) = f32x4{value_of<E4>(w[y][i] & 0xFFu, s), value_of<E4>(w[y][i] >> 8 & 0xFFu, s),
+                                                value_of<E4>(w[y][i] >> 16 & 0xFFu, s), value_of<E4>(w[y][i] >> 24, s)};
+        }
 }
-template <int D, bool E4>
-__global__ __launch_bounds__(D) void kv8_load_kernel(const Kv8LoadArgs a) {
-    if (a.k && !(a.v && blockIdx.z)) load_tile<D, E4, false>(a);
-    else load_tile<D, E4, true>(a);
+template <int D, bool E4, int Y>
+__global__ __launch_bounds__(2 * D / Y) void kv8_load_kernel(const Kv8LoadArgs a) {
+    if (a.k && !(a.v && blockIdx.z)) load_tile<D, E4, false, Y>(a);
+    else load_tile<D, E4, true, Y>(a);
 }
 
 // ------------------------------------------------------------- attention --
@@ -989,8 +993,8 @@ int kv8_attn_launch(const Kv8AttnArgs &in, int64_t part_floats, hipStream_t st) 
 template <int D>
 static void store_launch_d(const Kv8StoreArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)a.T + 62) >> 6) + 1, a.c.Hkv, 2);   // tiles of T rows from any position
-    if (a.c.e4m3) hipLaunchKernelGGL((kv8_store_kernel<D, true>), grid, dim3(D), 0, st, a);
-    else hipLaunchKernelGGL((kv8_store_kernel<D, false>), grid, dim3(D), 0, st, a);
+    if (a.c.e4m3) hipLaunchKernelGGL((kv8_store_kernel<D, true>), grid, dim3(2 * D), 0, st, a);
+    else hipLaunchKernelGGL((kv8_store_kernel<D, false>), grid, dim3(2 * D), 0, st, a);
 }
 int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st) {
     switch (a.c.D) {
@@ -1002,17 +1006,19 @@ int kv8_store_launch(const Kv8StoreArgs &a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-template <int D>
+// Two groups a thread (16 bytes of a dim's values) where the work-groups take turns on the CUs: 32000 positions of 4 heads of 256
+// 65 us, 69 with one; one where all are there at once: 77 positions of one head of 128 3.1 us, 3.9 with two, 2100 of 4 of 256 6.0 and 7.0.
+template <int D, bool E4>
 static void load_launch_d(const Kv8LoadArgs &a, hipStream_t st) {
     const dim3 grid(((a.pos0 + a.n - 1) >> 6) - (a.pos0 >> 6) + 1, a.c.Hkv, a.k && a.v ? 2 : 1);
-    if (a.c.e4m3) hipLaunchKernelGGL((kv8_load_kernel<D, true>), grid, dim3(D), 0, st, a);
-    else hipLaunchKernelGGL((kv8_load_kernel<D, false>), grid, dim3(D), 0, st, a);
+    if ((int64_t)grid.x * grid.y * grid.z > 1024) hipLaunchKernelGGL((kv8_load_kernel<D, E4, 2>), grid, dim3(D), 0, st, a);
+    else hipLaunchKernelGGL((kv8_load_kernel<D, E4, 1>), grid, dim3(2 * D), 0, st, a);
 }
 int kv8_load_launch(const Kv8LoadArgs &a, hipStream_t st) {
     switch (a.c.D) {
-    case 64: load_launch_d<64>(a, st); break;
-    case 128: load_launch_d<128>(a, st); break;
-    case 256: load_launch_d<256>(a, st); break;
+    case 64: a.c.e4m3 ? load_launch_d<64, true>(a, st) : load_launch_d<64, false>(a, st); break;
+    case 128: a.c.e4m3 ? load_launch_d<128, true>(a, st) : load_launch_d<128, false>(a, st); break;
+    case 256: a.c.e4m3 ? load_launch_d<256, true>(a, st) : load_launch_d<256, false>(a, st); break;
     default: return -1;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
