@@ -437,6 +437,9 @@ int xjh_delta_chunked(int H, int S, int T, int chunk, const float *q, const floa
  * buffers belong to the current device, need no alignment beyond their type's
  * (the cache and the work area: 16 bytes) and are complete when the stream
  * reaches the call. Strides are in elements. T = 0 does nothing.
+ * (The other per-op entries run on the library's own stream, which does not wait
+ * for any other: xjh_sync before one that reads what these wrote.) Outputs do not
+ * overlap inputs unless stated.
  * Where a call takes n_past_dev (may be NULL), the tokens' position is read
  * there on the GPU instead of n_past, which then is an upper bound for it, so
  * that one captured graph serves every step; a value outside [0, n_past] counts

@@ -557,3 +557,222 @@ def test_run_together_against_the_fp16_attention():
             rel = np.linalg.norm(got - want) / np.linalg.norm(want)
             assert rel < 0.03 if key[0] == I8 else rel < 0.08, (key, n, T, rel)
         n += T
+
+
+# ------------------------------------------- streams, graphs, sizes, positions --
+
+def _call(name, *args):
+    err = C.create_string_buffer(xp.ERR)
+    assert getattr(xp.lib(), name)(*args, err, xp.ERR) == 0, err.value
+
+
+class Hip:
+    """Streams and graphs of the HIP runtime that the library has loaded."""
+
+    def __init__(self):
+        xp.lib()
+        with open("/proc/self/maps") as f:
+            path = next(line.split()[-1] for line in f if "libamdhip64" in line)
+        self.rt = C.CDLL(path)
+
+    def __call__(self, name, *args):
+        assert getattr(self.rt, name)(*args) == 0, name
+
+    def stream(self):
+        st = C.c_void_p()
+        self("hipStreamCreate", C.byref(st))
+        return st
+
+    def capture(self, st, work):
+        graph, run = C.c_void_p(), C.c_void_p()
+        self("hipStreamBeginCapture", st, C.c_int(0))
+        work(st)
+        self("hipStreamEndCapture", st, C.byref(graph))
+        self("hipGraphInstantiate", C.byref(run), graph, None, None, C.c_size_t(0))
+        return run
+
+    def sync(self):
+        self("hipDeviceSynchronize")
+
+
+class _Step:
+    """One layer step of T tokens on a stream, position and buffers on the device: rope of queries and keys, store, attention."""
+
+    def __init__(self, Hkv, G, D, n_ctx, block, kind, T, n_max, window=0, n_sink=0):
+        self.H, self.T, self.n_max, self.window, self.n_sink = Hkv * G, T, n_max, window, n_sink
+        self.cache = xp.Kv8(Hkv, D, n_ctx, block, kind)
+        self.cache.put_bytes(np.full(self.cache.c.bytes, 0xFF, np.uint8))
+        self.q, self.qr, self.k, self.kr, self.v, self.out = (xp.Dev(nbytes=T * h * D * 4) for h in (self.H, self.H, Hkv, Hkv, Hkv, self.H))
+        self.pos, self.n_past = xp.Dev(nbytes=4 * T), xp.Dev(nbytes=4)
+        self.cfg = xp.XjhRopeCfg(pairs=0, n_rot=D // 2, base=1e5, **YARN)
+        self.wb = xp.lib().xjh_attn_kv8_work_bytes(C.byref(self.cache.c), T, self.H, n_max, window, n_sink)
+        self.work = xp.Dev(nbytes=max(self.wb, 16))
+
+    def run(self, st):
+        c = self.cache.c
+        cc, D, T, H, row = C.byref(c), c.D, self.T, self.H, c.Hkv * c.D
+        for x, y, h in ((self.q, self.qr, H), (self.k, self.kr, c.Hkv)):
+            _call("xjh_rope_scaled", x.ptr, h * D, D, y.ptr, h * D, D, T, h, D, C.byref(self.cfg), self.pos.ptr, 0, st)
+        _call("xjh_kv8_store", cc, self.kr.ptr, row, self.v.ptr, row, T, self.n_max, self.n_past.ptr, st)
+        _call("xjh_attn_kv8", cc, self.qr.ptr, H * D, D, None, 0, 0, T, H, self.n_max, self.n_past.ptr, self.window, self.n_sink, D ** -0.5,
+              self.out.ptr, H * D, self.work.ptr, self.wb, st)
+
+    def feed(self, q, k, v, n):
+        for d, a in ((self.q, q), (self.k, k), (self.v, v)):
+            d.put(a)
+        self.n_past.put(np.array([n], np.int32))
+        self.pos.put(np.arange(n, n + self.T, dtype=np.int32))
+
+    def result(self, d=None):
+        return (d or self.out).get(np.float32, (self.T, self.H, self.cache.c.D))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hkv,G,D,T,window,n_sink", [(2, 4, 256, 1, 0, 0), (1, 2, 128, 5, 100, 3), (2, 1, 64, 40, 0, 0)])
+def test_captured_steps_replay_at_every_position(Hkv, G, D, T, window, n_sink):
+    """The four calls captured once, with the position read on the device, and replayed over a sequence with eager work and
+    synchronisations between; two graphs with a cache and a work area each, on two streams at once. Every replay equals
+    the eager calls bit for bit and, at the end, the float64 form."""
+    rng = np.random.default_rng(D)
+    hip, steps = Hip(), 9
+    n_ctx = T * steps + 3
+    graphs = [_Step(Hkv, G, D, n_ctx, 16, kind, T, n_ctx - T, window, n_sink) for kind in (I8, E4)]
+    eager = [_Step(Hkv, G, D, n_ctx, 16, kind, T, n_ctx - T, window, n_sink) for kind in (I8, E4)]
+    streams = [hip.stream() for _ in graphs]
+    captured = [hip.capture(st, s.run) for s, st in zip(graphs, streams)]
+    for n in range(0, T * steps, T):
+        q, k, v = rng.standard_normal((T, Hkv * G, D)).astype(np.float32), rows(rng, T, Hkv, D), rows(rng, T, Hkv, D)
+        for s in graphs + eager:
+            s.feed(q, k, v, n)
+        for g, st in zip(captured, streams):
+            hip("hipGraphLaunch", g, st)
+        for s in eager:
+            s.run(None)
+        hip.sync()
+        for s, e in zip(graphs, eager):
+            assert np.array_equal(s.result().view(np.uint32), e.result().view(np.uint32)), n
+            assert np.array_equal(s.cache.bytes(), e.cache.bytes()), n
+    for e in eager:
+        kv = np.stack(e.cache.load(0, T * steps))
+        _check_attn(e.result(), *attend64(kv, e.result(e.qr), T * (steps - 1), window=window, n_sink=n_sink))
+    for g in captured:
+        hip("hipGraphExecDestroy", g)
+    for st in streams:
+        hip("hipStreamDestroy", st)
+
+
+@pytest.mark.gpu
+def test_device_positions_outside_the_range_count_as_its_ends():
+    rng = np.random.default_rng(20)
+    hip = Hip()
+    for given, meant in ((-5, 0), (1000, 37), (-(1 << 31), 0), ((1 << 31) - 1, 37), (20, 20)):
+        a, b = (_Step(1, 2, 64, 40, 8, I8, 3, 37) for _ in range(2))
+        x = [rng.standard_normal((37, 1, 64)).astype(np.float32) for _ in range(2)]
+        q, k, v = (rng.standard_normal((3, h, 64)).astype(np.float32) for h in (2, 1, 1))
+        for s, n in ((a, given), (b, meant)):
+            s.cache.store(x[0], x[1], 0)
+            s.feed(q, k, v, 0)
+            s.n_past.put(np.array([n], np.int32))
+            s.run(None)
+        hip.sync()
+        assert np.array_equal(a.result(), b.result()) and np.array_equal(a.cache.bytes(), b.cache.bytes()) and np.all(np.isfinite(a.result()))
+
+
+@pytest.mark.gpu
+def test_calls_follow_their_stream():
+    """Work enqueued before on the caller's stream is done when the calls run: inputs that a side stream copies in behind
+    half a gigabyte of other copies."""
+    rng = np.random.default_rng(21)
+    hip = Hip()
+    s, e = (_Step(2, 2, 128, 300, 32, I8, 4, 200) for _ in range(2))
+    x, q, k, v = (rng.standard_normal(n).astype(np.float32) for n in ((200, 2, 128), (4, 4, 128), (4, 2, 128), (4, 2, 128)))
+    for step in (s, e):
+        step.cache.store(x, x, 0)
+    e.feed(q, k, v, 200)
+    e.run(None)
+    s.feed(q * 0, k * 0, v * 0, 200)
+    src, big = [xp.Dev(y) for y in (q, k, v)], [xp.Dev(nbytes=1 << 26) for _ in range(2)]
+    st = hip.stream()
+    hip.sync()
+    for _ in range(8):
+        hip("hipMemcpyAsync", C.c_void_p(big[0].ptr), C.c_void_p(big[1].ptr), C.c_size_t(1 << 26), C.c_int(3), st)
+    for d, y in zip((s.q, s.k, s.v), src):
+        hip("hipMemcpyAsync", C.c_void_p(d.ptr), C.c_void_p(y.ptr), C.c_size_t(y.nbytes), C.c_int(3), st)
+    s.run(st)
+    hip.sync()
+    hip("hipStreamDestroy", st)
+    assert np.array_equal(s.result().view(np.uint32), e.result().view(np.uint32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_cache_beyond_four_gigabytes(kind):
+    """Eight heads of 256 over 2 million positions: codes past 2^32 bytes. A window's rows far into it."""
+    rng = np.random.default_rng(22)
+    Hkv, D, n_ctx, W = 8, 256, 1 << 21, 150
+    c = xp.XjhKv8(type=kind, Hkv=Hkv, D=D, n_ctx=n_ctx, block=64)
+    c.bytes = xp.lib().xjh_kv8_bytes(C.byref(c))
+    assert c.bytes > 1 << 33
+    buf = xp.Dev(nbytes=c.bytes)
+    c.data = buf.ptr
+    n, n0, T = 300, n_ctx - 300, 3
+    k, v, q = rows(rng, n, Hkv, D), rows(rng, n, Hkv, D), rng.standard_normal((T, 16, D)).astype(np.float32)
+    dk, dv, dq = xp.Dev(k), xp.Dev(v), xp.Dev(q)
+    ok, ov, out = xp.Dev(nbytes=k.nbytes), xp.Dev(nbytes=k.nbytes), xp.Dev(nbytes=q.nbytes)
+    row, cc = Hkv * D, C.byref(c)
+    wb = xp.lib().xjh_attn_kv8_work_bytes(cc, T, 16, n_ctx - T, W, 0)
+    work = xp.Dev(nbytes=max(wb, 16))
+    _call("xjh_kv8_store", cc, dk.ptr, row, dv.ptr, row, n, n0, None, None)
+    _call("xjh_kv8_load", cc, n0, n, ok.ptr, row, ov.ptr, row, None)
+    _call("xjh_attn_kv8", cc, dq.ptr, 16 * D, D, None, 0, 0, T, 16, n_ctx - T, None, W, 0, D ** -0.5, out.ptr, 16 * D, work.ptr, wb, None)
+    xp.lib().xjh_sync()
+    shift = n0 % 64   # the same blocks at the start of a small cache
+    ref = Ref(Hkv, D, n + 64, 64, kind)
+    ref.store(k, v, shift)
+    want = ref.values(shift, n).astype(np.float32)
+    assert np.array_equal(ok.get(np.float32, k.shape), want[0]) and np.array_equal(ov.get(np.float32, k.shape), want[1])
+    _check_attn(out.get(np.float32, q.shape), *attend64(want, q, n - T, window=W))
+    buf.free()
+
+
+@pytest.mark.gpu
+def test_many_heads_and_many_rows():
+    """64 kv heads (loads of more work-groups than are on the GPU at once), and a chunk of 80000 query rows checked at some."""
+    rng = np.random.default_rng(23)
+    cache, ref = xp.Kv8(64, 64, 700, 32, E4), Ref(64, 64, 700, 32, E4)
+    k, v = rows(rng, 690, 64, 64), rows(rng, 690, 64, 64)
+    cache.store(k, v, 3)
+    ref.store(k, v, 3)
+    want = ref.values(3, 690)
+    gk, gv = cache.load(3, 690)
+    assert np.array_equal(gk, want[0].astype(np.float32)) and np.array_equal(gv, want[1].astype(np.float32))
+    T, H = 5000, 16
+    cache, kv = _filled(rng, 2, 64, T, 64, I8)
+    q = rng.standard_normal((T, H, 64)).astype(np.float32)
+    got = cache.attend(q, 0).reshape(T, H, 64)
+    assert np.all(np.isfinite(got))
+    for t in (0, 1, 63, 64, 2500, 4999):
+        _check_attn(got[t:t + 1], *attend64(kv[:, :t + 1], q[t:t + 1], t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n_past", [(1, 3000), (3, 3000), (40, 3000), (300, 0)])
+def test_the_same_call_gives_the_same_bits(T, n_past):
+    rng = np.random.default_rng(24)
+    cache, _ = _filled(rng, 4, 128, n_past + T, 32, I8)
+    q = rng.standard_normal((T, 8, 128)).astype(np.float32)
+    a = cache.attend(q, n_past)
+    for _ in range(3):
+        assert np.array_equal(a.view(np.uint32), cache.attend(q, n_past).view(np.uint32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_attention_scales_of_any_sign(scale):
+    rng = np.random.default_rng(25)
+    for T, n_past in ((1, 200), (60, 70)):
+        for kind in (I8, E4):
+            cache, kv = _filled(rng, 1, 64, n_past + T, 32, kind)
+            q = rng.standard_normal((T, 2, 64)).astype(np.float32)
+            _check_attn(cache.attend(q, n_past, scale=scale, window=90, n_sink=2),
+                        *attend64(kv, q, n_past, scale=scale, window=90, n_sink=2))
