@@ -883,22 +883,27 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     const int ns = (tl.n + a.per_split - 1) / a.per_split;
     const float *part = a.part + ((int64_t)g * rows + rr) * a.n_split * (D + 4);
     const int t = rr / G, h = g * G + rr % G;
-    float M = -INFINITY;
-    for (int s = l; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
-    M = xjd::wave_max(M);
-    vec y = 0.f;
-    float L = 0.f;
     constexpr int U = 8;
-    for (int s = w; s < ns; s += U * W) {
-        vec v[U];
-        float m[U], c[U];
+    vec v[U];
+    float m[U], c[U];
+    auto load = [&](int s) {   // (past the end: the last one again, with weight 0)
 #pragma unroll
-        for (int i = 0; i < U; i++) {   // (past the end: the last one again, with weight 0)
+        for (int i = 0; i < U; i++) {
             const float *p = part + (int64_t)min(s + i * W, ns - 1) * (D + 4);
             m[i] = p[0];
             c[i] = p[1];
             __builtin_memcpy(&v[i], p + 4 + V * l, sizeof(vec));
         }
+    };
+    float M = -INFINITY;
+    if (l < ns) M = part[(int64_t)l * (D + 4)];
+    load(w);   // with the maxima
+    for (int s = l + 64; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
+    M = xjd::wave_max(M);
+    vec y = 0.f;
+    float L = 0.f;
+    for (int s = w; s < ns; s += U * W) {
+        if (s > w) load(s);
 #pragma unroll
         for (int i = 0; i < U; i++) {
             const float f = s + i * W >= ns || m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
