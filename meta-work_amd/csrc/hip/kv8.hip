@@ -11,6 +11,7 @@
 // which are the weights that it multiplies with those values.
 #include "common.h"
 #include "kernels.h"
+#include <algorithm>
 
 namespace xjk {
 
@@ -951,14 +952,21 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
-// Splits of the tiles. Up to 16 rows: three work-groups per CU, a tile each if there are no more (one token at 4000 positions in 16,
-// 32, 63 splits: 15.9, 14.7, 11.2 us; at 131000 in 64, 128, 256: 63, 55, 60). More rows: one per CU, two tiles each at least (333 tokens
-// with a window of 1024 in 2, 3, 6 splits: 28, 25, 26 us; 5 tokens with a window of 4096 in 16, 32, 65: 18, 15, 17).
+// Splits of the tiles. The registers let a CU hold two work-groups, and two hide each other's waits: splits for 512 where every one
+// has its tiles. Up to 16 rows a tile is enough, but the merge reads every split, so 256 at most (microseconds with 16 heads, 4 of keys,
+// 256 dims, int8, for 256, 384, 512 and 768 work-groups: one token at 131000 positions 70, 60, 56, 57, four 77, 66, 58, 67; at 4000 in 16,
+// 32, 63 splits 15.9, 14.7, 11.2; one token of 16 heads on one at 32000 in 128, 256, 512 splits 16.5, 16.8, 22). With more rows the
+// second work-group of a CU has to come with eight tiles a split (for 256 and 512: 8 tokens at 131000 78 and 68, 32 at 32000 58 and 50,
+// 512 at 32000 684 and 515, but 512 tokens of an empty cache, 9 tiles, 20 and 27) and the first with two (333 tokens with a window
+// of 1024 in 2, 3, 6 splits: 28, 25, 26). From 257 to 341 work-groups thirds in two turns beat wholes in one, which leave every
+// other CU one work-group alone (600 tokens at 32000 636 and 912); from there on nothing is split.
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
-    const int64_t n = (R == 32 ? 256 : 768) / wgs, most = R == 32 ? (tiles + 1) / 2 : tiles;
-    return n < 1 ? 1 : (int)(n < most ? n : most);
+    int64_t n;
+    if (R < 32) n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
+    else n = std::max(std::min<int64_t>(256 / wgs, (tiles + 1) / 2), std::min<int64_t>((wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs, tiles / 8));
+    return n < 1 ? 1 : (int)n;
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
     const int n = splits_of(a);
