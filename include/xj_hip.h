@@ -504,8 +504,10 @@ uint64_t xjh_kv8_bytes(const xjh_kv8 *c);
 /* Quantise the rows k, v [T][Hkv*D] (token strides k_tok, v_tok) into positions
  * n_past .. n_past+T-1. A block that positions before n_past began keeps the
  * larger of its scale and the new rows'; where that grew, its older codes are
- * rounded again to it. Blocks written from their first position start anew. No
- * other byte is touched. n_past_dev: see above. */
+ * rounded again to it; if those were never stored, clear the memory first. Blocks
+ * written from their first position start anew. Every
+ * other byte keeps its value, but tiles of 64 positions are rewritten whole: what
+ * stores into a tile or reads it is ordered with this call. n_past_dev: see above. */
 int xjh_kv8_store(const xjh_kv8 *c, const float *k, int64_t k_tok, const float *v, int64_t v_tok, int T, int n_past,
                   const int32_t *n_past_dev, void *stream, char *err, size_t errlen);
 /* Read positions pos0 .. pos0+n-1 back: k, v [n][Hkv*D] (token strides k_tok, v_tok); either may be NULL. */
@@ -521,8 +523,9 @@ int xjh_kv8_load(const xjh_kv8 *c, int pos0, int n, float *k, int64_t k_tok, flo
  * work: xjh_attn_kv8_work_bytes bytes, for splitting the positions over the
  * GPU; a smaller area (or NULL) splits less. It holds nothing between calls, but
  * calls that may run at the same time (other streams, other graphs) need one each.
- * Positions that no row sees are not read beyond their tile of 64, whatever they
- * hold. A query that is not finite leaves its own row not finite and no other. */
+ * Positions that no token sees need not be stored: what they hold, tiles that no
+ * token sees even a position of unread, counts for nothing. A query that is not
+ * finite leaves its own row not finite and no other. T * H is at most 2^28. */
 int xjh_attn_kv8(const xjh_kv8 *c, const float *q, int64_t q_tok, int64_t q_head, const float *gate, int64_t g_tok,
                  int64_t g_head, int T, int H, int n_past, const int32_t *n_past_dev, int window, int n_sink, float scale,
                  float *out, int64_t o_tok, void *work, size_t work_bytes, void *stream, char *err, size_t errlen);

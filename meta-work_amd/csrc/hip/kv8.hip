@@ -347,15 +347,20 @@ __device__ __forceinline__ float add_ror8(float v) {
 __device__ __forceinline__ bool tile_edge(const Kv8AttnArgs &a, int j0, int p0, int p1) {
     return j0 + 63 > p0 || (a.window && j0 <= p1 - a.window && j0 + 63 >= a.sinks);
 }
-// The lane's bytes of a values unit at j0 that positions after `last` do not hold: an e4m3 code not written yet may be a NaN,
-// which a weight of 0 does not take out.
-__device__ __forceinline__ u32x4 written(int j0, int last) {
+// Positions j that no row of the work-group sees may never have been stored: they have no scale, and where their e4m3 codes
+// are NaN a weight of 0 does not take them out. Those after `last`, the call's last token, and from `sinks` up to `lo`, where
+// the first row's window begins (0 without).
+__device__ __forceinline__ bool held(int j, int sinks, int lo, int last) { return j <= last && (j >= lo || j < sinks); }
+// Not every position of the tile at j0 is held; the lane's bytes of one of its values units that are.
+__device__ __forceinline__ bool tile_part(int j0, int sinks, int lo, int last) { return j0 + 63 > last || (j0 < lo && j0 + 63 >= sinks); }
+__device__ __forceinline__ u32x4 held_bytes(int j0, int sinks, int lo, int last) {
     const int kq = (threadIdx.x & 63) >> 4;
     u32x4 m;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-        const int n = last + 1 - (j0 + 16 * u + 4 * kq);
-        m[u] = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        m[u] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) m[u] |= held(j0 + 16 * u + 4 * kq + r, sinks, lo, last) ? 0xFFu << (8 * r) : 0u;
     }
     return m;
 }
@@ -410,8 +415,9 @@ __device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int
 //   scores   16 keys each: K units from the cache to registers, the queries stay in registers
 //   weights  a quarter of the (row, key) pairs each: scores and weights pass through LDS (a few KB a tile)
 //   sums     a quarter of the dims each
-// A wavefront's part of the next tile (8 KB at D = 256) is always in flight, three or four work-groups share a CU: a long
-// cache streams (one token at 131000 positions of the 4B shape: 268 MB in 49.4 us, 5.4 TB/s; a 1 GiB copy reaches 5.15).
+// A wavefront's part of the next tile (8 KB at D = 256) is always in flight, two work-groups or more share a CU: a long cache
+// streams (one token at 131000 positions, 16 heads on 4 of 256 dims: 268 MB in 48.2 us, 5.6 TB/s; a 1 GiB copy reaches 5.15). A short
+// one is bound by latency: 4000 positions, 8.4 MB, 5.8 us, most of it the first loads and the way of a tile through the steps.
 // An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; R = 16: one plane after the
 // other.
 template <int D, bool E4, int R>
@@ -429,6 +435,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
     const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = (int)blockIdx.x / a.c.Hkv * R;
     const int p0 = np + r0 / G, p1 = np + min(r0 + R - 1, rows - 1) / G, last = np + a.T - 1;
+    const int lo = a.window ? max(p0 - a.window + 1, 0) : 0;
     const Tiles tl = tiles_of(p0, p1, a.window, a.sinks);
     const int i0 = sp * a.per_split, i1 = min(i0 + a.per_split, tl.n);
     if (i0 >= tl.n) return;
@@ -437,10 +444,10 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     u32x4 kr[NS], vr[NV];
     float s1 = 0.f;   // wavefront 0: the keys' scale of position l; 1: the values'
     auto tile = [&](int i) { return i < tl.ns ? i : tl.f + i - tl.ns; };
-    auto load_k = [&](int kt) {   // positions not written yet have no scale
+    auto load_k = [&](int kt) {
         load_units<NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
         const int j = kt * 64 + l;
-        if (w < 2) s1 = j <= last ? (w ? a.c.vs : a.c.ks)[s0 + (j >> a.c.lg)] : 0.f;
+        if (w < 2) s1 = held(j, a.sinks, lo, last) ? (w ? a.c.vs : a.c.ks)[s0 + (j >> a.c.lg)] : 0.f;
     };
     auto load_v = [&](int kt) { load_units<NV>(vc + (int64_t)kt * 64 * D, l * 16, vr); };
     load_k(tile(i0));
@@ -574,8 +581,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
         if (__any(al != 1.f))
 #pragma unroll
             for (int d = 0; d < NV; d++) o[d] *= al;
-        if (E4 && j0 + 63 > last) {
-            const u32x4 m = written(j0, last);
+        if (E4 && tile_part(j0, a.sinks, lo, last)) {
+            const u32x4 m = held_bytes(j0, a.sinks, lo, last);
 #pragma unroll
             for (int d = 0; d < NV; d++) vr[d] &= m;
         }
@@ -613,9 +620,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 //   sums             a quarter of the dims for all rows
 // int8 keys are matrix operands as they are: the queries are 24-bit integers per row in three signed digits of 8 bits
 // (x = X 2^e, |X| <= 2^22), every product and sum is exact until the digits' sums are joined in fp32.
-// Bound by the two units of a SIMD, whose times add up here: of 64 rows' tile of 64 keys at D = 256 (3750 cycles) the products are
-// 1792 and the vector instructions (conversions, softmax, two planes) 1600. Measured the same with the operands of 64 rows shared
-// through LDS, with its two groups of wavefronts in opposite steps, and with vector instructions placed among the products.
+// 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 87 us, 400 TFLOP/s (twice that in matrix instructions' f16 rate); at
+// 6144 positions 465 us, 515. Bound by a wavefront's own chain: of a step's 3480 cycles at D = 256 the scores take 780, the weights
+// 570, the softmax's end 800, the sums 950 and barrier and loads 350, and two work-groups a CU overlap only part of it (the products
+// alone would be 1800 cycles of a SIMD for both, the vector instructions 1600). Measured the same or slower: operands of
+// 64 rows shared through LDS, two groups of wavefronts in opposite steps, wavefronts with different roles, and the vector
+// instructions placed among the products.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <int D, bool E4>
 __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) {
@@ -629,6 +639,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
     const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = ((int)gridDim.x / a.c.Hkv - 1 - (int)blockIdx.x / a.c.Hkv) * 32;
     const int p0 = np + r0 / G, p1 = np + min(r0 + 31, rows - 1) / G, last = np + a.T - 1;
+    const int lo = a.window ? max(p0 - a.window + 1, 0) : 0;
     const Tiles tl = tiles_of(p0, p1, a.window, a.sinks);
     const int i0 = sp * a.per_split, nt = min(a.per_split, tl.n - i0);
     if (nt <= 0) return;
@@ -640,8 +651,8 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     auto load_k = [&](int i) { load_units<2 * NS>(kc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, kr); };
     auto load_v = [&](int i) { load_units<NV>(vc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, vr); };
     auto load_s = [&](int i) { s1 = scp[min(tile(min(i, nt - 1)) * 64 + l, last) >> a.c.lg]; };
-    auto put_s = [&](int i) {   // positions not written yet have no scale (every pair of wavefronts the same)
-        const float x = tile(min(i, nt - 1)) * 64 + l <= last ? s1 : 0.f;
+    auto put_s = [&](int i) {   // (every pair of wavefronts the same)
+        const float x = held(tile(min(i, nt - 1)) * 64 + l, a.sinks, lo, last) ? s1 : 0.f;
         sc[i & 3][w & 1][l] = w & 1 ? x * kP : x;
         sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-100f));
     };
@@ -735,8 +746,8 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
                     for (int d = 0; d < NV; d++) o[c][d] *= al[c];
             if (E4) {
                 const int j0 = tile(i - 2) * 64;
-                if (j0 + 63 > last) {
-                    const u32x4 m = written(j0, last);
+                if (tile_part(j0, a.sinks, lo, last)) {
+                    const u32x4 m = held_bytes(j0, a.sinks, lo, last);
 #pragma unroll
                     for (int d = 0; d < NV; d++) vr[d] &= m;
                 }
@@ -870,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
 }
 
 // The splits of a row joined in order: W wavefronts take every W-th split each (a lane D / 64 dims), their sums are added in
-// order. W = 1: four rows per work-group.
+// order. W = 1: four rows per work-group. Latency bound: 63 splits of 16 rows of 256 3.9 us, 128 5.3; a launch alone is 3.
 template <int D, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const Kv8AttnArgs a, int R) {
     constexpr int V = D / 64;
@@ -938,8 +949,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
 
-// Rows of a work-group: up to 8 share every product between their planes (half the matrix instructions), up to 16 have the kernel
-// with the shorter way through one tile (one token at 4000 positions: 5.9 us, 13 in the other one).
+// Rows of a work-group. Up to 8 share every product between their planes, half the matrix instructions (one token of 32 heads on as
+// many of 128 dims at 32000 positions: 65 us, 69 as 16 rows; of 16 heads on 4 of 256 56 either way). Up to 16 take the kernel that
+// shares a tile's work out (4 tokens of those at 131000: 58 us, 61 as 32 rows, 83 as two times 8), more the one that has 32 in
+// a pass over the cache (8 tokens: 68 us, 90 as two times 16).
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
     return n <= 8 ? 8 : n <= 16 ? 16 : 32;

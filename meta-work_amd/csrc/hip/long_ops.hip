@@ -143,7 +143,7 @@ extern "C" int xjh_kv8_load(const xjh_kv8 *c, int pos0, int n, float *k, int64_t
 
 static bool attn_shape_ok(const xjh_kv8 *c, int T, int H, int n_past, int window, int n_sink) {
     return T >= 0 && H >= c->Hkv && H % c->Hkv == 0 && n_past >= 0 && (int64_t)n_past + T <= c->n_ctx && window >= 0 &&
-           n_sink >= 0 && (int64_t)T * H <= (1 << 30);
+           n_sink >= 0 && (int64_t)T * H <= (1 << 28);
 }
 
 extern "C" int xjh_attn_kv8(const xjh_kv8 *c, const float *q, int64_t q_tok, int64_t q_head, const float *gate,

@@ -807,18 +807,37 @@ def delta_step(qkv, k_off, v_off, beta_raw, alpha_raw, dt, A, Hk, Hv, S, eps, qs
 
 # ---------------------------------------------------------- long contexts --
 
+def _rows(a, dims, what):
+    """a as contiguous float32 rows of these dims (None: any); the GPU reads all of them."""
+    a = np.ascontiguousarray(a, np.float32)
+    if a.ndim != len(dims) or any(d is not None and d != n for d, n in zip(dims, a.shape)):
+        raise XjError(f"{what}: shape {a.shape}, expected {tuple('any' if d is None else d for d in dims)}")
+    return a
+
+
+def _opt(arr):
+    """A device copy of an array, or no buffer for none and for an empty one; its address."""
+    d = Dev(arr) if arr is not None and arr.size else None
+    return d, d.ptr if d else None
+
+
 def rope_scaled(x, n_rot, base, pos, pairs=ROPE_HALF, in_place=False, **scaling):
     """Rotary positions on the GPU of x [T][heads][D]; pos: the first token's position, or an
     int32 array of every token's. scaling: the other fields of XjhRopeCfg."""
-    x = np.ascontiguousarray(x, np.float32)
+    x = _rows(x, (None, None, None), "rope_scaled: x")
     T, H, D = x.shape
     cfg = XjhRopeCfg(pairs=pairs, n_rot=n_rot, base=base, **scaling)
-    dx = Dev(x)
-    do = dx if in_place else Dev(nbytes=max(x.nbytes, 1))
-    dp = None if np.isscalar(pos) else Dev(np.ascontiguousarray(pos, np.int32))
+    own = None if np.isscalar(pos) else np.ascontiguousarray(pos, np.int32)
+    if own is not None and own.shape != (T,):
+        raise XjError(f"rope_scaled: {own.shape} positions of {T} tokens")
+    dx, xp = _opt(x)
+    do = dx if in_place or not x.size else Dev(nbytes=x.nbytes)
+    dp, pp = _opt(own)
     err = _err()
-    _check(lib().xjh_rope_scaled(dx.ptr, H * D, D, do.ptr, H * D, D, T, H, D, C.byref(cfg), dp.ptr if dp else None,
-                                 0 if dp else int(pos), None, err, ERR), err, "rope_scaled")
+    _check(lib().xjh_rope_scaled(xp, H * D, D, do.ptr if do else None, H * D, D, T, H, D, C.byref(cfg), pp,
+                                 0 if own is not None else int(pos), None, err, ERR), err, "rope_scaled")
+    if not x.size:
+        return x
     lib().xjh_sync()
     return do.get(np.float32, x.shape)
 
@@ -842,10 +861,10 @@ class Kv8:
 
     def store(self, k, v, n_past):
         """k, v [T][Hkv][D] into positions n_past .."""
-        k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
-        dk, dv, row, err = Dev(k), Dev(v), self.c.Hkv * self.c.D, _err()
-        _check(lib().xjh_kv8_store(C.byref(self.c), dk.ptr, row, dv.ptr, row, k.shape[0], n_past, None, None, err, ERR), err,
-               "kv8_store")
+        k = _rows(k, (None, self.c.Hkv, self.c.D), "kv8_store: k")
+        v = _rows(v, k.shape, "kv8_store: v")
+        (dk, kp), (dv, vp), row, err = _opt(k), _opt(v), self.c.Hkv * self.c.D, _err()
+        _check(lib().xjh_kv8_store(C.byref(self.c), kp, row, vp, row, k.shape[0], n_past, None, None, err, ERR), err, "kv8_store")
         lib().xjh_sync()
 
     def load(self, pos0, n):
@@ -860,15 +879,16 @@ class Kv8:
     def attend(self, q, n_past, gate=None, window=0, n_sink=0, scale=None, work_bytes=None):
         """Attention of q [T][H][D] at positions n_past .. over the cache, [T][H*D]. work_bytes: the
         work area (default: what the library asks for)."""
-        q = np.ascontiguousarray(q, np.float32)
+        q = _rows(q, (None, None, self.c.D), "attn_kv8: q")
         T, H, D = q.shape
-        dq, do, err = Dev(q), Dev(nbytes=max(1, q.nbytes)), _err()
-        dg = Dev(np.ascontiguousarray(gate, np.float32)) if gate is not None else None
+        (dq, qp), err = _opt(q), _err()
+        do = Dev(nbytes=max(1, q.nbytes))
+        dg, gp = _opt(_rows(gate, q.shape, "attn_kv8: gate") if gate is not None else None)
         if work_bytes is None:
             work_bytes = lib().xjh_attn_kv8_work_bytes(C.byref(self.c), T, H, n_past, window, n_sink)
         dw = Dev(nbytes=work_bytes) if work_bytes else None
-        _check(lib().xjh_attn_kv8(C.byref(self.c), dq.ptr, H * D, D, dg.ptr if dg else None, H * D, D, T, H, n_past, None, window,
-                                  n_sink, D ** -0.5 if scale is None else scale, do.ptr, H * D, dw.ptr if dw else None, work_bytes,
+        _check(lib().xjh_attn_kv8(C.byref(self.c), qp, H * D, D, gp, H * D, D, T, H, n_past, None, window, n_sink,
+                                  D ** -0.5 if scale is None else scale, do.ptr, H * D, dw.ptr if dw else None, work_bytes,
                                   None, err, ERR), err, "attn_kv8")
         lib().xjh_sync()
         return do.get(np.float32, (T, H * D))

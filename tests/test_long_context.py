@@ -776,3 +776,52 @@ def test_attention_scales_of_any_sign(scale):
             q = rng.standard_normal((T, 2, 64)).astype(np.float32)
             _check_attn(cache.attend(q, n_past, scale=scale, window=90, n_sink=2),
                         *attend64(kv, q, n_past, scale=scale, window=90, n_sink=2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("T,H", [(1, 4), (2, 4), (4, 4), (9, 4), (50, 2)])   # 4, 8, 16 rows a work-group and more
+@pytest.mark.parametrize("window,n_sink,n_past", [(100, 4, 700), (70, 0, 300), (1, 70, 200), (65, 64, 129)])
+def test_attention_of_positions_that_were_never_stored(window, n_sink, n_past, T, H, kind):
+    """Only the first tokens and the window's are in the cache; every other byte is a NaN code or scale."""
+    rng = np.random.default_rng(26)
+    D, n = 64, n_past + T
+    lo = n_past - window + 1
+    k, v = rows(rng, n, 2, D), rows(rng, n, 2, D)
+    cache, ref = xp.Kv8(2, D, n + 80, 1, kind), Ref(2, D, n + 80, 1, kind)
+    cache.put_bytes(np.full(cache.c.bytes, 0xFF, np.uint8))
+    for p0, p1 in ((0, n_sink), (lo, n)):
+        cache.store(k[p0:p1], v[p0:p1], p0)
+        ref.store(k[p0:p1], v[p0:p1], p0)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    _check_attn(cache.attend(q, n_past, window=window, n_sink=n_sink),
+                *attend64(ref.values(0, n), q, n_past, window=window, n_sink=n_sink))
+
+
+@pytest.mark.gpu
+def test_rope_scaled_of_very_many_tokens():
+    """2^24 + 3 tokens, two elements each: more work-groups than one dimension of a grid takes."""
+    T, D = (1 << 24) + 3, 2
+    cfg = xp.XjhRopeCfg(pairs=0, n_rot=2, base=1e4, scaling=0, factor=1.0)
+    x = np.random.default_rng(27).standard_normal((T, 1, D)).astype(np.float32)
+    got = xp.rope_scaled(x, 2, 1e4, 5)
+    for t0 in (0, (1 << 23) - 2, (1 << 24) - 2):
+        want, length = rope64(x[t0:t0 + 5], cfg, 5 + t0 + np.arange(5))
+        assert np.all(np.abs(got[t0:t0 + 5] - want) <= 4 * 2.0 ** -24 * length[..., :1] + 1e-37)
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_arrays_of_other_shapes_and_take_empty_ones():
+    rng = np.random.default_rng(28)
+    cache = xp.Kv8(2, 64, 100)
+    x = rows(rng, 5, 2, 64)
+    for call in (lambda: cache.store(x, x[:4], 0), lambda: cache.store(x[:, :1], x[:, :1], 0), lambda: cache.store(x[..., :32], x[..., :32], 0),
+                 lambda: cache.attend(np.zeros((1, 2, 128)), 0), lambda: cache.attend(x, 0, gate=x[:3]), lambda: cache.attend(x[0], 0),
+                 lambda: xp.rope_scaled(x, 64, 1e4, np.zeros(4, np.int32)), lambda: xp.rope_scaled(x[0], 64, 1e4, 0)):
+        with pytest.raises(xp.XjError):
+            call()
+    assert not np.any(cache.bytes())
+    cache.store(x[:0], x[:0], 100)
+    assert not np.any(cache.bytes())
+    assert cache.attend(x[:0], 100).shape == (0, 128) and xp.rope_scaled(x[:0], 64, 1e4, 0).shape == (0, 2, 64)
+    assert cache.load(100, 0)[0].shape == (0, 2, 64)
