@@ -391,8 +391,8 @@ struct Kv8AttnArgs {
     float *part;                  // split partials
     int32_t n_split, per_split;   // set by kv8_attn_launch
 };
-// part_floats: the partials' capacity (any); kv8_attn_part_floats: what the
-// launch would use with enough.
+// part_floats: the partials' capacity (any); kv8_attn_part_floats: at least what the
+// launch would use with enough, for this and every smaller npast.
 int kv8_attn_launch(const Kv8AttnArgs &a, int64_t part_floats, hipStream_t st);
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a);
 

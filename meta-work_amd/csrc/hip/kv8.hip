@@ -949,14 +949,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
 
-// Rows of a work-group. Up to 8 share every product between their planes, half the matrix instructions (one token of 32 heads on as
-// many of 128 dims at 32000 positions: 65 us, 69 as 16 rows; of 16 heads on 4 of 256 56 either way). Up to 16 take the kernel that
-// shares a tile's work out (4 tokens of those at 131000: 58 us, 61 as 32 rows, 83 as two times 8), more the one that has 32 in
-// a pass over the cache (8 tokens: 68 us, 90 as two times 16).
-static int rows_of(const Kv8AttnArgs &a) {
-    const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
-    return n <= 8 ? 8 : n <= 16 ? 16 : 32;
-}
 // Tiles that R rows see at most.
 static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int all = (a.npast + a.T - 1) / 64 + 1;
@@ -965,7 +957,19 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
     const int64_t n = ((int64_t)a.sinks + 63) / 64 + ((int64_t)a.window + span + 62) / 64 + 1;
     return n < all ? (int)n : all;
 }
-// Splits of the tiles. The registers let a CU hold two work-groups, and two hide each other's waits: splits for 512 where every one
+// Rows of a work-group (times of 16 heads on 4 of 256 dims, int8, as replayed graphs). Up to 8 share every product between their planes,
+// half the matrix instructions: one token of 32 heads on as many of 128 dims at 32000 positions 65 us, 69 as 16 rows. 16 is the
+// kernel that shares a tile's work out, the shorter way through it, 32 the one that has more rows in a pass over the cache: up to 16 rows
+// the first (4 tokens at 131000: 58 us, 61 as 32), and as long as its work-groups have a tile each, e4m3, whose scores cost the second
+// more, two and a half (5 tokens at 200 positions 9.4 us, 12.3 as 32; 64 at 0 7.0 and 9.9; 16 at 1000 12.2 and 14.1;
+// beyond: 32 at 4000 20.6 and 19.8, 64 at 8000 43 and 35; e4m3 20 at 4000 17.3 and 18.9, 64 at 2000 20.4 and 20.8).
+static int64_t groups16(const Kv8AttnArgs &a) { return ((int64_t)a.T * (a.H / a.c.Hkv) + 15) / 16 * a.c.Hkv; }
+static int rows_of(const Kv8AttnArgs &a) {
+    const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
+    return n <= 8 ? 8 : n <= 16 || groups16(a) * most_tiles(a, 16) <= (a.c.e4m3 ? 1280 : 512) ? 16 : 32;
+}
+// Splits of the tiles, from four on: below, the merge costs more (one token at 64 positions, two tiles, 8.5 us split and 7.6 not, at
+// 128 8.7 and 8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9 and 12.5, at 192 13.1 and 13.7). The registers let a CU hold two work-groups, and two hide each other's waits: splits for 512 where every one
 // has its tiles. Up to 16 rows a tile is enough, but the merge reads every split, so 256 at most (microseconds with 16 heads, 4 of keys,
 // 256 dims, int8, for 256, 384, 512 and 768 work-groups: one token at 131000 positions 70, 60, 56, 57, four 77, 66, 58, 67; at 4000 in 16,
 // 32, 63 splits 15.9, 14.7, 11.2; one token of 16 heads on one at 32000 in 128, 256, 512 splits 16.5, 16.8, 22). With more rows the
@@ -977,12 +981,14 @@ static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
     int64_t n;
+    if (tiles <= 3) return 1;
     if (R < 32) n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
     else n = std::max(std::min<int64_t>(256 / wgs, (tiles + 1) / 2), std::min<int64_t>((wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs, tiles / 8));
     return n < 1 ? 1 : (int)n;
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
-    const int n = splits_of(a);
+    int64_t n = splits_of(a);
+    if (most_tiles(a, 16) > 3) n = std::max(n, std::min<int64_t>(512 / groups16(a), std::min(most_tiles(a, 16), 256)));   // what fewer tiles may take as 16 rows
     return n > 1 ? (int64_t)a.T * a.H * n * (a.c.D + 4) : 0;
 }
 
@@ -994,8 +1000,9 @@ static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     else if (R == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), grid, dim3(256), 0, st, a);
     if (a.n_split == 1) return;
-    // eight wavefronts a row while the rows do not fill the GPU by themselves
-    if (a.n_split <= 16 || rows * a.c.Hkv > 1024) hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((rows + 3) / 4, a.c.Hkv), dim3(256), 0, st, a, R);
+    // eight wavefronts a row where there is more than a round of one's loads and the rows do not fill the GPU by themselves (one token at
+    // 576 positions, 10 splits, 9.8 us with one and 9.4 with eight, at 256, 5 splits, 8.6 and 9.1; 64 of 8 heads of 64 dims at 500 9.3 and 10.2)
+    if (a.n_split <= 8 || rows * a.c.Hkv > (a.n_split <= 16 ? 256 : 1024)) hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((rows + 3) / 4, a.c.Hkv), dim3(256), 0, st, a, R);
     else hipLaunchKernelGGL((kv8_merge_kernel<D, 8>), dim3(rows, a.c.Hkv), dim3(512), 0, st, a, R);
 }
 

@@ -230,6 +230,14 @@ def test_empty_calls_do_nothing():
     assert L.xjh_attn_kv8(c, None, 0, 0, None, 0, 0, 0, 2, 100, None, 0, 0, 1.0, None, 0, None, 0, None, err, xp.ERR) == 0
 
 
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("T,H,Hkv,window", [(1, 16, 4, 0), (5, 16, 4, 0), (20, 8, 1, 0), (64, 16, 4, 0), (200, 16, 4, 0), (5, 16, 4, 3000), (700, 8, 2, 0)])
+def test_work_area_serves_every_earlier_position(T, H, Hkv, window, kind):
+    c = _kv(type=kind, Hkv=Hkv, D=128, n_ctx=1 << 20)
+    need = [xp.lib().xjh_attn_kv8_work_bytes(c, T, H, n, window, 4) for n in [*range(0, 20000, 61), 50000, 131000, 1000000]]
+    assert all(a <= b for a, b in zip(need, need[1:]))
+
+
 # -------------------------------------------------------------------- rope --
 
 def _rope_close(x, cfg_kw, pos, T, **kw):
