@@ -636,7 +636,8 @@ class _Step:
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("Hkv,G,D,T,window,n_sink", [(2, 4, 256, 1, 0, 0), (1, 2, 128, 5, 100, 3), (2, 1, 64, 40, 0, 0)])
+@pytest.mark.parametrize("Hkv,G,D,T,window,n_sink", [(2, 4, 256, 1, 0, 0), (1, 2, 128, 5, 100, 3), (2, 1, 64, 40, 0, 0),
+                                                         (2, 4, 256, 200, 0, 0), (1, 4, 64, 900, 100, 70)])
 def test_captured_steps_replay_at_every_position(Hkv, G, D, T, window, n_sink):
     """The four calls captured once, with the position read on the device, and replayed over a sequence with eager work and
     synchronisations between; two graphs with a cache and a work area each, on two streams at once. Every replay equals
@@ -764,7 +765,7 @@ def test_many_heads_and_many_rows():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,n_past", [(1, 3000), (3, 3000), (40, 3000), (300, 0)])
+@pytest.mark.parametrize("T,n_past", [(1, 3000), (3, 3000), (40, 3000), (300, 0), (9, 20000), (300, 3000)])
 def test_the_same_call_gives_the_same_bits(T, n_past):
     rng = np.random.default_rng(24)
     cache, _ = _filled(rng, 4, 128, n_past + T, 32, I8)
@@ -833,3 +834,69 @@ def test_wrappers_refuse_arrays_of_other_shapes_and_take_empty_ones():
     assert not np.any(cache.bytes())
     assert cache.attend(x[:0], 100).shape == (0, 128) and xp.rope_scaled(x[:0], 64, 1e4, 0).shape == (0, 2, 64)
     assert cache.load(100, 0)[0].shape == (0, 2, 64)
+
+
+# Enough rows and tiles for the kernel that takes 32 rows at a time (fewer go to the one that takes 8 or 16).
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("H,Hkv,D,block,n_past,T", [(8, 2, 256, 32, 400, 300), (8, 2, 128, 1, 390, 301), (16, 4, 64, 64, 411, 170), (3, 1, 256, 16, 1200, 299)])
+def test_attention_of_many_rows_matches_float64(H, Hkv, D, block, n_past, T, kind):
+    rng = np.random.default_rng(H * D + n_past)
+    n = n_past + T
+    cache, kv = _filled(rng, Hkv, D, n, block, kind, n_ctx=n + 70)
+    q, gate = (rng.standard_normal((T, H, D)).astype(np.float32) for _ in range(2))
+    _check_attn(cache.attend(q, n_past, gate), *attend64(kv, q, n_past, gate))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (7, 4), (65, 64), (100, 130), (300, 2), (200, 0), (100, 4)])
+def test_windows_of_many_rows(window, n_sink, kind):
+    """Of the positions before the call only the first tokens and the window's are stored, the other bytes are NaN codes and scales."""
+    rng = np.random.default_rng(30)
+    T, H, D, n_past = 700, 8, 64, 430
+    n, lo = n_past + T, n_past - window + 1
+    k, v = rows(rng, n, 2, D), rows(rng, n, 2, D)
+    cache, ref = xp.Kv8(2, D, n + 80, 1, kind), Ref(2, D, n + 80, 1, kind)
+    cache.put_bytes(np.full(cache.c.bytes, 0xFF, np.uint8))
+    for p0, p1 in ((0, n_sink), (lo, n)):
+        cache.store(k[p0:p1], v[p0:p1], p0)
+        ref.store(k[p0:p1], v[p0:p1], p0)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    _check_attn(cache.attend(q, n_past, window=window, n_sink=n_sink),
+                *attend64(ref.values(0, n), q, n_past, window=window, n_sink=n_sink))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("work_bytes", [0, 200000, None])
+def test_split_rows_of_a_long_context(work_bytes, kind):
+    rng = np.random.default_rng(31)
+    T, n = 9, 20009
+    cache, kv = _filled(rng, 4, 64, n, 32, kind)
+    q = rng.standard_normal((T, 16, 64)).astype(np.float32)
+    _check_attn(cache.attend(q, n - T, work_bytes=work_bytes), *attend64(kv, q, n - T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_many_rows_of_sharp_scores_and_rows_that_are_not_finite(kind):
+    """Scores that rise to 60 from key to key, or reach it on one key; a query that is not finite stays in its own row."""
+    rng = np.random.default_rng(32)
+    D, n, T, H = 128, 1500, 300, 4
+    u = rng.standard_normal(D)
+    u /= np.linalg.norm(u)
+    for k in (np.arange(n)[:, None, None] / n * 60 * u, np.where(np.arange(n)[:, None, None] == 317, 60 * u, 0.1 * rng.standard_normal((n, 1, D)))):
+        cache = xp.Kv8(1, D, n, 16, kind)
+        cache.store(k.astype(np.float32), rows(rng, n, 1, D), 0)
+        kv = np.stack(cache.load(0, n))
+        q = np.tile(u.astype(np.float32), (T, H, 1)) + (rng.standard_normal((T, H, D)) * 0.01).astype(np.float32)
+        want, mag = attend64(kv, q, n - T, scale=1.0)
+        # a score of 60 is off by 4 roundings: 60 * 1.44 * 4 * 2^-24 = 2e-5 in a weight
+        _check_attn(cache.attend(q, n - T, scale=1.0), want, mag + 1e-30, bar_row=4e-5, bar=2e-5)
+        q[5, 1, 7], q[250, 3, 0], q[299, 0, 127] = np.nan, np.inf, -np.inf
+        bad = ~np.isfinite(q).all(-1)
+        got = cache.attend(q, n - T, scale=1.0).reshape(q.shape)
+        assert not np.any(np.isfinite(got[bad])) and bad.sum() == 3
+        assert np.max(np.abs(got - want)[~bad] / (mag.max(-1)[~bad][:, None] + 1e-30)) <= 4e-5
