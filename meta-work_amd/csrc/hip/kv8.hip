@@ -968,22 +968,27 @@ static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
     return n <= 8 ? 8 : n <= 16 || groups16(a) * most_tiles(a, 16) <= (a.c.e4m3 ? 1280 : 512) ? 16 : 32;
 }
-// Splits of the tiles, from four on: below, the merge costs more (one token at 64 positions, two tiles, 8.5 us split and 7.6 not, at
-// 128 8.7 and 8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9 and 12.5, at 192 13.1 and 13.7). The registers let a CU hold two work-groups, and two hide each other's waits: splits for 512 where every one
-// has its tiles. Up to 16 rows a tile is enough, but the merge reads every split, so 256 at most (microseconds with 16 heads, 4 of keys,
-// 256 dims, int8, for 256, 384, 512 and 768 work-groups: one token at 131000 positions 70, 60, 56, 57, four 77, 66, 58, 67; at 4000 in 16,
-// 32, 63 splits 15.9, 14.7, 11.2; one token of 16 heads on one at 32000 in 128, 256, 512 splits 16.5, 16.8, 22). With more rows the
-// second work-group of a CU has to come with eight tiles a split (for 256 and 512: 8 tokens at 131000 78 and 68, 32 at 32000 58 and 50,
-// 512 at 32000 684 and 515, but 512 tokens of an empty cache, 9 tiles, 20 and 27) and the first with two (333 tokens with a window
-// of 1024 in 2, 3, 6 splits: 28, 25, 26). From 257 to 341 work-groups thirds in two turns beat wholes in one, which leave every
-// other CU one work-group alone (600 tokens at 32000 636 and 912); from there on nothing is split.
+// Splits of the tiles (times of 16 heads on 4 of 256 dims, int8, as replayed graphs). Below four tiles the merge costs more than it
+// saves: one token at 64 positions 8.5 us split and 7.6 not, at 128 8.7 and 8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9
+// and 12.5. A CU holds two work-groups, by their registers, and the two hide each other's waits: 512 in all.
+// Up to 16 rows a tile each is enough, but the merge reads every split, so 256 at most: for 256, 384, 512 and 768
+// work-groups one token at 131000 positions takes 70, 60, 56 and 57, four 77, 66, 58 and 67; one token of 16 heads on one at 32000 in
+// 128, 256 and 512 splits 16.5, 16.8 and 22.
+// With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32, 512 at
+// 32000 684 and 515), else 256 of two at least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23;
+// a number between the two leaves some CUs one work-group and others two). From 257 to 341 row groups thirds in two turns
+// beat wholes in one, which leave every other CU one work-group alone (600 at 32000 636 and 912); from there on nothing is split.
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
-    int64_t n;
     if (tiles <= 3) return 1;
-    if (R < 32) n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
-    else n = std::max(std::min<int64_t>(256 / wgs, (tiles + 1) / 2), std::min<int64_t>((wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs, tiles / 8));
+    int64_t n;
+    if (R < 32) {
+        n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
+    } else {
+        n = (wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs;
+        if (tiles < 4 * n) n = std::min<int64_t>(256 / wgs, (tiles + 1) / 2);
+    }
     return n < 1 ? 1 : (int)n;
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
