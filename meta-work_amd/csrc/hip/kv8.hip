@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 //   sums             a quarter of the dims for all rows
 // int8 keys are matrix operands as they are: the queries are 24-bit integers per row in three signed digits of 8 bits
 // (x = X 2^e, |X| <= 2^22), every product and sum is exact until the digits' sums are joined in fp32.
-// 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 87 us, 400 TFLOP/s (twice that in matrix instructions' f16 rate); at
+// 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 87 to 90 us, 390 TFLOP/s (twice that in matrix instructions' f16 rate); at
 // 6144 positions 465 us, 515. Bound by a wavefront's own chain: of a step's 3480 cycles at D = 256 the scores take 780, the weights
 // 570, the softmax's end 800, the sums 950 and barrier and loads 350, and two work-groups a CU overlap only part of it (the products
 // alone would be 1800 cycles of a SIMD for both, the vector instructions 1600). Measured the same or slower: operands of
