@@ -945,9 +945,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
             __builtin_memcpy(&v[i], p + 4 + V * l, sizeof(vec));
         }
     };
+    vec gate = 0.f;
     float M = -INFINITY;
     if (l < ns) M = part[(int64_t)l * (D + 4)];
     load(w);   // with the maxima
+    if (a.gate && w == 0) __builtin_memcpy(&gate, a.gate + t * a.g_tok + h * a.g_head + V * l, sizeof(vec));
     for (int s = l + 64; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 4)]);
     M = xjd::wave_max(M);
     vec y = 0.f;
@@ -978,11 +980,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
     }
     y *= (1.f / kP) / L;
     float *op = a.out + t * a.o_tok + (int64_t)h * D + V * l;
-    if (a.gate) {
-        const float *gp = a.gate + t * a.g_tok + h * a.g_head + V * l;
+    if (a.gate)
 #pragma unroll
-        for (int i = 0; i < V; i++) ((float *)&y)[i] *= sigm_fast(gp[i]);
-    }
+        for (int i = 0; i < V; i++) ((float *)&y)[i] *= sigm_fast(((float *)&gate)[i]);
 #pragma unroll
     for (int i = 0; i < V; i++) op[i] = ((float *)&y)[i];
 }
@@ -998,13 +998,14 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
 // Rows of a work-group (times of 16 heads on 4 of 256 dims, int8, as replayed graphs). Up to 8 share every product between their planes,
 // half the matrix instructions: one token of 32 heads on as many of 128 dims at 32000 positions 65 us, 69 as 16 rows. 16 is the
 // kernel that shares a tile's work out, the shorter way through it, 32 the one that has more rows in a pass over the cache: up to 16 rows
-// the first (4 tokens at 131000: 58 us, 61 as 32), and as long as its work-groups have a tile each, e4m3, whose scores cost the second
-// more, two and a half (5 tokens at 200 positions 9.4 us, 12.3 as 32; 64 at 0 7.0 and 9.9; 16 at 1000 12.2 and 14.1;
-// beyond: 32 at 4000 20.6 and 19.8, 64 at 8000 43 and 35; e4m3 20 at 4000 17.3 and 18.9, 64 at 2000 20.4 and 20.8).
+// the first (4 tokens at 131000: 58 us, 61 as 32), and as long as its work-groups have a tile each (5 tokens at 200 positions 9.4 us,
+// 12.3 as 32; 64 at 0 7.0 and 9.9; 16 at 1000 12.2 and 14.1; beyond: 32 at 4000 20.6 and 19.8, 64 at 8000 43 and 35). With e4m3 the scores of
+// 32 rows are no integer products, and 16 rows hold out for 20 D tiles (of 256 dims 64 tokens at 4000 25.5 and 26.5, of 128 at
+// 2000, 2112 tiles, 15.1 and 15.2, 128 at 2000, 4352 tiles, 21.3 and 20.8, of 64 on 8 heads 40 at 4000, 1536 tiles, 13.0 and 12.1).
 static int64_t groups16(const Kv8AttnArgs &a) { return ((int64_t)a.T * (a.H / a.c.Hkv) + 15) / 16 * a.c.Hkv; }
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
-    return n <= 8 ? 8 : n <= 16 || groups16(a) * most_tiles(a, 16) <= (a.c.e4m3 ? 1280 : 512) ? 16 : 32;
+    return n <= 8 ? 8 : n <= 16 || groups16(a) * most_tiles(a, 16) <= (a.c.e4m3 ? 20 * a.c.D : 512) ? 16 : 32;
 }
 // Splits of the tiles (times of 16 heads on 4 of 256 dims, int8, as replayed graphs). Below four tiles the merge costs more than it
 // saves: one token at 64 positions 8.5 us split and 7.6 not, at 128 8.7 and 8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9
@@ -1012,10 +1013,12 @@ static int rows_of(const Kv8AttnArgs &a) {
 // Up to 16 rows a tile each is enough, but the merge reads every split, so 256 at most: for 256, 384, 512 and 768
 // work-groups one token at 131000 positions takes 70, 60, 56 and 57, four 77, 66, 58 and 67; one token of 16 heads on one at 32000 in
 // 128, 256 and 512 splits 16.5, 16.8 and 22.
-// With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32, 512 at
-// 32000 684 and 515), else 256 of two at least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23;
-// a number between the two leaves some CUs one work-group and others two). From 257 to 341 row groups thirds in two turns
-// beat wholes in one, which leave every other CU one work-group alone (600 at 32000 636 and 912); from there on nothing is split.
+// With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32), else 256 of two at
+// least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23; a number between the two
+// leaves some CUs one work-group and others two). From 129 row groups on the other choice is no split and no merge: worth
+// five tiles a third up to 170 groups (333 tokens at 500 positions 29.0 whole, 29.6 in thirds, at 1000 40.0 and 34.5), twelve a half or a
+// third beyond (512 at 500 33.5 whole, 37.1 in halves, at 1000 44.1 and 45.5, at 2000 64 and 59, at 32000 684 and 515; 600, thirds in two
+// turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636). From 342 on nothing is split.
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
@@ -1025,7 +1028,7 @@ static int splits_of(const Kv8AttnArgs &a) {
         n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
     } else {
         n = (wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs;
-        if (tiles < 4 * n) n = std::min<int64_t>(256 / wgs, (tiles + 1) / 2);
+        if (tiles < (wgs <= 128 ? 4 : wgs <= 170 ? 5 : 12) * n) n = std::min<int64_t>(256 / wgs, (tiles + 1) / 2);
     }
     return n < 1 ? 1 : (int)n;
 }
