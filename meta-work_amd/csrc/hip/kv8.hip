@@ -447,7 +447,7 @@ __device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int
     }
 }
 
-// Attention of up to 16 rows (row = token * G + head of the kv head): a work-group takes R of them and a split of the tiles. Its
+// Attention of 8 or 16 rows (row = token * G + head of the kv head): a work-group takes R of them and a split of the tiles. Its
 // four wavefronts share every tile, each a part of every step, so nothing is converted or summed twice and one tile (a
 // short context's) takes a quarter of the time:
 //   scores   16 keys each: K units from the cache to registers, the queries stay in registers
@@ -456,9 +456,10 @@ __device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int
 // A wavefront's part of the next tile (8 KB at D = 256) is always in flight, two work-groups or more share a CU: a long cache
 // streams (one token at 131000 positions, 16 heads on 4 of 256 dims: 268 MB in 48.2 us, 5.6 TB/s; a 1 GiB copy reaches 5.15). A short
 // one is bound by latency: 4000 positions, 8.4 MB, 5.8 us, most of it the first loads and the way of a tile through the steps.
+// A: tiles requested ahead of the one in use.
 // An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; R = 16: one plane after the
 // other.
-template <int D, bool E4, int R>
+template <int D, bool E4, int R, int A>
 __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     constexpr int NS = D / 64, NV = D / 64, NQ = 2 * NS;   // a wavefront's units of keys and of values; 32-dim steps of a score
     constexpr bool ST = R == 8;
@@ -479,17 +480,22 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     if (i0 >= tl.n) return;
     const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + w * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
     const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
-    u32x4 kr[NS], vr[NV];
-    float s1 = 0.f;   // wavefront 0: the keys' scale of position l; 1: the values'
+    u32x4 kr[A][NS], vr[A][NV];
+    float s1[A] = {};   // wavefront 0: the keys' scale of position l; 1: the values'
     auto tile = [&](int i) { return i < tl.ns ? i : tl.f + i - tl.ns; };
-    auto load_k = [&](int kt) {
+    auto load_k = [&](int kt, u32x4 (&kr)[NS], float &s1) {
         load_units<NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
         const int j = kt * 64 + l;
         if (w < 2) s1 = held(j, a.sinks, lo, last) ? (w ? a.c.vs : a.c.ks)[s0 + (j >> a.c.lg)] : 0.f;
     };
-    auto load_v = [&](int kt) { load_units<NV>(vc + (int64_t)kt * 64 * D, l * 16, vr); };
-    load_k(tile(i0));
-    load_v(tile(i0));
+    auto load_v = [&](int kt, u32x4 (&vr)[NV]) { load_units<NV>(vc + (int64_t)kt * 64 * D, l * 16, vr); };
+    load_k(tile(i0), kr[0], s1[0]);
+    load_v(tile(i0), vr[0]);
+    auto ahead = [&](int i) { return tile(A > 1 ? min(i + A, i1 - 1) : i + A); };   // (past the end: the last one again, so that the waits know how many are in flight)
+    if constexpr (A > 1) {
+        load_k(ahead(i0 - 1), kr[A - 1], s1[A - 1]);
+        load_v(ahead(i0 - 1), vr[A - 1]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     const int row = r0 + (li & (R - 1)), rq = min(row, rows - 1), t = rq / G, h = g * G + rq % G, pos = np + t;
     // the queries as operands, step i = 2 s + e the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo, e per row
@@ -537,9 +543,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < NV; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
-    for (int i = i0; i < i1; i++) {
+    auto step = [&](int i, u32x4 (&kr)[NS], u32x4 (&vr)[NV], float &s1) {
         const int kt = tile(i), j0 = kt * 64, par = i & 1;
-        const bool more = i + 1 < i1;
+        const bool more = A > 1 || i + A < i1;
         {   // scores
             f32x4 x[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -556,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
             if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
             sb[w][l] = v;
         }
-        if (more) load_k(tile(i + 1));
+        if (more) load_k(ahead(i), kr, s1);
         lds_barrier();
         {   // weights: the maximum over all keys, the terms of the wavefront's 16
             f32x4 s[4];   // of the sets of 16 keys from w on, around
@@ -636,7 +642,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
                 for (int x = NP - 1; x >= 0; x--) o[d] = mfma16(v, p[x], o[d]);
             }
         }
-        if (more) load_v(tile(i + 1));
+        if (more) load_v(ahead(i), vr);
+    };
+    for (int i = i0; i < i1; i += A) {
+        step(i, kr[0], vr[0], s1[0]);
+        if (A > 1 && i + 1 < i1) step(i + 1, kr[A - 1], vr[A - 1], s1[A - 1]);
     }
     // the rows' totals
     L += __shfl_xor(L, 16, 64);
@@ -1012,29 +1022,36 @@ static int rows_of(const Kv8AttnArgs &a) {
 // and 12.5. A CU holds two work-groups, by their registers, and the two hide each other's waits: 512 in all.
 // Up to 16 rows a tile each is enough, but the merge reads every split, so 256 at most: for 256, 384, 512 and 768
 // work-groups one token at 131000 positions takes 70, 60, 56 and 57, four 77, 66, 58 and 67; one token of 16 heads on one at 32000 in
-// 128, 256 and 512 splits 16.5, 16.8 and 22.
+// 128, 256 and 512 splits 16.5, 16.8 and 22. Of 64 dims, whose registers leave a CU more of them, 1024 up to 128 splits (one token of
+// 32 heads on 8 at 131000 43 with 512 and 36 with 1024, of 16 on 4 at 32000 13.1 in 128 splits and 15.2 in 256).
 // With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32), else 256 of two at
 // least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23; a number between the two
 // leaves some CUs one work-group and others two). From 129 row groups on the other choice is no split and no merge: worth
 // five tiles a third up to 170 groups (333 tokens at 500 positions 29.0 whole, 29.6 in thirds, at 1000 40.0 and 34.5), twelve a half or a
 // third beyond (512 at 500 33.5 whole, 37.1 in halves, at 1000 44.1 and 45.5, at 2000 64 and 59, at 32000 684 and 515; 600, thirds in two
-// turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636). From 342 on nothing is split.
+// turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636). From 342 on nothing is split. Of 128 and 64 dims a CU holds three and
+// four, which take eight tiles each, and no more than 64 splits (128 dims, for 512 and 768 in all: 512 tokens at 32000 351 and 320,
+// 700 at 8000 178 and 131, 128 at 4000, five tiles, 25.7 and 26.6, 8 at 131000, 64 and 96 splits, 44.1 and 45.7; 64 dims of 32 heads on 8, for 512
+// and 1024: 256 at 32000 313 and 248).
+static int64_t splits_few(const Kv8AttnArgs &a, int64_t wgs, int tiles) {
+    int64_t n = 512 / wgs;
+    if (a.c.D == 64) n = std::max(n, std::min<int64_t>(1024 / wgs, 128));
+    return std::min<int64_t>(n, std::min(tiles, 256));
+}
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
     const int64_t rows = (int64_t)a.T * (a.H / a.c.Hkv), wgs = (rows + R - 1) / R * a.c.Hkv;
     if (tiles <= 3) return 1;
-    int64_t n;
-    if (R < 32) {
-        n = std::min<int64_t>(512 / wgs, std::min(tiles, 256));
-    } else {
-        n = (wgs > 256 && wgs <= 341 ? 1024 : 512) / wgs;
-        if (tiles < (wgs <= 128 ? 4 : wgs <= 170 ? 5 : 12) * n) n = std::min<int64_t>(256 / wgs, (tiles + 1) / 2);
+    if (R < 32) return std::max<int64_t>(splits_few(a, wgs, tiles), 1);
+    for (int per = a.c.D == 64 ? 4 : a.c.D == 128 ? 3 : 2; per > 1; per--) {
+        const int64_t n = (per == 2 && wgs > 256 && wgs <= 341 ? 1024 : 256 * per) / wgs;
+        if (tiles >= (wgs > 170 ? 12 : per > 2 ? 8 : wgs > 128 ? 5 : 4) * n && (per == 2 || n <= 64)) return n < 1 ? 1 : (int)n;
     }
-    return n < 1 ? 1 : (int)n;
+    return (int)std::max<int64_t>(std::min<int64_t>(256 / wgs, (tiles + 1) / 2), 1);
 }
 int64_t kv8_attn_part_floats(const Kv8AttnArgs &a) {
     int64_t n = splits_of(a);
-    if (most_tiles(a, 16) > 3) n = std::max(n, std::min<int64_t>(512 / groups16(a), std::min(most_tiles(a, 16), 256)));   // what fewer tiles may take as 16 rows
+    if (most_tiles(a, 16) > 3) n = std::max(n, splits_few(a, groups16(a), most_tiles(a, 16)));   // what fewer tiles may take as 16 rows
     return n > 1 ? (int64_t)a.T * a.H * n * (a.c.D + 4) : 0;
 }
 
@@ -1042,8 +1059,15 @@ template <int D, bool E4>
 static void attn_launch_d(const Kv8AttnArgs &a, int R, hipStream_t st) {
     const int rows = a.T * (a.H / a.c.Hkv);
     const dim3 grid((rows + R - 1) / R * a.c.Hkv, a.n_split);
-    if (R == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 8>), grid, dim3(256), 0, st, a);
-    else if (R == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16>), grid, dim3(256), 0, st, a);
+    // Two tiles ahead where a tile is small and a work-group has some: one token of 32 heads on as many of 128 dims at 32000 positions, 32
+    // tiles, 57 us with two and 68 with one, at 8000, 8 tiles, 19.4 and 20.4; of 16 heads on 4 at 32000, 4 tiles, 15.4 and 15.2, at 4000,
+    // one tile, 8.7 and 8.5; of 256 dims, whose registers then leave a CU fewer work-groups, on 4 heads at 131000 60 and 58.
+    constexpr int A = D < 256 ? 2 : 1;
+    const bool ahead = A > 1 && a.per_split >= 6;
+    if (R == 8 && ahead) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 8, A>), grid, dim3(256), 0, st, a);
+    else if (R == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 8, 1>), grid, dim3(256), 0, st, a);
+    else if (R == 16 && ahead) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16, A>), grid, dim3(256), 0, st, a);
+    else if (R == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, E4, 16, 1>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv8_chunk_kernel<D, E4>), grid, dim3(256), 0, st, a);
     if (a.n_split == 1) return;
     // eight wavefronts a row where there is more than a round of one's loads and the rows do not fill the GPU by themselves (one token at

@@ -901,3 +901,16 @@ def test_many_rows_of_sharp_scores_and_rows_that_are_not_finite(kind):
         got = cache.attend(q, n - T, scale=1.0).reshape(q.shape)
         assert not np.any(np.isfinite(got[bad])) and bad.sum() == 3
         assert np.max(np.abs(got - want)[~bad] / (mag.max(-1)[~bad][:, None] + 1e-30)) <= 4e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("T,H,Hkv,D,n_past,window,n_sink", [(1, 4, 2, 128, 330, 0, 0), (1, 8, 1, 64, 447, 0, 0), (3, 4, 1, 128, 1000, 0, 0), (4, 8, 2, 64, 800, 0, 0),
+                                                            (1, 4, 2, 64, 1500, 500, 70), (4, 4, 1, 128, 1501, 500, 70), (12, 1, 1, 64, 378, 0, 0)])
+def test_unsplit_rows_of_many_tiles(T, H, Hkv, D, n_past, window, n_sink, kind):
+    """Work-groups of 6, 7, 8 and more tiles one after the other (no work area), the last one whole, begun or half in a window."""
+    rng = np.random.default_rng(n_past)
+    cache, kv = _filled(rng, Hkv, D, n_past + T, 8, kind, n_ctx=n_past + T + 64)
+    q, gate = (rng.standard_normal((T, H, D)).astype(np.float32) for _ in range(2))
+    _check_attn(cache.attend(q, n_past, gate, window=window, n_sink=n_sink, work_bytes=0),
+                *attend64(kv, q, n_past, gate, window=window, n_sink=n_sink))
