@@ -1022,7 +1022,8 @@ static int rows_of(const Kv8AttnArgs &a) {
 // and 12.5. A CU holds two work-groups, by their registers, and the two hide each other's waits: 512 in all.
 // Up to 16 rows a tile each is enough, but the merge reads every split, so 256 at most: for 256, 384, 512 and 768
 // work-groups one token at 131000 positions takes 70, 60, 56 and 57, four 77, 66, 58 and 67; one token of 16 heads on one at 32000 in
-// 128, 256 and 512 splits 16.5, 16.8 and 22. Of 64 dims, whose registers leave a CU more of them, 1024 up to 128 splits (one token of
+// 128, 256 and 512 splits 16.5, 16.8 and 22. More than 64 splits have to have two and a half tiles each (one token at 5000 positions in 64
+// and in 79 splits 10.3 and 11.8, at 12000 in 64 and 128 13.5 and 15.1, at 24000 18.3 and 17.5). Of 64 dims, whose registers leave a CU more of them, 1024 up to 128 splits (one token of
 // 32 heads on 8 at 131000 43 with 512 and 36 with 1024, of 16 on 4 at 32000 13.1 in 128 splits and 15.2 in 256).
 // With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32), else 256 of two at
 // least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23; a number between the two
@@ -1036,7 +1037,9 @@ static int rows_of(const Kv8AttnArgs &a) {
 static int64_t splits_few(const Kv8AttnArgs &a, int64_t wgs, int tiles) {
     int64_t n = 512 / wgs;
     if (a.c.D == 64) n = std::max(n, std::min<int64_t>(1024 / wgs, 128));
-    return std::min<int64_t>(n, std::min(tiles, 256));
+    n = std::min<int64_t>(n, 256);
+    if (n > 64 && 2 * tiles < 5 * n) n = std::max<int64_t>(n / 2, 64);
+    return std::min<int64_t>(n, tiles);
 }
 static int splits_of(const Kv8AttnArgs &a) {
     const int R = rows_of(a), tiles = most_tiles(a, R);
