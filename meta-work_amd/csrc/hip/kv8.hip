@@ -1017,23 +1017,24 @@ static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
     return n <= 8 ? 8 : n <= 16 || groups16(a) * most_tiles(a, 16) <= (a.c.e4m3 ? 20 * a.c.D : 512) ? 16 : 32;
 }
-// Splits of the tiles (times of 16 heads on 4 of 256 dims, int8, as replayed graphs). Below four tiles the merge costs more than it
-// saves: one token at 64 positions 8.5 us split and 7.6 not, at 128 8.7 and 8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9
-// and 12.5. A CU holds two work-groups, by their registers, and the two hide each other's waits: 512 in all.
-// Up to 16 rows a tile each is enough, but the merge reads every split, so 256 at most: for 256, 384, 512 and 768
-// work-groups one token at 131000 positions takes 70, 60, 56 and 57, four 77, 66, 58 and 67; one token of 16 heads on one at 32000 in
-// 128, 256 and 512 splits 16.5, 16.8 and 22. More than 64 splits have to have two and a half tiles each (one token at 5000 positions in 64
-// and in 79 splits 10.3 and 11.8, at 12000 in 64 and 128 13.5 and 15.1, at 24000 18.3 and 17.5). Of 64 dims, whose registers leave a CU more of them, 1024 up to 128 splits (one token of
-// 32 heads on 8 at 131000 43 with 512 and 36 with 1024, of 16 on 4 at 32000 13.1 in 128 splits and 15.2 in 256).
-// With more rows 512 if each then has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and 32), else 256 of two at
-// least (at three tiles in 512 or in between 40 at 4000 22 and 25, 100 at 2000 of 8 heads 19 and 23; a number between the two
-// leaves some CUs one work-group and others two). From 129 row groups on the other choice is no split and no merge: worth
-// five tiles a third up to 170 groups (333 tokens at 500 positions 29.0 whole, 29.6 in thirds, at 1000 40.0 and 34.5), twelve a half or a
-// third beyond (512 at 500 33.5 whole, 37.1 in halves, at 1000 44.1 and 45.5, at 2000 64 and 59, at 32000 684 and 515; 600, thirds in two
-// turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636). From 342 on nothing is split. Of 128 and 64 dims a CU holds three and
-// four, which take eight tiles each, and no more than 64 splits (128 dims, for 512 and 768 in all: 512 tokens at 32000 351 and 320,
-// 700 at 8000 178 and 131, 128 at 4000, five tiles, 25.7 and 26.6, 8 at 131000, 64 and 96 splits, 44.1 and 45.7; 64 dims of 32 heads on 8, for 512
-// and 1024: 256 at 32000 313 and 248).
+// Splits of the tiles (times in us of 16 heads on 4 of 256 dims, int8, as replayed graphs).
+//   Up to three tiles: none, the merge costs more than it saves (one token at 64 positions 8.5 split and 7.6 not, at 128 8.7 and
+//   8.9, at 192 8.6 and 10.3; 32 as 32 rows at 128 12.9 and 12.5).
+//   Two work-groups a CU, which their registers leave room for, hide each other's waits: 512 in all.
+//   Up to 16 rows a tile each is enough (for 256, 384, 512 and 768 work-groups one token at 131000 takes 70, 60, 56 and 57, four 77, 66,
+//   58 and 67). The merge reads every split: 256 at most (16 heads on one, one token at 32000 in 128, 256 and 512 16.5, 16.8 and
+//   22), and more than 64 have to have two and a half tiles each (one token at 5000 in 64 and in 79 splits 10.3 and 11.8, at 12000
+//   in 64 and 128 13.5 and 15.1, at 24000 18.3 and 17.5). Of 64 dims, whose registers leave room for more, 1024 up to 128
+//   splits (32 heads on 8 at 131000 43 with 512 and 36 with 1024; 16 on 4 at 32000 13.1 in 128 splits and 15.2 in 256).
+//   More rows, up to 128 groups of them: 512 if each has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and
+//   32), else 256 of two at least (at three tiles in 512 or in between 40 at 4000 22 and 25; a number in between leaves
+//   some CUs one work-group and others two).
+//   From 129 groups on the other choice is no split and no merge: worth five tiles a third up to 170 (333 tokens at 500 29.0 whole,
+//   29.6 in thirds, at 1000 40.0 and 34.5), twelve a half or a third beyond (512 at 500 33.5 whole, 37.1 in halves, at 2000 64 and
+//   59, at 32000 684 and 515; 600, thirds in two turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636).
+//   Of 128 and 64 dims a CU holds three and four of these, which take eight tiles each and at most 64 splits (128 dims, for 512 and 768 in
+//   all: 512 tokens at 32000 351 and 320, 128 at 4000, five tiles, 25.7 and 26.6, 8 at 131000, 64 and 96 splits, 44.1 and
+//   45.7; 64 dims, 32 heads on 8, for 512 and 1024: 256 at 32000 313 and 248).
 static int64_t splits_few(const Kv8AttnArgs &a, int64_t wgs, int tiles) {
     int64_t n = 512 / wgs;
     if (a.c.D == 64) n = std::max(n, std::min<int64_t>(1024 / wgs, 128));
