@@ -51,7 +51,7 @@ __device__ __forceinline__ float block_scale(float amax) {
 //   e4m3: s is a power of two, the product with 1 / s is exact and converts to nearest even.
 //   int8: the product, rounded by adding 1.5 * 2^23 (the sum's low byte is the code), is off by less than 2^-14. Where one lies
 //   nearer than that to a border (one value in 8000), the rests decide: x - c s is exact in one fma (it is below s
-//   and a multiple of the smaller ulp), and compared with s / 2.
+//   and a multiple of the smaller ulp), and twice it is compared with s (s / 2 is no float where s is below 2^-125 and odd).
 // FIN: they are finite, so no quotient is beyond the largest code by more than its rounding.
 template <bool E4, bool FIN>
 __device__ __forceinline__ uint32_t codes_of(const f32x4 x, float s, float inv) {
@@ -78,10 +78,10 @@ __device__ __forceinline__ uint32_t codes_of(const f32x4 x, float s, float inv) 
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float c = r[i] - kMagic;
-                const float rest = fmaf(-c, s, x[i]), half = 0.5f * s;
+                const float rest = fmaf(-c, s, x[i]), twice = rest + rest;
                 const bool odd = (int)c & 1;
-                if (rest > half || (rest == half && odd)) c += 1.f;
-                else if (rest < -half || (rest == -half && odd)) c -= 1.f;
+                if (twice > s || (twice == s && odd)) c += 1.f;
+                else if (twice < -s || (twice == -s && odd)) c -= 1.f;
                 r[i] = fminf(fmaxf(c, -127.f), 127.f) + kMagic;   // (an infinity's rest is one)
             }
         }

@@ -914,3 +914,26 @@ def test_unsplit_rows_of_many_tiles(T, H, Hkv, D, n_past, window, n_sink, kind):
     q, gate = (rng.standard_normal((T, H, D)).astype(np.float32) for _ in range(2))
     _check_attn(cache.attend(q, n_past, gate, window=window, n_sink=n_sink, work_bytes=0),
                 *attend64(kv, q, n_past, gate, window=window, n_sink=n_sink))
+
+
+@pytest.mark.gpu
+def test_store_borders_at_the_smallest_scales():
+    """int8 scales in [2^-126, 2^-125), half of which is no float when their last bit is odd: quotients on and next to every border."""
+    B, D = 4, 256
+    u = np.float32(2.0 ** -126)
+    tops = [np.float32(127 * (float(u) + i * 2.0 ** -149)) for i in (1, 2, 1025, 3333333, 4194303, 4194305, 7340033, 8388607)] + [np.float32(1.754825e-36)]
+    x = np.zeros((B * len(tops), 1, D), np.float32)
+    for i, top in enumerate(tops):
+        s = float(np.float32(float(top) / 127))
+        b = ((np.arange(-127, 127) + 0.5) * s).astype(np.float32)
+        x[B * i, 0, 0] = top
+        for j, y in enumerate((b, np.nextafter(b, np.float32(np.inf)), np.nextafter(b, np.float32(-np.inf)))):
+            x[B * i + 1 + j, 0, :254] = np.clip(y, -top, top)
+    cache, ref = xp.Kv8(1, D, len(x), B, I8), Ref(1, D, len(x), B, I8)
+    cache.store(x, -x, 0)
+    ref.store(x, -x, 0)
+    code, scale = unpack(cache)
+    n = len(tops)
+    assert np.all(ref.scale[:, :, :n] >= 2.0 ** -126) and np.all(ref.scale[:, :, :n] <= 2.0 ** -125)
+    assert np.array_equal(scale[:, :, :n], ref.scale[:, :, :n])
+    assert np.array_equal(code[:, :, :len(x)], ref.code[:, :, :len(x)])
