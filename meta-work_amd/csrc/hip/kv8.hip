@@ -366,8 +366,9 @@ __host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, i
 
 // Softmax state in powers of two. With t = score + log2(value scale), the weights are
 // kept relative to a reference M that is at least max t - kGrow: w = 2^(t - M) <= 2^kGrow
-// enters as two f16 planes of w * kP (22 bits), whatever the scales' range, the total is of
-// 2^(score - M). The sums are rescaled only when max t passes M by more than kGrow.
+// enters as two f16 planes of w * kP (22 bits), whatever the scales' range: the term 2 * 2^(score - M), of which the total is the
+// sum, times the value scale times kP / 2 (the largest scale, 2^128 / 127, times kP would be infinite). The sums are rescaled only
+// when max t passes M by more than kGrow.
 constexpr float kGrow = 8.f, kP = 128.f;
 
 // Work-group barrier ordering LDS accesses only (global loads in flight stay in flight).
@@ -431,7 +432,7 @@ __device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int
         return;
     }
     const int t = row / G, h = g * G + row % G;
-    const float inv = (1.f / kP) / total;
+    const float inv = (2.f / kP) / total;
     float *op = a.out + t * a.o_tok + (int64_t)h * D + d0;
     f32x4 x[N];
     if (a.gate)
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     __shared__ __align__(16) hf8 qs[NQ][NP][64];
     __shared__ __align__(16) f32x4 sb[4][64];          // scores [16 keys][lane]
     __shared__ __align__(16) uint8_t pb[2][NP][1024];  // weights as operands [32 keys][plane][lane]
-    __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys, of the values times kP, their log2
+    __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys, of the values times kP / 2, their log2
     __shared__ float alb[16], mx[4][16];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
@@ -555,8 +556,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
                 for (int p = NP - 1; p >= 0; p--) x[st & 1] = mfma16(k, q[st][p], x[st & 1]);
             }
             if (w < 2) {
-                sc[par][w][l] = w ? s1 * kP : s1;
-                if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-100f));
+                sc[par][w][l] = w ? s1 * (kP / 2) : s1;
+                if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-99f));
             }
             f32x4 v = x[0] + x[1];
             if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
@@ -598,7 +599,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
                 L *= al;
             }
             if (w == 0 && kq == 0) alb[li] = al;
-            const float ref = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+            const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
             const f32x4 vs = *(const f32x4 *)&sc[par][1][16 * w + 4 * kq];
             float y[4];
 #pragma unroll
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     constexpr int NS = D / 64, NQ = E4 ? 2 * NS : NS, NP = E4 ? 2 : 3;
     constexpr int CT = 2, NV = D / 64;   // columns; a wavefront's units of values
     __shared__ __align__(16) uint8_t pb[2][CT][2][2][1024];   // weights [tile parity][columns][32 keys][plane][lane]
-    __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP, their log2 (and unused)
+    __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP / 2, their log2 (and unused)
     __shared__ float alb[2][CT][16], mx[2][CT][2][16], ms[CT][16];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int cw = w >> 1, u0 = 2 * (w & 1);
@@ -701,8 +702,8 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     auto load_s = [&](int i) { s1 = scp[min(tile(min(i, nt - 1)) * 64 + l, last) >> a.c.lg]; };
     auto put_s = [&](int i) {   // (every pair of wavefronts the same)
         const float x = held(tile(min(i, nt - 1)) * 64 + l, a.sinks, lo, last) ? s1 : 0.f;
-        sc[i & 3][w & 1][l] = w & 1 ? x * kP : x;
-        sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-100f));
+        sc[i & 3][w & 1][l] = w & 1 ? x * (kP / 2) : x;
+        sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-99f));
     };
     load_s(0);
     load_k(0);
@@ -850,7 +851,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
             M = mn;
             L *= al;
             alb[pw][cw][li] = al;
-            const float ref = M == -INFINITY ? 0.f : M;   // (a row that has seen nothing yet: every term is 0)
+            const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
             hf2 hi[4], lo[4];
 #pragma unroll
             for (int v = 0; v < 2; v++) {
@@ -988,7 +989,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(const 
             for (int i = 0; i < V; i++) ((float *)&y)[i] += red[x][i][l];
         }
     }
-    y *= (1.f / kP) / L;
+    y *= (2.f / kP) / L;
     float *op = a.out + t * a.o_tok + (int64_t)h * D + V * l;
     if (a.gate)
 #pragma unroll

@@ -937,3 +937,26 @@ def test_store_borders_at_the_smallest_scales():
     assert np.all(ref.scale[:, :, :n] >= 2.0 ** -126) and np.all(ref.scale[:, :, :n] <= 2.0 ** -125)
     assert np.array_equal(scale[:, :, :n], ref.scale[:, :, :n])
     assert np.array_equal(code[:, :, :len(x)], ref.code[:, :, :len(x)])
+
+
+# (rows of 8, of 16 and of 32 a work-group)
+ROWS = [(3, 2, 700), (4, 4, 700), (200, 8, 1300)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,n", ROWS)
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_attention_of_the_largest_values(kind, T, H, n):
+    """Value blocks whose scale times 128 is no float any more (int8), equal scores."""
+    rng = np.random.default_rng(39)
+    D = 64
+    v = rows(rng, n, 1, D).astype(np.float64)
+    for b in range(0, n, 16):
+        v[b:b + 16] *= float(np.finfo(np.float32).max) * (0.995 if kind == I8 else 0.9) / np.abs(v[b:b + 16]).max()
+    v = v.astype(np.float32)
+    cache, ref = xp.Kv8(1, D, n, 16, kind), Ref(1, D, n, 16, kind)
+    cache.store(v * 0, v, 0)
+    ref.store(v * 0, v, 0)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    for work_bytes in (0, None):
+        _check_attn(cache.attend(q, n - T, work_bytes=work_bytes), *attend64(ref.values(0, n), q, n - T))
