@@ -960,3 +960,34 @@ def test_attention_of_the_largest_values(kind, T, H, n):
     q = rng.standard_normal((T, H, D)).astype(np.float32)
     for work_bytes in (0, None):
         _check_attn(cache.attend(q, n - T, work_bytes=work_bytes), *attend64(ref.values(0, n), q, n - T))
+
+
+def _sized(rng, sizes, n, D, kind):
+    """n positions whose blocks of 16 values have the largest magnitudes `sizes` in turn: the cache and its values in float64."""
+    k, v = rows(rng, n, 1, D), rows(rng, n, 1, D).astype(np.float64)
+    for b in range(0, n, 16):
+        v[b:b + 16] *= sizes[b // 16 % len(sizes)] / np.abs(v[b:b + 16]).max()
+    v = v.astype(np.float32)
+    cache, ref = xp.Kv8(1, D, n, 16, kind), Ref(1, D, n, 16, kind)
+    cache.store(k, v, 0)
+    ref.store(k, v, 0)
+    return cache, ref.values(0, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("work_bytes", [0, None])
+@pytest.mark.parametrize("T,H,n", ROWS)
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_attention_of_values_of_any_size(kind, T, H, n, work_bytes):
+    """Value blocks of very different size, up to the largest floats (those whose codes' values are still floats): everywhere, first, in the
+    middle, last, beside zeros. The small ones count in the total as much as the large ones. Bars as for any size: totals and
+    sums are rounded relative to themselves."""
+    rng = np.random.default_rng(40)
+    top = float(np.finfo(np.float32).max) * (0.995 if kind == I8 else 0.9)
+    q = rng.standard_normal((T, H, 64)).astype(np.float32)
+    blocks = n // 16 + 1
+    for sizes in (np.exp2(rng.integers(-30, 30, blocks)), [top], [1e37], [1e32, 1e-3],
+                  [top] + [1.0] * (blocks - 1), [1.0] * (blocks // 2) + [top] + [1.0] * blocks, [1e-6] * (blocks - 2) + [top] * 2, [1e-30], [0.0, 1e-6]):
+        cache, kv = _sized(rng, sizes, n, 64, kind)
+        want, mag = attend64(kv, q, n - T)
+        _check_attn(cache.attend(q, n - T, work_bytes=work_bytes), want, mag)
