@@ -370,16 +370,11 @@ __host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, i
 // sum, times the value scale times kP / 2 (the largest scale, 2^128 / 127, times kP would be infinite). The sums are rescaled only
 // when max t passes M by more than kGrow.
 constexpr float kGrow = 8.f, kP = 128.f;
-
-// Beside value scales of 2^100 and more the terms of a whole row are so small that the exponential instruction, which leaves out
-// what is below 2^-126, drops those of all but the row's best keys. A work-group that has met a value scale above kBig takes its
-// tiles again with the terms as denormals too (DEN; 2^-149 is 2^-28 of the smallest total). It looks at the end: a check of every
-// tile's sums instead cost the calls that have no such scale 1 to 4%, this none that shows.
-constexpr float kBig = 0x1p64f;
-template <bool DEN>
-__device__ __forceinline__ float term(float x) {
-    const float p = __builtin_amdgcn_exp2f(x);
-    return DEN && x < -100.f ? __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(x + 64.f), -64) : p;
+// 2^(2 x), to the smallest denormal: the exponential instruction leaves out what is below 2^-126, which beside value scales of 2^100 and
+// more are the terms of all but a row's best keys (2^-149 is 2^-28 of the smallest total). One product more for 1 ulp more.
+__device__ __forceinline__ float exp2_twice(float x) {
+    const float h = __builtin_amdgcn_exp2f(x);
+    return h * h;
 }
 
 // Work-group barrier ordering LDS accesses only (global loads in flight stay in flight).
@@ -482,7 +477,6 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     __shared__ __align__(16) uint8_t pb[2][NP][1024];  // weights as operands [32 keys][plane][lane]
     __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys, of the values times kP / 2, their log2
     __shared__ float alb[16], mx[4][16];
-    __shared__ int met;                                // a value scale above kBig
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
     const int g = blockIdx.x % a.c.Hkv, sp = blockIdx.y, r0 = (int)blockIdx.x / a.c.Hkv * R;
@@ -494,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + w * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
     const int64_t s0 = ((int64_t)g * a.c.n_tiles * 64) >> a.c.lg;
     u32x4 kr[A][NS], vr[A][NV];
-    float s1[A] = {}, top = 0.f;   // wavefront 0: the keys' scale of position l; 1: the values', and the largest so far
+    float s1[A] = {};   // wavefront 0: the keys' scale of position l; 1: the values'
     auto tile = [&](int i) { return i < tl.ns ? i : tl.f + i - tl.ns; };
     auto load_k = [&](int kt, u32x4 (&kr)[NS], float &s1) {
         load_units<NS>(kc + (int64_t)kt * 64 * D, l * 16, kr);
@@ -502,16 +496,13 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
         if (w < 2) s1 = held(j, a.sinks, lo, last) ? (w ? a.c.vs : a.c.ks)[s0 + (j >> a.c.lg)] : 0.f;
     };
     auto load_v = [&](int kt, u32x4 (&vr)[NV]) { load_units<NV>(vc + (int64_t)kt * 64 * D, l * 16, vr); };
+    load_k(tile(i0), kr[0], s1[0]);
+    load_v(tile(i0), vr[0]);
     auto ahead = [&](int i) { return tile(A > 1 ? min(i + A, i1 - 1) : i + A); };   // (past the end: the last one again, so that the waits know how many are in flight)
-    auto load_first = [&]() __attribute__((always_inline)) {
-        load_k(tile(i0), kr[0], s1[0]);
-        load_v(tile(i0), vr[0]);
-        if constexpr (A > 1) {
-            load_k(ahead(i0 - 1), kr[A - 1], s1[A - 1]);
-            load_v(ahead(i0 - 1), vr[A - 1]);
-        }
-    };
-    load_first();
+    if constexpr (A > 1) {
+        load_k(ahead(i0 - 1), kr[A - 1], s1[A - 1]);
+        load_v(ahead(i0 - 1), vr[A - 1]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     const int row = r0 + (li & (R - 1)), rq = min(row, rows - 1), t = rq / G, h = g * G + rq % G, pos = np + t;
     // the queries as operands, step i = 2 s + e the dims 64 s + 16 kq + 8 e .. + 7, x 2^-e = hi + lo, e per row
@@ -556,8 +547,10 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 #pragma unroll
         for (int p = 0; p < NP; p++) q[i][p] = qs[i][p][l];
     f32x4 o[NV];
-    float M, L;
-    auto step = [&](int i, u32x4 (&kr)[NS], u32x4 (&vr)[NV], float &s1, auto den) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < NV; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    auto step = [&](int i, u32x4 (&kr)[NS], u32x4 (&vr)[NV], float &s1) {
         const int kt = tile(i), j0 = kt * 64, par = i & 1;
         const bool more = A > 1 || i + A < i1;
         {   // scores
@@ -570,7 +563,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
             }
             if (w < 2) {
                 sc[par][w][l] = w ? s1 * (kP / 2) : s1;
-                if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-99f)), top = fmaxf(top, s1);
+                if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-99f));
             }
             f32x4 v = x[0] + x[1];
             if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
@@ -617,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
             float y[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float p = term<decltype(den)::value>(fmaf(s[0][r], qe, -ref));
+                const float p = exp2_twice(fmaf(s[0][r], 0.5f * qe, -0.5f * ref));
                 L += p;
                 y[r] = p * vs[r];
             }
@@ -658,26 +651,15 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
         }
         if (more) load_v(ahead(i), vr);
     };
-    auto tiles = [&](auto den) __attribute__((always_inline)) {
-#pragma unroll
-        for (int d = 0; d < NV; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        M = -INFINITY, L = 0.f;
-        for (int i = i0; i < i1; i += A) {
-            step(i, kr[0], vr[0], s1[0], den);
-            if (A > 1 && i + 1 < i1) step(i + 1, kr[A - 1], vr[A - 1], s1[A - 1], den);
-        }
-        // the rows' totals
-        L += __shfl_xor(L, 16, 64);
-        L += __shfl_xor(L, 32, 64);
-        if (l < 16) mx[w][l] = L;
-        if (w == 1) met = __any(top > kBig);
-        lds_barrier();
-    };
-    tiles(std::false_type{});
-    if (__builtin_amdgcn_readfirstlane(met)) {
-        load_first();
-        tiles(std::true_type{});
+    for (int i = i0; i < i1; i += A) {
+        step(i, kr[0], vr[0], s1[0]);
+        if (A > 1 && i + 1 < i1) step(i + 1, kr[A - 1], vr[A - 1], s1[A - 1]);
     }
+    // the rows' totals
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (l < 16) mx[w][l] = L;
+    lds_barrier();
     if constexpr (ST)
 #pragma unroll
         for (int d = 0; d < NV; d++) o[d] = f32x4{add_ror8(o[d].x), add_ror8(o[d].y), add_ror8(o[d].z), add_ror8(o[d].w)};
@@ -707,7 +689,6 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     __shared__ __align__(16) uint8_t pb[2][CT][2][2][1024];   // weights [tile parity][columns][32 keys][plane][lane]
     __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP / 2, their log2 (and unused)
     __shared__ float alb[2][CT][16], mx[2][CT][2][16], ms[CT][16];
-    __shared__ int met;                                      // a value scale above kBig
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int cw = w >> 1, u0 = 2 * (w & 1);
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
@@ -720,14 +701,13 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     const uint8_t *kc = a.c.k + (int64_t)g * a.c.n_tiles * 64 * D + u0 * NS * 1024, *vc = a.c.v + (int64_t)g * a.c.n_tiles * 64 * D + w * NV * 1024;
     const float *scp = (w & 1 ? a.c.vs : a.c.ks) + (((int64_t)g * a.c.n_tiles * 64) >> a.c.lg);
     u32x4 kr[2 * NS], vr[NV];
-    float s1, top = 0.f;   // even wavefronts: the keys' scale of a tile's position l; odd: the values'; the largest so far
+    float s1;   // even wavefronts: the keys' scale of a tile's position l; odd: the values'
     auto tile = [&](int i) { return i0 + i < tl.ns ? i0 + i : tl.f + i0 + i - tl.ns; };
     auto load_k = [&](int i) { load_units<2 * NS>(kc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, kr); };
     auto load_v = [&](int i) { load_units<NV>(vc + (int64_t)tile(min(i, nt - 1)) * 64 * D, l * 16, vr); };
     auto load_s = [&](int i) { s1 = scp[min(tile(min(i, nt - 1)) * 64 + l, last) >> a.c.lg]; };
     auto put_s = [&](int i) {   // (every pair of wavefronts the same)
         const float x = held(tile(min(i, nt - 1)) * 64 + l, a.sinks, lo, last) ? s1 : 0.f;
-        top = fmaxf(top, x);
         sc[i & 3][w & 1][l] = w & 1 ? x * (kP / 2) : x;
         sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-99f));
     };
@@ -786,178 +766,168 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
         }
     }
     f32x4 o[CT][NV], s[2];   // sums; products of the tile before with its keys' scales
-    float qe = 1.f, M, L, mt;   // what makes them powers of two; the rows' state and the tile's maximum
-    auto tiles = [&](auto den) __attribute__((always_inline)) {
+    float qe = 1.f;           // what makes them powers of two
 #pragma unroll
-        for (int c = 0; c < CT; c++)
+    for (int c = 0; c < CT; c++)
 #pragma unroll
-            for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        M = mt = -INFINITY, L = 0.f;
-        put_s(0);
-        load_s(1);
-        lds_barrier();
+        for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f, mt = -INFINITY;
+    put_s(0);
+    load_s(1);
+    lds_barrier();
 
-        // steps of the pipeline: the scores of tile i (S), the weights of tile i - 1 (W), the sums of tile i - 2 (P)
-        for (int i = 0; i < nt + 2; i++) {
-            const bool S = i < nt, W = i >= 1 && i <= nt, P = i >= 2;
-            const int par = i & 1, pw = par ^ 1;   // tile i and i - 2; tile i - 1
-            hf8 pf[2][CT];   // weights of half y >> 1, plane 1 - (y & 1): two groups of columns ahead
-            auto get_p = [&](int y) {
+    // steps of the pipeline: the scores of tile i (S), the weights of tile i - 1 (W), the sums of tile i - 2 (P)
+    for (int i = 0; i < nt + 2; i++) {
+        const bool S = i < nt, W = i >= 1 && i <= nt, P = i >= 2;
+        const int par = i & 1, pw = par ^ 1;   // tile i and i - 2; tile i - 1
+        hf8 pf[2][CT];   // weights of half y >> 1, plane 1 - (y & 1): two groups of columns ahead
+        auto get_p = [&](int y) {
 #pragma unroll
-                for (int c = 0; c < CT; c++) pf[y & 1][c] = *(const hf8 *)(pb[par][c][y >> 1][1 - (y & 1)] + l * 16);
-            };
-            if (P) {
-                float al[CT];
+            for (int c = 0; c < CT; c++) pf[y & 1][c] = *(const hf8 *)(pb[par][c][y >> 1][1 - (y & 1)] + l * 16);
+        };
+        if (P) {
+            float al[CT];
 #pragma unroll
-                for (int c = 0; c < CT; c++) al[c] = alb[par][c][li];
-                get_p(0);
-                get_p(1);
-                bool any = false;
+            for (int c = 0; c < CT; c++) al[c] = alb[par][c][li];
+            get_p(0);
+            get_p(1);
+            bool any = false;
 #pragma unroll
-                for (int c = 0; c < CT; c++) any |= al[c] != 1.f;
-                if (__any(any))
+            for (int c = 0; c < CT; c++) any |= al[c] != 1.f;
+            if (__any(any))
 #pragma unroll
-                    for (int c = 0; c < CT; c++)
+                for (int c = 0; c < CT; c++)
 #pragma unroll
-                        for (int d = 0; d < NV; d++) o[c][d] *= al[c];
-                if (E4) {
-                    const int j0 = tile(i - 2) * 64;
-                    if (tile_part(j0, a.sinks, lo, last)) {
-                        const u32x4 m = held_bytes(j0, a.sinks, lo, last);
+                    for (int d = 0; d < NV; d++) o[c][d] *= al[c];
+            if (E4) {
+                const int j0 = tile(i - 2) * 64;
+                if (tile_part(j0, a.sinks, lo, last)) {
+                    const u32x4 m = held_bytes(j0, a.sinks, lo, last);
 #pragma unroll
-                        for (int d = 0; d < NV; d++) vr[d] &= m;
-                    }
+                    for (int d = 0; d < NV; d++) vr[d] &= m;
                 }
             }
-            f32x4 y[2];
-            if (S) {
-                if constexpr (E4) {
-                    f32x4 x[2][2];
+        }
+        f32x4 y[2];
+        if (S) {
+            if constexpr (E4) {
+                f32x4 x[2][2];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) x[u][0] = x[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < 2; u++) x[u][0] = x[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int st = 0; st < NQ; st++)
+                for (int st = 0; st < NQ; st++)
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const u32x4 &k4 = kr[u * NS + (st >> 1)];
-                            const hf8 k = to_half<E4>(k4[2 * (st & 1)], k4[2 * (st & 1) + 1]);
+                    for (int u = 0; u < 2; u++) {
+                        const u32x4 &k4 = kr[u * NS + (st >> 1)];
+                        const hf8 k = to_half<E4>(k4[2 * (st & 1)], k4[2 * (st & 1) + 1]);
 #pragma unroll
-                            for (int p = 0; p < 2; p++) {
-                                hf8 qq;
-                                __builtin_memcpy(&qq, &q[st][p], 16);
-                                x[u][p] = mfma16(k, qq, x[u][p]);
-                            }
+                        for (int p = 0; p < 2; p++) {
+                            hf8 qq;
+                            __builtin_memcpy(&qq, &q[st][p], 16);
+                            x[u][p] = mfma16(k, qq, x[u][p]);
                         }
+                    }
 #pragma unroll
-                    for (int u = 0; u < 2; u++) y[u] = x[u][0] + x[u][1];
-                } else {
-                    i32x4 x[2][3];
+                for (int u = 0; u < 2; u++) y[u] = x[u][0] + x[u][1];
+            } else {
+                i32x4 x[2][3];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int p = 0; p < 3; p++) x[u][p] = i32x4{0, 0, 0, 0};
+                    for (int p = 0; p < 3; p++) x[u][p] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int st = 0; st < NS; st++)
+                for (int st = 0; st < NS; st++)
 #pragma unroll
-                        for (int p = 0; p < 3; p++)
+                    for (int p = 0; p < 3; p++)
 #pragma unroll
-                            for (int u = 0; u < 2; u++)
-                                x[u][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)kr[u * NS + st], (i32x4)q[st][p], x[u][p], 0, 0, 0);
+                        for (int u = 0; u < 2; u++)
+                            x[u][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)kr[u * NS + st], (i32x4)q[st][p], x[u][p], 0, 0, 0);
 #pragma unroll
-                    for (int u = 0; u < 2; u++)   // a digit's sum is below 2^23
+                for (int u = 0; u < 2; u++)   // a digit's sum is below 2^23
 #pragma unroll
-                        for (int r = 0; r < 4; r++) y[u][r] = fmaf((float)x[u][2][r], 65536.f, (float)((x[u][1][r] << 8) + x[u][0][r]));
-                }
-                load_k(i + 1);
+                    for (int r = 0; r < 4; r++) y[u][r] = fmaf((float)x[u][2][r], 65536.f, (float)((x[u][1][r] << 8) + x[u][0][r]));
             }
-            if (W) {
-                const float mm = fmaxf(mt, mx[pw][cw][1 - (w & 1)][li]);
-                // (the two wavefronts of the rows agree)
-                const float mn = mm > M + kGrow || M == -INFINITY ? fmaxf(M, mm) : M;
-                const float ah = mn == M ? 1.f : __builtin_amdgcn_exp2f(0.5f * (M - mn));
-                M = mn;
-                L = L * ah * ah;
-                alb[pw][cw][li] = ah * ah;
-                const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
-                hf2 hi[4], lo[4];
+            load_k(i + 1);
+        }
+        if (W) {
+            const float mm = fmaxf(mt, mx[pw][cw][1 - (w & 1)][li]);
+            // (the two wavefronts of the rows agree)
+            const float mn = mm > M + kGrow || M == -INFINITY ? fmaxf(M, mm) : M;
+            const float h = mn == M ? 1.f : __builtin_amdgcn_exp2f(0.5f * (M - mn));
+            M = mn;
+            L = L * h * h;   // (in steps: a float where h * h may be none)
+            alb[pw][cw][li] = h * h;
+            const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
+            hf2 hi[4], lo[4];
 #pragma unroll
-                for (int v = 0; v < 2; v++) {
-                    const f32x4 vs = *(const f32x4 *)&sc[(i - 1) & 3][1][16 * (u0 + v) + 4 * kq];
-                    float z[4];
+            for (int v = 0; v < 2; v++) {
+                const f32x4 vs = *(const f32x4 *)&sc[(i - 1) & 3][1][16 * (u0 + v) + 4 * kq];
+                float z[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float p = exp2_twice(fmaf(s[v][r], 0.5f * qe, -0.5f * ref));
+                    L += p;
+                    z[r] = p * vs[r];
+                }
+                split2(z[0], z[1], hi[2 * v], lo[2 * v]);
+                split2(z[2], z[3], hi[2 * v + 1], lo[2 * v + 1]);
+            }
+            *(hf8 *)(pb[pw][cw][w & 1][0] + l * 16) = join8(hi[0], hi[1], hi[2], hi[3]);
+            *(hf8 *)(pb[pw][cw][w & 1][1] + l * 16) = join8(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (S) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
+            const int j0 = tile(i) * 64;
+            qe = qsc;
+            if (tile_edge(a, j0, p0, p1)) {
+                qe = 1.f;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float p = term<decltype(den)::value>(fmaf(s[v][r], qe, -ref));
-                        L += p;
-                        z[r] = p * vs[r];
+                        const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
+                        const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+                        s[u][r] = see ? s[u][r] * qsc : -INFINITY;
                     }
-                    split2(z[0], z[1], hi[2 * v], lo[2 * v]);
-                    split2(z[2], z[3], hi[2 * v + 1], lo[2 * v + 1]);
-                }
-                *(hf8 *)(pb[pw][cw][w & 1][0] + l * 16) = join8(hi[0], hi[1], hi[2], hi[3]);
-                *(hf8 *)(pb[pw][cw][w & 1][1] + l * 16) = join8(lo[0], lo[1], lo[2], lo[3]);
             }
-            if (S) {
+            mt = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
-                const int j0 = tile(i) * 64;
-                qe = qsc;
-                if (tile_edge(a, j0, p0, p1)) {
-                    qe = 1.f;
+            for (int u = 0; u < 2; u++) {
+                const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
-                            const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-                            s[u][r] = see ? s[u][r] * qsc : -INFINITY;
-                        }
-                }
-                mt = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
-                }
-                mt = max_x16(max_x32(mt));
-                mx[par][cw][w & 1][li] = mt;
-                put_s(i + 1);
-                load_s(i + 2);
+                for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
             }
-            if (P) {
-                hf8 v[NV];
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    if (!(x & 1))
-#pragma unroll
-                        for (int d = 0; d < NV; d++) v[d] = to_half<E4>(vr[d][x], vr[d][x + 1]);
-#pragma unroll
-                    for (int d = 0; d < NV; d++)
-#pragma unroll
-                        for (int c = 0; c < CT; c++) o[c][d] = mfma16(v[d], pf[x & 1][c], o[c][d]);
-                    if (x < 2) get_p(x + 2);
-                }
-                load_v(i - 1);
-            }
-            lds_barrier();
+            mt = max_x16(max_x32(mt));
+            mx[par][cw][w & 1][li] = mt;
+            put_s(i + 1);
+            load_s(i + 2);
         }
-        // the rows' totals
-        L += __shfl_xor(L, 16, 64);
-        L += __shfl_xor(L, 32, 64);
-        if (l < 16) {
-            mx[0][cw][w & 1][l] = L;
-            if (u0 == 0) ms[cw][l] = M;
+        if (P) {
+            hf8 v[NV];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                if (!(x & 1))
+#pragma unroll
+                    for (int d = 0; d < NV; d++) v[d] = to_half<E4>(vr[d][x], vr[d][x + 1]);
+#pragma unroll
+                for (int d = 0; d < NV; d++)
+#pragma unroll
+                    for (int c = 0; c < CT; c++) o[c][d] = mfma16(v[d], pf[x & 1][c], o[c][d]);
+                if (x < 2) get_p(x + 2);
+            }
+            load_v(i - 1);
         }
-        if (w == 1) met = __any(top > kBig);
         lds_barrier();
-    };
-    tiles(std::false_type{});
-    if (__builtin_amdgcn_readfirstlane(met)) {
-        load_s(0);
-        load_k(0);
-        load_v(0);
-        tiles(std::true_type{});
     }
+    // the rows' totals
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    if (l < 16) {
+        mx[0][cw][w & 1][l] = L;
+        if (u0 == 0) ms[cw][l] = M;
+    }
+    lds_barrier();
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         const int row = r0 + 16 * c + li;   // register r of o[d]: dim 16 (w NV + d) + 4 kq + r
