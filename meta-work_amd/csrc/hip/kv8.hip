@@ -673,8 +673,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 //   scores, weights  16 rows (w >> 1) by 32 keys (w & 1): the rows' queries and the scores stay in registers, the two
 //                    wavefronts of the rows exchange their maxima and all of them the weights through LDS
 //   sums             a quarter of the dims for all rows
-// int8 keys are matrix operands as they are: the queries are 24-bit integers per row in three signed digits of 8 bits
-// (x = X 2^e, |X| <= 2^22), every product and sum is exact until the digits' sums are joined in fp32.
+// int8 keys are matrix operands as they are: the queries are integers per row in signed digits of 8 bits (x = X 2^e, |X| <= 2^30),
+// every product and sum is exact until the digits' sums are joined in fp32. Three digits hold an element of 2^-k of its row's
+// largest to 22 - k bits: at most 2^-19 of the mean magnitude where the largest is 8 times that, as little as fp32's own roundings
+// of a score. Work-groups with a row whose largest is above that (a channel far above the others; three digits are off by 1e-4 in a
+// weight at 1000 times) take four digits, 30 - k bits, for 3 to 7% of the time.
 // 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 87 to 90 us, 390 TFLOP/s (twice that in matrix instructions' f16 rate); at
 // 6144 positions 465 us, 515. Bound by a wavefront's own chain: of a step's 3480 cycles at D = 256 the scores take 780, the weights
 // 570, the softmax's end 800, the sums 950 and barrier and loads 350, and two work-groups a CU overlap only part of it (the products
@@ -682,6 +685,17 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 // 64 rows shared through LDS, two groups of wavefronts in opposite steps, wavefronts with different roles, and the vector
 // instructions placed among the products.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// Four values times 2^(16 - e) as integers, the bytes of X + 0x80808080; each less 128 is one of X's signed digits. Digit p of the four.
+__device__ __forceinline__ u32x4 digits(const f32x4 x, int e) {
+    u32x4 X;
+#pragma unroll
+    for (int r = 0; r < 4; r++) X[r] = ((uint32_t)(int)rintf(ldexpf(x[r], 16 - e)) + 0x80808080u) ^ 0x80808080u;
+    return X;
+}
+__device__ __forceinline__ uint32_t digit(const u32x4 X, int p) {
+    const uint32_t sel = (uint32_t)p | (uint32_t)(4 + p) << 8 | 0x0c0c0000u;
+    return __builtin_amdgcn_perm(X[1], X[0], sel) | __builtin_amdgcn_perm(X[3], X[2], sel) << 16;
+}
 template <int D, bool E4>
 __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) {
     constexpr int NS = D / 64, NQ = E4 ? 2 * NS : NS, NP = E4 ? 2 : 3;
@@ -689,6 +703,8 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     __shared__ __align__(16) uint8_t pb[2][CT][2][2][1024];   // weights [tile parity][columns][32 keys][plane][lane]
     __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP / 2, their log2 (and unused)
     __shared__ float alb[2][CT][16], mx[2][CT][2][16], ms[CT][16];
+    __shared__ __align__(16) u32x4 qd[CT][E4 ? 1 : NS][64];   // int8: the queries' fourth digits
+    __shared__ int large[4];                                  // int8: a row has a large channel
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int cw = w >> 1, u0 = 2 * (w & 1);
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
@@ -717,26 +733,31 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     __builtin_amdgcn_sched_barrier(0);
     // the wavefront's queries as operands, an exponent per row; the two wavefronts of the rows prepare them both
     const int rq = min(r0 + 16 * cw + li, rows - 1), tq = rq / G, pos = np + tq;
-    u32x4 q[NQ][NP];
+    u32x4 q[NQ][NP];   // int8: the first three digits
     float qsc;
     {
         const float *qp = a.q + tq * a.q_tok + (g * G + rq % G) * a.q_head + 16 * kq;
         f32x4 x[4 * NS];
-        float m = 0.f;
+        float m = 0.f, sum = 0.f;
         bool fin = true;
 #pragma unroll
         for (int i = 0; i < 4 * NS; i++) {
             x[i] = *(const f32x4_u *)(qp + 64 * (i >> 2) + 4 * (i & 3));
 #pragma unroll
-            for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[i][r])), fin &= fabsf(x[i][r]) < INFINITY;
+            for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[i][r])), sum += fabsf(x[i][r]), fin &= fabsf(x[i][r]) < INFINITY;
         }
         m = max_x16(max_x32(m));
+        if constexpr (!E4) {
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            large[w] = __any(m * (D / 8) > sum);
+        }
         const uint64_t bad = ~__ballot(fin);   // a NaN or infinity, which integers do not hold, is put into the row's factor
         fin = !((bad >> li | bad >> (li + 16) | bad >> (li + 32) | bad >> (li + 48)) & 1);
         int e = 0;
         if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-        e = max(e, -100) - (E4 ? 14 : 22);
-        qsc = fin ? ldexpf(a.scale * 1.44269504088896341f, e) : NAN;   // what a product is multiplied with
+        e = max(e, -100) - 14;
+        qsc = fin ? ldexpf(a.scale * 1.44269504088896341f, e) : NAN;   // what a product (of int8, its 2^-16) is multiplied with
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             if constexpr (E4) {
@@ -751,175 +772,188 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
                     __builtin_memcpy(&q[2 * s + y][1], &ql, 16);
                 }
             } else {
+                u32x4 q4;
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    uint32_t X[4];   // the bytes of X + 0x808080, each less 128, are its signed digits
+                    const u32x4 X = digits(x[4 * s + y], e);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) X[r] = ((uint32_t)(int)rintf(ldexpf(x[4 * s + y][r], -e)) + 0x808080u) ^ 0x808080u;
-#pragma unroll
-                    for (int p = 0; p < 3; p++) {
-                        const uint32_t sel = (uint32_t)p | (uint32_t)(4 + p) << 8 | 0x0c0c0000u;
-                        q[s][p][y] = __builtin_amdgcn_perm(X[1], X[0], sel) | __builtin_amdgcn_perm(X[3], X[2], sel) << 16;
-                    }
+                    for (int p = 0; p < 3; p++) q[s][p][y] = digit(X, 3 - p);
+                    q4[y] = digit(X, 0);
                 }
+                if (u0 == 0) qd[cw][s][l] = q4;
             }
         }
     }
     f32x4 o[CT][NV], s[2];   // sums; products of the tile before with its keys' scales
-    float qe = 1.f;           // what makes them powers of two
-#pragma unroll
-    for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float M = -INFINITY, L = 0.f, mt = -INFINITY;
+    float qe = 1.f, M, L, mt;   // what makes them powers of two
     put_s(0);
     load_s(1);
     lds_barrier();
 
-    // steps of the pipeline: the scores of tile i (S), the weights of tile i - 1 (W), the sums of tile i - 2 (P)
-    for (int i = 0; i < nt + 2; i++) {
-        const bool S = i < nt, W = i >= 1 && i <= nt, P = i >= 2;
-        const int par = i & 1, pw = par ^ 1;   // tile i and i - 2; tile i - 1
-        hf8 pf[2][CT];   // weights of half y >> 1, plane 1 - (y & 1): two groups of columns ahead
-        auto get_p = [&](int y) {
+    auto tiles = [&](auto n_digits) __attribute__((always_inline)) {
+        constexpr int ND = decltype(n_digits)::value;
 #pragma unroll
-            for (int c = 0; c < CT; c++) pf[y & 1][c] = *(const hf8 *)(pb[par][c][y >> 1][1 - (y & 1)] + l * 16);
-        };
-        if (P) {
-            float al[CT];
+        for (int c = 0; c < CT; c++)
 #pragma unroll
-            for (int c = 0; c < CT; c++) al[c] = alb[par][c][li];
-            get_p(0);
-            get_p(1);
-            bool any = false;
+            for (int d = 0; d < NV; d++) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        M = mt = -INFINITY, L = 0.f;
+        u32x4 q4[ND > 3 ? NS : 1];
+        if constexpr (ND > 3)
 #pragma unroll
-            for (int c = 0; c < CT; c++) any |= al[c] != 1.f;
-            if (__any(any))
+            for (int st = 0; st < NS; st++) q4[st] = qd[cw][st][l];
+
+        // steps of the pipeline: the scores of tile i (S), the weights of tile i - 1 (W), the sums of tile i - 2 (P)
+        for (int i = 0; i < nt + 2; i++) {
+            const bool S = i < nt, W = i >= 1 && i <= nt, P = i >= 2;
+            const int par = i & 1, pw = par ^ 1;   // tile i and i - 2; tile i - 1
+            hf8 pf[2][CT];   // weights of half y >> 1, plane 1 - (y & 1): two groups of columns ahead
+            auto get_p = [&](int y) {
 #pragma unroll
-                for (int c = 0; c < CT; c++)
+                for (int c = 0; c < CT; c++) pf[y & 1][c] = *(const hf8 *)(pb[par][c][y >> 1][1 - (y & 1)] + l * 16);
+            };
+            if (P) {
+                float al[CT];
 #pragma unroll
-                    for (int d = 0; d < NV; d++) o[c][d] *= al[c];
-            if (E4) {
-                const int j0 = tile(i - 2) * 64;
-                if (tile_part(j0, a.sinks, lo, last)) {
-                    const u32x4 m = held_bytes(j0, a.sinks, lo, last);
+                for (int c = 0; c < CT; c++) al[c] = alb[par][c][li];
+                get_p(0);
+                get_p(1);
+                bool any = false;
 #pragma unroll
-                    for (int d = 0; d < NV; d++) vr[d] &= m;
-                }
-            }
-        }
-        f32x4 y[2];
-        if (S) {
-            if constexpr (E4) {
-                f32x4 x[2][2];
+                for (int c = 0; c < CT; c++) any |= al[c] != 1.f;
+                if (__any(any))
 #pragma unroll
-                for (int u = 0; u < 2; u++) x[u][0] = x[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int st = 0; st < NQ; st++)
+                        for (int d = 0; d < NV; d++) o[c][d] *= al[c];
+                if (E4) {
+                    const int j0 = tile(i - 2) * 64;
+                    if (tile_part(j0, a.sinks, lo, last)) {
+                        const u32x4 m = held_bytes(j0, a.sinks, lo, last);
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const u32x4 &k4 = kr[u * NS + (st >> 1)];
-                        const hf8 k = to_half<E4>(k4[2 * (st & 1)], k4[2 * (st & 1) + 1]);
-#pragma unroll
-                        for (int p = 0; p < 2; p++) {
-                            hf8 qq;
-                            __builtin_memcpy(&qq, &q[st][p], 16);
-                            x[u][p] = mfma16(k, qq, x[u][p]);
-                        }
+                        for (int d = 0; d < NV; d++) vr[d] &= m;
                     }
-#pragma unroll
-                for (int u = 0; u < 2; u++) y[u] = x[u][0] + x[u][1];
-            } else {
-                i32x4 x[2][3];
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int p = 0; p < 3; p++) x[u][p] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int st = 0; st < NS; st++)
-#pragma unroll
-                    for (int p = 0; p < 3; p++)
-#pragma unroll
-                        for (int u = 0; u < 2; u++)
-                            x[u][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)kr[u * NS + st], (i32x4)q[st][p], x[u][p], 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 2; u++)   // a digit's sum is below 2^23
-#pragma unroll
-                    for (int r = 0; r < 4; r++) y[u][r] = fmaf((float)x[u][2][r], 65536.f, (float)((x[u][1][r] << 8) + x[u][0][r]));
-            }
-            load_k(i + 1);
-        }
-        if (W) {
-            const float mm = fmaxf(mt, mx[pw][cw][1 - (w & 1)][li]);
-            // (the two wavefronts of the rows agree)
-            const float mn = mm > M + kGrow || M == -INFINITY ? fmaxf(M, mm) : M;
-            const float h = mn == M ? 1.f : __builtin_amdgcn_exp2f(0.5f * (M - mn));
-            M = mn;
-            L = L * h * h;   // (in steps: a float where h * h may be none)
-            alb[pw][cw][li] = h * h;
-            const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
-            hf2 hi[4], lo[4];
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const f32x4 vs = *(const f32x4 *)&sc[(i - 1) & 3][1][16 * (u0 + v) + 4 * kq];
-                float z[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float p = exp2_twice(fmaf(s[v][r], 0.5f * qe, -0.5f * ref));
-                    L += p;
-                    z[r] = p * vs[r];
                 }
-                split2(z[0], z[1], hi[2 * v], lo[2 * v]);
-                split2(z[2], z[3], hi[2 * v + 1], lo[2 * v + 1]);
             }
-            *(hf8 *)(pb[pw][cw][w & 1][0] + l * 16) = join8(hi[0], hi[1], hi[2], hi[3]);
-            *(hf8 *)(pb[pw][cw][w & 1][1] + l * 16) = join8(lo[0], lo[1], lo[2], lo[3]);
-        }
-        if (S) {
+            f32x4 y[2];
+            if (S) {
+                if constexpr (E4) {
+                    f32x4 x[2][2];
 #pragma unroll
-            for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
-            const int j0 = tile(i) * 64;
-            qe = qsc;
-            if (tile_edge(a, j0, p0, p1)) {
-                qe = 1.f;
+                    for (int u = 0; u < 2; u++) x[u][0] = x[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                    for (int st = 0; st < NQ; st++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const u32x4 &k4 = kr[u * NS + (st >> 1)];
+                            const hf8 k = to_half<E4>(k4[2 * (st & 1)], k4[2 * (st & 1) + 1]);
+#pragma unroll
+                            for (int p = 0; p < 2; p++) {
+                                hf8 qq;
+                                __builtin_memcpy(&qq, &q[st][p], 16);
+                                x[u][p] = mfma16(k, qq, x[u][p]);
+                            }
+                        }
+#pragma unroll
+                    for (int u = 0; u < 2; u++) y[u] = x[u][0] + x[u][1];
+                } else {
+                    i32x4 x[2][ND];
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int p = 0; p < ND; p++) x[u][p] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int st = 0; st < NS; st++)
+#pragma unroll
+                        for (int p = 0; p < ND; p++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++)
+                                x[u][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8((i32x4)kr[u * NS + st], (i32x4)(p < 3 ? q[st][p] : q4[st]), x[u][p], 0, 0, 0);
+#pragma unroll
+                    for (int u = 0; u < 2; u++)   // a digit's sum is 2^22 at most
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int hi = (x[u][0][r] << 8) + x[u][1][r], lo = ND > 3 ? (x[u][2][r] << 8) + x[u][ND - 1][r] : x[u][2][r];
+                            y[u][r] = fmaf((float)lo, ND > 3 ? 0x1p-16f : 0x1p-8f, (float)hi);
+                        }
+                }
+                load_k(i + 1);
+            }
+            if (W) {
+                const float mm = fmaxf(mt, mx[pw][cw][1 - (w & 1)][li]);
+                // (the two wavefronts of the rows agree)
+                const float mn = mm > M + kGrow || M == -INFINITY ? fmaxf(M, mm) : M;
+                const float h = mn == M ? 1.f : __builtin_amdgcn_exp2f(0.5f * (M - mn));
+                M = mn;
+                L = L * h * h;   // (in steps: a float where h * h may be none)
+                alb[pw][cw][li] = h * h;
+                const float ref = M == -INFINITY ? 0.f : M - 1.f;   // (a row that has seen nothing yet: every term is 0)
+                hf2 hi[4], lo[4];
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const f32x4 vs = *(const f32x4 *)&sc[(i - 1) & 3][1][16 * (u0 + v) + 4 * kq];
+                    float z[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
-                        const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-                        s[u][r] = see ? s[u][r] * qsc : -INFINITY;
+                        const float p = exp2_twice(fmaf(s[v][r], 0.5f * qe, -0.5f * ref));
+                        L += p;
+                        z[r] = p * vs[r];
                     }
+                    split2(z[0], z[1], hi[2 * v], lo[2 * v]);
+                    split2(z[2], z[3], hi[2 * v + 1], lo[2 * v + 1]);
+                }
+                *(hf8 *)(pb[pw][cw][w & 1][0] + l * 16) = join8(hi[0], hi[1], hi[2], hi[3]);
+                *(hf8 *)(pb[pw][cw][w & 1][1] + l * 16) = join8(lo[0], lo[1], lo[2], lo[3]);
             }
-            mt = -INFINITY;
+            if (S) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
+                for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
+                const int j0 = tile(i) * 64;
+                qe = qsc;
+                if (tile_edge(a, j0, p0, p1)) {
+                    qe = 1.f;
 #pragma unroll
-                for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
+                            const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+                            s[u][r] = see ? s[u][r] * qsc : -INFINITY;
+                        }
+                }
+                mt = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
+                }
+                mt = max_x16(max_x32(mt));
+                mx[par][cw][w & 1][li] = mt;
+                put_s(i + 1);
+                load_s(i + 2);
             }
-            mt = max_x16(max_x32(mt));
-            mx[par][cw][w & 1][li] = mt;
-            put_s(i + 1);
-            load_s(i + 2);
+            if (P) {
+                hf8 v[NV];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    if (!(x & 1))
+#pragma unroll
+                        for (int d = 0; d < NV; d++) v[d] = to_half<E4>(vr[d][x], vr[d][x + 1]);
+#pragma unroll
+                    for (int d = 0; d < NV; d++)
+#pragma unroll
+                        for (int c = 0; c < CT; c++) o[c][d] = mfma16(v[d], pf[x & 1][c], o[c][d]);
+                    if (x < 2) get_p(x + 2);
+                }
+                load_v(i - 1);
+            }
+            lds_barrier();
         }
-        if (P) {
-            hf8 v[NV];
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                if (!(x & 1))
-#pragma unroll
-                    for (int d = 0; d < NV; d++) v[d] = to_half<E4>(vr[d][x], vr[d][x + 1]);
-#pragma unroll
-                for (int d = 0; d < NV; d++)
-#pragma unroll
-                    for (int c = 0; c < CT; c++) o[c][d] = mfma16(v[d], pf[x & 1][c], o[c][d]);
-                if (x < 2) get_p(x + 2);
-            }
-            load_v(i - 1);
-        }
-        lds_barrier();
-    }
+    };
+    int four = E4 ? 0 : __builtin_amdgcn_readfirstlane(large[0] | large[2]);
+    if (!four) tiles(std::integral_constant<int, 3>{});
+    if (!E4) asm volatile("" : "+s"(four));   // (as one choice of two the loops take 20 registers more, and spill at D = 256)
+    if (four) tiles(std::integral_constant<int, 4>{});
     // the rows' totals
     L += __shfl_xor(L, 16, 64);
     L += __shfl_xor(L, 32, 64);

@@ -991,3 +991,24 @@ def test_attention_of_values_of_any_size(kind, T, H, n, work_bytes):
         cache, kv = _sized(rng, sizes, n, 64, kind)
         want, mag = attend64(kv, q, n - T)
         _check_attn(cache.attend(q, n - T, work_bytes=work_bytes), want, mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,n", ROWS)
+@pytest.mark.parametrize("ratio,D", [(4, 64), (16, 128), (100, 256), (1000, 64)])
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_attention_of_queries_with_a_large_channel(kind, ratio, D, T, H, n):
+    """Queries with one channel `ratio` times the others, keys that are small in it, so that every channel moves the scores alike. A query
+    element is off by 2^-22 of itself or by 2^-30 of its row's largest, about 4 `ratio`: 4e-6 at 1000, a third of which, on the root of mean squares,
+    enters a score of D channels over the root of D, so 1.3e-6 of a weight and, over hundreds of independent weights, less than the bars of any query."""
+    rng = np.random.default_rng(41)
+    c = 11
+    k, v = rows(rng, n, 1, D), rows(rng, n, 1, D)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    k[..., c] /= ratio
+    q[..., c] *= ratio
+    # a block's scale is its largest element's: the small channel's keys are few codes, which the float64 form takes as they are
+    cache = xp.Kv8(1, D, n, 1, kind)
+    cache.store(k, v, 0)
+    kv = np.stack(cache.load(0, n))
+    _check_attn(cache.attend(q, n - T), *attend64(kv, q, n - T))
