@@ -470,7 +470,7 @@ typedef struct {
  * t*x_tok + h*x_head, out likewise), token t at position pos[t] (device, may be
  * negative) or, with pos NULL, pos0 + t. out == x with equal strides rotates
  * in place; other overlaps are not allowed. The angles are formed in double, so far positions keep
- * theirs (xjh_rope evaluates them in float, as the reference does). */
+ * theirs (xjh_rope evaluates them in float, as the reference does). n_heads * D is at most 2^30. */
 int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, float *out, int64_t o_tok, int64_t o_head, int T,
                     int n_heads, int D, const xjh_rope_cfg *cfg, const int32_t *pos, int pos0, void *stream,
                     char *err, size_t errlen);

@@ -69,7 +69,7 @@ bool range_ok(const xjh_kv8 *c, int T, int n_past, const char *what, char *err, 
 extern "C" int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, float *out, int64_t o_tok, int64_t o_head,
                                int T, int n_heads, int D, const xjh_rope_cfg *cfg, const int32_t *pos, int pos0,
                                void *stream, char *err, size_t errlen) {
-    if (!cfg || T < 0 || n_heads < 0 || D < 2 || cfg->n_rot < 2 || cfg->n_rot % 2 || cfg->n_rot > D ||
+    if (!cfg || T < 0 || n_heads < 0 || D < 2 || (int64_t)n_heads * D > (1 << 30) || cfg->n_rot < 2 || cfg->n_rot % 2 || cfg->n_rot > D ||
         cfg->n_rot / 2 > kRopeMaxPairs || (cfg->pairs != XJH_ROPE_HALF && cfg->pairs != XJH_ROPE_INTERLEAVED)) {
         snprintf(err, errlen, "rope_scaled: bad shape (T=%d, heads=%d, D=%d, n_rot=%d, pairs=%d)", T, n_heads, D,
                  cfg ? cfg->n_rot : 0, cfg ? cfg->pairs : 0);

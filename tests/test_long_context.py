@@ -1012,3 +1012,13 @@ def test_attention_of_queries_with_a_large_channel(kind, ratio, D, T, H, n):
     cache.store(k, v, 0)
     kv = np.stack(cache.load(0, n))
     _check_attn(cache.attend(q, n - T), *attend64(kv, q, n - T))
+
+
+@pytest.mark.parametrize("n_heads,D", [((1 << 31) - 1, 2), ((1 << 23) + 1, 128), (1, (1 << 30) + 1), (1 << 20, 1 << 20)])
+def test_rope_refuses_tokens_of_more_elements_than_a_work_group_counts(n_heads, D):
+    """n_heads * D above 2^30: the kernel's index of a token's elements would pass 31 bits."""
+    err = C.create_string_buffer(xp.ERR)
+    for T in (0, 1):
+        assert xp.lib().xjh_rope_scaled(4096, D, D, 4096, D, D, T, n_heads, D, _cfg(n_rot=2), None, 0, None, err, xp.ERR) == -1
+        assert b"bad shape" in err.value
+    assert xp.lib().xjh_rope_scaled(4096, 128, 128, 4096, 128, 128, 0, 1 << 23, 128, _cfg(n_rot=2), None, 0, None, err, xp.ERR) == 0
