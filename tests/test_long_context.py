@@ -1022,3 +1022,67 @@ def test_rope_refuses_tokens_of_more_elements_than_a_work_group_counts(n_heads, 
         assert xp.lib().xjh_rope_scaled(4096, D, D, 4096, D, D, T, n_heads, D, _cfg(n_rot=2), None, 0, None, err, xp.ERR) == -1
         assert b"bad shape" in err.value
     assert xp.lib().xjh_rope_scaled(4096, 128, 128, 4096, 128, 128, 0, 1 << 23, 128, _cfg(n_rot=2), None, 0, None, err, xp.ERR) == 0
+
+
+@pytest.mark.gpu
+def test_cache_beyond_four_gigabytes_of_cleared_memory():
+    """As test_cache_beyond_four_gigabytes, with the begun block's bytes and scale cleared first, as the store asks for."""
+    rng = np.random.default_rng(42)
+    hip, Hkv, D, n_ctx = Hip(), 8, 256, 1 << 21
+    for kind in (I8, E4):
+        c = xp.XjhKv8(type=kind, Hkv=Hkv, D=D, n_ctx=n_ctx, block=64)
+        c.bytes = xp.lib().xjh_kv8_bytes(C.byref(c))
+        assert c.bytes > 1 << 33
+        buf = xp.Dev(nbytes=c.bytes)
+        c.data = buf.ptr
+        hip("hipMemset", C.c_void_p(buf.ptr), C.c_int(0), C.c_size_t(c.bytes))
+        n, n0 = 300, n_ctx - 300
+        k, v = rows(rng, n, Hkv, D), rows(rng, n, Hkv, D)
+        dk, dv, ok, ov = xp.Dev(k), xp.Dev(v), xp.Dev(nbytes=k.nbytes), xp.Dev(nbytes=v.nbytes)
+        row, cc = Hkv * D, C.byref(c)
+        _call("xjh_kv8_store", cc, dk.ptr, row, dv.ptr, row, n, n0, None, None)
+        _call("xjh_kv8_load", cc, n0, n, ok.ptr, row, ov.ptr, row, None)
+        xp.lib().xjh_sync()
+        ref = Ref(Hkv, D, n + 64, 64, kind)
+        ref.store(k, v, n0 % 64)
+        want = ref.values(n0 % 64, n).astype(np.float32)
+        assert np.array_equal(ok.get(np.float32, k.shape), want[0]) and np.array_equal(ov.get(np.float32, k.shape), want[1])
+        buf.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("Hkv,G,D,T,window,n_sink", [(2, 4, 64, 1, 0, 0), (1, 4, 128, 5, 0, 0), (1, 4, 64, 40, 0, 0), (1, 4, 64, 5, 1000, 70)])
+def test_captured_step_far_below_its_bound(Hkv, G, D, T, window, n_sink, kind):
+    """A step captured with a bound of 60000 positions and replayed at a few hundred and a few thousand, from the first on."""
+    rng = np.random.default_rng(43)
+    hip, n_max = Hip(), 60000
+    s = _Step(Hkv, G, D, n_max + T, 32, kind, T, n_max, window, n_sink)
+    st = hip.stream()
+    g = hip.capture(st, s.run)
+    n = 0
+    for gap in (0, 3, 190, 1, 2100, 2500):
+        if gap:
+            s.cache.store(rows(rng, gap, Hkv, D), rows(rng, gap, Hkv, D), n)
+            n += gap
+        s.feed(rng.standard_normal((T, Hkv * G, D)).astype(np.float32), rows(rng, T, Hkv, D), rows(rng, T, Hkv, D), n)
+        hip.sync()
+        for _ in range(2):
+            hip("hipGraphLaunch", g, st)
+        hip.sync()
+        kv = np.stack(s.cache.load(0, n + T))
+        _check_attn(s.result(), *attend64(kv, s.result(s.qr), n, window=window, n_sink=n_sink))
+        n += T
+    hip("hipGraphExecDestroy", g)
+    hip("hipStreamDestroy", st)
+
+
+@pytest.mark.parametrize("kind", [I8, E4])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H,Hkv,window", [(1, 16, 4, 0), (1, 8, 2, 0), (1, 2, 1, 0), (2, 16, 16, 0), (5, 16, 4, 0), (33, 16, 4, 0), (64, 32, 8, 0),
+                                            (300, 16, 4, 0), (340, 16, 4, 0), (5, 16, 4, 3000), (700, 8, 2, 2000)])
+def test_work_area_serves_every_earlier_position_of_any_dims(T, H, Hkv, window, D, kind):
+    """The splits' rules differ by dims and heads: the area asked for is never less at a later position."""
+    c = _kv(type=kind, Hkv=Hkv, D=D, n_ctx=1 << 20)
+    need = [xp.lib().xjh_attn_kv8_work_bytes(c, T, H, n, window, 4) for n in [*range(0, 20000, 61), 24000, 30000, 50000, 131000, 1000000]]
+    assert all(a <= b for a, b in zip(need, need[1:]))
