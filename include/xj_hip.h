@@ -522,7 +522,7 @@ int xjh_kv8_load(const xjh_kv8 *c, int pos0, int n, float *k, int64_t k_tok, flo
  * not NULL. Codes are exact operands, sums are fp32. A query's elements and the
  * weights enter with 22 bits, the elements, where a work-group has 32 rows over
  * int8 keys, to 2^-19 of their row's mean magnitude or, if the largest is more
- * than 8 times that, to 2^-30 of the largest.
+ * than 8 times that, to 2^-30 of the largest (2^-132 at least).
  * work: xjh_attn_kv8_work_bytes bytes, for splitting the positions over the
  * GPU; a smaller area (or NULL) splits less. It holds nothing between calls, but
  * calls that may run at the same time (other streams, other graphs) need one each.

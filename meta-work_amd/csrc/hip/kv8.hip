@@ -369,7 +369,15 @@ __host__ __device__ __forceinline__ Tiles tiles_of(int p0, int p1, int window, i
 // enters as two f16 planes of w * kP (22 bits), whatever the scales' range: the term 2 * 2^(score - M), of which the total is the
 // sum, times the value scale times kP / 2 (the largest scale, 2^128 / 127, times kP would be infinite). The sums are rescaled only
 // when max t passes M by more than kGrow.
-constexpr float kGrow = 8.f, kP = 128.f;
+// A score is a sum of codes by queries, times what the queries were divided by over kK, times the key's scale times kK (2^127 at most, so
+// that the product before it is as small as can be): no step is beyond float's range where the score is well within it. It is
+// rounded before M is formed of it: one of 2^24 and more then lies on the grid that M has, and the largest's term is still near 1 (with an
+// exact product in the sums, M's rounding alone would be a power of two; plus() keeps the compiler from that).
+__device__ __forceinline__ float plus(float a, float b) {
+#pragma clang fp contract(off)
+    return a + b;
+}
+constexpr float kGrow = 8.f, kP = 128.f, kK = 64.f;
 // 2^(2 x), to the smallest denormal: the exponential instruction leaves out what is below 2^-126, which beside value scales of 2^100 and
 // more are the terms of all but a row's best keys (2^-149 is 2^-28 of the smallest total). One product more for 1 ulp more.
 __device__ __forceinline__ float exp2_twice(float x) {
@@ -475,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
     __shared__ __align__(16) hf8 qs[NQ][NP][64];
     __shared__ __align__(16) f32x4 sb[4][64];          // scores [16 keys][lane]
     __shared__ __align__(16) uint8_t pb[2][NP][1024];  // weights as operands [32 keys][plane][lane]
-    __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys, of the values times kP / 2, their log2
+    __shared__ __align__(16) float sc[2][3][64];       // [tile parity] scales of the keys times kK, of the values times kP / 2, their log2
     __shared__ float alb[16], mx[4][16];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, kq = l >> 4;
     const int G = a.H / a.c.Hkv, rows = a.T * G, np = clamp_past(a.npast, a.npast_dev);
@@ -527,8 +535,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
         m = fmaxf(fmaxf(mx[0][li], mx[1][li]), fmaxf(mx[2][li], mx[3][li]));
         int e = 0;
         if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-        e = max(e, -100) - 14;
-        qsc = ldexpf(a.scale * 1.44269504088896341f, e);   // what a product is multiplied with
+        e = max(e, -102) - 14;
+        qsc = ldexpf(a.scale * (1.44269504088896341f / kK), e);   // what a product is multiplied with
 #pragma unroll
         for (int i = 0; i < QW; i++) {
             hf2 hi[4], lo[4];
@@ -562,39 +570,37 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
                 for (int p = NP - 1; p >= 0; p--) x[st & 1] = mfma16(k, q[st][p], x[st & 1]);
             }
             if (w < 2) {
-                sc[par][w][l] = w ? s1 * (kP / 2) : s1;
+                sc[par][w][l] = s1 * (w ? kP / 2 : kK);
                 if (w) sc[par][2][l] = log2f(fmaxf(s1, 0x1p-99f));
             }
             f32x4 v = x[0] + x[1];
             if constexpr (ST) v = f32x4{add_ror8(v.x), add_ror8(v.y), add_ror8(v.z), add_ror8(v.w)};
-            sb[w][l] = v;
+            sb[w][l] = v * qsc;
         }
         if (more) load_k(ahead(i), kr, s1);
         lds_barrier();
         {   // weights: the maximum over all keys, the terms of the wavefront's 16
             f32x4 s[4];   // of the sets of 16 keys from w on, around
-            float mt = -INFINITY, qe = qsc;
+            float mt = -INFINITY;
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const int u = (w + v) & 3;
                 s[v] = sb[u][l] * *(const f32x4 *)&sc[par][0][16 * u + 4 * kq];
             }
-            if (tile_edge(a, j0, p0, p1)) {
-                qe = 1.f;
+            if (tile_edge(a, j0, p0, p1))
 #pragma unroll
                 for (int v = 0; v < 4; v++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int j = j0 + 16 * ((w + v) & 3) + 4 * kq + r;
                         const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-                        s[v][r] = see ? s[v][r] * qsc : -INFINITY;
+                        s[v][r] = see ? s[v][r] : -INFINITY;
                     }
-            }
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const f32x4 lv = *(const f32x4 *)&sc[par][2][16 * ((w + v) & 3) + 4 * kq];
 #pragma unroll
-                for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[v][r], qe, lv[r]));
+                for (int r = 0; r < 4; r++) mt = fmaxf(mt, plus(s[v][r], lv[r]));
             }
             mt = max_x16(max_x32(mt));
             float al = 1.f;
@@ -610,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
             float y[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float p = exp2_twice(fmaf(s[0][r], 0.5f * qe, -0.5f * ref));
+                const float p = exp2_twice(fmaf(s[0][r], 0.5f, -0.5f * ref));
                 L += p;
                 y[r] = p * vs[r];
             }
@@ -701,7 +707,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     constexpr int NS = D / 64, NQ = E4 ? 2 * NS : NS, NP = E4 ? 2 : 3;
     constexpr int CT = 2, NV = D / 64;   // columns; a wavefront's units of values
     __shared__ __align__(16) uint8_t pb[2][CT][2][2][1024];   // weights [tile parity][columns][32 keys][plane][lane]
-    __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys, of the values times kP / 2, their log2 (and unused)
+    __shared__ __align__(16) float sc[4][4][64];             // [tile & 3] scales of the keys times kK, of the values times kP / 2, their log2 (and unused)
     __shared__ float alb[2][CT][16], mx[2][CT][2][16], ms[CT][16];
     __shared__ __align__(16) u32x4 qd[CT][E4 ? 1 : NS][64];   // int8: the queries' fourth digits
     __shared__ int large[4];                                  // int8: a row has a large channel
@@ -724,7 +730,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
     auto load_s = [&](int i) { s1 = scp[min(tile(min(i, nt - 1)) * 64 + l, last) >> a.c.lg]; };
     auto put_s = [&](int i) {   // (every pair of wavefronts the same)
         const float x = held(tile(min(i, nt - 1)) * 64 + l, a.sinks, lo, last) ? s1 : 0.f;
-        sc[i & 3][w & 1][l] = w & 1 ? x * (kP / 2) : x;
+        sc[i & 3][w & 1][l] = x * (w & 1 ? kP / 2 : kK);
         sc[i & 3][2 + (~w & 1)][l] = log2f(fmaxf(x, 0x1p-99f));
     };
     load_s(0);
@@ -750,14 +756,14 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
         if constexpr (!E4) {
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
-            large[w] = __any(m * (D / 8) > sum);
+            large[w] = __any(m * (D / 8) > sum || m < 0x1p-102f);   // (below, where the exponent stops, the bits are needed too)
         }
         const uint64_t bad = ~__ballot(fin);   // a NaN or infinity, which integers do not hold, is put into the row's factor
         fin = !((bad >> li | bad >> (li + 16) | bad >> (li + 32) | bad >> (li + 48)) & 1);
         int e = 0;
         if (m < INFINITY) (void)frexpf(m, &e);   // m < 2^e
-        e = max(e, -100) - 14;
-        qsc = fin ? ldexpf(a.scale * 1.44269504088896341f, e) : NAN;   // what a product (of int8, its 2^-16) is multiplied with
+        e = max(e, -102) - 14;
+        qsc = fin ? ldexpf(a.scale * (1.44269504088896341f / kK), e) : NAN;   // what a product (of int8, its 2^-16) is multiplied with
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             if constexpr (E4) {
@@ -785,7 +791,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
         }
     }
     f32x4 o[CT][NV], s[2];   // sums; products of the tile before with its keys' scales
-    float qe = 1.f, M, L, mt;   // what makes them powers of two
+    float M, L, mt;
     put_s(0);
     load_s(1);
     lds_barrier();
@@ -894,7 +900,7 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
                     float z[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float p = exp2_twice(fmaf(s[v][r], 0.5f * qe, -0.5f * ref));
+                        const float p = exp2_twice(fmaf(s[v][r], 0.5f, -0.5f * ref));
                         L += p;
                         z[r] = p * vs[r];
                     }
@@ -906,26 +912,23 @@ __global__ __launch_bounds__(256, 2) void kv8_chunk_kernel(const Kv8AttnArgs a) 
             }
             if (S) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) s[u] = y[u] * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
+                for (int u = 0; u < 2; u++) s[u] = y[u] * qsc * *(const f32x4 *)&sc[i & 3][0][16 * (u0 + u) + 4 * kq];
                 const int j0 = tile(i) * 64;
-                qe = qsc;
-                if (tile_edge(a, j0, p0, p1)) {
-                    qe = 1.f;
+                if (tile_edge(a, j0, p0, p1))
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const int j = j0 + 16 * (u0 + u) + 4 * kq + r;
                             const bool see = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-                            s[u][r] = see ? s[u][r] * qsc : -INFINITY;
+                            s[u][r] = see ? s[u][r] : -INFINITY;
                         }
-                }
                 mt = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const f32x4 lv = *(const f32x4 *)&sc[i & 3][2][16 * (u0 + u) + 4 * kq];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) mt = fmaxf(mt, fmaf(s[u][r], qe, lv[r]));
+                    for (int r = 0; r < 4; r++) mt = fmaxf(mt, plus(s[u][r], lv[r]));
                 }
                 mt = max_x16(max_x32(mt));
                 mx[par][cw][w & 1][li] = mt;

@@ -1086,3 +1086,19 @@ def test_work_area_serves_every_earlier_position_of_any_dims(T, H, Hkv, window, 
     c = _kv(type=kind, Hkv=Hkv, D=D, n_ctx=1 << 20)
     need = [xp.lib().xjh_attn_kv8_work_bytes(c, T, H, n, window, 4) for n in [*range(0, 20000, 61), 24000, 30000, 50000, 131000, 1000000]]
     assert all(a <= b for a, b in zip(need, need[1:]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,n", ROWS)
+@pytest.mark.parametrize("kind", [I8, E4])
+def test_attention_of_keys_of_any_size(kind, T, H, n):
+    """Keys up to 1e37: of queries as small as they are large, and of others, whose scores of 1e6 to 1e37 leave one key a row."""
+    rng = np.random.default_rng(44)
+    D = 64
+    k, v, q = rows(rng, n, 1, D), rows(rng, n, 1, D), rng.standard_normal((T, H, D)).astype(np.float32)
+    for fk, fq in ((1e34, 1e-34), (1e30, 1e-30), (1e-28, 1e28), (1e6, 1.0), (3.0, 3e8), (1e4, 1e7), (1e34, 1.0), (3e36, 1.0), (1.0, 1e36)):
+        cache, ref = xp.Kv8(1, D, n, 16, kind), Ref(1, D, n, 16, kind)
+        kf, qf = k * np.float32(fk), q * np.float32(fq)
+        cache.store(kf, v, 0)
+        ref.store(kf, v, 0)
+        _check_attn(cache.attend(qf, n - T), *attend64(ref.values(0, n), qf, n - T))
