@@ -443,7 +443,10 @@ int xjh_delta_chunked(int H, int S, int T, int chunk, const float *q, const floa
  * Where a call takes n_past_dev (may be NULL), the tokens' position is read
  * there on the GPU instead of n_past, which then is an upper bound for it, so
  * that one captured graph serves every step; a value outside [0, n_past] counts
- * as the nearer end. */
+ * as the nearer end. The bound shapes the launch: attention far below it is right
+ * but slower than a call that knows its position (one token of 16 heads on 4 of 256
+ * dims at 4000 of at most 131000: 28 us, 9.4 known), so that a long context is
+ * better served by a few graphs of growing bounds. */
 
 /* Rotary positions. pairs: which elements of a head turn together, (i, i +
  * n_rot/2) or (2i, 2i + 1), i < n_rot/2; the elements past n_rot do not turn.
@@ -453,7 +456,12 @@ int xjh_delta_chunked(int H, int S, int T, int chunk, const float *q, const floa
  *   XJH_ROPE_YARN    with r = n_ctx_orig * base^(-2i/n_rot) / (2 pi) turns over the
  *                    trained context and g = (r - beta_slow) / (beta_fast - beta_slow)
  *                    clamped to [0, 1]: (g + (1 - g) / factor) of it
- * and is multiplied by mscale (0: 0.1 ln(factor) + 1 for YARN, else 1). */
+ * and is multiplied by mscale (0: 0.1 ln(factor) + 1 for YARN, else 1).
+ * YARN's g is linear in the turns r, the form in which the method was published.
+ * Programs that run scaled checkpoints (and the yarn fields of GGUF files) commonly
+ * take g linear in the pair's index i, between the pairs that make beta_fast and
+ * beta_slow turns: other frequencies between those two (by up to 1.7 for n_rot 64,
+ * base 1e7, 32768 positions, factor 4, betas 32 and 1), which this call does not form. */
 enum { XJH_ROPE_HALF = 0, XJH_ROPE_INTERLEAVED = 1 };
 enum { XJH_ROPE_PLAIN = 0, XJH_ROPE_LINEAR = 1, XJH_ROPE_YARN = 2 };
 typedef struct {
@@ -483,7 +491,9 @@ int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, float *out, i
  *                with largest magnitude <= 448 scale, code = nearest e4m3 of x / scale
  * Ties go to the even code and every code is that of the exact quotient. A block
  * of zeros has scale 0. NaN is stored as 0 and an infinity as the largest code;
- * neither counts for the scale, so the cache never holds them.
+ * neither counts for the scale, so the cache never holds them (a code of rows within
+ * a step of the largest float may stand for a value just beyond it: that loads as
+ * an infinity).
  * The bytes at data, N = n_ctx rounded up to 64 positions:
  *   keys   [Hkv][N/64][4 groups of 16 positions][D/64][4 x 16 dims][16 positions][16 dims]
  *   values [Hkv][N/64][D/16 groups of 16 dims][4 q][16 dims][4 u][4 r], byte (q, u, r)
@@ -504,8 +514,9 @@ uint64_t xjh_kv8_bytes(const xjh_kv8 *c);
 /* Quantise the rows k, v [T][Hkv*D] (token strides k_tok, v_tok) into positions
  * n_past .. n_past+T-1. A block that positions before n_past began keeps the
  * larger of its scale and the new rows'; where that grew, its older codes are
- * rounded again to it; if those were never stored, clear the memory first. Blocks
- * written from their first position start anew. Every
+ * rounded again to it; if those were never stored, clear the memory first. So after
+ * going back within a block (a rejected draft) it keeps the scale that the rows
+ * given up had made. Blocks written from their first position start anew. Every
  * other byte keeps its value, but tiles of 64 positions are rewritten whole: what
  * stores into a tile or reads it is ordered with this call. n_past_dev: see above. */
 int xjh_kv8_store(const xjh_kv8 *c, const float *k, int64_t k_tok, const float *v, int64_t v_tok, int T, int n_past,

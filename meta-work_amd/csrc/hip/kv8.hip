@@ -469,7 +469,7 @@ __device__ __forceinline__ void finish(const Kv8AttnArgs &a, int g, int row, int
 //   weights  a quarter of the (row, key) pairs each: scores and weights pass through LDS (a few KB a tile)
 //   sums     a quarter of the dims each
 // A wavefront's part of the next tile (8 KB at D = 256) is always in flight, two work-groups or more share a CU: a long cache
-// streams (one token at 131000 positions, 16 heads on 4 of 256 dims: 268 MB in 48.2 us, 5.6 TB/s; a 1 GiB copy reaches 5.15). A short
+// streams (one token at 131000 positions, 16 heads on 4 of 256 dims: 268 MB in 48.8 us, 5.5 TB/s; a 1 GiB copy reaches 5.15). A short
 // one is bound by latency: 4000 positions, 8.4 MB, 5.8 us, most of it the first loads and the way of a tile through the steps.
 // A: tiles requested ahead of the one in use.
 // An operand has 16 columns. R = 8: both planes of 8 rows, so a product costs one instruction; R = 16: one plane after the
@@ -684,12 +684,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(const Kv8AttnArgs a) {
 // largest to 22 - k bits: at most 2^-19 of the mean magnitude where the largest is 8 times that, as little as fp32's own roundings
 // of a score. Work-groups with a row whose largest is above that (a channel far above the others; three digits are off by 1e-4 in a
 // weight at 1000 times) take four digits, 30 - k bits, for 3 to 7% of the time.
-// 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 87 to 90 us, 390 TFLOP/s (twice that in matrix instructions' f16 rate); at
-// 6144 positions 465 us, 515. Bound by a wavefront's own chain: of a step's 3480 cycles at D = 256 the scores take 780, the weights
-// 570, the softmax's end 800, the sums 950 and barrier and loads 350, and two work-groups a CU overlap only part of it (the products
-// alone would be 1800 cycles of a SIMD for both, the vector instructions 1600). Measured the same or slower: operands of
-// 64 rows shared through LDS, two groups of wavefronts in opposite steps, wavefronts with different roles, and the vector
-// instructions placed among the products.
+// 2048 tokens of an empty cache, 16 heads on 4 of 256 dims: 90 to 96 us, 380 TFLOP/s (twice that in matrix instructions' f16 rate); at
+// 6144 positions 466 us, 515 (with four digits 97 and 487). Bound by a wavefront's own chain: of a step's 3480 cycles at D = 256 the scores
+// take 780, the weights 570, the softmax's end 800, the sums 950 and barrier and loads 350 (before scores and terms took a product more
+// each, some 60 cycles), and two work-groups a CU overlap only part of it (the products alone would be 1800 cycles of a SIMD for both, the
+// vector instructions 1600). Measured the same or slower: operands of 64 rows shared through LDS, two groups of wavefronts in
+// opposite steps, wavefronts with different roles, and the vector instructions placed among the products.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 // Four values times 2^(16 - e) as integers, the bytes of X + 0x80808080; each less 128 is one of X's signed digits. Digit p of the four.
 __device__ __forceinline__ u32x4 digits(const f32x4 x, int e) {
@@ -1053,9 +1053,10 @@ static int most_tiles(const Kv8AttnArgs &a, int R) {
 // half the matrix instructions: one token of 32 heads on as many of 128 dims at 32000 positions 65 us, 69 as 16 rows. 16 is the
 // kernel that shares a tile's work out, the shorter way through it, 32 the one that has more rows in a pass over the cache: up to 16 rows
 // the first (4 tokens at 131000: 58 us, 61 as 32), and as long as its work-groups have a tile each (5 tokens at 200 positions 9.4 us,
-// 12.3 as 32; 64 at 0 7.0 and 9.9; 16 at 1000 12.2 and 14.1; beyond: 32 at 4000 20.6 and 19.8, 64 at 8000 43 and 35). With e4m3 the scores of
-// 32 rows are no integer products, and 16 rows hold out for 20 D tiles (of 256 dims 64 tokens at 4000 25.5 and 26.5, of 128 at
-// 2000, 2112 tiles, 15.1 and 15.2, 128 at 2000, 4352 tiles, 21.3 and 20.8, of 64 on 8 heads 40 at 4000, 1536 tiles, 13.0 and 12.1).
+// 12.3 as 32; 64 at 0 7.0 and 9.9; 16 at 1000, 256 of them, 12.2 and 14.1; beyond: 32 at 4000, 2016, 20.6 and 19.8, 64 at 8000 43 and
+// 35; not measured between). With e4m3 the scores of 32 rows are no integer products, and 16 rows hold out for 20 D tiles (of 256
+// dims 64 tokens at 4000 25.5 and 26.5, of 128 at 2000, 2112 tiles, 15.1 and 15.2, 128 at 2000, 4352 tiles, 21.3 and 20.8, of 64 on 8
+// heads 40 at 4000, 1536 tiles, 13.0 and 12.1).
 static int64_t groups16(const Kv8AttnArgs &a) { return ((int64_t)a.T * (a.H / a.c.Hkv) + 15) / 16 * a.c.Hkv; }
 static int rows_of(const Kv8AttnArgs &a) {
     const int64_t n = (int64_t)a.T * (a.H / a.c.Hkv);
@@ -1067,15 +1068,19 @@ static int rows_of(const Kv8AttnArgs &a) {
 //   Two work-groups a CU, which their registers leave room for, hide each other's waits: 512 in all.
 //   Up to 16 rows a tile each is enough (for 256, 384, 512 and 768 work-groups one token at 131000 takes 70, 60, 56 and 57, four 77, 66,
 //   58 and 67). The merge reads every split: 256 at most (16 heads on one, one token at 32000 in 128, 256 and 512 16.5, 16.8 and
-//   22), and more than 64 have to have two and a half tiles each (one token at 5000 in 64 and in 79 splits 10.3 and 11.8, at 12000
-//   in 64 and 128 13.5 and 15.1, at 24000 18.3 and 17.5). Of 64 dims, whose registers leave room for more, 1024 up to 128
+//   22), and above 64 half as many, once, where they would have less than two and a half tiles each: with four kv heads 64 for 128
+//   (one token at 5000, 79 tiles, in 40 splits 10.3 and in 79 11.8, at 12000 in 63 13.5 and in 94 15.1, at 24000 in 63 18.3 and in
+//   126 17.5), with one or two 128 for 256, where 64 would be the better on one side only (8 heads on 2, one token at 5000 in
+//   79 splits 10.6 and in 40 10.1, at 12000 in 94 12.5 and in 63 11.6, but at 4200 in 66 9.9 and in 33 10.5, at 16000 in 126 12.9 and in
+//   63 13.8). Of 64 dims, whose registers leave room for more, 1024 up to 128
 //   splits (32 heads on 8 at 131000 43 with 512 and 36 with 1024; 16 on 4 at 32000 13.1 in 128 splits and 15.2 in 256).
 //   More rows, up to 128 groups of them: 512 if each has four tiles (for 256 and 512: 8 tokens at 131000 78 and 68, 200 at 2000 35 and
 //   32), else 256 of two at least (at three tiles in 512 or in between 40 at 4000 22 and 25; a number in between leaves
 //   some CUs one work-group and others two).
-//   From 129 groups on the other choice is no split and no merge: worth five tiles a third up to 170 (333 tokens at 500 29.0 whole,
-//   29.6 in thirds, at 1000 40.0 and 34.5), twelve a half or a third beyond (512 at 500 33.5 whole, 37.1 in halves, at 2000 64 and
-//   59, at 32000 684 and 515; 600, thirds in two turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636).
+//   From 129 groups on the other choice is no split and no merge (256 dims; of fewer the last paragraph decides first where a group
+//   has enough tiles): worth five tiles a third up to 170 (333 tokens at 500 29.0 whole, 29.6 in thirds, at 1000 40.0 and 34.5), twelve
+//   a half or a third beyond (512 at 500 33.5 whole, 37.1 in halves, at 2000 64 and 59, at 32000 684 and 515; 600, thirds in two
+//   turns, at 1000 48 and 54, at 2000 77 and 73, at 32000 912 and 636).
 //   Of 128 and 64 dims a CU holds three and four of these, which take eight tiles each and at most 64 splits (128 dims, for 512 and 768 in
 //   all: 512 tokens at 32000 351 and 320, 128 at 4000, five tiles, 25.7 and 26.6, 8 at 131000, 64 and 96 splits, 44.1 and
 //   45.7; 64 dims, 32 heads on 8, for 512 and 1024: 256 at 32000 313 and 248).
