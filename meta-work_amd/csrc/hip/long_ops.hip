@@ -13,6 +13,10 @@ namespace {
 // A stream of another device would run the launch there, on this device's pointers.
 bool stream_ok(void *stream, const char *what, char *err, size_t errlen) {
     if (!stream) return true;
+    if ((uintptr_t)stream < 4096) {   // hipStreamLegacy, hipStreamPerThread: no pointers, which hipStreamGetDevice takes them for
+        snprintf(err, errlen, "%s: predefined stream handles are not supported (NULL: the default stream)", what);
+        return false;
+    }
     int cur = 0;
     hipDevice_t dev = 0;
     if (hipGetDevice(&cur) != hipSuccess || hipStreamGetDevice((hipStream_t)stream, &dev) != hipSuccess) {

@@ -1102,3 +1102,15 @@ def test_attention_of_keys_of_any_size(kind, T, H, n):
         cache.store(kf, v, 0)
         ref.store(kf, v, 0)
         _check_attn(cache.attend(qf, n - T), *attend64(ref.values(0, n), qf, n - T))
+
+
+@pytest.mark.parametrize("handle", [1, 2])
+def test_predefined_stream_handles_are_refused(handle):
+    """hipStreamLegacy and hipStreamPerThread are small numbers, no pointers: refused before the runtime sees them."""
+    err, c, L = C.create_string_buffer(xp.ERR), _kv(), xp.lib()
+    for call in (lambda: L.xjh_rope_scaled(4096, 128, 128, 4096, 128, 128, 1, 1, 128, _cfg(), None, 0, handle, err, xp.ERR),
+                 lambda: L.xjh_kv8_store(c, 4096, 256, 4096, 256, 1, 0, None, handle, err, xp.ERR),
+                 lambda: L.xjh_kv8_load(c, 0, 1, 4096, 256, 4096, 256, handle, err, xp.ERR),
+                 lambda: L.xjh_attn_kv8(c, 4096, 256, 128, None, 0, 0, 1, 2, 0, None, 0, 0, 1.0, 4096, 256, None, 0, handle, err, xp.ERR)):
+        err.value = b""
+        assert call() == -1 and b"predefined stream" in err.value
