@@ -431,9 +431,9 @@ int xjh_delta_chunked(int H, int S, int T, int chunk, const float *q, const floa
  * reference: rotary positions with scaled frequencies, a cache of keys and
  * values in 8 bits, and attention over it with an optional sliding window.
  *
- * Unlike the other per-op entries these enqueue on `stream` (a created hipStream_t of
- * the current device; NULL: its default stream; the predefined handles
- * hipStreamLegacy and hipStreamPerThread are refused) and return without waiting
+ * Unlike the other per-op entries these enqueue on `stream` (a hipStream_t of
+ * the current device, hipStreamPerThread among them; NULL and hipStreamLegacy: its
+ * default stream) and return without waiting
  * (xjh_sync waits), never allocate and can be captured into a HIP graph. Device
  * buffers belong to the current device, need no alignment beyond their type's
  * (the cache and the work area: 16 bytes) and are complete when the stream

@@ -10,16 +10,14 @@ using namespace xjk;
 
 namespace {
 
-// A stream of another device would run the launch there, on this device's pointers.
-bool stream_ok(void *stream, const char *what, char *err, size_t errlen) {
-    if (!stream) return true;
-    if ((uintptr_t)stream < 4096) {   // hipStreamLegacy, hipStreamPerThread: no pointers, which hipStreamGetDevice takes them for
-        snprintf(err, errlen, "%s: predefined stream handles are not supported (NULL: the default stream)", what);
-        return false;
-    }
+// The stream to launch on. One of another device would run the launch there, on this device's pointers. The predefined handles
+// are of the current device and no pointers, which hipStreamGetDevice takes them for.
+bool stream_of(void *stream, hipStream_t &st, const char *what, char *err, size_t errlen) {
+    st = (hipStream_t)stream == hipStreamLegacy ? nullptr : (hipStream_t)stream;
+    if (!st || st == hipStreamPerThread) return true;
     int cur = 0;
     hipDevice_t dev = 0;
-    if (hipGetDevice(&cur) != hipSuccess || hipStreamGetDevice((hipStream_t)stream, &dev) != hipSuccess) {
+    if (hipGetDevice(&cur) != hipSuccess || hipStreamGetDevice(st, &dev) != hipSuccess) {
         (void)hipGetLastError();
         snprintf(err, errlen, "%s: not a usable stream", what);
         return false;
@@ -92,7 +90,8 @@ extern "C" int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, fl
         snprintf(err, errlen, "rope_scaled: no buffer, or in place with other strides");
         return -1;
     }
-    if (!stream_ok(stream, "rope_scaled", err, errlen)) return -1;
+    hipStream_t st;
+    if (!stream_of(stream, st, "rope_scaled", err, errlen)) return -1;
     RopeArgs a{};
     a.x = x; a.x_tok = x_tok; a.x_head = x_head;
     a.out = out; a.o_tok = o_tok; a.o_head = o_head;
@@ -110,7 +109,7 @@ extern "C" int xjh_rope_scaled(const float *x, int64_t x_tok, int64_t x_head, fl
         }
         a.f[i] = f / two_pi;
     }
-    if (rope_scaled_launch(a, (hipStream_t)stream)) { snprintf(err, errlen, "rope_scaled launch failed"); return -1; }
+    if (rope_scaled_launch(a, st)) { snprintf(err, errlen, "rope_scaled launch failed"); return -1; }
     return 0;
 }
 
@@ -126,10 +125,11 @@ extern "C" int xjh_kv8_store(const xjh_kv8 *c, const float *k, int64_t k_tok, co
     if (!cache_ok(c, "kv8_store", a.c, err, errlen) || !range_ok(c, T, n_past, "kv8_store", err, errlen)) return -1;
     if (!T) return 0;
     if (!k || !v) { snprintf(err, errlen, "kv8_store: no rows"); return -1; }
-    if (!stream_ok(stream, "kv8_store", err, errlen)) return -1;
+    hipStream_t st;
+    if (!stream_of(stream, st, "kv8_store", err, errlen)) return -1;
     a.k = k; a.k_tok = k_tok; a.v = v; a.v_tok = v_tok;
     a.T = T; a.npast = n_past; a.npast_dev = n_past_dev;
-    if (kv8_store_launch(a, (hipStream_t)stream)) { snprintf(err, errlen, "kv8_store launch failed"); return -1; }
+    if (kv8_store_launch(a, st)) { snprintf(err, errlen, "kv8_store launch failed"); return -1; }
     return 0;
 }
 
@@ -138,10 +138,11 @@ extern "C" int xjh_kv8_load(const xjh_kv8 *c, int pos0, int n, float *k, int64_t
     Kv8LoadArgs a{};
     if (!cache_ok(c, "kv8_load", a.c, err, errlen) || !range_ok(c, n, pos0, "kv8_load", err, errlen)) return -1;
     if (!n || (!k && !v)) return 0;
-    if (!stream_ok(stream, "kv8_load", err, errlen)) return -1;
+    hipStream_t st;
+    if (!stream_of(stream, st, "kv8_load", err, errlen)) return -1;
     a.k = k; a.k_tok = k_tok; a.v = v; a.v_tok = v_tok;
     a.pos0 = pos0; a.n = n;
-    if (kv8_load_launch(a, (hipStream_t)stream)) { snprintf(err, errlen, "kv8_load launch failed"); return -1; }
+    if (kv8_load_launch(a, st)) { snprintf(err, errlen, "kv8_load launch failed"); return -1; }
     return 0;
 }
 
@@ -163,14 +164,15 @@ extern "C" int xjh_attn_kv8(const xjh_kv8 *c, const float *q, int64_t q_tok, int
     }
     if (!T) return 0;
     if (!q || !out || ((uintptr_t)work & 15)) { snprintf(err, errlen, "attn_kv8: no buffer, or an unaligned work area"); return -1; }
-    if (!stream_ok(stream, "attn_kv8", err, errlen)) return -1;
+    hipStream_t st;
+    if (!stream_of(stream, st, "attn_kv8", err, errlen)) return -1;
     a.q = q; a.q_tok = q_tok; a.q_head = q_head;
     a.gate = gate; a.g_tok = g_tok; a.g_head = g_head;
     a.out = out; a.o_tok = o_tok;
     a.T = T; a.H = H; a.npast = n_past; a.npast_dev = n_past_dev;
     a.window = window; a.sinks = n_sink; a.scale = scale;
     a.part = (float *)work;
-    if (kv8_attn_launch(a, work ? (int64_t)(work_bytes / sizeof(float)) : 0, (hipStream_t)stream)) {
+    if (kv8_attn_launch(a, work ? (int64_t)(work_bytes / sizeof(float)) : 0, st)) {
         snprintf(err, errlen, "attn_kv8 launch failed");
         return -1;
     }

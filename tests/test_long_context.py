@@ -1104,13 +1104,21 @@ def test_attention_of_keys_of_any_size(kind, T, H, n):
         _check_attn(cache.attend(qf, n - T), *attend64(ref.values(0, n), qf, n - T))
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("handle", [1, 2])
-def test_predefined_stream_handles_are_refused(handle):
-    """hipStreamLegacy and hipStreamPerThread are small numbers, no pointers: refused before the runtime sees them."""
-    err, c, L = C.create_string_buffer(xp.ERR), _kv(), xp.lib()
-    for call in (lambda: L.xjh_rope_scaled(4096, 128, 128, 4096, 128, 128, 1, 1, 128, _cfg(), None, 0, handle, err, xp.ERR),
-                 lambda: L.xjh_kv8_store(c, 4096, 256, 4096, 256, 1, 0, None, handle, err, xp.ERR),
-                 lambda: L.xjh_kv8_load(c, 0, 1, 4096, 256, 4096, 256, handle, err, xp.ERR),
-                 lambda: L.xjh_attn_kv8(c, 4096, 256, 128, None, 0, 0, 1, 2, 0, None, 0, 0, 1.0, 4096, 256, None, 0, handle, err, xp.ERR)):
-        err.value = b""
-        assert call() == -1 and b"predefined stream" in err.value
+def test_predefined_stream_handles(handle):
+    """hipStreamLegacy and hipStreamPerThread, small numbers instead of pointers: a layer step on each gives the default stream's bits."""
+    rng = np.random.default_rng(45)
+    a, b = (_Step(2, 2, 64, 200, 16, I8, 3, 100) for _ in range(2))
+    x = rng.standard_normal((100, 2, 64)).astype(np.float32)
+    q, k, v = (rng.standard_normal((3, h, 64)).astype(np.float32) for h in (4, 2, 2))
+    for s, stream in ((a, handle), (b, None)):
+        s.cache.store(x, x, 0)
+        s.feed(q, k, v, 100)
+        s.run(stream)
+        xp.lib().xjh_sync()
+    assert np.array_equal(a.result().view(np.uint32), b.result().view(np.uint32)) and np.array_equal(a.cache.bytes(), b.cache.bytes())
+    out = xp.Dev(nbytes=3 * 2 * 64 * 4)
+    _call("xjh_kv8_load", C.byref(a.cache.c), 100, 3, out.ptr, 128, None, 0, handle)
+    xp.lib().xjh_sync()
+    assert np.array_equal(out.get(np.float32, (3, 2, 64)), a.cache.load(100, 3)[0])
