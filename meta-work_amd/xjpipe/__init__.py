@@ -821,21 +821,30 @@ def _opt(arr):
     return d, d.ptr if d else None
 
 
+def _i32(n, what):
+    """n, which ctypes would cut to 32 bits."""
+    if not -1 << 31 <= n < 1 << 31:
+        raise XjError(f"{what}: {n} is no int32")
+    return int(n)
+
+
 def rope_scaled(x, n_rot, base, pos, pairs=ROPE_HALF, in_place=False, **scaling):
     """Rotary positions on the GPU of x [T][heads][D]; pos: the first token's position, or an
     int32 array of every token's. scaling: the other fields of XjhRopeCfg."""
     x = _rows(x, (None, None, None), "rope_scaled: x")
     T, H, D = x.shape
     cfg = XjhRopeCfg(pairs=pairs, n_rot=n_rot, base=base, **scaling)
-    own = None if np.isscalar(pos) else np.ascontiguousarray(pos, np.int32)
-    if own is not None and own.shape != (T,):
-        raise XjError(f"rope_scaled: {own.shape} positions of {T} tokens")
+    own, pos0 = (None, _i32(pos, "rope_scaled: pos")) if np.isscalar(pos) else (np.asarray(pos), 0)
+    if own is not None:
+        if own.shape != (T,):
+            raise XjError(f"rope_scaled: {own.shape} positions of {T} tokens")
+        own = np.ascontiguousarray([_i32(n, "rope_scaled: pos") for n in own.tolist()], np.int32)
     dx, xp = _opt(x)
     do = dx if in_place or not x.size else Dev(nbytes=x.nbytes)
     dp, pp = _opt(own)
     err = _err()
     _check(lib().xjh_rope_scaled(xp, H * D, D, do.ptr if do else None, H * D, D, T, H, D, C.byref(cfg), pp,
-                                 0 if own is not None else int(pos), None, err, ERR), err, "rope_scaled")
+                                 pos0, None, err, ERR), err, "rope_scaled")
     if not x.size:
         return x
     lib().xjh_sync()
@@ -846,7 +855,7 @@ class Kv8:
     """An 8-bit key/value cache on the GPU (xjh_kv8); arrays in and out are numpy, every call waits."""
 
     def __init__(self, Hkv, D, n_ctx, block=32, type=KV_I8):
-        self.c = XjhKv8(type=type, Hkv=Hkv, D=D, n_ctx=n_ctx, block=block)
+        self.c = XjhKv8(*(_i32(n, "kv8") for n in (type, Hkv, D, n_ctx, block)))
         n = lib().xjh_kv8_bytes(C.byref(self.c))
         if not n:
             raise XjError(f"unsupported cache (Hkv={Hkv}, D={D}, n_ctx={n_ctx}, block={block}, type={type})")
@@ -863,12 +872,14 @@ class Kv8:
         """k, v [T][Hkv][D] into positions n_past .."""
         k = _rows(k, (None, self.c.Hkv, self.c.D), "kv8_store: k")
         v = _rows(v, k.shape, "kv8_store: v")
+        n_past = _i32(n_past, "kv8_store: n_past")
         (dk, kp), (dv, vp), row, err = _opt(k), _opt(v), self.c.Hkv * self.c.D, _err()
         _check(lib().xjh_kv8_store(C.byref(self.c), kp, row, vp, row, k.shape[0], n_past, None, None, err, ERR), err, "kv8_store")
         lib().xjh_sync()
 
     def load(self, pos0, n):
         """(k, v) [n][Hkv][D] of the positions pos0 .. pos0 + n - 1."""
+        pos0, n = _i32(pos0, "kv8_load: pos0"), _i32(n, "kv8_load: n")
         row, err = self.c.Hkv * self.c.D, _err()
         dk, dv = Dev(nbytes=max(1, n * row * 4)), Dev(nbytes=max(1, n * row * 4))
         _check(lib().xjh_kv8_load(C.byref(self.c), pos0, n, dk.ptr, row, dv.ptr, row, None, err, ERR), err, "kv8_load")
@@ -881,6 +892,7 @@ class Kv8:
         work area (default: what the library asks for)."""
         q = _rows(q, (None, None, self.c.D), "attn_kv8: q")
         T, H, D = q.shape
+        n_past, window, n_sink = (_i32(n, f"attn_kv8: {w}") for n, w in ((n_past, "n_past"), (window, "window"), (n_sink, "n_sink")))
         (dq, qp), err = _opt(q), _err()
         do = Dev(nbytes=max(1, q.nbytes))
         dg, gp = _opt(_rows(gate, q.shape, "attn_kv8: gate") if gate is not None else None)

@@ -1122,3 +1122,16 @@ def test_predefined_stream_handles(handle):
     _call("xjh_kv8_load", C.byref(a.cache.c), 100, 3, out.ptr, 128, None, 0, handle)
     xp.lib().xjh_sync()
     assert np.array_equal(out.get(np.float32, (3, 2, 64)), a.cache.load(100, 3)[0])
+
+
+def test_wrappers_refuse_numbers_that_are_no_int32():
+    """ctypes cuts them: position 2^32 would be 0."""
+    x = np.zeros((2, 2, 64), np.float32)
+    cache = xp.Kv8.__new__(xp.Kv8)   # (without memory: nothing is launched)
+    cache.c = xp.XjhKv8(type=I8, Hkv=2, D=64, n_ctx=100, block=8)
+    for call in (lambda: xp.rope_scaled(x, 64, 1e4, 1 << 31), lambda: xp.rope_scaled(x, 64, 1e4, np.array([0, 1 << 32])),
+                 lambda: xp.rope_scaled(x, 64, 1e4, [0, -(1 << 31) - 1]), lambda: cache.store(x, x, 1 << 32), lambda: cache.load(1 << 32, 1),
+                 lambda: cache.load(0, 1 << 32), lambda: cache.attend(x, 1 << 32), lambda: cache.attend(x, 5, window=1 << 32),
+                 lambda: cache.attend(x, 5, n_sink=1 << 32), lambda: xp.Kv8(2, 64, (1 << 32) + 1), lambda: xp.Kv8((1 << 32) + 2, 64, 1)):
+        with pytest.raises(xp.XjError, match="int32"):
+            call()
