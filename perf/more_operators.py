@@ -241,10 +241,11 @@ def _plain_plan(i):
     r = torch.searchsorted(rel_cu[1:], k - n_free, right=True).clamp(max=len(past) - 1)
     given = i.table[r, (need[r] + k - n_free - rel_cu[r]).clamp(0, i.max_blocks - 1)]
     stack = torch.where(k < n_free, i.free, given)                          # the free pages, then the released ones
-    left = (total - take_cu[-1]).clamp(min=0)
+    enough = take_cu[-1] <= total                                           # else none is taken
+    left = torch.where(enough, total - take_cu[-1], total)
     b = torch.arange(i.max_blocks, device=DEV)[None]
     src = total - 1 - (take_cu[:-1, None] + b - have[:, None])
-    page = torch.where(src >= 0, stack[src.clamp(0, i.n_pages - 1)], -1)
+    page = torch.where(enough, stack[src.clamp(0, i.n_pages - 1)], -1)
     taking = (b >= have[:, None]) & (b < need[:, None])
     i.table.copy_(torch.where(taking, page, i.table))
     i.free.copy_(torch.where((k >= n_free) & (k < left), stack, i.free))
@@ -416,14 +417,14 @@ def _exact_plan(case, i):
     P, L = case["page"], i.max_blocks * case["page"]
     table, free = i.table.tolist(), i.free.tolist()
     stack = free[:i.n_free.item()]
-    cu, kv_len, pos, slot, missing = [0], [], [], [], 0
+    cu, kv_len, pos, slot = [0], [], [], []
     for (held, past, new), row in zip(i.lens, table):
         kv_len.append(min(past + new, L))
         stack += row[_pages(kv_len[-1], P):_pages(held, P)]
+    missing = max(0, sum(max(0, _pages(n, P) - _pages(held, P)) for (held, _, _), n in zip(i.lens, kv_len)) - len(stack))
     for (held, past, new), row, n in zip(i.lens, table, kv_len):
         for b in range(_pages(held, P), _pages(n, P)):
-            missing += not stack
-            row[b] = stack.pop() if stack else -1
+            row[b] = -1 if missing else stack.pop()
         cu.append(cu[-1] + new)
         pos += range(past, past + new)
         slot += [row[p // P] * P + p % P if p < L and row[p // P] >= 0 else -1 for p in range(past, past + new)]
