@@ -548,6 +548,68 @@ int xjh_attn_kv8(const xjh_kv8 *c, const float *q, int64_t q_tok, int64_t q_head
  * n_past), window and n_sink; 0 when they are not supported. */
 size_t xjh_attn_kv8_work_bytes(const xjh_kv8 *c, int T, int H, int n_past, int window, int n_sink);
 
+/* ------------------------------------------------------ several requests -- */
+
+/* What a program needs that runs its own layer loop over several requests at
+ * once, no counterpart in the reference: a key/value cache in pages that any
+ * request may own, the tables of who owns them, and attention over batches of
+ * requests of different lengths. As the long-context calls these enqueue on
+ * `stream` and return without waiting, never allocate, can be captured, and read
+ * every length on the GPU, so that one captured step serves them all; buffers,
+ * strides and work areas follow the rules there. Row types are ggml ids (XJ_F32, XJ_F16,
+ * XJ_BF16). */
+
+/* Pages of `page` positions: which are free, and which hold a request's blocks
+ * (block b of request r, its positions b*page .. b*page + page-1, lies in page
+ * table[r*max_blocks + b]). */
+typedef struct {
+    int32_t  page;               /* 16, 32, 64, 128 or 256 */
+    int32_t  n_pages;            /* n_pages * page < 2^31 */
+    int32_t  max_blocks;         /* entries of a table row; max_blocks * page < 2^31 */
+    int32_t *table;              /* device [n_req][max_blocks] */
+    int32_t *free_list;          /* device [n_pages] */
+} xjh_pages;
+/* Prepare a step in which request r (row r of the table) adds n_new[r] tokens behind
+ * n_past[r], while its row holds the pages of held[r] positions (held NULL: n_past):
+ * pages beyond those that n_past + n_new positions need go back to the free list,
+ * missing ones are taken from it. So n_past < held gives up the positions of rejected
+ * drafts, and n_past = n_new = 0 a request that is over. All arrays are on the device.
+ *   free_list  its first *n_free entries are the free pages. Those given back are put behind them
+ *              (requests and blocks in order), then pages are taken from the end (requests and
+ *              blocks in order); *n_free_out (may be n_free) is how many are left. Entries from there on keep their
+ *              values, and so do table entries of blocks that are not taken.
+ *   cu         [n_req+1] the requests' first rows in the step's batch, and their sum
+ *   kv_len     [n_req] n_past + n_new, at most max_blocks * page
+ *   pos, slot  [T] of every row its position, and page * table entry + offset for xjh_paged_store (either may be
+ *              NULL); rows from the sum on get position 0 and slot -1
+ *   status     [4] pages missing, positions beyond the table's rows (slot -1), rows beyond T, rows.
+ *              With pages missing none is taken: the wanted blocks' table entries and their tokens' slots are
+ *              -1, what was given back stays given back, and the step can be tried again with less (held as
+ *              it was for requests that wanted pages, n_past for those that gave some).
+ * Negative lengths count as 0, n_past and held beyond the rows as the whole row; the sum of n_new is
+ * below 2^31. n_req is at most 65536, n_req * max_blocks 2^30. Calls on the same pages are ordered. work: xjh_page_plan_work_bytes
+ * bytes, 16-byte aligned. */
+int xjh_page_plan(const xjh_pages *p, const int32_t *held, const int32_t *n_past, const int32_t *n_new, int n_req,
+                  const int32_t *n_free, int32_t *n_free_out, int T, int32_t *cu, int32_t *kv_len, int32_t *pos,
+                  int32_t *slot, int32_t *status, void *work, size_t work_bytes, void *stream, char *err, size_t errlen);
+size_t xjh_page_plan_work_bytes(int n_req);
+
+/* A layer's keys and values in pages, [n_pages][Hkv][page][D] each. */
+typedef struct {
+    int32_t  type;               /* XJ_F16 or XJ_BF16 */
+    int32_t  Hkv, D;             /* D: 64, 128 or 256 */
+    int32_t  page, n_pages;      /* as in xjh_pages */
+    void    *k, *v;              /* device, 16-byte aligned */
+    uint64_t bytes;              /* at k and at v, at least xjh_paged_bytes each */
+} xjh_paged;
+/* Bytes of the keys (and of the values) of these heads, page and n_pages; 0 when they are not supported. */
+uint64_t xjh_paged_bytes(const xjh_paged *c);
+/* Rows k, v [T][Hkv*D] (token strides k_tok, v_tok) of `type` (XJ_F32 or the cache's) into their
+ * slots: row t goes to offset slot[t] % page of page slot[t] / page, rounded to nearest (beyond the type's
+ * range: infinity). A slot outside [0, n_pages * page) skips its row. The slots of a call differ. */
+int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, const void *v, int64_t v_tok, int T,
+                    const int32_t *slot, void *stream, char *err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,111 @@
+// C entries of the operators for several requests (the "several requests" part of xj_hip.h): argument checks
+// and the launches on the caller's stream.
+#include "common.h"
+#include "kernels.h"
+#include "xj_hip.h"
+
+#include <cmath>
+
+using namespace xjk;
+
+namespace {
+
+bool page_ok(int page, int n_pages) {
+    return page >= 16 && page <= 256 && (page & (page - 1)) == 0 && n_pages >= 1 && (int64_t)n_pages * page <= INT32_MAX;
+}
+
+bool shape_ok(const xjh_paged *c) {
+    return c && (c->type == XJ_F16 || c->type == XJ_BF16) && c->Hkv >= 1 && c->Hkv <= 1024 &&
+           (c->D == 64 || c->D == 128 || c->D == 256) && page_ok(c->page, c->n_pages);
+}
+
+bool cache_ok(const xjh_paged *c, const char *what, Paged &out, char *err, size_t errlen) {
+    if (!shape_ok(c)) {
+        if (!c) snprintf(err, errlen, "%s: no cache", what);
+        else
+            snprintf(err, errlen, "%s: unsupported cache (type=%d (f16|bf16), Hkv=%d, D=%d (64|128|256), page=%d (16|32|64|128|256), n_pages=%d)",
+                     what, c->type, c->Hkv, c->D, c->page, c->n_pages);
+        return false;
+    }
+    if (!c->k || !c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15) || c->bytes < xjh_paged_bytes(c)) {
+        snprintf(err, errlen, "%s: the cache's memory is missing, not 16-byte aligned or below its %llu bytes", what,
+                 (unsigned long long)xjh_paged_bytes(c));
+        return false;
+    }
+    out.k = c->k;
+    out.v = c->v;
+    out.bf16 = c->type == XJ_BF16;
+    out.Hkv = c->Hkv;
+    out.D = c->D;
+    out.lg = __builtin_ctz((unsigned)c->page);
+    out.n_pages = c->n_pages;
+    return true;
+}
+
+int row_type(int type) { return type == XJ_F32 ? kRowF32 : type == XJ_F16 ? kRowF16 : type == XJ_BF16 ? kRowBf16 : -1; }
+
+constexpr int kMaxReq = 65536;
+
+}  // namespace
+
+extern "C" size_t xjh_page_plan_work_bytes(int n_req) {
+    return n_req < 0 || n_req > kMaxReq ? 0 : (2 * ((size_t)n_req + 1) + 4) * sizeof(int32_t);
+}
+
+extern "C" int xjh_page_plan(const xjh_pages *p, const int32_t *held, const int32_t *n_past, const int32_t *n_new, int n_req,
+                             const int32_t *n_free, int32_t *n_free_out, int T, int32_t *cu, int32_t *kv_len, int32_t *pos,
+                             int32_t *slot, int32_t *status, void *work, size_t work_bytes, void *stream, char *err,
+                             size_t errlen) {
+    if (!p || !page_ok(p->page, p->n_pages) || p->max_blocks < 1 || (int64_t)p->max_blocks * p->page > INT32_MAX || n_req < 0 ||
+        n_req > kMaxReq || (int64_t)n_req * p->max_blocks > (1 << 30) || T < 0) {
+        snprintf(err, errlen, "page_plan: bad shape (page=%d (16|32|64|128|256), n_pages=%d, max_blocks=%d, n_req=%d, T=%d)",
+                 p ? p->page : 0, p ? p->n_pages : 0, p ? p->max_blocks : 0, n_req, T);
+        return -1;
+    }
+    if (!p->free_list || !n_free || !n_free_out || !cu || !status || (n_req && (!p->table || !n_past || !n_new || !kv_len))) {
+        snprintf(err, errlen, "page_plan: a buffer is missing");
+        return -1;
+    }
+    if (!work || ((uintptr_t)work & 15) || work_bytes < xjh_page_plan_work_bytes(n_req)) {
+        snprintf(err, errlen, "page_plan: the work area is missing, not 16-byte aligned or below its %llu bytes",
+                 (unsigned long long)xjh_page_plan_work_bytes(n_req));
+        return -1;
+    }
+    hipStream_t st;
+    if (!stream_of(stream, st, "page_plan", err, errlen)) return -1;
+    PlanArgs a{};
+    a.lg = __builtin_ctz((unsigned)p->page);
+    a.n_pages = p->n_pages; a.max_blocks = p->max_blocks;
+    a.table = p->table; a.free_list = p->free_list;
+    a.held = held; a.n_past = n_past; a.n_new = n_new;
+    a.n_req = n_req; a.T = T;
+    a.n_free = n_free; a.n_free_out = n_free_out;
+    a.cu = cu; a.kv_len = kv_len; a.pos = pos; a.slot = slot; a.status = status;
+    a.sum = (int32_t *)work;
+    a.rel_cu = a.sum + 4;
+    a.take_cu = a.rel_cu + n_req + 1;
+    if (page_plan_launch(a, st)) { snprintf(err, errlen, "page_plan launch failed"); return -1; }
+    return 0;
+}
+
+extern "C" uint64_t xjh_paged_bytes(const xjh_paged *c) {
+    return shape_ok(c) ? 2 * (uint64_t)c->n_pages * c->page * c->Hkv * c->D : 0;
+}
+
+extern "C" int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, const void *v, int64_t v_tok, int T,
+                               const int32_t *slot, void *stream, char *err, size_t errlen) {
+    PagedStoreArgs a{};
+    if (!cache_ok(c, "paged_store", a.c, err, errlen)) return -1;
+    if (T < 0 || (int64_t)T * c->Hkv > (1 << 28) || (type != XJ_F32 && type != c->type)) {
+        snprintf(err, errlen, "paged_store: bad rows (T=%d, type=%d into a cache of type %d)", T, type, c->type);
+        return -1;
+    }
+    if (!T) return 0;
+    if (!k || !v || !slot) { snprintf(err, errlen, "paged_store: no rows or no slots"); return -1; }
+    hipStream_t st;
+    if (!stream_of(stream, st, "paged_store", err, errlen)) return -1;
+    a.k = k; a.k_tok = k_tok; a.v = v; a.v_tok = v_tok;
+    a.type = row_type(type); a.T = T; a.slot = slot;
+    if (paged_store_launch(a, st)) { snprintf(err, errlen, "paged_store launch failed"); return -1; }
+    return 0;
+}

@@ -409,4 +409,35 @@ struct RopeArgs {
 };
 int rope_scaled_launch(const RopeArgs &a, hipStream_t st);
 
+// The stream that a call which takes one launches on (long_ops.hip): false, with a message, when it is not
+// one of the current device.
+bool stream_of(void *stream, hipStream_t &st, const char *what, char *err, size_t errlen);
+
+// Page tables (paged.hip), as xjh_page_plan in xj_hip.h.
+struct PlanArgs {
+    int32_t lg, n_pages, max_blocks;   // pages of 1 << lg positions
+    int32_t *table, *free_list;
+    const int32_t *held, *n_past, *n_new;
+    int32_t n_req, T;
+    const int32_t *n_free;
+    int32_t *n_free_out, *cu, *kv_len, *pos, *slot, *status;
+    int32_t *rel_cu, *take_cu, *sum;   // work area: [n_req + 1] each, [4]
+};
+int page_plan_launch(const PlanArgs &a, hipStream_t st);
+// Element types of rows and caches.
+enum RowType { kRowF32 = 0, kRowF16 = 1, kRowBf16 = 2 };
+// Keys and values in pages, [n_pages][Hkv][1 << lg][D] each.
+struct Paged {
+    void *k, *v;
+    int32_t bf16, Hkv, D, lg, n_pages;
+};
+struct PagedStoreArgs {
+    Paged c;
+    const void *k, *v;
+    int64_t k_tok, v_tok;
+    int32_t type, T;
+    const int32_t *slot;
+};
+int paged_store_launch(const PagedStoreArgs &a, hipStream_t st);
+
 }  // namespace xjk

@@ -8,7 +8,7 @@
 
 using namespace xjk;
 
-namespace {
+namespace xjk {
 
 // The stream to launch on. One of another device would run the launch there, on this device's pointers. The predefined handles
 // are of the current device and no pointers, which hipStreamGetDevice takes them for.
@@ -26,6 +26,10 @@ bool stream_of(void *stream, hipStream_t &st, const char *what, char *err, size_
     snprintf(err, errlen, "%s: the stream belongs to device %d, the current device is %d", what, (int)dev, cur);
     return false;
 }
+
+}  // namespace xjk
+
+namespace {
 
 bool shape_ok(const xjh_kv8 *c) {
     return c && (c->type == XJH_KV_I8 || c->type == XJH_KV_E4M3) && c->Hkv >= 1 && c->Hkv <= 1024 &&

@@ -1,0 +1,187 @@
+// A key/value cache in pages (gfx950): who owns which page (xjh_page_plan), and new rows into their slots (xjh_paged_store).
+#include "common.h"
+#include "kernels.h"
+#include <algorithm>
+
+namespace xjk {
+
+// ------------------------------------------------------------- page plan --
+
+// A request's row of the table: `have` blocks are there, `need` will be, `past` tokens before `fresh` new ones.
+struct Req {
+    int past, fresh, have, need, kv;
+    int64_t beyond;   // positions that do not fit the row
+};
+__device__ __forceinline__ Req request(const PlanArgs &a, int r) {
+    const int L = a.max_blocks << a.lg, up = (1 << a.lg) - 1;
+    Req q;
+    q.past = min(max(a.n_past[r], 0), L);
+    q.fresh = max(a.n_new[r], 0);
+    const int held = a.held ? min(max(a.held[r], 0), L) : q.past;
+    const int64_t n = (int64_t)q.past + q.fresh;
+    q.kv = (int)min(n, (int64_t)L);
+    q.beyond = n - q.kv;
+    q.have = (int)(((int64_t)held + up) >> a.lg);
+    q.need = (int)(((int64_t)q.kv + up) >> a.lg);
+    return q;
+}
+// The last of n entries cu[0] = 0 <= cu[1] <= .. with cu[i] <= x (x >= 0), that is the one whose run holds x.
+__device__ __forceinline__ int run_of(const int32_t *cu, int n, int x) {
+    int lo = 0, hi = n;   // cu[lo] <= x < cu[hi]
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (cu[m] <= x) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Sums over the requests before each: rows, pages given back, pages taken. One work-group, the requests in runs of its threads.
+__device__ __forceinline__ void plan_scan(const PlanArgs &a) {
+    __shared__ int64_t red[3][kPlanThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int64_t base[3] = {0, 0, 0}, beyond = 0;
+    for (int r0 = 0; r0 < a.n_req; r0 += kPlanThreads) {
+        const int r = r0 + tid;
+        Req q{};
+        if (r < a.n_req) q = request(a, r);
+        beyond += q.beyond;
+        const int64_t own[3] = {q.fresh, max(q.have - q.need, 0), max(q.need - q.have, 0)};
+        int64_t x[3];
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            x[i] = own[i];
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t y = __shfl_up(x[i], o, 64);
+                if (lane >= o) x[i] += y;
+            }
+            if (lane == 63) red[i][w] = x[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            int64_t all = 0, before = 0;
+            for (int k = 0; k < kPlanThreads / 64; k++) {
+                if (k == w) before = all;
+                all += red[i][k];
+            }
+            x[i] += base[i] + before;
+            base[i] += all;
+        }
+        if (r < a.n_req) {
+            a.cu[r + 1] = (int)min(x[0], (int64_t)INT32_MAX);
+            a.rel_cu[r + 1] = (int)min(x[1], (int64_t)INT32_MAX);
+            a.take_cu[r + 1] = (int)min(x[2], (int64_t)INT32_MAX);
+            a.kv_len[r] = q.kv;
+        }
+        __syncthreads();
+    }
+    for (int o = 32; o; o >>= 1) beyond += __shfl_xor(beyond, o, 64);
+    if (lane == 0) red[0][w] = beyond;
+    __syncthreads();
+    if (tid == 0) {
+        beyond = 0;
+        for (int k = 0; k < kPlanThreads / 64; k++) beyond += red[0][k];
+        const int n_free = min(max(*a.n_free, 0), a.n_pages);
+        const int all = (int)min(n_free + base[1], (int64_t)a.n_pages);
+        const int64_t left = base[2] > all ? all : all - base[2];   // pages missing: none is taken
+        const int64_t big = INT32_MAX;
+        a.cu[0] = a.rel_cu[0] = a.take_cu[0] = 0;
+        a.sum[0] = n_free;
+        a.sum[1] = all;
+        a.sum[2] = (int)left;
+        a.sum[3] = (int)min(base[2], big);
+        *a.n_free_out = (int)left;
+        a.status[0] = (int)min(max(base[2] - all, (int64_t)0), big);
+        a.status[1] = (int)min(beyond, big);
+        a.status[2] = (int)min(max(base[0] - a.T, (int64_t)0), big);
+        a.status[3] = (int)min(base[0], big);
+    }
+}
+// Entry i of the free pages with those given back behind them.
+__device__ __forceinline__ int stack_at(const PlanArgs &a, int n_free, int i) {
+    if (i < n_free) return a.free_list[i];
+    const int k = i - n_free, r = run_of(a.rel_cu, a.n_req, k);
+    return a.table[(int64_t)r * a.max_blocks + request(a, r).need + k - a.rel_cu[r]];
+}
+// The pages that move, and the rows' positions and slots, each by a thread of its own. (What is read here of the table and of the
+// free list is not what is written: rows give or take, and pages are taken from `left` on, put back below it.)
+__device__ __forceinline__ void plan_expand(const PlanArgs &a) {
+    const int n_free = a.sum[0], all = a.sum[1], left = a.sum[2], takes = a.sum[3];
+    const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+    auto taken = [&](int i) { return takes <= all ? stack_at(a, n_free, all - 1 - i) : -1; };
+    for (int64_t i = first; i < takes; i += step) {
+        const int r = run_of(a.take_cu, a.n_req, (int)i);
+        a.table[(int64_t)r * a.max_blocks + request(a, r).have + (int)i - a.take_cu[r]] = taken((int)i);
+    }
+    for (int64_t i = n_free + first; i < left; i += step) a.free_list[i] = stack_at(a, n_free, (int)i);
+    const int rows = a.n_req ? a.cu[a.n_req] : 0;
+    for (int64_t t = first; t < a.T; t += step) {
+        int pos = 0, slot = -1;
+        if (t < rows) {
+            const int r = run_of(a.cu, a.n_req, (int)t);
+            const Req q = request(a, r);
+            const int64_t p = (int64_t)q.past + (t - a.cu[r]);
+            pos = (int)min(p, (int64_t)INT32_MAX);
+            if (p < q.kv) {
+                const int b = (int)(p >> a.lg);
+                const int page = b < q.have ? a.table[(int64_t)r * a.max_blocks + b] : taken(a.take_cu[r] + b - q.have);
+                if (page >= 0 && page < a.n_pages) slot = (page << a.lg) + (int)(p & ((1 << a.lg) - 1));
+            }
+        }
+        if (a.pos) a.pos[t] = pos;
+        if (a.slot) a.slot[t] = slot;
+    }
+}
+__global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(const PlanArgs a) { plan_scan(a); }
+__global__ __launch_bounds__(256) void plan_expand_kernel(const PlanArgs a) { plan_expand(a); }
+
+int page_plan_launch(const PlanArgs &a, hipStream_t st) {
+    plan_scan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+    plan_expand_kernel<<<std::min(1024, std::max(16, (a.T + 255) / 256)), 256, 0, st>>>(a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+// ----------------------------------------------------------------- store --
+
+typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+typedef unsigned short us8_u __attribute__((ext_vector_type(8), aligned(2)));   // rows of any 2-byte alignment
+typedef float f32x8_u __attribute__((ext_vector_type(8), aligned(4)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+template <int TYPE, bool BF>
+__global__ __launch_bounds__(256) void paged_store_kernel(const PagedStoreArgs a) {
+    const int per = a.c.Hkv * a.c.D / 8;   // pieces of a row
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)a.T * per) return;
+    const int t = (int)(i / per), c = (int)(i - (int64_t)t * per) * 8, slot = a.slot[t];
+    if (slot < 0 || (slot >> a.c.lg) >= a.c.n_pages) return;
+    const void *x = blockIdx.y ? a.v : a.k;
+    const int64_t at = t * (blockIdx.y ? a.v_tok : a.k_tok) + c;
+    us8 y;
+    if constexpr (TYPE == kRowF32) {
+        const f32x8_u f = *(const f32x8_u *)((const float *)x + at);
+        if constexpr (BF) y = __builtin_bit_cast(us8, __builtin_convertvector(f, bf8));
+        else y = __builtin_bit_cast(us8, __builtin_convertvector(f, hf8));
+    } else {
+        y = *(const us8_u *)((const unsigned short *)x + at);
+    }
+    const int h = c / a.c.D, d = c - h * a.c.D;
+    unsigned short *out = (unsigned short *)(blockIdx.y ? a.c.v : a.c.k);
+    const int64_t row = ((((int64_t)(slot >> a.c.lg) * a.c.Hkv + h) << a.c.lg) + (slot & ((1 << a.c.lg) - 1)));
+    *(us8 *)(out + row * a.c.D + d) = y;
+}
+
+int paged_store_launch(const PagedStoreArgs &a, hipStream_t st) {
+    const int64_t n = (int64_t)a.T * (a.c.Hkv * a.c.D / 8);
+    const dim3 grid((unsigned)((n + 255) / 256), 2);
+    if (a.type == kRowF32 && a.c.bf16) paged_store_kernel<kRowF32, true><<<grid, 256, 0, st>>>(a);
+    else if (a.type == kRowF32) paged_store_kernel<kRowF32, false><<<grid, 256, 0, st>>>(a);
+    else paged_store_kernel<kRowF16, false><<<grid, 256, 0, st>>>(a);   // 16 bits of either type as they are
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace xjk

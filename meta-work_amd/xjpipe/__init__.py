@@ -110,6 +110,15 @@ class XjhKv8(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("type", "Hkv", "D", "n_ctx", "block")] + [("data", C.c_void_p), ("bytes", C.c_uint64)]
 
 
+class XjhPages(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("page", "n_pages", "max_blocks")] + [("table", C.c_void_p), ("free_list", C.c_void_p)]
+
+
+class XjhPaged(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "Hkv", "D", "page", "n_pages")] + \
+               [("k", C.c_void_p), ("v", C.c_void_p), ("bytes", C.c_uint64)]
+
+
 # -------------------------------------------------------------- library --
 
 _lib = None
@@ -206,6 +215,11 @@ def lib():
     _sig(L, "xjh_kv8_load", I, PK, I, I, P, I64, P, I64, P, CP, S)
     _sig(L, "xjh_attn_kv8", I, PK, P, I64, I64, P, I64, I64, I, I, I, P, I, I, F, P, I64, P, S, P, CP, S)
     _sig(L, "xjh_attn_kv8_work_bytes", S, PK, I, I, I, I, I)
+    PB = C.POINTER(XjhPaged)
+    _sig(L, "xjh_page_plan", I, C.POINTER(XjhPages), P, P, P, I, P, P, I, P, P, P, P, P, P, S, P, CP, S)
+    _sig(L, "xjh_page_plan_work_bytes", S, I)
+    _sig(L, "xjh_paged_bytes", U64, PB)
+    _sig(L, "xjh_paged_store", I, PB, I, P, I64, P, I64, I, P, P, CP, S)
     _lib = L
     return L
 
@@ -904,6 +918,95 @@ class Kv8:
                                   None, err, ERR), err, "attn_kv8")
         lib().xjh_sync()
         return do.get(np.float32, (T, H * D))
+
+
+# ------------------------------------------------------- several requests --
+
+_ROW_TYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}   # bf16 as its bits
+
+
+def _typed(a, dims, what):
+    """a as contiguous rows of float32, float16 or bf16 bits (uint16), and its ggml type id."""
+    a = np.ascontiguousarray(a)
+    if a.dtype not in _ROW_TYPES or a.ndim != len(dims) or any(d is not None and d != n for d, n in zip(dims, a.shape)):
+        raise XjError(f"{what}: {a.dtype} {a.shape}, expected float32, float16 or uint16 (bf16) of {tuple('any' if d is None else d for d in dims)}")
+    return a, _ROW_TYPES[a.dtype]
+
+
+def _ints(a, n, what):
+    """a as n int32; None: any number."""
+    a = np.asarray(a)
+    if a.ndim != 1 or (n is not None and a.shape[0] != n):
+        raise XjError(f"{what}: shape {a.shape}, expected ({'any' if n is None else n},)")
+    return np.ascontiguousarray([_i32(x, what) for x in a.tolist()], np.int32)
+
+
+class PagePool:
+    """The pages of several requests' caches on the GPU (xjh_pages), all of them free at first; numpy in and out, every call waits."""
+
+    def __init__(self, page, n_pages, n_req, max_blocks):
+        page, n_pages, self.n_req, max_blocks = (_i32(n, "page_plan") for n in (page, n_pages, n_req, max_blocks))
+        if min(page, n_pages, max_blocks) < 1 or self.n_req < 0 or n_pages * page >= 1 << 31 or self.n_req * max_blocks > 1 << 30:
+            raise XjError(f"page_plan: bad shape (page={page}, n_pages={n_pages}, n_req={self.n_req}, max_blocks={max_blocks})")
+        self._table = Dev(np.full((max(1, self.n_req), max_blocks), -1, np.int32))
+        self._free, self._n_free = Dev(np.arange(n_pages, dtype=np.int32)), Dev(np.array([n_pages], np.int32))
+        self.p = XjhPages(page, n_pages, max_blocks, self._table.ptr, self._free.ptr)
+
+    @property
+    def table(self):
+        return self._table.get(np.int32, (self.n_req, self.p.max_blocks))
+
+    @property
+    def free(self):
+        """The free pages; the last is taken first."""
+        return self._free.get(np.int32, (self.p.n_pages,))[:self._n_free.get(np.int32, (1,))[0]]
+
+    def plan(self, n_past, n_new, held=None, T=None):
+        """xjh_page_plan for a step of T rows (default: as many as n_new asks for): a dict of cu, kv_len, pos, slot and status."""
+        past, new = _ints(n_past, self.n_req, "page_plan: n_past"), _ints(n_new, self.n_req, "page_plan: n_new")
+        if T is None:
+            T = int(np.maximum(new, 0).sum(dtype=np.int64))
+        T = _i32(T, "page_plan: T")
+        (dp, pp), (dn, pn) = _opt(past), _opt(new)
+        dh, ph = _opt(_ints(held, self.n_req, "page_plan: held") if held is not None else None)
+        out = {"cu": self.n_req + 1, "kv_len": self.n_req, "pos": T, "slot": T, "status": 4}
+        d = {k: Dev(nbytes=max(4, 4 * n)) for k, n in out.items()}
+        n = lib().xjh_page_plan_work_bytes(self.n_req)
+        work, err = Dev(nbytes=max(16, n)), _err()
+        _check(lib().xjh_page_plan(C.byref(self.p), ph, pp, pn, self.n_req, self._n_free.ptr, self._n_free.ptr, T, d["cu"].ptr,
+                                   d["kv_len"].ptr, d["pos"].ptr, d["slot"].ptr, d["status"].ptr, work.ptr, n, None, err, ERR),
+               err, "page_plan")
+        lib().xjh_sync()
+        return {k: d[k].get(np.int32, (n,)) for k, n in out.items()}
+
+
+class PagedKv:
+    """A layer's keys and values in pages on the GPU (xjh_paged), float16 or bf16 (as uint16); numpy in and out, every call waits."""
+
+    def __init__(self, Hkv, D, page, n_pages, type=F16):
+        self.c = XjhPaged(*(_i32(n, "paged") for n in (type, Hkv, D, page, n_pages)))
+        n = lib().xjh_paged_bytes(C.byref(self.c))
+        if not n:
+            raise XjError(f"unsupported cache (type={type}, Hkv={Hkv}, D={D}, page={page}, n_pages={n_pages})")
+        self.k, self.v = Dev(np.zeros(n, np.uint8)), Dev(np.zeros(n, np.uint8))
+        self.c.k, self.c.v, self.c.bytes = self.k.ptr, self.v.ptr, n
+
+    def pages(self):
+        """(k, v) [n_pages][Hkv][page][D]"""
+        dt = np.float16 if self.c.type == F16 else np.uint16
+        shape = (self.c.n_pages, self.c.Hkv, self.c.page, self.c.D)
+        return self.k.get(dt, shape), self.v.get(dt, shape)
+
+    def store(self, k, v, slot):
+        """Rows k, v [T][Hkv][D] into their slots; slots outside the pages skip theirs."""
+        k, t = _typed(k, (None, self.c.Hkv, self.c.D), "paged_store: k")
+        v, tv = _typed(v, k.shape, "paged_store: v")
+        slot = _ints(slot, k.shape[0], "paged_store: slot")
+        if t != tv or np.unique(slot[slot >= 0]).size != np.count_nonzero(slot >= 0):
+            raise XjError("paged_store: k and v of two types, or a slot twice")
+        (dk, kp), (dv, vp), (ds, sp), row, err = _opt(k), _opt(v), _opt(slot), self.c.Hkv * self.c.D, _err()
+        _check(lib().xjh_paged_store(C.byref(self.c), t, kp, row, vp, row, k.shape[0], sp, None, err, ERR), err, "paged_store")
+        lib().xjh_sync()
 
 
 def device_name():
