@@ -609,6 +609,38 @@ uint64_t xjh_paged_bytes(const xjh_paged *c);
  * range: infinity). A slot outside [0, n_pages * page) skips its row. The slots of a call differ. */
 int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, const void *v, int64_t v_tok, int T,
                     const int32_t *slot, void *stream, char *err, size_t errlen);
+/* Attention of every request's new tokens over its pages: request r's are the rows cu[r] .. cu[r+1]-1
+ * of q, gate and out (elements of `type`, XJ_F32 or the cache's; rows from T on do not exist), at positions
+ * kv_len[r] - n .. kv_len[r]-1, n = cu[r+1] - cu[r], and their keys and values are in the cache already.
+ * Query head h (q + row*q_tok + h*q_head, D elements) of the token at p reads kv head
+ * h / (H/Hkv) and sees the positions j <= p, with window > 0 only those with j > p - window or j < n_sink
+ * (the first tokens stay visible); out[row*o_tok + h*D ..] = softmax(scale q.K^T) V, times
+ * sigmoid(gate[row*g_tok + h*g_head ..]) when gate is not NULL. A row that sees nothing (a position
+ * below 0) is 0; rows that belong to no request keep their values. table [n_req][max_blocks] as in
+ * xjh_pages (max_blocks * page <= 2^30; kv_len beyond that counts as it); requests may share pages.
+ * A table entry outside [0, n_pages) stands for positions that are not seen. What lies at positions
+ * that a row does not see, NaN too, counts for nothing in it; a value that it sees and is not finite leaves it not finite.
+ * Products of 16-bit elements are exact and sums are fp32. Weights enter with the cache's bits; with float rows the
+ * queries and the weights enter with 22 bits over f16 (queries to 2^-40 of the row's largest element,
+ * weights to 2^-40 of the row's largest) and 24 over bf16.
+ * max_new: the largest n, as far as the program knows (0: it does not); it decides which kernel runs, and a
+ * larger n is right too. The result does not depend on it, or on the work area, beyond the rounding of sums.
+ * T * H is at most 2^28, n_req 65536. */
+int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, int64_t q_head, const void *gate, int64_t g_tok,
+                   int64_t g_head, const int32_t *table, int max_blocks, const int32_t *cu, const int32_t *kv_len, int n_req,
+                   int T, int max_new, int H, int window, int n_sink, float scale, void *out, int64_t o_tok, void *work,
+                   size_t work_bytes, void *stream, char *err, size_t errlen);
+/* The work area beyond which nothing is gained for these; 0 when they are not supported. */
+size_t xjh_attn_paged_work_bytes(const xjh_paged *c, int type, int T, int H, int n_req, int max_new, int max_blocks);
+/* The same for whole sequences that lie packed in rows: sequence s is the rows cu[s] .. cu[s+1]-1 of q, k, v, gate and
+ * out (all of `type`, XJ_F32, XJ_F16 or XJ_BF16), the first at position 0; kv head g of a row at k + row*k_tok +
+ * g*k_head, D elements (64, 128 or 256). Float queries, keys, values and weights enter with 24 bits. Rows of k and v
+ * whose addresses are multiples of 16 bytes are read faster. */
+int xjh_attn_packed(int type, const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
+                    const void *v, int64_t v_tok, int64_t v_head, const void *gate, int64_t g_tok, int64_t g_head,
+                    const int32_t *cu, int n_seq, int T, int H, int Hkv, int D, int window, int n_sink, float scale, void *out,
+                    int64_t o_tok, void *work, size_t work_bytes, void *stream, char *err, size_t errlen);
+size_t xjh_attn_packed_work_bytes(int type, int T, int H, int Hkv, int D, int n_seq);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,223 @@
+// Attention over batches of requests of different lengths: what its kernels share (gfx950).
+//
+// The rows of a request and kv head are its new tokens times the G = H / Hkv query heads that read that kv head, row R being
+// token R / G, query head R % G. A work item is a tile of BM rows of a request and a kv head over a piece of the key tiles
+// (of BN positions) that they see. The kernels form S^T = K Q^T, so that a lane holds scores of one row only, and O^T = V^T P^T
+// straight from them: with the keys of an instruction taken in the order in which the first product leaves them, the weights
+// are the second one's operand as they are.
+#pragma once
+#include "common.h"
+#include "kernels.h"
+
+namespace xjk {
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4_u __attribute__((ext_vector_type(4), aligned(2)));   // rows of any 2-byte alignment
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8_u __attribute__((ext_vector_type(8), aligned(4)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+// Operands of the matrix cores.
+template <class E>
+struct Op;
+template <>
+struct Op<_Float16> {
+    typedef hf8 v8;
+    static constexpr uint32_t kExp = 0x7C00, kOne = 0x3C00;
+    static constexpr float kLift = 15.f;   // weights enter as 2^15 p, at most 32768: f16 loses them from 2^-29 on only
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Op<__bf16> {
+    typedef bf8 v8;
+    static constexpr uint32_t kExp = 0x7F80, kOne = 0x3F80;
+    static constexpr float kLift = 0.f;
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <class E>
+using V8 = typename Op<E>::v8;
+
+// Eight numbers as NP planes that add up to them: one plane rounds to nearest; f16 in two keeps 22 bits (of numbers scaled so that
+// the planes are no subnormals); bf16 in three, each the leading 8 bits of what is left, is exact. (An infinity's further
+// planes are NaN: a product with it is not finite.)
+template <class E, int NP>
+__device__ __forceinline__ void planes(const float (&x)[8], V8<E> (&p)[NP]) {
+    if constexpr (NP == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[0][i] = (E)x[i];
+    } else if constexpr (NP == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[0][i] = (E)x[i];
+            p[1][i] = (E)(x[i] - (float)p[0][i]);
+        }
+    } else {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            uint32_t u[3], v[3];
+            float a = x[i], b = x[i + 1];
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                u[k] = __float_as_uint(a) & 0xFFFF0000u;
+                v[k] = __float_as_uint(b) & 0xFFFF0000u;
+                a -= __uint_as_float(u[k]);
+                b -= __uint_as_float(v[k]);
+                w[k][i / 2] = __builtin_amdgcn_perm(v[k], u[k], 0x07060302u);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) p[k] = __builtin_bit_cast(V8<E>, u32x4{w[k][0], w[k][1], w[k][2], w[k][3]});
+    }
+}
+
+// The larger of a lane's value and that of lane l ^ 16, l ^ 32.
+__device__ __forceinline__ float max_x16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The rows of one request.
+struct Seq {
+    int r, start, rows, pos0;   // its rows of q, the first one's position
+    int tiles, len;             // row tiles; key tiles that the last of them sees
+};
+// The key tiles that rows at positions pf .. pl see: n of them, tile(i) the i-th.
+struct Range {
+    int first, n_sink, n;
+    __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
+};
+template <int BN>
+__device__ __forceinline__ Range range_of(const BatchAttnArgs &a, int pf, int pl) {
+    Range g{0, 0, 0};
+    if (pl < 0) return g;
+    if (a.window) {
+        g.first = max(0, pf - a.window + 1) / BN;
+        g.n_sink = min((min(a.sinks, pl + 1) + BN - 1) / BN, g.first);
+    }
+    g.n = g.n_sink + pl / BN - g.first + 1;
+    return g;
+}
+template <int BM, int BN>
+__device__ __forceinline__ Seq seq_of(const BatchAttnArgs &a, int r) {
+    Seq s{};
+    if (r >= a.n_req) return s;
+    const int c0 = a.cu[r], c1 = a.cu[r + 1];
+    s.r = r;
+    s.start = min(max(c0, 0), a.T);
+    s.rows = min(max(c1, s.start), a.T) - s.start;
+    if (a.kv_len) s.pos0 = (int)max((int64_t)min(max(a.kv_len[r], 0), a.max_blocks << a.lg) - ((int64_t)c1 - c0), (int64_t)(-1 << 30));
+    s.tiles = (s.rows * a.G + BM - 1) / BM;
+    if (s.tiles) s.len = range_of<BN>(a, s.pos0 + (s.tiles - 1) * BM / a.G, s.pos0 + s.rows - 1).n;
+    return s;
+}
+__device__ __forceinline__ int wave_scan(int v) {   // sums up to and with this lane
+    const int lane = threadIdx.x & 63;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(v, o, 64);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+struct Item {
+    Seq s;
+    int tile, head, piece, pieces, slot;
+};
+// Work item `item` (with MERGE: row tile and head `item` of those in more than one piece); false beyond the last. Every
+// wavefront finds its own, from the lengths, 64 requests at a time: with U key tiles over all row tiles and heads, a piece is about U / a.target
+// of them and no fewer than a.least, so that the pieces are alike whatever the lengths. At most a.target + (row tiles * heads) items,
+// 2 a.target of them in pieces: a request is cut only if it has more than a piece's tiles.
+template <int BM, int BN, bool MERGE>
+__device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item &it) {
+    const int lane = threadIdx.x & 63;
+    int per = INT32_MAX;
+    Seq s{};
+    if (a.target) {
+        float u = 0.f;
+        for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+            s = seq_of<BM, BN>(a, r0 + lane);
+            u += (float)s.tiles * (float)s.len;
+        }
+        for (int o = 32; o; o >>= 1) u += __shfl_xor(u, o, 64);
+        per = max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1);
+    }
+    int items = 0, slots = 0;
+    for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+        if (a.n_req > 64 || !a.target) s = seq_of<BM, BN>(a, r0 + lane);
+        const int pieces = max(1, (int)(((int64_t)s.len + per - 1) / per)), heads = s.tiles * a.Hkv;
+        const int n_slot = pieces > 1 ? heads * pieces : 0, n = MERGE ? (pieces > 1 ? heads : 0) : heads * pieces;
+        const int to = items + wave_scan(n), slot_to = slots + wave_scan(n_slot);
+        const unsigned long long m = __ballot(to > item);
+        if (m) {
+            const int l = __builtin_ctzll(m);
+            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            it.s = Seq{get(s.r), get(s.start), get(s.rows), get(s.pos0), get(s.tiles), get(s.len)};
+            it.pieces = get(pieces);
+            const int local = item - get(to - n), slot = get(slot_to - n_slot);
+            it.head = local % a.Hkv;
+            const int q = local / a.Hkv;
+            it.piece = MERGE ? 0 : q % it.pieces;
+            const int i = MERGE ? q : q / it.pieces;
+            it.tile = it.s.tiles - 1 - i;   // those that see most first
+            it.slot = slot + (i * it.pieces + it.piece) * a.Hkv + it.head;   // the next piece's is Hkv further
+            return true;
+        }
+        items = __builtin_amdgcn_readlane(to, 63);
+        slots = __builtin_amdgcn_readlane(slot_to, 63);
+    }
+    return false;
+}
+
+// A page of the request's row for position j, uniform over the wavefront, or -1. (Read as a constant: a vector load would be
+// waited for behind the keys and values on their way.)
+__device__ __forceinline__ int page_at(const BatchAttnArgs &a, const int32_t *row, int j) {
+    const int b = __builtin_amdgcn_readfirstlane(j) >> a.lg;
+    const int p = b < a.max_blocks ? ((const __attribute__((address_space(4))) int32_t *)row)[b] : -1;
+    return p >= 0 && p < a.n_pages ? p : -1;
+}
+__device__ __forceinline__ bool sees(const BatchAttnArgs &a, int p, int j) {
+    return j <= p && (!a.window || j > p - a.window || j < a.sinks);
+}
+
+// State of the splits in the work area: [slots][BM][D] unscaled sums, then [slots][BM] of (the largest score in powers of two,
+// the weights' sum). A row that has seen nothing yet has the largest score -infinity.
+__device__ __forceinline__ float *part_sums(const BatchAttnArgs &a, int64_t row, int D) { return a.part + row * D; }
+__device__ __forceinline__ float2 *part_stat(const BatchAttnArgs &a, int64_t row, int BM, int D) {
+    return (float2 *)(a.part + (int64_t)a.slots * BM * D) + row;
+}
+
+template <int RT>
+struct Row;
+template <>
+struct Row<kRowF32> {
+    typedef float t;
+};
+template <>
+struct Row<kRowF16> {
+    typedef _Float16 t;
+};
+template <>
+struct Row<kRowBf16> {
+    typedef __bf16 t;
+};
+
+// Scores that underflow every weight still count as seen: the running maximum (in powers of two, rounded up) stays finite.
+constexpr float kLowest = -1e38f;
+
+int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st);
+int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
+int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
+constexpr int kFewRows = 16, kFewKeys = 32;
+constexpr int kManyRows = 128;
+constexpr int many_keys(int D) { return D == 256 ? 32 : 64; }
+
+}  // namespace xjk

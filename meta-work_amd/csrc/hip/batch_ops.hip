@@ -109,3 +109,107 @@ extern "C" int xjh_paged_store(const xjh_paged *c, int type, const void *k, int6
     if (paged_store_launch(a, st)) { snprintf(err, errlen, "paged_store launch failed"); return -1; }
     return 0;
 }
+
+static bool batch_ok(int n_req, int T, int H, int Hkv, int window, int n_sink) {
+    return n_req >= 0 && n_req <= kMaxReq && T >= 0 && Hkv >= 1 && Hkv <= 1024 && H >= Hkv && H % Hkv == 0 && (int64_t)T * H <= (1 << 28) &&
+           window >= 0 && n_sink >= 0;
+}
+static bool paged_batch_ok(const xjh_paged *c, int type, int T, int H, int n_req, int max_blocks) {
+    return (type == XJ_F32 || type == c->type) && batch_ok(n_req, T, H, c->Hkv, 0, 0) && max_blocks >= 1 &&
+           (int64_t)max_blocks * c->page <= (1 << 30);
+}
+static bool packed_batch_ok(int type, int T, int H, int Hkv, int D, int n_seq) {
+    return row_type(type) >= 0 && batch_ok(n_seq, T, H, Hkv, 0, 0) && (D == 64 || D == 128 || D == 256);
+}
+static void batch_args(BatchAttnArgs &a, int type, int n_req, int T, int H, int Hkv, int D, int window, int n_sink) {
+    a.type = row_type(type);
+    a.n_req = n_req; a.T = T; a.H = H; a.Hkv = Hkv; a.D = D; a.G = H / Hkv;
+    a.window = window < (1 << 30) ? window : 0;   // positions are below 2^30
+    a.sinks = n_sink;
+}
+
+extern "C" int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, int64_t q_head, const void *gate,
+                              int64_t g_tok, int64_t g_head, const int32_t *table, int max_blocks, const int32_t *cu,
+                              const int32_t *kv_len, int n_req, int T, int max_new, int H, int window, int n_sink, float scale,
+                              void *out, int64_t o_tok, void *work, size_t work_bytes, void *stream, char *err, size_t errlen) {
+    Paged p;
+    if (!cache_ok(c, "attn_paged", p, err, errlen)) return -1;
+    if (!paged_batch_ok(c, type, T, H, n_req, max_blocks) || window < 0 || n_sink < 0 || !std::isfinite(scale)) {
+        snprintf(err, errlen, "attn_paged: bad shape (type=%d over %d, n_req=%d, T=%d, H=%d on %d kv heads, max_blocks=%d, window=%d, n_sink=%d, scale=%g)",
+                 type, c->type, n_req, T, H, c->Hkv, max_blocks, window, n_sink, scale);
+        return -1;
+    }
+    if (!T || !n_req) return 0;
+    if (!q || !out || !table || !cu || !kv_len || ((uintptr_t)work & 15)) {
+        snprintf(err, errlen, "attn_paged: a buffer is missing, or an unaligned work area");
+        return -1;
+    }
+    hipStream_t st;
+    if (!stream_of(stream, st, "attn_paged", err, errlen)) return -1;
+    BatchAttnArgs a{};
+    batch_args(a, type, n_req, T, H, p.Hkv, p.D, window, n_sink);
+    a.q = q; a.q_tok = q_tok; a.q_head = q_head;
+    a.gate = gate; a.g_tok = g_tok; a.g_head = g_head;
+    a.out = out; a.o_tok = o_tok;
+    a.k = p.k; a.v = p.v;
+    a.kv_type = p.bf16 ? kRowBf16 : kRowF16;
+    a.table = table; a.kv_len = kv_len; a.cu = cu;
+    a.lg = p.lg; a.n_pages = p.n_pages; a.max_blocks = max_blocks;
+    a.max_new = max_new; a.scale = scale;
+    a.part = (float *)work;
+    if (batch_attn_launch(a, work ? (int64_t)(work_bytes / sizeof(float)) : 0, st)) {
+        snprintf(err, errlen, "attn_paged launch failed");
+        return -1;
+    }
+    return 0;
+}
+
+extern "C" size_t xjh_attn_paged_work_bytes(const xjh_paged *c, int type, int T, int H, int n_req, int max_new, int max_blocks) {
+    if (!shape_ok(c) || !paged_batch_ok(c, type, T, H, n_req, max_blocks)) return 0;
+    BatchAttnArgs a{};
+    batch_args(a, type, n_req, T, H, c->Hkv, c->D, 0, 0);
+    a.table = (const int32_t *)c;   // pages
+    a.lg = __builtin_ctz((unsigned)c->page); a.max_blocks = max_blocks; a.max_new = max_new;
+    return (size_t)batch_attn_part_floats(a) * sizeof(float);
+}
+
+extern "C" int xjh_attn_packed(int type, const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
+                               const void *v, int64_t v_tok, int64_t v_head, const void *gate, int64_t g_tok, int64_t g_head,
+                               const int32_t *cu, int n_seq, int T, int H, int Hkv, int D, int window, int n_sink, float scale,
+                               void *out, int64_t o_tok, void *work, size_t work_bytes, void *stream, char *err, size_t errlen) {
+    if (!packed_batch_ok(type, T, H, Hkv, D, n_seq) || window < 0 || n_sink < 0 || !std::isfinite(scale)) {
+        snprintf(err, errlen, "attn_packed: bad shape (type=%d, n_seq=%d, T=%d, H=%d on %d kv heads of %d (64|128|256), window=%d, n_sink=%d, scale=%g)",
+                 type, n_seq, T, H, Hkv, D, window, n_sink, scale);
+        return -1;
+    }
+    if (!T || !n_seq) return 0;
+    if (!q || !k || !v || !out || !cu || ((uintptr_t)work & 15)) {
+        snprintf(err, errlen, "attn_packed: a buffer is missing, or an unaligned work area");
+        return -1;
+    }
+    hipStream_t st;
+    if (!stream_of(stream, st, "attn_packed", err, errlen)) return -1;
+    BatchAttnArgs a{};
+    batch_args(a, type, n_seq, T, H, Hkv, D, window, n_sink);
+    a.q = q; a.q_tok = q_tok; a.q_head = q_head;
+    a.gate = gate; a.g_tok = g_tok; a.g_head = g_head;
+    a.out = out; a.o_tok = o_tok;
+    a.k = k; a.k_tok = k_tok; a.k_head = k_head;
+    a.v = v; a.v_tok = v_tok; a.v_head = v_head;
+    a.kv_type = a.type;
+    a.cu = cu;
+    a.scale = scale;
+    a.part = (float *)work;
+    if (batch_attn_launch(a, work ? (int64_t)(work_bytes / sizeof(float)) : 0, st)) {
+        snprintf(err, errlen, "attn_packed launch failed");
+        return -1;
+    }
+    return 0;
+}
+
+extern "C" size_t xjh_attn_packed_work_bytes(int type, int T, int H, int Hkv, int D, int n_seq) {
+    if (!packed_batch_ok(type, T, H, Hkv, D, n_seq)) return 0;
+    BatchAttnArgs a{};
+    batch_args(a, type, n_seq, T, H, Hkv, D, 0, 0);
+    return (size_t)batch_attn_part_floats(a) * sizeof(float);
+}

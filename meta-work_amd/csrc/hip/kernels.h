@@ -439,5 +439,24 @@ struct PagedStoreArgs {
     const int32_t *slot;
 };
 int paged_store_launch(const PagedStoreArgs &a, hipStream_t st);
+// Attention over batches of requests (batch_attn*.hip), as xjh_attn_paged and xjh_attn_packed in xj_hip.h.
+struct BatchAttnArgs {
+    const void *q; int64_t q_tok, q_head;
+    const void *gate; int64_t g_tok, g_head;      // optional
+    void *out; int64_t o_tok;
+    const void *k; int64_t k_tok, k_head;         // pages: the cache's k and v, no strides
+    const void *v; int64_t v_tok, v_head;
+    const int32_t *table, *kv_len;                // pages only
+    const int32_t *cu;
+    int32_t lg, n_pages, max_blocks;
+    int32_t n_req, T, max_new, H, Hkv, D, G;
+    int32_t type, kv_type;                        // RowType of q, gate, out, and of k, v
+    int32_t window, sinks;
+    float scale;
+    float *part;                                  // split partials
+    int32_t target, least, slots;                 // set by batch_attn_launch: pieces aimed at, key tiles a piece at least, the partials' room
+};
+int batch_attn_launch(const BatchAttnArgs &a, int64_t part_floats, hipStream_t st);
+int64_t batch_attn_part_floats(const BatchAttnArgs &a);      // beyond this nothing is gained
 
 }  // namespace xjk

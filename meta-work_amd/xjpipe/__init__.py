@@ -220,6 +220,10 @@ def lib():
     _sig(L, "xjh_page_plan_work_bytes", S, I)
     _sig(L, "xjh_paged_bytes", U64, PB)
     _sig(L, "xjh_paged_store", I, PB, I, P, I64, P, I64, I, P, P, CP, S)
+    _sig(L, "xjh_attn_paged", I, PB, I, P, I64, I64, P, I64, I64, P, I, P, P, I, I, I, I, I, I, F, P, I64, P, S, P, CP, S)
+    _sig(L, "xjh_attn_paged_work_bytes", S, PB, I, I, I, I, I, I)
+    _sig(L, "xjh_attn_packed", I, I, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, P, I, I, I, I, I, I, I, F, P, I64, P, S, P, CP, S)
+    _sig(L, "xjh_attn_packed_work_bytes", S, I, I, I, I, I, I)
     _lib = L
     return L
 
@@ -1007,6 +1011,69 @@ class PagedKv:
         (dk, kp), (dv, vp), (ds, sp), row, err = _opt(k), _opt(v), _opt(slot), self.c.Hkv * self.c.D, _err()
         _check(lib().xjh_paged_store(C.byref(self.c), t, kp, row, vp, row, k.shape[0], sp, None, err, ERR), err, "paged_store")
         lib().xjh_sync()
+
+    def attend(self, q, table, cu, kv_len, gate=None, window=0, n_sink=0, scale=None, max_new=None, work_bytes=None):
+        """Attention of q [T][H][D], request r's rows cu[r] .. cu[r+1]-1 at the positions before kv_len[r], over the pages
+        that the table [n_req][max_blocks] names; [T][H*D] of q's type. Rows of no request are 0. max_new: what the library is told
+        (default: the largest); work_bytes: the work area (default: what it asks for)."""
+        q, t = _typed(q, (None, None, self.c.D), "attn_paged: q")
+        T, H, D = q.shape
+        table = np.asarray(table)
+        if table.ndim != 2:
+            raise XjError(f"attn_paged: table {table.shape}")
+        n_req, blocks = table.shape
+        tab = _ints(table.reshape(-1), None, "attn_paged: table")
+        cu, kv_len = _ints(cu, n_req + 1, "attn_paged: cu"), _ints(kv_len, n_req, "attn_paged: kv_len")
+        window, n_sink = _i32(window, "attn_paged: window"), _i32(n_sink, "attn_paged: n_sink")
+        max_new = max(int(np.diff(cu.astype(np.int64)).max(initial=0)), 0) if max_new is None else max_new
+        max_new = _i32(max_new, "attn_paged: max_new")
+        (dq, qp), (dt, tp), (dc, cp), (dk, kp) = _opt(q), _opt(tab), _opt(cu), _opt(kv_len)
+        dg, gp = _opt(_gate(gate, q, t, "attn_paged: gate"))
+        do, err = Dev(np.zeros(max(1, q.size), q.dtype)), _err()
+        if work_bytes is None:
+            work_bytes = lib().xjh_attn_paged_work_bytes(C.byref(self.c), t, T, H, n_req, max_new, blocks)
+        dw = Dev(nbytes=work_bytes) if work_bytes else None
+        _check(lib().xjh_attn_paged(C.byref(self.c), t, qp, H * D, D, gp, H * D, D, tp, blocks, cp, kp, n_req, T, max_new, H, window,
+                                    n_sink, D ** -0.5 if scale is None else scale, do.ptr, H * D, dw.ptr if dw else None, work_bytes,
+                                    None, err, ERR), err, "attn_paged")
+        lib().xjh_sync()
+        return do.get(q.dtype, (T, H * D))
+
+
+def _gate(gate, q, t, what):
+    if gate is None:
+        return None
+    gate, tg = _typed(gate, q.shape, what)
+    if tg != t:
+        raise XjError(f"{what}: {gate.dtype}, the queries are {q.dtype}")
+    return gate
+
+
+def attn_packed(q, k, v, cu, gate=None, window=0, n_sink=0, scale=None, work_bytes=None):
+    """Causal attention of whole sequences on the GPU: q [T][H][D], k, v [T][Hkv][D], sequence s the rows cu[s] .. cu[s+1]-1;
+    [T][H*D] of q's type, rows of no sequence 0."""
+    q, t = _typed(q, (None, None, None), "attn_packed: q")
+    T, H, D = q.shape
+    k, tk = _typed(k, (T, None, D), "attn_packed: k")
+    v, tv = _typed(v, k.shape, "attn_packed: v")
+    if tk != t or tv != t:
+        raise XjError(f"attn_packed: rows of {q.dtype}, {k.dtype} and {v.dtype}")
+    Hkv, cu = k.shape[1], _ints(cu, None, "attn_packed: cu")
+    n = cu.shape[0] - 1
+    if n < 0:
+        raise XjError("attn_packed: cu is empty")
+    window, n_sink = _i32(window, "attn_packed: window"), _i32(n_sink, "attn_packed: n_sink")
+    (dq, qp), (dk, kp), (dv, vp), (dc, cp) = _opt(q), _opt(k), _opt(v), _opt(cu)
+    dg, gp = _opt(_gate(gate, q, t, "attn_packed: gate"))
+    do, err = Dev(np.zeros(max(1, q.size), q.dtype)), _err()
+    if work_bytes is None:
+        work_bytes = lib().xjh_attn_packed_work_bytes(t, T, H, Hkv, D, n)
+    dw = Dev(nbytes=work_bytes) if work_bytes else None
+    _check(lib().xjh_attn_packed(t, qp, H * D, D, kp, Hkv * D, D, vp, Hkv * D, D, gp, H * D, D, cp, n, T, H, Hkv, D, window, n_sink,
+                                 (D ** -0.5 if D else 0.0) if scale is None else scale, do.ptr, H * D, dw.ptr if dw else None, work_bytes, None,
+                                 err, ERR), err, "attn_packed")
+    lib().xjh_sync()
+    return do.get(q.dtype, (T, H * D))
 
 
 def device_name():

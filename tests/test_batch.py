@@ -2,6 +2,10 @@
 forms written here from the text of xj_hip.h, and what they refuse (on the CPU, where nothing is launched).
 
 Tables, lengths and slots are whole numbers and equal. A stored element is its row's, rounded once to nearest: equal bits.
+Attention, with u the half step of the rows' type (f16 2^-11, bf16 2^-8): every weight is rounded once (u of it) and so is
+the result, so an element is off by at most u of itself and u + 1e-5 of its row's sum_j p_j |v_j| (the 1e-5: fp32 sums and scores up to
+20, off by a few of their own roundings: 20 * 1.44 * 4 * 2^-24 = 7e-6 in a weight). Float rows have no u, and 2e-6 over the norm of all rows, where
+the roundings are independent.
 """
 import ctypes as C
 
@@ -9,6 +13,7 @@ import numpy as np
 import pytest
 
 import xjpipe as xp
+from test_long_context import Hip
 
 
 # ------------------------------------------------------------ plain forms --
@@ -214,3 +219,403 @@ def test_store_refusals():
     assert store(T=0, x=None, slot=None) == 0
     assert L.xjh_paged_store(None, xp.F32, one, 64, one, 64, 1, one, None, err, 512) == -1
     assert L.xjh_paged_bytes(None) == 0
+
+
+# -------------------------------------------------------------- attention --
+
+IDS = {"f32": xp.F32, "f16": xp.F16, "bf16": xp.BF16}
+HALF = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def to_type(x, t):
+    return bf16_bits(x) if t == "bf16" else x.astype(np.float16 if t == "f16" else np.float32)
+
+
+def value(x):
+    """The numbers that an array of float32, float16 or bf16 bits holds, in float64."""
+    return (from_bf16(x) if x.dtype == np.uint16 else x).astype(np.float64)
+
+
+def attend64(q, k, v, pos, seen=None, gate=None, window=0, n_sink=0, scale=None):
+    """q [n][H][D] at positions pos .., k, v [m][Hkv][D], float64: (out, sum of p |v|). seen [m]: positions that exist."""
+    n, H, D = q.shape
+    m, G = k.shape[0], H // k.shape[1]
+    p, j = pos + np.arange(n)[:, None], np.arange(m)[None]
+    see = (j <= p) & ((window == 0) | (j > p - window) | (j < n_sink))
+    if seen is not None:
+        see = see & seen[None]
+    out, mag = np.zeros((n, H, D)), np.zeros((n, H, D))
+    for h in range(H):
+        s = np.where(see, q[:, h] @ k[:, h // G].T * (D ** -0.5 if scale is None else scale), -np.inf)
+        top = s.max(1, initial=-np.inf, keepdims=True)
+        w = np.exp(s - np.where(np.isfinite(top), top, 0))
+        w = np.divide(w, w.sum(1, keepdims=True), out=np.zeros_like(w), where=see.any(1, keepdims=True))
+        out[:, h], mag[:, h] = w @ v[:, h // G], w @ np.abs(v[:, h // G])
+        if gate is not None:
+            sg = 1 / (1 + np.exp(-gate[:, h]))
+            out[:, h], mag[:, h] = out[:, h] * sg, mag[:, h] * sg
+    return out, mag
+
+
+def check(got, want, mag, t):
+    got = value(got).reshape(want.shape)
+    u = HALF[t]
+    assert np.all(np.isfinite(got))
+    err, bar = np.abs(got - want), u * np.abs(want) + (u + 1e-5) * mag + (2.0 ** -24 if t == "f16" else 0)   # f16's smallest step
+    assert np.all(err <= bar), (float((err / np.maximum(bar, 1e-300)).max()), np.unravel_index(np.argmax(err - bar), err.shape))
+    if t == "f32" and np.linalg.norm(mag):
+        assert np.linalg.norm(err) <= 2e-6 * np.linalg.norm(mag)
+
+
+def kv_rows(rng, n, Hkv, D):
+    x = rng.standard_normal((n, Hkv, D)) * np.exp(0.3 * rng.standard_normal((1, Hkv, D)) + 0.2 * rng.standard_normal((n, Hkv, 1)))
+    return (x + 0.5 * rng.standard_normal((1, Hkv, D))).astype(np.float32)
+
+
+class Batch:
+    """Requests of (kv length, new rows) in shuffled pages whose other positions hold NaN."""
+
+    def __init__(self, rng, lens, H, Hkv, D, page, rows="f16", cache="f16", spare=0, kv=None):
+        self.lens, self.rows, self.D, self.H = lens, rows, D, H
+        blocks = [up(max(n, 0), page) for n, _ in lens]
+        n_pages = sum(blocks) + 2
+        order = rng.permutation(n_pages)[:sum(blocks)].tolist()
+        self.table = np.full((len(lens), max(blocks + [1]) + spare), -1, np.int32)
+        nan = np.uint16(0x7E00 if cache == "f16" else 0x7FC0)
+        pool = np.full((2, n_pages, Hkv, page, D), nan, np.uint16)
+        self.kv = []
+        for r, (n, _) in enumerate(lens):
+            x = [to_type(a, cache) for a in (kv(r, n) if kv else (kv_rows(rng, n, Hkv, D), kv_rows(rng, n, Hkv, D)))]
+            self.kv.append([value(a) for a in x])
+            for b in range(blocks[r]):
+                self.table[r, b] = g = order.pop()
+                for w in range(2):
+                    part = x[w][b * page:(b + 1) * page].view(np.uint16)
+                    pool[w, g, :, :part.shape[0]] = part.transpose(1, 0, 2)
+        self.cache = xp.PagedKv(Hkv, D, page, n_pages, type=IDS[cache])
+        self.cache.k.put(pool[0]), self.cache.v.put(pool[1])
+        self.cu = np.cumsum([0] + [m for _, m in lens])
+        T = int(self.cu[-1])
+        self.q, self.gate = (to_type((rng.standard_normal((T, H, D)) * 1.5).astype(np.float32), rows) for _ in range(2))
+
+    def want(self, gate=False, **kw):
+        got = []
+        for r, (n, m) in enumerate(self.lens):
+            rs = slice(int(self.cu[r]), int(self.cu[r + 1]))
+            got.append(attend64(value(self.q[rs]), *self.kv[r], n - m, gate=value(self.gate[rs]) if gate else None, **kw))
+        return tuple(np.concatenate([x[i] for x in got]) for i in range(2))
+
+    def attend(self, gate=False, **kw):
+        return self.cache.attend(self.q, self.table, self.cu, [n for n, _ in self.lens], gate=self.gate if gate else None, **kw)
+
+    def check(self, max_new=None, work_bytes=None, **kw):
+        got = self.attend(max_new=max_new, work_bytes=work_bytes, **kw)
+        check(got, *self.want(**kw), self.rows)
+        return got
+
+
+EDGES = [(1, 1), (2, 1), (15, 1), (16, 2), (17, 3), (31, 1), (32, 4), (33, 1), (63, 2), (64, 1), (65, 5), (127, 1), (128, 1), (129, 1), (257, 7)]
+PAIRS = [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [None, 0])   # few rows, many rows
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("H,Hkv,D,page", [(2, 1, 128, 16), (16, 4, 256, 64), (8, 8, 64, 256), (15, 3, 64, 32), (6, 2, 128, 128), (3, 1, 256, 16)])
+def test_paged_attention_of_few_rows(H, Hkv, D, page, rows, cache, max_new):
+    b = Batch(np.random.default_rng(H + D), EDGES, H, Hkv, D, page, rows, cache)
+    b.check(gate=True, max_new=1 if max_new is None else max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [None, 1])   # many rows, and the other kernel told wrongly
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("H,Hkv,D,page", [(2, 1, 128, 16), (16, 4, 256, 64), (8, 8, 64, 256), (15, 3, 64, 32), (3, 1, 256, 16)])
+def test_paged_attention_of_chunks(H, Hkv, D, page, rows, cache, max_new):
+    lens = [(300, 300), (150, 33), (90, 90), (1, 1), (401, 129), (64, 64), (0, 0), (200, 0), (130, 1)]
+    Batch(np.random.default_rng(H * D), lens, H, Hkv, D, page, rows, cache).check(max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (1, 1), (7, 4), (64, 0), (65, 64), (100, 130), (300, 2), (1 << 30, 5), ((1 << 31) - 1, 0), (50, (1 << 31) - 1)])
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("H,Hkv,D", [(4, 2, 128), (4, 1, 64), (8, 2, 256)])
+def test_paged_windows_and_first_tokens(H, Hkv, D, max_new, window, n_sink):
+    """Positions behind the window are in no page."""
+    lens = [(517, 1), (300, 6), (200, 70), (64, 64), (33, 1)]
+    b = Batch(np.random.default_rng(window % 999), lens, H, Hkv, D, 16, "f32", "f16")
+    for r, (n, m) in enumerate(lens):
+        for i in range(up(n, 16)):
+            if 16 * i + 15 <= n - m - window and 16 * i >= n_sink:
+                b.table[r, i] = [-1, 1 << 30, -1 << 31][i % 3]
+    b.check(window=window, n_sink=n_sink, max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("work_bytes", [None, 0, 64, 100000, 1 << 20])
+def test_paged_splits(work_bytes, max_new, rows, cache):
+    lens = [(5000, 1), (17, 1), (2100, 3), (640, 1), (1, 1)]
+    Batch(np.random.default_rng(9), lens, 8, 2, 128, 32, rows, cache, spare=40).check(gate=True, max_new=max_new, work_bytes=work_bytes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("n_req", [63, 64, 65, 300])
+def test_paged_many_requests(n_req, max_new):
+    rng = np.random.default_rng(n_req)
+    lens = [(int(n), 1) for n in rng.integers(1, 700, n_req)]
+    lens[n_req // 2] = (9000, 2)
+    Batch(rng, lens, 4, 2, 64, 16, "bf16", "bf16").check(max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+def test_paged_rows_before_the_first_position_and_of_no_request(max_new):
+    """More new rows than positions: those before position 0 see nothing and are 0; rows past the last request keep their values."""
+    rng, err = np.random.default_rng(3), C.create_string_buffer(512)
+    b = Batch(rng, [(5, 5), (40, 3)], 4, 2, 64, 16, "f32", "f16")
+    T, cu, kv = 12, np.array([0, 6, 9], np.int32), np.array([4, 40], np.int32)
+    q = rng.standard_normal((T, 4, 64)).astype(np.float32)
+    out = np.full((T, 4, 64), 7.0, np.float32)
+    dq, do, dt, dc, dk = (xp.Dev(x) for x in (q, out, b.table, cu, kv))
+    assert xp.lib().xjh_attn_paged(C.byref(b.cache.c), xp.F32, dq.ptr, 256, 64, None, 0, 0, dt.ptr, b.table.shape[1], dc.ptr, dk.ptr, 2, T, max_new, 4, 0, 0,
+                                   0.125, do.ptr, 256, None, 0, None, err, 512) == 0
+    xp.lib().xjh_sync()
+    got = do.get(np.float32, out.shape)
+    assert np.all(got[:2] == 0) and np.all(got[9:] == 7)
+    w0 = attend64(q[2:6].astype(np.float64), b.kv[0][0][:4], b.kv[0][1][:4], 0)
+    w1 = attend64(q[6:9].astype(np.float64), *b.kv[1], 37)
+    check(got[2:6], *w0, "f32")
+    check(got[6:9], *w1, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("cu,kv_len", [([0, 5, 3, 9], [20, 20, 20]), ([-4, 2, 100, 200], [20, 20, 20]), ([9, 0, 9, 9], [-3, 5, 1 << 30]),
+                                       ([0, 3, 6, 9], [-1 << 31, 0, (1 << 31) - 1])])
+def test_paged_lengths_that_make_no_sense_stay_in_bounds(cu, kv_len, max_new):
+    b = Batch(np.random.default_rng(4), [(20, 3)] * 3, 2, 1, 64, 16)
+    out = value(b.cache.attend(b.q, b.table, cu, kv_len, max_new=max_new))
+    assert out.shape == (9, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_paged_values_that_are_not_finite(D, rows, cache, max_new):
+    """Rows that do not see them are as without them; rows that do are not finite, in the dims concerned at least."""
+    lens = [(90, 40), (70, 6), (33, 1)]
+    for bad, at in ((np.inf, 60), (-np.inf, 75), (np.nan, 66)):
+        def kv(r, n):
+            rng = np.random.default_rng(r)
+            return kv_rows(rng, n, 2, D), kv_rows(rng, n, 2, D)
+
+        def spoilt(r, n):
+            k, v = kv(r, n)
+            if n > at:
+                v[at, 1, D // 2 + 1] = bad
+            return k, v
+
+        clean = Batch(np.random.default_rng(1), lens, 4, 2, D, 16, rows, cache, kv=kv)
+        b = Batch(np.random.default_rng(1), lens, 4, 2, D, 16, rows, cache, kv=spoilt)
+        want, got = (value(x.attend(max_new=max_new)).reshape(-1, 4, D) for x in (clean, b))
+        t = 0
+        for n, m in lens:
+            for p in range(n - m, n):
+                hit = at < n and p >= at
+                if hit:
+                    assert not np.isfinite(got[t, 2:, D // 2 + 1]).any()
+                    got[t, 2:, D // 2 + 1] = want[t, 2:, D // 2 + 1]
+                assert np.array_equal(got[t], want[t]), (bad, n, p)
+                t += 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("rows,cache", PAIRS)
+def test_paged_keys_and_queries_that_are_not_finite(rows, cache, max_new):
+    lens, D = [(80, 30), (50, 5)], 128
+    def kv(r, n):
+        rng = np.random.default_rng(r)
+        return kv_rows(rng, n, 1, D), kv_rows(rng, n, 1, D)
+
+    def spoilt(r, n):
+        k, v = kv(r, n)
+        k[47 + r, 0, 5] = np.nan
+        return k, v
+
+    clean = Batch(np.random.default_rng(1), lens, 2, 1, D, 32, rows, cache, kv=kv)
+    b = Batch(np.random.default_rng(1), lens, 2, 1, D, 32, rows, cache, kv=spoilt)
+    want, got = (value(x.attend(max_new=max_new)).reshape(-1, 2, D) for x in (clean, b))
+    for t, (r, p) in enumerate([(r, p) for r, (n, m) in enumerate(lens) for p in range(n - m, n)]):
+        if p >= 47 + r:
+            assert not np.isfinite(got[t]).any()
+        else:
+            assert np.array_equal(got[t], want[t]), (r, p)
+    q = clean.q.copy()
+    q[7, 1, 3] = np.float32(np.inf) if rows == "f32" else {"f16": np.float16(np.inf), "bf16": np.uint16(0x7F80)}[rows]
+    clean.q = q
+    got = value(clean.attend(max_new=max_new)).reshape(-1, 2, D)
+    assert not np.isfinite(got[7, 1]).any()
+    got[7, 1] = want[7, 1]
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 4.0])
+def test_paged_scales_of_any_sign(scale, max_new):
+    """4.0: scores of some hundred, a weight each in 64 bits compared in norm by the rounding of such scores (2^-24 of 400 * 1.44, a few of them)."""
+    b = Batch(np.random.default_rng(2), [(150, 40), (70, 1)], 4, 2, 64, 16, "f32", "f16")
+    got, (want, mag) = b.attend(scale=scale, max_new=max_new), b.want(scale=scale)
+    if scale != 4.0:
+        check(got, want, mag, "f32")
+    else:
+        assert np.linalg.norm(value(got).reshape(want.shape) - want) <= 4 * 400 * 1.44 * 2.0 ** -24 * np.linalg.norm(mag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1e6, 1e30])
+def test_paged_float_queries_of_any_size(size, max_new):
+    """Queries of a size and a scale that undoes it: the scores are ordinary."""
+    for cache in ("f16", "bf16"):
+        b = Batch(np.random.default_rng(2), [(150, 40), (70, 1)], 4, 2, 64, 16, "f32", cache)
+        b.q = (b.q * np.float32(size)).astype(np.float32)
+        b.check(scale=0.125 / size, max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+def test_paged_requests_that_share_pages(max_new):
+    rng = np.random.default_rng(8)
+    b = Batch(rng, [(100, 4), (100, 4), (40, 1)], 4, 1, 128, 16, "f16", "f16")
+    b.table[1, :5], b.kv[1] = b.table[0, :5], [np.concatenate([x[:80], y[80:]]) for x, y in zip(b.kv[0], b.kv[1])]
+    b.check(max_new=max_new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new,work_bytes", [(1, None), (1, 0), (0, None)])
+def test_paged_same_bits_again_and_in_any_batch(max_new, work_bytes):
+    """The same call gives the same bits."""
+    lens = [(3000, 1), (200, 60), (17, 3)]
+    b = Batch(np.random.default_rng(2), lens, 8, 2, 128, 16, "bf16", "bf16")
+    one = b.attend(max_new=max_new, work_bytes=work_bytes)
+    for _ in range(3):
+        assert np.array_equal(one, b.attend(max_new=max_new, work_bytes=work_bytes))
+
+
+PROMPTS = [300, 1, 0, 33, 128, 5, 129, 64, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("H,Hkv,D", [(2, 1, 128), (16, 4, 256), (8, 8, 64), (15, 3, 64), (3, 1, 256), (32, 8, 128)])
+@pytest.mark.parametrize("window,n_sink", [(0, 0), (50, 3)])
+def test_packed(H, Hkv, D, rows, window, n_sink):
+    rng = np.random.default_rng(H + D)
+    T, cu = sum(PROMPTS), np.cumsum([0] + PROMPTS)
+    q, gate = (to_type((rng.standard_normal((T, H, D)) * 1.5).astype(np.float32), rows) for _ in range(2))
+    k, v = (to_type(kv_rows(rng, T, Hkv, D), rows) for _ in range(2))
+    got = xp.attn_packed(q, k, v, cu, gate=gate, window=window, n_sink=n_sink)
+    w = [attend64(*(value(x[a:b]) for x in (q, k, v)), 0, gate=value(gate[a:b]), window=window, n_sink=n_sink) for a, b in zip(cu, cu[1:])]
+    check(got, *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("work_bytes", [None, 0, 300000])
+def test_packed_long(rows, work_bytes):
+    rng = np.random.default_rng(1)
+    T, H, Hkv, D = 2050, 2, 1, 64
+    q = to_type((rng.standard_normal((T, H, D)) * 1.5).astype(np.float32), rows)
+    k, v = (to_type(kv_rows(rng, T, Hkv, D), rows) for _ in range(2))
+    got = xp.attn_packed(q, k, v, [0, 1900, T], work_bytes=work_bytes)
+    w = [attend64(*(value(x[a:b]) for x in (q, k, v)), 0) for a, b in ((0, 1900), (1900, T))]
+    check(got, *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("D,shift,tok,head", [(64, 0, 0, 0), (64, 8, 16, 8), (128, 1, 3, 1), (128, 2, 8, 8), (256, 4, 8, 0), (64, 8, 1, 8)])
+def test_packed_strides_and_alignment(D, shift, tok, head, rows):
+    """Rows that begin at any element, heads and tokens apart, q k v and gate in one buffer; what lies between is left alone."""
+    rng, err = np.random.default_rng(5), C.create_string_buffer(512)
+    H, Hkv, cu, T = 4, 2, np.array([0, 40, 41, 90], np.int32), 93
+    hs = D + head
+    ts = 2 * H * hs + 2 * Hkv * hs + tok
+    buf = to_type(rng.standard_normal(shift + T * ts + 8 * D).astype(np.float32), rows)
+    o_tok = H * D + 3
+    out = np.full(T * o_tok, 9, buf.dtype)
+    db, do, dc = xp.Dev(buf), xp.Dev(out), xp.Dev(cu)
+    size = buf.itemsize
+    at = [shift + x * hs for x in (0, H, H + Hkv, H + 2 * Hkv)]   # q, k, v, gate
+    ptr = [db.ptr + x * size for x in at]
+    wb = xp.lib().xjh_attn_packed_work_bytes(IDS[rows], T, H, Hkv, D, 3)
+    work = xp.Dev(nbytes=max(16, wb))
+    assert xp.lib().xjh_attn_packed(IDS[rows], ptr[0], ts, hs, ptr[1], ts, hs, ptr[2], ts, hs, ptr[3], ts, hs, dc.ptr, 3, T, H, Hkv, D, 0, 0,
+                                    D ** -0.5, do.ptr, o_tok, work.ptr, wb, None, err, 512) == 0, err.value
+    xp.lib().xjh_sync()
+    got = do.get(buf.dtype, out.shape).reshape(T, o_tok)
+    assert np.all(got[:, H * D:] == 9) and np.all(got[90:] == 9)
+    def take(x, n):
+        return value(np.stack([[buf[x + t * ts + h * hs:x + t * ts + h * hs + D] for h in range(n)] for t in range(T)]))
+
+    q, k, v, g = take(at[0], H), take(at[1], Hkv), take(at[2], Hkv), take(at[3], H)
+    w = [attend64(q[a:b], k[a:b], v[a:b], 0, gate=g[a:b]) for a, b in zip(cu, cu[1:])]
+    check(np.ascontiguousarray(got[:90, :H * D]), *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+def test_packed_values_that_are_not_finite(rows):
+    """One prompt's do not reach another's rows, nor earlier ones of its own."""
+    rng = np.random.default_rng(2)
+    T, D, cu = 120, 64, [0, 70, 120]
+    q = to_type(rng.standard_normal((T, 2, D)).astype(np.float32), rows)
+    k, v = (kv_rows(rng, T, 1, D) for _ in range(2))
+    want = value(xp.attn_packed(q, to_type(k, rows), to_type(v, rows), cu))
+    v[50, 0, 9], k[110, 0, 3] = np.inf, np.nan
+    got = value(xp.attn_packed(q, to_type(k, rows), to_type(v, rows), cu))
+    assert not np.isfinite(got.reshape(T, 2, D)[50:70, :, 9]).any() and not np.isfinite(got[110:]).any()
+    assert np.array_equal(got[:50], want[:50]) and np.array_equal(got[70:110], want[70:110])
+
+
+def test_attention_refusals():
+    L, err, one = xp.lib(), C.create_string_buffer(512), C.c_void_p(16)
+
+    def paged(type=xp.F16, Hkv=2, D=64, page=16, n_pages=2, k=16, v=16, bytes=1 << 20, rows=xp.F32, q=one, out=one, table=one, blocks=4, cu=one,
+              kv=one, n_req=1, T=1, H=4, window=0, n_sink=0, scale=1.0, work=None):
+        c = xp.XjhPaged(type, Hkv, D, page, n_pages, k, v, bytes)
+        return L.xjh_attn_paged(C.byref(c), rows, q, 256, 64, None, 0, 0, table, blocks, cu, kv, n_req, T, 1, H, window, n_sink, scale, out, 256,
+                                work, 0, None, err, 512)
+
+    for bad in ({"type": xp.F32}, {"Hkv": 0}, {"D": 32}, {"page": 1}, {"page": 512}, {"n_pages": 0}):
+        assert paged(**bad) == -1 and b"unsupported cache" in err.value, bad
+    for bad in ({"k": None}, {"v": 20}, {"bytes": 100}):
+        assert paged(**bad) == -1 and b"memory" in err.value, bad
+    for bad in ({"rows": xp.BF16}, {"rows": xp.Q8_0}, {"blocks": 0}, {"blocks": (1 << 26) + 1}, {"n_req": -1}, {"n_req": 65537}, {"T": -1}, {"T": 1 << 27},
+                {"H": 3}, {"H": 0}, {"H": -2}, {"window": -1}, {"n_sink": -1}, {"scale": float("nan")}, {"scale": float("inf")}):
+        assert paged(**bad) == -1 and b"bad shape" in err.value, bad
+    for bad in ({"q": None}, {"out": None}, {"table": None}, {"cu": None}, {"kv": None}, {"work": C.c_void_p(8)}):
+        assert paged(**bad) == -1 and b"buffer is missing" in err.value, bad
+    assert paged(T=0, q=None) == 0 and paged(n_req=0, table=None) == 0
+
+    def packed(type=xp.F32, q=one, k=one, v=one, out=one, cu=one, n=1, T=1, H=4, Hkv=2, D=64, window=0, n_sink=0, scale=1.0, work=None):
+        return L.xjh_attn_packed(type, q, 256, 64, k, 128, 64, v, 128, 64, None, 0, 0, cu, n, T, H, Hkv, D, window, n_sink, scale, out, 256, work, 0, None,
+                                 err, 512)
+
+    for bad in ({"type": xp.Q8_0}, {"n": -1}, {"T": -1}, {"T": 1 << 27}, {"H": 3}, {"Hkv": 0}, {"Hkv": 1025, "H": 1025}, {"D": 80}, {"window": -1},
+                {"n_sink": -2}, {"scale": float("-inf")}):
+        assert packed(**bad) == -1 and b"bad shape" in err.value, bad
+    for bad in ({"q": None}, {"k": None}, {"v": None}, {"out": None}, {"cu": None}, {"work": C.c_void_p(4)}):
+        assert packed(**bad) == -1 and b"buffer is missing" in err.value, bad
+    assert packed(T=0, q=None) == 0 and packed(n=0, cu=None) == 0
+    c = xp.XjhPaged(xp.F16, 2, 64, 16, 2, None, None, 0)
+    assert L.xjh_attn_paged_work_bytes(C.byref(c), xp.BF16, 1, 4, 1, 1, 4) == 0 and L.xjh_attn_packed_work_bytes(xp.F32, 1, 3, 2, 64, 1) == 0
+    # enough for any smaller batch
+    n = [L.xjh_attn_paged_work_bytes(C.byref(c), xp.F16, T, 4, T, 1, 4096) for T in (1, 2, 8, 64)]
+    assert n[0] > 0 and n == sorted(n)
