@@ -622,7 +622,7 @@ int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, 
  * that a row does not see, NaN too, counts for nothing in it; a value that it sees and is not finite leaves it not finite.
  * Products of 16-bit elements are exact and sums are fp32. Weights enter with the cache's bits; with float rows the
  * queries and the weights enter with 22 bits over f16 (queries to 2^-40 of the row's largest element,
- * weights to 2^-40 of the row's largest) and 24 over bf16.
+ * weights to 2^-33 of the row's largest) and 24 over bf16.
  * max_new: the largest n, as far as the program knows (0: it does not); it decides which kernel runs, and a
  * larger n is right too. The result does not depend on it, or on the work area, beyond the rounding of sums.
  * T * H is at most 2^28, n_req 65536. */

@@ -27,7 +27,9 @@ template <>
 struct Op<_Float16> {
     typedef hf8 v8;
     static constexpr uint32_t kExp = 0x7C00, kOne = 0x3C00;
-    static constexpr float kLift = 15.f;   // weights enter as 2^15 p, at most 32768: f16 loses them from 2^-29 on only
+    // Weights are 2^kLift p to a reference that the running maximum may exceed by kTol before the sums are rescaled to it (on random
+    // scores nearly every tile raises some row's maximum a little), 2^15 at most: bits are lost from 2^-22 of the largest on only.
+    static constexpr float kLift = 8.f, kTol = 7.f;
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -35,7 +37,7 @@ template <>
 struct Op<__bf16> {
     typedef bf8 v8;
     static constexpr uint32_t kExp = 0x7F80, kOne = 0x3F80;
-    static constexpr float kLift = 0.f;
+    static constexpr float kLift = -8.f, kTol = 8.f;   // 1 at most: no sum of theirs is beyond the largest value
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -43,27 +45,27 @@ template <class E>
 using V8 = typename Op<E>::v8;
 
 // Eight numbers as NP planes that add up to them: one plane rounds to nearest; f16 in two keeps 22 bits (of numbers scaled so that
-// the planes are no subnormals); bf16 in three, each the leading 8 bits of what is left, is exact. (An infinity's further
+// the planes are no subnormals); bf16 takes the leading 8 bits of what is left in each, 16 in two, all in three. (An infinity's further
 // planes are NaN: a product with it is not finite.)
 template <class E, int NP>
 __device__ __forceinline__ void planes(const float (&x)[8], V8<E> (&p)[NP]) {
     if constexpr (NP == 1) {
 #pragma unroll
         for (int i = 0; i < 8; i++) p[0][i] = (E)x[i];
-    } else if constexpr (NP == 2) {
+    } else if constexpr (__is_same(E, _Float16)) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             p[0][i] = (E)x[i];
             p[1][i] = (E)(x[i] - (float)p[0][i]);
         }
     } else {
-        uint32_t w[3][4];
+        uint32_t w[NP][4];
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            uint32_t u[3], v[3];
+            uint32_t u[NP], v[NP];
             float a = x[i], b = x[i + 1];
 #pragma unroll
-            for (int k = 0; k < 3; k++) {
+            for (int k = 0; k < NP; k++) {
                 u[k] = __float_as_uint(a) & 0xFFFF0000u;
                 v[k] = __float_as_uint(b) & 0xFFFF0000u;
                 a -= __uint_as_float(u[k]);
@@ -72,7 +74,7 @@ __device__ __forceinline__ void planes(const float (&x)[8], V8<E> (&p)[NP]) {
             }
         }
 #pragma unroll
-        for (int k = 0; k < 3; k++) p[k] = __builtin_bit_cast(V8<E>, u32x4{w[k][0], w[k][1], w[k][2], w[k][3]});
+        for (int k = 0; k < NP; k++) p[k] = __builtin_bit_cast(V8<E>, u32x4{w[k][0], w[k][1], w[k][2], w[k][3]});
     }
 }
 
@@ -86,6 +88,11 @@ __device__ __forceinline__ float max_x32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// x / G of a row x < 2^28.
+__device__ __forceinline__ int token_of(const BatchAttnArgs &a, int x) {
+    const int q = (int)__umulhi((uint32_t)x, a.inv_g);   // or one less
+    return q + (x - q * a.G >= a.G);
+}
 // The rows of one request.
 struct Seq {
     int r, start, rows, pos0;   // its rows of q, the first one's position
@@ -117,16 +124,28 @@ __device__ __forceinline__ Seq seq_of(const BatchAttnArgs &a, int r) {
     s.rows = min(max(c1, s.start), a.T) - s.start;
     if (a.kv_len) s.pos0 = (int)max((int64_t)min(max(a.kv_len[r], 0), a.max_blocks << a.lg) - ((int64_t)c1 - c0), (int64_t)(-1 << 30));
     s.tiles = (s.rows * a.G + BM - 1) / BM;
-    if (s.tiles) s.len = range_of<BN>(a, s.pos0 + (s.tiles - 1) * BM / a.G, s.pos0 + s.rows - 1).n;
+    if (s.tiles) s.len = range_of<BN>(a, s.pos0 + token_of(a, (s.tiles - 1) * BM), s.pos0 + s.rows - 1).n;
     return s;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
 __device__ __forceinline__ int wave_scan(int v) {   // sums up to and with this lane
-    const int lane = threadIdx.x & 63;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(v, o, 64);
-        if (lane >= o) v += y;
-    }
-    return v;
+    v = dpp_add<0x111, 0xF>(v);   // the lane 1, 2, 4, 8 below in its row of 16
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);   // lane 15 to row 1, lane 47 to row 3
+    return dpp_add<0x143, 0xC>(v);   // lane 31 to rows 2 and 3
+}
+__device__ __forceinline__ float wave_sum(float v) {   // the same for every lane and in the same order
+    v = xjd::row16_sum(v);
+    auto at = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+    return (at(0) + at(16)) + (at(32) + at(48));
+}
+// Part `piece` of n tiles in `pieces` parts.
+__device__ __forceinline__ int part_from(int n, int piece, int pieces) {
+    const int q = n / pieces;
+    return q * piece + min(piece, n - q * pieces);
 }
 struct Item {
     Seq s;
@@ -147,13 +166,13 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
             s = seq_of<BM, BN>(a, r0 + lane);
             u += (float)s.tiles * (float)s.len;
         }
-        for (int o = 32; o; o >>= 1) u += __shfl_xor(u, o, 64);
+        u = wave_sum(u);
         per = max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1);
     }
     int items = 0, slots = 0;
     for (int r0 = 0; r0 < a.n_req; r0 += 64) {
         if (a.n_req > 64 || !a.target) s = seq_of<BM, BN>(a, r0 + lane);
-        const int pieces = max(1, (int)(((int64_t)s.len + per - 1) / per)), heads = s.tiles * a.Hkv;
+        const int pieces = s.len > per ? (int)((uint32_t)(s.len + per - 1) / (uint32_t)per) : 1, heads = s.tiles * a.Hkv;
         const int n_slot = pieces > 1 ? heads * pieces : 0, n = MERGE ? (pieces > 1 ? heads : 0) : heads * pieces;
         const int to = items + wave_scan(n), slot_to = slots + wave_scan(n_slot);
         const unsigned long long m = __ballot(to > item);
@@ -209,6 +228,30 @@ template <>
 struct Row<kRowBf16> {
     typedef __bf16 t;
 };
+
+// N elements of rows of any alignment.
+template <class R, int N>
+using Rows = R __attribute__((ext_vector_type(N), aligned(sizeof(R))));
+// 1 / (1 + e^-g), for rows of 16 bits to 2^-20.
+template <class R>
+__device__ __forceinline__ float gate_of(float g) {
+    if constexpr (sizeof(R) == 4) return xjd::sigm(g);
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f));
+}
+// Four finished elements of a row: y times 1 / l, through the gate.
+template <class R>
+__device__ __forceinline__ void finish4(f32x4 y, float inv, const R *gate, R *out) {
+    Rows<R, 4> z;
+    y *= inv;
+    if (gate) {
+        const Rows<R, 4> g = *(const Rows<R, 4> *)gate;
+#pragma unroll
+        for (int k = 0; k < 4; k++) y[k] *= gate_of<R>((float)g[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) z[k] = (R)y[k];
+    *(Rows<R, 4> *)out = z;
+}
 
 // Scores that underflow every weight still count as seen: the running maximum (in powers of two, rounded up) stays finite.
 constexpr float kLowest = -1e38f;

@@ -5,90 +5,117 @@ namespace xjk {
 
 // A tile of 16 rows, the key tiles of the piece dealt to four wavefronts, which join at the end. Lane l: li = l & 15, kq = l >> 4.
 // Keys come straight into the operand's registers (key li, dims 32 s + 8 kq ..); values are read as
-// the lane's VW dims of the eight keys whose weights it holds and turned in registers.
+// the lane's VW dims of the eight keys whose weights it holds and turned in registers. A tile's keys are requested as soon as the scores of
+// the one before are there, its values behind that one's sums. Weights enter in two planes at least: the
+// matrix cores wait for memory here.
 template <int D, class E, int NP, int RT>
 __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
-    constexpr int NS = D / 32, VW = D >= 128 ? 8 : 4, NB = D / (16 * VW), PAD = D + 4;
+    constexpr int NS = D / 32, VW = D >= 128 ? 8 : 4, NB = D / (16 * VW), PAD = D + 4, NW = NP > 2 ? NP : 2;
     __shared__ __align__(16) float so[4][16][PAD];
     __shared__ float sm[4][16], sl[4][16];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, kq = lane >> 4;
     Item it;
     if (!find_item<kFewRows, kFewKeys, false>(a, blockIdx.x, it)) return;
-    const int row = it.tile * 16 + li, n_rows = it.s.rows * a.G;
-    const int tok = min(row / a.G, it.s.rows - 1), p = it.s.pos0 + tok;
-    const int pf = it.s.pos0 + it.tile * 16 / a.G, pl = it.s.pos0 + min((it.tile * 16 + 15) / a.G, it.s.rows - 1);
+    const int row = it.tile * 16 + li, n_rows = it.s.rows * a.G, last = min(it.tile * 16 + 15, n_rows - 1);
+    const int rq = min(row, n_rows - 1), tok = token_of(a, rq), p = it.s.pos0 + tok;
+    const int pf = it.s.pos0 + token_of(a, it.tile * 16), pl = it.s.pos0 + token_of(a, last);
     const Range g = range_of<kFewKeys>(a, pf, pl);
-    const int i0 = (int)((int64_t)g.n * it.piece / it.pieces), i1 = (int)((int64_t)g.n * (it.piece + 1) / it.pieces);
+    const int i0 = part_from(g.n, it.piece, it.pieces) + w, i1 = part_from(g.n, it.piece + 1, it.pieces);
 
-    // queries, with the scale's sign; float ones scaled to 2^14 .. 2^15 before they become f16 planes
-    V8<E> q[NS][NP];
-    float c = fabsf(a.scale) * 1.44269504088896340736f;
+    // ---- a tile: its pages, keys and values
+    const int32_t *tab = a.table + (int64_t)it.s.r * a.max_blocks;
+    struct Pages {
+        int j0, page[2];
+    };
+    auto pages_of = [&](int i) {
+        Pages x;
+        x.j0 = g.tile(min(i, i1 - 1)) * kFewKeys;
+#pragma unroll
+        for (int u = 0; u < 2; u++) x.page[u] = page_at(a, tab, x.j0 + 16 * u);
+        return x;
+    };
+    auto at = [&](const Pages &x, int u) {   // of a page that is none, page 0's, which counts for nothing
+        const int j = x.j0 + 16 * u;
+        return (((((int64_t)max(x.page[u], 0) * a.Hkv + it.head) << a.lg) + (j & ((1 << a.lg) - 1)))) * D;
+    };
+    V8<E> kf[2][NS];
+    uint32_t vv[8][NB][VW / 2];
+    auto load_keys = [&](const Pages &x) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const E *kp = (const E *)a.k + at(x, u) + li * D + 8 * kq;
+#pragma unroll
+            for (int s = 0; s < NS; s++) kf[u][s] = *(const V8<E> *)(kp + 32 * s);
+        }
+    };
+    auto load_values = [&](const Pages &x) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const E *vp = (const E *)a.v + at(x, u) + 4 * kq * D + VW * li;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) __builtin_memcpy(vv[4 * u + r][b], __builtin_assume_aligned(vp + r * D + 16 * VW * b, 2 * VW), 2 * VW);
+        }
+    };
+    // ---- queries, with the scale's sign; float ones scaled to 2^14 .. 2^15 before they become f16 planes
+    Rows<R, 8> x[NS];
     {
-        const R *x = (const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + min(row, n_rows - 1) % a.G) * a.q_head + 8 * kq;
-        float f[NS][8], top = 0.f;
+        const R *qp = (const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head + 8 * kq;
+#pragma unroll
+        for (int s = 0; s < NS; s++) x[s] = *(const Rows<R, 8> *)(qp + 32 * s);
+    }
+    Pages now{}, next{};
+    if (i0 < i1) {
+        now = pages_of(i0);
+        load_keys(now);
+        load_values(now);
+        next = pages_of(i0 + 4);
+    }
+    V8<E> q[NS][NP];
+    float c = fabsf(a.scale) * 1.44269504088896340736f, up = a.scale < 0.f ? -1.f : 1.f;
+    if constexpr (NP == 2) {
+        float top = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; s++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                f[s][i] = (float)x[32 * s + i];
-                top = fmaxf(top, fabsf(f[s][i]));
-            }
-        float up = a.scale < 0.f ? -1.f : 1.f;
-        if constexpr (NP == 2) {
-            top = max_x32(max_x16(top));
-            int e = 15;
-            if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
-            e = max(e, -100);
-            up = ldexpf(up, 15 - e);
-            c = ldexpf(c, e - 15);
-        }
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf((float)x[s][i]));
+        top = max_x32(max_x16(top));
+        int e = 15;
+        if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
+        e = max(e, -100);
+        up = ldexpf(up, 15 - e);
+        c = ldexpf(c, e - 15);
+    }
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
+    for (int s = 0; s < NS; s++) {
+        float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[s][i] *= up;
-            planes<E, NP>(f[s], q[s]);
-        }
+        for (int i = 0; i < 8; i++) f[i] = (float)x[s][i] * up;
+        planes<E, NP>(f, q[s]);
     }
     f32x4 o[D / 16];
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;   // m: a whole number, so that every rescaling is exact
 
-    const int32_t *tab = a.table + (int64_t)it.s.r * a.max_blocks;
-    for (int i = i0 + w; i < i1; i += 4) {
-        const int j0 = g.tile(i) * kFewKeys;
-        bool ok[2];
-        const E *kp[2], *vp[2];
+    for (int i = i0; i < i1; i += 4) {
+        f32x4 s[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int j = j0 + 16 * u, page = page_at(a, tab, j);
-            ok[u] = page >= 0;
-            const int64_t at = (((((int64_t)max(page, 0) * a.Hkv + it.head) << a.lg) + (j & ((1 << a.lg) - 1)))) * D;
-            kp[u] = (const E *)a.k + at + li * D + 8 * kq;
-            vp[u] = (const E *)a.v + at + 4 * kq * D + VW * li;
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < NS; st++)
+#pragma unroll
+                for (int k = NP - 1; k >= 0; k--) s[u] = Op<E>::mfma16(kf[u][st], q[st][k], s[u]);
         }
-        V8<E> kf[2][NS];
-        uint32_t vv[8][NB][VW / 2];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int s = 0; s < NS; s++) kf[u][s] = *(const V8<E> *)(kp[u] + 32 * s);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int b = 0; b < NB; b++) __builtin_memcpy(vv[4 * u + r][b], __builtin_assume_aligned(vp[u] + r * D + 16 * VW * b, 2 * VW), 2 * VW);
-
-        f32x4 x[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int k = NP - 1; k >= 0; k--) x[u] = Op<E>::mfma16(kf[u][s], q[s][k], x[u]);
+        const int j0 = now.j0;
+        const bool ok[2] = {now.page[0] >= 0, now.page[1] >= 0};
+        now = next;
+        if (i + 4 < i1) {
+            load_keys(now);
+            next = pages_of(i + 8);
         }
         const bool full = ok[0] && ok[1] && j0 + 31 <= pf && (!a.window || j0 > pl - a.window || j0 + 31 < a.sinks);
         uint32_t vis = 0xFFu;
@@ -116,33 +143,34 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
                         inf |= ((y & 0xFFFFu) == Op<E>::kExp) | ((y >> 16) == Op<E>::kExp);
                     }
                 bad |= inf != 0;
-                if (vis >> n & 1) top = fmaxf(top, x[n >> 2][n & 3]);
+                if (vis >> n & 1) top = fmaxf(top, s[n >> 2][n & 3]);
             }
             bad = __any(bad);
             const unsigned long long any = __ballot(vis != 0);
             seen = ((any >> li | any >> (16 + li) | any >> (32 + li) | any >> (48 + li)) & 1) != 0;
         } else {
 #pragma unroll
-            for (int n = 0; n < 8; n++) top = fmaxf(top, x[n >> 2][n & 3]);
+            for (int n = 0; n < 8; n++) top = fmaxf(top, s[n >> 2][n & 3]);
         }
         top = max_x32(max_x16(top));
-        const float mn = fmaxf(m, seen ? fmaxf(ceilf(top * c), kLowest) : -INFINITY);
-        if (__any(mn > m)) {
-            const float up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= up;
+        const float high = seen ? fmaxf(ceilf(top * c), kLowest) : -INFINITY;
+        const bool higher = high > m + Op<E>::kTol;
+        if (__any(higher)) {
+            const float mn = higher ? high : m, f = higher ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+            l *= f;
 #pragma unroll
-            for (int d = 0; d < D / 16; d++) o[d] *= up;
+            for (int d = 0; d < D / 16; d++) o[d] *= f;
             m = mn;
         }
         float pr[8];
 #pragma unroll
         for (int n = 0; n < 8; n++) {
-            pr[n] = __builtin_amdgcn_exp2f(fmaf(x[n >> 2][n & 3], c, Op<E>::kLift - m));
+            pr[n] = __builtin_amdgcn_exp2f(fmaf(s[n >> 2][n & 3], c, Op<E>::kLift - m));
             if (!full && !(vis >> n & 1)) pr[n] = 0.f;
             l += pr[n];
         }
-        V8<E> pp[NP];
-        planes<E, NP>(pr, pp);
+        V8<E> pp[NW];
+        planes<E, NW>(pr, pp);
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -165,13 +193,14 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
                     for (int k = 0; k < 4; k++) acc[k] += n[k] > 0.f ? NAN : 0.f;
                 }
 #pragma unroll
-                for (int k = NP - 1; k >= 0; k--) acc = Op<E>::mfma16(__builtin_bit_cast(V8<E>, t), pp[k], acc);
+                for (int k = NW - 1; k >= 0; k--) acc = Op<E>::mfma16(__builtin_bit_cast(V8<E>, t), pp[k], acc);
             }
+        if (i + 4 < i1) load_values(now);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    // the four wavefronts' sums
+    // ---- the four wavefronts' sums
     if (kq == 0) sm[w][li] = m, sl[w][li] = l;
     if (row < n_rows)
 #pragma unroll
@@ -198,27 +227,19 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
         L += mw[k] * sl[k][rt];
     }
     const bool whole = it.pieces == 1;
-    const int t = R0 / a.G, h = it.head * a.G + R0 - t * a.G;
-    const int64_t at = (int64_t)it.slot * 16 + rt;
-    if (!whole && (tid & 15) == 0) *part_stat(a, at, 16, D) = float2{M, L};
+    const float inv = M == -INFINITY ? 0.f : 1.f / L;   // a row that has seen nothing is 0
+    const int t = token_of(a, R0), h = it.head * a.G + R0 - t * a.G, d0 = 4 * (tid & 15);
+    const int64_t to = (int64_t)it.slot * 16 + rt;
+    if (!whole && d0 == 0) *part_stat(a, to, 16, D) = float2{M, L};
+    R *out = (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d0;
+    const R *gate = a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d0 : nullptr;
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += 64) {
-        const int d = d0 + 4 * (tid & 15);
+    for (int d = 0; d < D; d += 64) {
         f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; k++) y += mw[k] * *(const f32x4 *)&so[k][rt][d];
-        if (!whole) {
-            *(f32x4 *)(part_sums(a, at, D) + d) = y;
-            continue;
-        }
-        R *out = (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d;
-        const R *gate = a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            float z = M == -INFINITY ? 0.f : y[k] / L;
-            if (gate) z *= xjd::sigm((float)gate[k]);
-            out[k] = (R)z;
-        }
+        for (int k = 0; k < 4; k++) y += mw[k] * *(const f32x4 *)&so[k][rt][d0 + d];
+        if (whole) finish4(y, inv, gate ? gate + d : nullptr, out + d);
+        else *(f32x4 *)(part_sums(a, to, D) + d0 + d) = y;
     }
 }
 
@@ -239,47 +260,44 @@ int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
 
 // ----------------------------------------------------------------- merge --
 
-// Rows in more than one piece: a wavefront joins a row's pieces.
+// Rows in more than one piece: a work-group joins a row's pieces, D / 4 threads taking one piece at a time, the others the next ones.
 template <int D, int BM, int BN, int RT>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
-    constexpr int N = D / 64;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int TD = D / 4, TP = 256 / TD;
+    __shared__ __align__(16) float so[TP][D];
+    __shared__ float sl[TP];
+    const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % TD), tp = tid / TD;
     Item it;
     if (!find_item<BM, BN, true>(a, blockIdx.x, it)) return;
-    const int n_rows = min(it.s.rows * a.G - it.tile * BM, BM);
-    for (int i = blockIdx.y * 4 + w; i < n_rows; i += gridDim.y * 4) {
-        const int64_t at = (int64_t)it.slot * BM + i, step = (int64_t)a.Hkv * BM;
-        float M = -INFINITY, L = 0.f, y[N];
-#pragma unroll
-        for (int k = 0; k < N; k++) y[k] = 0.f;
-        for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
-        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-        if (M != -INFINITY)
-            for (int p0 = 0; p0 < it.pieces; p0 += 64) {
-                const int n = min(64, it.pieces - p0);
-                const float2 s = lane < n ? *part_stat(a, at + (p0 + lane) * step, BM, D) : float2{-INFINITY, 0.f};
-                const float mine = __builtin_amdgcn_exp2f(s.x - M);
-                L += mine * s.y;
-#pragma unroll 8
-                for (int p = 0; p < n; p++) {
-                    const float f = __shfl(mine, p, 64);
-                    const float *x = part_sums(a, at + (p0 + p) * step, D);
-#pragma unroll
-                    for (int k = 0; k < N; k++) y[k] += f * x[lane + 64 * k];
-                }
-            }
-        for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
-        const int row = it.tile * BM + i, t = row / a.G, h = it.head * a.G + row - t * a.G;
-        R *out = (R *)a.out + (it.s.start + t) * a.o_tok + h * D;
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-            const int d = lane + 64 * k;
-            float z = M == -INFINITY ? 0.f : y[k] / L;
-            if (a.gate) z *= xjd::sigm((float)((const R *)a.gate)[(it.s.start + t) * a.g_tok + h * a.g_head + d]);
-            out[d] = (R)z;
+    const int i = blockIdx.y;
+    if (i >= it.s.rows * a.G - it.tile * BM) return;
+    const int64_t at = (int64_t)it.slot * BM + i, step = (int64_t)a.Hkv * BM;
+    float M = -INFINITY, L = 0.f;
+    for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
+    M = xjd::wave_max(M);
+    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (M != -INFINITY)
+#pragma unroll 4
+        for (int p = tp; p < it.pieces; p += TP) {
+            const float2 s = *part_stat(a, at + p * step, BM, D);
+            const f32x4 x = *(const f32x4 *)(part_sums(a, at + p * step, D) + d);
+            const float f = __builtin_amdgcn_exp2f(s.x - M);
+            L += f * s.y;
+            y += f * x;
         }
+    *(f32x4 *)&so[tp][d] = y;
+    if (d == 0) sl[tp] = L;
+    __syncthreads();
+    if (tp) return;
+#pragma unroll
+    for (int k = 1; k < TP; k++) {
+        y += *(const f32x4 *)&so[k][d];
+        L += sl[k];
     }
+    const int row = it.tile * BM + i, t = token_of(a, row), h = it.head * a.G + row - t * a.G;
+    finish4(y, M == -INFINITY ? 0.f : 1.f / L, a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr,
+            (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d);
 }
 template <int D, int BM, int BN>
 static void merge(const BatchAttnArgs &a, dim3 grid, hipStream_t st) {
@@ -293,7 +311,7 @@ static void merge(const BatchAttnArgs &a, dim3 grid, hipStream_t st) {
     else merge<D, BM, many_keys(D)>(a, grid, st);
 }
 int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st) {
-    const dim3 grid((unsigned)groups, BM / 16);
+    const dim3 grid((unsigned)groups, BM);
     if (BM == kFewRows) {
         if (a.D == 64) merge<kFewRows, 64>(a, grid, st);
         else if (a.D == 128) merge<kFewRows, 128>(a, grid, st);

@@ -1,6 +1,7 @@
 // Attention over pages or packed rows for requests of many rows (gfx950): prompts and pieces of them. See batch_attn.h.
 #include "batch_attn.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace xjk {
 
@@ -9,6 +10,10 @@ __device__ const u32x4 kZeros[1] = {};
 // Lane l: 16 bytes at p to LDS offset off + 16 l; off is uniform over the wavefront.
 __device__ __forceinline__ void dma16(const void *p, uint32_t off) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(off) : "memory", "m0");
+}
+// The same with a uniform base and a lane's offset from it.
+__device__ __forceinline__ void dma16(const void *base, uint32_t lane_off, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(off) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -21,106 +26,66 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Where the keys come from: pages, rows that 16 bytes at a time can be copied from, any other rows.
-enum { kPages = 0, kRows16 = 1, kRowsAny = 2 };
+// Where the keys come from: pages, or rows that can be copied 16 bytes at a time.
+enum { kPages = 0, kRows16 = 1 };
 
-// A row's 16-byte chunks lie permuted in LDS, so that what an instruction reads falls on all banks: 16 rows' chunk c of the keys,
-// 4 rows' chunks 4 c .. 4 c + 3 of the values.
-template <int D>
-__device__ __forceinline__ int key_swz(int row) { return D >= 128 ? row & 15 : (row >> 1) & 7; }
-template <int D>
-__device__ __forceinline__ int val_swz(int row) { return D >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2; }
-
-// A tile of 128 rows, 32 a wavefront; tiles of BN keys and values pass through LDS, the next one on its way meanwhile.
-// Lane l: row l & 31, half h = l >> 5.
-template <int D, class E, int NP, int NK, int RT, int SRC>
-__global__ __launch_bounds__(256, D <= 128 && NP == 1 ? 2 : 1) void attn_many_kernel(const BatchAttnArgs a) {
-    typedef typename Row<RT>::t R;
-    constexpr int BN = many_keys(D), NB = BN / 32, NS = D / 16, ND = D / 32, CH = D / 8;
-    constexpr int PLANE = BN * D * 2, TENSOR = NK * PLANE, BUF = 2 * TENSOR;
-    constexpr int COPIES = BN * CH / 256;   // of 16 bytes a lane and tensor
-    extern __shared__ __align__(1024) char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    Item it;
-    if (!find_item<kManyRows, BN, false>(a, blockIdx.x, it)) return;
-    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    const int R0 = it.tile * kManyRows, n_rows = it.s.rows * a.G;
-    const int row = R0 + 32 * w + (lane & 31), tok = min(row / a.G, it.s.rows - 1), p = it.s.pos0 + tok;
-    const int pf = it.s.pos0 + R0 / a.G, pl = it.s.pos0 + min((R0 + kManyRows - 1) / a.G, it.s.rows - 1);
-    const int wf = it.s.pos0 + min((R0 + 32 * w) / a.G, it.s.rows - 1), wl = it.s.pos0 + min((R0 + 32 * w + 31) / a.G, it.s.rows - 1);
-    const bool rows_here = R0 + 32 * w < n_rows;
-    const Range g = range_of<BN>(a, pf, pl);
-    const int i0 = (int)((int64_t)g.n * it.piece / it.pieces), i1 = (int)((int64_t)g.n * (it.piece + 1) / it.pieces);
-    const int32_t *tab = SRC == kPages ? a.table + (int64_t)it.s.r * a.max_blocks : nullptr;
-
-    // ---- a tile's keys and values into LDS: chunk (row, x ^ swizzle) of plane 0 .. NK - 1
-    auto any_sees = [&](int j) { return j <= pl && (!a.window || j > pf - a.window || j < a.sinks); };
-    auto copy = [&](int i, int buf) {
-        const int j0 = g.tile(i) * BN;
-#pragma unroll
-        for (int n = 0; n < COPIES; n++) {
-            const int c0 = (n * 4 + w) * 64, r0 = c0 / CH;   // the wavefront's chunks, all in rows of one page
-            const int c = c0 + lane, r = c / CH, x = c % CH, j = j0 + r;
-            const int page = SRC == kPages ? page_at(a, tab, j0 + r0) : 0;
-            const bool use = page >= 0 && any_sees(j);
-            const void *kp, *vp;
-            if (SRC == kPages) {
-                const int64_t at = (((((int64_t)page * a.Hkv + it.head) << a.lg) + (j & ((1 << a.lg) - 1)))) * D;
-                kp = (const E *)a.k + at + 8 * (x ^ key_swz<D>(r));
-                vp = (const E *)a.v + at + 8 * (x ^ val_swz<D>(r));
-            } else {
-                kp = (const E *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * (x ^ key_swz<D>(r));
-                vp = (const E *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * (x ^ val_swz<D>(r));
-            }
-            // what no row sees counts for nothing, whatever lies there
-            dma16(use ? kp : kZeros, base + buf * BUF + 16 * c0);
-            dma16(use ? vp : kZeros, base + buf * BUF + TENSOR + 16 * c0);
-        }
-    };
-    auto through_registers = [&](int i) {
-        const int j0 = g.tile(i) * BN;
-#pragma unroll 2
-        for (int n = 0; n < COPIES; n++) {
-            const int c = n * 256 + tid, r = c / CH, x = c % CH, j = j0 + r;
-            const bool use = any_sees(j);
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int64_t at = t ? (it.s.start + j) * a.v_tok + it.head * a.v_head : (it.s.start + j) * a.k_tok + it.head * a.k_head;
-                char *to = lds + t * TENSOR + 16 * (r * CH + (x ^ (t ? val_swz<D>(r) : key_swz<D>(r))));
-                if constexpr (RT == kRowF32) {
-                    float f[8] = {};
-                    if (use) {
-                        const f32x8_u y = *(const f32x8_u *)((const float *)(t ? a.v : a.k) + at + 8 * x);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) f[e] = y[e];
-                    }
-                    V8<E> q[NK];
-                    planes<E, NK>(f, q);
-#pragma unroll
-                    for (int k = 0; k < NK; k++) *(V8<E> *)(to + k * PLANE) = q[k];
-                } else {
-                    u32x4 y = u32x4{0, 0, 0, 0};
-                    if (use) y = *(const u32x4_u *)((const uint16_t *)(t ? a.v : a.k) + at + 8 * x);
-                    *(u32x4 *)to = y;
-                }
-            }
-        }
-    };
-    if (SRC != kRowsAny && i0 < i1) copy(i0, 0);
-
-    // ---- queries, with the scale's sign; float ones over f16 scaled to 2^14 .. 2^15 before they become planes
+template <class T>
+__device__ __forceinline__ T lds_read(uint32_t at, uint32_t off) {
+    return *(const __attribute__((address_space(3))) T *)(uintptr_t)(at + off);
+}
+// Of 16 lanes, each at 4 dims of a key (l / 4 % 4 of 4 keys): the four keys of dim l % 16.
+__device__ __forceinline__ u32x2 lds_read_turned(uint32_t at, uint32_t off) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(at + off)));
+}
+// What a wavefront holds of its M rows, 32 or 16, on the instruction of M by M by 512 / M. Lane l: row l % M, part h = l / M of the keys.
+// With 32 rows every operand read from LDS feeds one instruction of 32 clocks, which is as fast as LDS can be; it needs D / 2 registers for the sums and
+// D / 4 for the queries, and with 256 dims the compiler does not keep both in the 256 that two wavefronts a SIMD leave it. With 16 rows it is half of
+// each, LDS the bound for 16-bit rows, but not for float ones, whose planes use an operand two or three times.
+template <int D, class E, int NP, int NK, class R, int M>
+struct WaveRows {
+    static constexpr int BN = many_keys(D), NS = D * M / 512, ND = D / M, CH = D / 8, KI = 512 / M;   // KI: keys a step of the second product
+    static constexpr int PER = M * M / 64, NB = BN / M, NE = NB * PER;                                  // scores a block, blocks, scores a lane
+    static constexpr int PLANE = BN * D * 2, TENSOR = NK * PLANE;
+    typedef float F __attribute__((ext_vector_type(PER)));
     V8<E> q[NS][NP];
-    float c = fabsf(a.scale) * 1.44269504088896340736f;
-    {
-        const R *x = (const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + min(row, n_rows - 1) % a.G) * a.q_head + 8 * h;
-        float up = a.scale < 0.f ? -1.f : 1.f;
+    F o[ND];
+    float m, l, c;   // the reference in powers of two (a whole number, so that every rescaling is exact), the weights' sum, the scale
+    int lane, h;
+
+    static __device__ __forceinline__ F mfma(V8<E> a, V8<E> b, F x) {
+        if constexpr (M == 32) return Op<E>::mfma32(a, b, x);
+        else return Op<E>::mfma16(a, b, x);
+    }
+    static __device__ __forceinline__ int key_of(int e, int h) {   // of a lane's element e
+        const int r = e % PER;
+        return M * (e / PER) + 8 * (r >> 2) + 4 * h + (r & 3);
+    }
+    static __device__ __forceinline__ float most(float x) { return M == 32 ? max_x32(x) : max_x32(max_x16(x)); }
+    // A row's 16-byte chunks lie permuted in LDS, so that what an instruction reads falls on all banks: 16 rows' chunk c of the keys;
+    // of the values 4 rows' chunks 4 c .. 4 c + 3 (M = 32), 8 rows' chunks 2 c, 2 c + 1 (M = 16).
+    static __device__ __forceinline__ int key_swz(int row) { return D >= 128 ? row & 15 : (row >> 1) & 7; }
+    static __device__ __forceinline__ int val_swz(int row) {
+        if (D < 128) row >>= 1;
+        return M == 32 ? (row & (D >= 128 ? 3 : 1)) << 2 : (row & (D >= 128 ? 7 : 3)) << 1;
+    }
+
+    // Queries, with the scale's sign; float ones over f16 scaled to 2^14 .. 2^15 before they become planes.
+    __device__ __forceinline__ void start(const R *qp, float scale) {
+        lane = threadIdx.x & 63;
+        h = lane / M;
+        c = fabsf(scale) * 1.44269504088896340736f;
+        float up = scale < 0.f ? -1.f : 1.f;
+        Rows<R, 8> x[NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) x[s] = *(const Rows<R, 8> *)(qp + KI * s + 8 * h);
         if constexpr (NP == 2) {
             float top = 0.f;
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf((float)x[16 * s + i]));
-            top = max_x32(top);
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf((float)x[s][i]));
+            top = most(top);
             int e = 15;
             if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
             e = max(e, -100);
@@ -131,203 +96,426 @@ __global__ __launch_bounds__(256, D <= 128 && NP == 1 ? 2 : 1) void attn_many_ke
         for (int s = 0; s < NS; s++) {
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = (float)x[16 * s + i] * up;
+            for (int i = 0; i < 8; i++) f[i] = (float)x[s][i] * up;
             planes<E, NP>(f, q[s]);
         }
-    }
-    f32x16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
-    float m = -INFINITY, l = 0.f;   // m: a whole number, so that every rescaling is exact
-
-    for (int i = i0; i < i1; i++) {
-        const int buf = SRC == kRowsAny ? 0 : (i - i0) & 1, j0 = g.tile(i) * BN;
-        if constexpr (SRC == kRowsAny) {
-            lds_barrier();
-            through_registers(i);
-            __syncthreads();
-        } else {
-            if (i + 1 < i1) {
-                copy(i + 1, buf ^ 1);
-                wait_vm<2 * COPIES>();
-            } else {
-                wait_vm<0>();
-            }
-            lds_barrier();
-        }
-        const char *kb = lds + buf * BUF, *vb = kb + TENSOR;
-        if (rows_here && j0 <= wl) {
-            f32x16 s[NB];
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[b][r] = 0.f;
-                const int kr = 32 * b + (lane & 31);
-#pragma unroll
-                for (int st = 0; st < NS; st++) {
-                    const char *at = kb + 16 * (kr * CH + ((2 * st + h) ^ key_swz<D>(kr)));
-#pragma unroll
-                    for (int k = NK - 1; k >= 0; k--) {
-                        const V8<E> kf = *(const V8<E> *)(at + k * PLANE);
-#pragma unroll
-                        for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--) s[b] = Op<E>::mfma32(kf, q[st][n], s[b]);
-                    }
-                }
-            }
-            bool full = j0 + BN - 1 <= wf && (!a.window || j0 > wl - a.window || j0 + BN - 1 < a.sinks);
-            uint32_t page_ok = 0xFFFFFFFFu;   // a bit for 16 keys
-            if (SRC == kPages) {
-#pragma unroll
-                for (int u = 0; u < BN / 16; u++)
-                    if (page_at(a, tab, j0 + 16 * u) < 0) page_ok &= ~(1u << u);
-                full = full && page_ok == 0xFFFFFFFFu;
-            }
-            uint32_t vis[NB];
-            bool seen = true, bad = false;
-            float top = -INFINITY;
-            if (!full) {
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    vis[b] = 0;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int kj = 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                        if (sees(a, p, j0 + kj) && (page_ok >> (kj >> 4) & 1)) {
-                            vis[b] |= 1u << r;
-                            top = fmaxf(top, s[b][r]);
-                        }
-                    }
-                }
-                uint32_t any = 0;
-#pragma unroll
-                for (int b = 0; b < NB; b++) any |= vis[b];
-                const unsigned long long all = __ballot(any != 0);
-                seen = ((all >> (lane & 31) | all >> (32 + (lane & 31))) & 1) != 0;
-                // values that are not finite make the rows that see them so, and no other (0 times infinity)
-                for (int n = lane; n < TENSOR / 16; n += 64) {
-                    const u32x4 y = *(const u32x4 *)(vb + 16 * n);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) bad |= (y[k] & Op<E>::kExp) == Op<E>::kExp || (y[k] >> 16 & Op<E>::kExp) == Op<E>::kExp;
-                }
-                bad = __any(bad);
-            } else {
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) top = fmaxf(top, s[b][r]);
-            }
-            top = max_x32(top);
-            const float mn = fmaxf(m, seen ? fmaxf(ceilf(top * c), kLowest) : -INFINITY);
-            if (__any(mn > m)) {
-                const float up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                l *= up;
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= up;
-                m = mn;
-            }
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    float pr[8];
-#pragma unroll
-                    for (int n = 0; n < 8; n++) {
-                        pr[n] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * t + n], c, Op<E>::kLift - m));
-                        if (!full && !(vis[b] >> (8 * t + n) & 1)) pr[n] = 0.f;
-                        l += pr[n];
-                    }
-                    V8<E> pp[NP];
-                    planes<E, NP>(pr, pp);
-                    // keys 32 b + 16 t + 4 h + (0 .. 3, 8 .. 11): this lane fetches 4 of one of them for the others
-                    const int key = 32 * b + 16 * t + 4 * h + ((lane & 15) >> 2);
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const int chunk = 4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
-                        const char *at = vb + 16 * (key * CH + (chunk ^ val_swz<D>(key))) + 8 * (lane & 1);
-                        const char *at8 = vb + 16 * ((key + 8) * CH + (chunk ^ val_swz<D>(key + 8))) + 8 * (lane & 1);
-#pragma unroll
-                        for (int k = NK - 1; k >= 0; k--) {
-                            typedef short s16x4 __attribute__((ext_vector_type(4)));
-                            typedef __attribute__((address_space(3))) s16x4 *lp;
-                            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + k * PLANE)));
-                            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at8 + k * PLANE)));
-                            u32x4 v = u32x4{x[0], x[1], y[0], y[1]};
-                            if (bad) {
-                                u32x4 mark, sight;
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const bool lo = (v[e] & Op<E>::kExp) == Op<E>::kExp, hi = (v[e] >> 16 & Op<E>::kExp) == Op<E>::kExp;
-                                    mark[e] = (lo ? Op<E>::kOne : 0u) | (hi ? Op<E>::kOne << 16 : 0u);
-                                    v[e] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
-                                    const uint32_t bits = full ? 3u : vis[b] >> (8 * t + 2 * e);
-                                    sight[e] = (bits & 1 ? Op<E>::kOne : 0u) | (bits & 2 ? Op<E>::kOne << 16 : 0u);
-                                }
-                                f32x16 z;
-#pragma unroll
-                                for (int r = 0; r < 16; r++) z[r] = 0.f;
-                                z = Op<E>::mfma32(__builtin_bit_cast(V8<E>, mark), __builtin_bit_cast(V8<E>, sight), z);
-#pragma unroll
-                                for (int r = 0; r < 16; r++) o[d][r] += z[r] > 0.f ? NAN : 0.f;
-                            }
-#pragma unroll
-                            for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--)
-                                o[d] = Op<E>::mfma32(__builtin_bit_cast(V8<E>, v), pp[n], o[d]);
-                        }
-                    }
-                }
-        }
-        if (SRC != kRowsAny) lds_barrier();
-    }
-    l += __shfl_xor(l, 32, 64);
-    if (row >= n_rows) return;
-    if (it.pieces > 1) {
-        const int64_t at = (int64_t)it.slot * kManyRows + row - R0;
-        if (h == 0) *part_stat(a, at, kManyRows, D) = float2{m, l};
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                *(f32x4 *)(part_sums(a, at, D) + 32 * d + 8 * r + 4 * h) = f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
-        return;
+            for (int r = 0; r < PER; r++) o[d][r] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
     }
-    const int head = it.head * a.G + row % a.G;
-    R *out = (R *)a.out + (it.s.start + tok) * a.o_tok + head * D + 4 * h;
-    const R *gate = a.gate ? (const R *)a.gate + (it.s.start + tok) * a.g_tok + head * a.g_head + 4 * h : nullptr;
+    // Scores of a tile whose keys begin at LDS address kb.
+    __device__ __forceinline__ void scores(uint32_t kb, F (&s)[NB]) const {
+        const int kr = lane % M;
+        const uint32_t at = (kb + kr * 2 * D) | (16 * (h ^ key_swz(kr)));   // chunk KI / 8 * st + h: exclusive or with 2 KI st
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+        for (int b = 0; b < NB; b++) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            float z = m == -INFINITY ? 0.f : o[d][r] / l;
-            const int at = 32 * d + 8 * (r >> 2) + (r & 3);
-            if (gate) z *= xjd::sigm((float)gate[at]);
-            out[at] = (R)z;
+            for (int r = 0; r < PER; r++) s[b][r] = 0.f;
+#pragma unroll
+            for (int st = 0; st < NS; st++)
+#pragma unroll
+                for (int k = NK - 1; k >= 0; k--) {
+                    const V8<E> kf = lds_read<V8<E>>(at ^ (2 * KI * st), k * PLANE + 2 * M * b * D);
+#pragma unroll
+                    for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--) s[b] = mfma(kf, q[st][n], s[b]);
+                }
         }
+    }
+    // The running maximum with this tile's scores. (One that underflows every weight counts as seen.)
+    template <bool MASKED>
+    __device__ __forceinline__ void raise(const F (&s)[NB], uint32_t vis, bool seen) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < NE; e++)
+            if (!MASKED || (vis >> e & 1)) top = fmaxf(top, s[e / PER][e % PER]);
+        top = most(top);
+        const float now = !MASKED || seen ? fmaxf(ceilf(top * c), kLowest) : -INFINITY;
+        const bool higher = now > m + Op<E>::kTol;
+        if (__builtin_expect(__any(higher), 0)) {
+            const float mn = higher ? now : m, up = higher ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+            l *= up;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= up;
+            m = mn;
+        }
+    }
+    // Weights and sums.
+    template <bool MASKED>
+    __device__ __forceinline__ void weigh(uint32_t vb, const F (&s)[NB], uint32_t vis) {
+        const float lift = Op<E>::kLift - m;
+        // the lane fetches 4 dims of one key of a step's first (second) half for the others
+        const int key = 4 * h + (lane >> 2 & 3), low = (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (lane & 3);
+        const uint32_t at = (vb + key * 2 * D) | (low ^ 16 * val_swz(key));
+        constexpr int DX = 128 / M;   // dims within which chunks are permuted, over M
+#pragma unroll
+        for (int u = 0; u < NE / 8; u++) {
+            float pr[8];
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const int e = 8 * u + n;
+                pr[n] = __builtin_amdgcn_exp2f(fmaf(s[e / PER][e % PER], c, lift));
+                if (MASKED && !(vis >> e & 1)) pr[n] = 0.f;
+                l += pr[n];
+            }
+            V8<E> pp[NP];
+            planes<E, NP>(pr, pp);
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int k = NK - 1; k >= 0; k--) {
+                    const uint32_t from = at ^ (2 * M * (d % DX)), off = k * PLANE + 256 * (d / DX) + KI * u * 2 * D;
+                    const u32x2 x = lds_read_turned(from, off), y = lds_read_turned(from, off + 256 / M * 2 * D);
+                    const V8<E> v = __builtin_bit_cast(V8<E>, u32x4{x[0], x[1], y[0], y[1]});
+#pragma unroll
+                    for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--) o[d] = mfma(v, pp[n], o[d]);
+                }
+        }
+    }
+    // Which keys of a tile this lane's row sees, a bit an element; page_ok: a bit for 16 keys. Whether the row sees any.
+    __device__ __forceinline__ bool look(const BatchAttnArgs &a, int p, int j0, uint32_t page_ok, uint32_t &vis) const {
+        vis = 0;
+#pragma unroll
+        for (int e = 0; e < NE; e++) {
+            const int kj = key_of(e, h);
+            if (sees(a, p, j0 + kj) && (page_ok >> (kj >> 4) & 1)) vis |= 1u << e;
+        }
+        unsigned long long all = __ballot(vis != 0);
+        all |= all >> 32;
+        if (M == 16) all |= all >> 16;
+        return (all >> (lane % M) & 1) != 0;
+    }
+    // Values that are not finite make the rows that see them so, and no other, where 0 times infinity would not do: the work-group
+    // takes them out of a tile that some row does not see whole and leaves marks [BN][CH], a bit for each of a chunk's 8 dims, from which the
+    // rows take them.
+    __device__ __forceinline__ static bool find_spoilt(const char *vb) {
+        uint32_t bad = 0;
+        for (int n = threadIdx.x; n < TENSOR / 16; n += blockDim.x) {
+            const u32x4 y = *(const u32x4 *)(vb + 16 * n);
+#pragma unroll
+            for (int k = 0; k < 4; k++) bad |= ((y[k] & Op<E>::kExp) == Op<E>::kExp) | ((y[k] >> 16 & Op<E>::kExp) == Op<E>::kExp);
+        }
+        return bad != 0;
+    }
+    __device__ static __attribute__((noinline)) void mark_spoilt(char *vb, uint8_t *marks) {
+        for (int n = threadIdx.x; n < BN * CH; n += blockDim.x) {
+            const int key = n / CH, x = n % CH;
+            uint32_t mark = 0;
+            for (int k = 0; k < NK; k++) {
+                u32x4 *at = (u32x4 *)(vb + k * PLANE + 16 * (key * CH + (x ^ val_swz(key))));
+                u32x4 y = *at;
+                for (int e = 0; e < 4; e++) {
+                    const bool lo = (y[e] & Op<E>::kExp) == Op<E>::kExp, hi = (y[e] >> 16 & Op<E>::kExp) == Op<E>::kExp;
+                    mark |= (uint32_t)lo << (2 * e) | (uint32_t)hi << (2 * e + 1);
+                    y[e] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+                }
+                *at = y;
+            }
+            marks[n] = (uint8_t)mark;
+        }
+    }
+    __device__ __forceinline__ void take_spoilt(const BatchAttnArgs &a, int p, int j0, uint32_t page_ok, const uint8_t *marks) {
+#pragma unroll 1
+        for (int key = 0; key < BN; key++) {
+            const bool see = sees(a, p, j0 + key) && (page_ok >> (key >> 4) & 1);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                uint32_t w;
+                if constexpr (M == 32) w = *(const uint32_t *)(marks + key * CH + 4 * d);
+                else w = *(const uint16_t *)(marks + key * CH + 2 * d);
+                w = see ? w >> (4 * h) : 0u;
+                if (__any(w != 0))
+#pragma unroll
+                    for (int r = 0; r < PER; r++)
+                        if (w >> (8 * (r >> 2) + (r & 3)) & 1) o[d][r] = NAN;
+            }
+        }
+    }
+    // The rows' results, or their part of them.
+    __device__ __forceinline__ void finish(const BatchAttnArgs &a, const Item &it, int row, int tok) {
+        if (M == 16) l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (row >= it.s.rows * a.G) return;
+        if (it.pieces > 1) {
+            const int64_t at = (int64_t)it.slot * kManyRows + row - it.tile * kManyRows;
+            if (h == 0) *part_stat(a, at, kManyRows, D) = float2{m, l};
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int r = 0; r < PER / 4; r++)
+                    *(f32x4 *)(part_sums(a, at, D) + M * d + 8 * r + 4 * h) = f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+            return;
+        }
+        const int head = it.head * a.G + row - tok * a.G;
+        R *out = (R *)a.out + (it.s.start + tok) * a.o_tok + head * D + 4 * h;
+        const R *gate = a.gate ? (const R *)a.gate + (it.s.start + tok) * a.g_tok + head * a.g_head + 4 * h : nullptr;
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;   // a row that has seen nothing is 0
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < PER / 4; r++)
+                finish4(f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]}, inv, gate ? gate + M * d + 8 * r : nullptr,
+                        out + M * d + 8 * r);
+    }
+};
+// LDS beside the tiles: marks of values that are not finite, and whether there are any.
+constexpr int many_marks(int D) { return many_keys(D) * D / 8; }
+
+// A tile of 128 rows, M a wavefront; tiles of BN keys and values pass through LDS. While a tile's weights are made and its values
+// summed, the next one's scores are, and the keys behind it and its values are on their way: a barrier a tile.
+template <int D, class E, int NP, int RT, int SRC, int M>
+__global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnArgs a) {
+    typedef typename Row<RT>::t R;
+    typedef WaveRows<D, E, NP, 1, R, M> X;
+    constexpr int BN = X::BN, NB = X::NB, CH = X::CH, TENSOR = X::TENSOR;
+    constexpr int W = kManyRows / M, COPIES = BN * CH / (64 * W);   // wavefronts; copies of 16 bytes a lane and tensor
+    extern __shared__ __align__(1024) char lds[];   // keys, keys, values, values, marks, flag
+    char *const vals = lds + 2 * TENSOR;
+    uint8_t *const marks = (uint8_t *)lds + 4 * TENSOR;
+    int *const flag = (int *)(marks + many_marks(D));
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Item it;
+    if (!find_item<kManyRows, BN, false>(a, blockIdx.x, it)) return;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const int R0 = it.tile * kManyRows, n_rows = it.s.rows * a.G;
+    const int row = R0 + M * w + lane % M, rq = min(row, n_rows - 1), tok = token_of(a, rq), p = it.s.pos0 + tok;
+    const int pf = it.s.pos0 + token_of(a, R0), pl = it.s.pos0 + token_of(a, min(R0 + kManyRows, n_rows) - 1);
+    const int wf = it.s.pos0 + token_of(a, min(R0 + M * w, n_rows - 1)), wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
+    const Range g = range_of<BN>(a, pf, pl);
+    const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
+    const int32_t *tab = SRC == kPages ? a.table + (int64_t)it.s.r * a.max_blocks : nullptr;
+
+    // ---- a tile's keys or values into LDS: chunk (row, x ^ swizzle). A wavefront's copy is of 64 chunks, in rows r0 .. of one page;
+    // its lanes' offsets are of two kinds at most (the keys' with D = 256: odd copies)
+    const int64_t k_row = SRC == kPages ? D : a.k_tok, v_row = SRC == kPages ? D : a.v_tok;
+    uint32_t k_off[2], v_off;
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        const int c = (n * W + w) * 64 + lane, r = c / CH, x = c % CH;
+        k_off[n] = (uint32_t)(lane / CH) * (uint32_t)k_row * 2 + 16 * (x ^ X::key_swz(r));
+        if (n == 0) v_off = (uint32_t)(lane / CH) * (uint32_t)v_row * 2 + 16 * (x ^ X::val_swz(r));
+    }
+    auto whole_tile = [&](int f, int l, int j0) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
+    auto copy = [&](auto values, int t) {
+        constexpr bool V = decltype(values)::value;
+        const int j0 = g.tile(i0 + t) * BN;
+        const bool every = whole_tile(pl, pf, j0);   // some row sees each of its keys
+#pragma unroll
+        for (int n = 0; n < COPIES; n++) {
+            const int c0 = (n * W + w) * 64, r0 = c0 / CH;
+            const int page = SRC == kPages ? page_at(a, tab, j0 + r0) : 0;
+            const uint32_t off = V ? v_off : k_off[n & 1], to = base + (V ? 2 + (t & 1) : t & 1) * TENSOR + 16 * c0;
+            const E *from = (const E *)(V ? a.v : a.k);
+            if (SRC == kPages) from += (((((int64_t)max(page, 0) * a.Hkv + it.head) << a.lg) + ((j0 + r0) & ((1 << a.lg) - 1)))) * D;
+            else from += (it.s.start + j0 + r0) * (V ? v_row : k_row) + it.head * (V ? a.v_head : a.k_head);
+            if (every && page >= 0) {
+                dma16(from, off, to);
+            } else {   // what no row sees counts for nothing, whatever lies there
+                const int j = j0 + r0 + lane / CH;
+                const bool use = page >= 0 && j <= pl && (!a.window || j > pf - a.window || j < a.sinks);
+                dma16(use ? (const char *)from + off : (const char *)kZeros, to);
+            }
+        }
+    };
+    const std::false_type keys;
+    const std::true_type values;
+    if (n_tiles > 0) {
+        copy(keys, 0);
+        copy(values, 0);
+    }
+    if (n_tiles > 1) copy(keys, 1);
+    if (tid == 0) *flag = 0;
+    X x;
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale);
+    wait_vm<0>();
+    lds_barrier();
+    typename X::F s[NB];
+    auto has_keys = [&](int t) { return R0 + M * w < n_rows && t < n_tiles && g.tile(i0 + t) * BN <= wl; };
+    if (has_keys(0)) x.scores(base, s);
+
+    for (int t = 0; t < n_tiles; t++) {
+        const int j0 = g.tile(i0 + t) * BN;
+        if (t) wait_vm<0>();
+        lds_barrier();
+        if (t + 2 < n_tiles) copy(keys, t + 2);
+        if (t + 1 < n_tiles) copy(values, t + 1);
+        uint32_t page_ok = 0xFFFFFFFFu;   // a bit for 16 keys
+        if (SRC == kPages)
+#pragma unroll
+            for (int u = 0; u < BN / 16; u++)
+                if (page_at(a, tab, j0 + 16 * u) < 0) page_ok &= ~(1u << u);
+        const bool pages = page_ok == 0xFFFFFFFFu, all_whole = pages && whole_tile(pf, pl, j0);
+        char *const vt = vals + (t & 1) * TENSOR;
+        const uint32_t kb = base + ((t + 1) & 1) * TENSOR, vb = base + (2 + (t & 1)) * TENSOR;
+        if (pages && whole_tile(wf, wl, j0) && all_whole && has_keys(t + 1)) {
+            x.template raise<false>(s, 0, true);
+            typename X::F s2[NB];
+            x.scores(kb, s2);
+            x.template weigh<false>(vb, s, 0);
+#pragma unroll
+            for (int b = 0; b < NB; b++) s[b] = s2[b];
+            continue;
+        }
+        bool spoilt = false;
+        if (!all_whole) {
+            if (X::find_spoilt(vt)) *flag = 1;
+            lds_barrier();
+            spoilt = *flag != 0;
+            if (spoilt) {
+                lds_barrier();
+                if (tid == 0) *flag = 0;
+                X::mark_spoilt(vt, marks);
+                lds_barrier();
+            }
+        }
+        if (has_keys(t)) {
+            uint32_t vis;
+            const bool seen = x.look(a, p, j0, page_ok, vis);
+            x.template raise<true>(s, vis, seen);
+            x.template weigh<true>(vb, s, vis);
+            if (spoilt) x.take_spoilt(a, p, j0, page_ok, marks);
+        }
+        if (has_keys(t + 1)) x.scores(kb, s);
+    }
+    x.finish(a, it, row, tok);
 }
 
-template <int D, class E, int NP, int NK, int RT, int SRC>
-static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
-    constexpr int bytes = 2 * NK * many_keys(D) * D * 2 * (SRC == kRowsAny ? 1 : 2);
-    auto *f = attn_many_kernel<D, E, NP, NK, RT, SRC>;
-    if (bytes > 65536 && hipFuncSetAttribute((const void *)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return -1;
-    f<<<dim3((unsigned)items), 256, bytes, st>>>(a);
+// The same with keys and values that pass through registers: rows of any alignment, and floats in NK planes. A tile at a time; the next one
+// is requested before this one's products.
+template <int D, class E, int NP, int NK, int RT, int M>
+__global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchAttnArgs a) {
+    typedef typename Row<RT>::t R;
+    typedef WaveRows<D, E, NP, NK, R, M> X;
+    constexpr int BN = X::BN, NB = X::NB, CH = X::CH, TENSOR = X::TENSOR, PLANE = X::PLANE;
+    constexpr int W = kManyRows / M, COPIES = BN * CH / (64 * W);   // wavefronts; pieces of 8 elements a lane and tensor
+    extern __shared__ __align__(1024) char lds[];   // keys, values, marks, flag
+    char *const vb = lds + TENSOR;
+    uint8_t *const marks = (uint8_t *)lds + 2 * TENSOR;
+    int *const flag = (int *)(marks + many_marks(D));
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Item it;
+    if (!find_item<kManyRows, BN, false>(a, blockIdx.x, it)) return;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const int R0 = it.tile * kManyRows, n_rows = it.s.rows * a.G;
+    const int row = R0 + M * w + lane % M, rq = min(row, n_rows - 1), tok = token_of(a, rq), p = it.s.pos0 + tok;
+    const int pf = it.s.pos0 + token_of(a, R0), pl = it.s.pos0 + token_of(a, min(R0 + kManyRows, n_rows) - 1);
+    const int wf = it.s.pos0 + token_of(a, min(R0 + M * w, n_rows - 1)), wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
+    const Range g = range_of<BN>(a, pf, pl);
+    const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
+    Rows<R, 8> kx[COPIES], vx[COPIES];
+    auto request = [&](int t) {
+        const int j0 = g.tile(i0 + t) * BN;
+#pragma unroll
+        for (int n = 0; n < COPIES; n++) {
+            const int c = n * 64 * W + tid, r = c / CH, e = c % CH, j = j0 + r;
+            kx[n] = vx[n] = R(0);
+            if (j <= pl && (!a.window || j > pf - a.window || j < a.sinks)) {   // what no row sees counts for nothing, whatever lies there
+                kx[n] = *(const Rows<R, 8> *)((const R *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * e);
+                vx[n] = *(const Rows<R, 8> *)((const R *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * e);
+            }
+        }
+    };
+    auto put = [&]() {
+#pragma unroll
+        for (int n = 0; n < COPIES; n++) {
+            const int c = n * 64 * W + tid, r = c / CH, e = c % CH;
+            V8<E> kp[NK], vp[NK];
+            if constexpr (NK == 1) {
+                kp[0] = __builtin_bit_cast(V8<E>, kx[n]);
+                vp[0] = __builtin_bit_cast(V8<E>, vx[n]);
+            } else {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) f[i] = (float)kx[n][i];
+                planes<E, NK>(f, kp);
+#pragma unroll
+                for (int i = 0; i < 8; i++) f[i] = (float)vx[n][i];
+                planes<E, NK>(f, vp);
+            }
+#pragma unroll
+            for (int k = 0; k < NK; k++) {
+                *(V8<E> *)(lds + k * PLANE + 16 * (r * CH + (e ^ X::key_swz(r)))) = kp[k];
+                *(V8<E> *)(vb + k * PLANE + 16 * (r * CH + (e ^ X::val_swz(r)))) = vp[k];
+            }
+        }
+    };
+    if (n_tiles > 0) request(0);
+    if (tid == 0) *flag = 0;
+    X x;
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale);
+    for (int t = 0; t < n_tiles; t++) {
+        const int j0 = g.tile(i0 + t) * BN;
+        if (t) lds_barrier();
+        put();
+        lds_barrier();
+        if (t + 1 < n_tiles) request(t + 1);
+        auto whole_tile = [&](int f, int l) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
+        bool spoilt = false;
+        if (!whole_tile(pf, pl)) {
+            if (X::find_spoilt(vb)) *flag = 1;
+            lds_barrier();
+            spoilt = *flag != 0;
+            if (spoilt) {
+                lds_barrier();
+                if (tid == 0) *flag = 0;
+                X::mark_spoilt(vb, marks);
+                lds_barrier();
+            }
+        }
+        if (R0 + M * w < n_rows && j0 <= wl) {
+            typename X::F s[NB];
+            x.scores(base, s);
+            if (whole_tile(wf, wl)) {
+                x.template raise<false>(s, 0, true);
+                x.template weigh<false>(base + TENSOR, s, 0);
+            } else {
+                uint32_t vis;
+                const bool seen = x.look(a, p, j0, 0xFFFFFFFFu, vis);
+                x.template raise<true>(s, vis, seen);
+                x.template weigh<true>(base + TENSOR, s, vis);
+            }
+            if (spoilt) x.take_spoilt(a, p, j0, 0xFFFFFFFFu, marks);
+        }
+    }
+    x.finish(a, it, row, tok);
+}
+
+template <class F>
+static int many_run(F *f, int threads, int bytes, const BatchAttnArgs &a, int64_t items, hipStream_t st) {
+    if (hipFuncSetAttribute((const void *)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return -1;
+    f<<<dim3((unsigned)items), threads, bytes, st>>>(a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+// Rows a wavefront: 32 where their registers allow it (WaveRows).
+constexpr int many_wave(int D, int NP) { return D <= 128 && NP == 1 ? 32 : 16; }
+template <int D, class E, int NP, int RT, int SRC>
+static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
+    constexpr int M = many_wave(D, NP);
+    return many_run(attn_many_kernel<D, E, NP, RT, SRC, M>, 8192 / M, 4 * many_keys(D) * D * 2 + many_marks(D) + 16, a, items, st);
+}
+template <int D, class E, int NP, int NK, int RT>
+static int many_any(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
+    constexpr int M = many_wave(D, NP);
+    return many_run(attn_many_any_kernel<D, E, NP, NK, RT, M>, 8192 / M, 2 * NK * many_keys(D) * D * 2 + many_marks(D) + 16, a, items, st);
 }
 template <int D>
 static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
     if (a.table) {
-        if (a.type == kRowF16) return many<D, _Float16, 1, 1, kRowF16, kPages>(a, items, st);
-        if (a.type == kRowBf16) return many<D, __bf16, 1, 1, kRowBf16, kPages>(a, items, st);
-        if (a.kv_type == kRowF16) return many<D, _Float16, 2, 1, kRowF32, kPages>(a, items, st);
-        return many<D, __bf16, 3, 1, kRowF32, kPages>(a, items, st);
+        if (a.type == kRowF16) return many<D, _Float16, 1, kRowF16, kPages>(a, items, st);
+        if (a.type == kRowBf16) return many<D, __bf16, 1, kRowBf16, kPages>(a, items, st);
+        if (a.kv_type == kRowF16) return many<D, _Float16, 2, kRowF32, kPages>(a, items, st);
+        return many<D, __bf16, 3, kRowF32, kPages>(a, items, st);
     }
-    if (a.type == kRowF32) return many<D, __bf16, 3, 3, kRowF32, kRowsAny>(a, items, st);
-    const bool whole = !(((uintptr_t)a.k | (uintptr_t)a.v) & 15) && !((a.k_tok | a.k_head | a.v_tok | a.v_head) & 7);
+    if (a.type == kRowF32) return many_any<D, __bf16, 3, 3, kRowF32>(a, items, st);
+    // (a lane's offset within a copy, 8 rows at most, has 32 bits)
+    const bool whole = !(((uintptr_t)a.k | (uintptr_t)a.v) & 15) && !((a.k_tok | a.k_head | a.v_tok | a.v_head) & 7) &&
+                       a.k_tok >= 0 && a.v_tok >= 0 && std::max(a.k_tok, a.v_tok) < (1 << 27);
     if (a.type == kRowF16) {
-        return whole ? many<D, _Float16, 1, 1, kRowF16, kRows16>(a, items, st) : many<D, _Float16, 1, 1, kRowF16, kRowsAny>(a, items, st);
+        return whole ? many<D, _Float16, 1, kRowF16, kRows16>(a, items, st) : many_any<D, _Float16, 1, 1, kRowF16>(a, items, st);
     }
-    return whole ? many<D, __bf16, 1, 1, kRowBf16, kRows16>(a, items, st) : many<D, __bf16, 1, 1, kRowBf16, kRowsAny>(a, items, st);
+    return whole ? many<D, __bf16, 1, kRowBf16, kRows16>(a, items, st) : many_any<D, __bf16, 1, 1, kRowBf16>(a, items, st);
 }
 int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
     return a.D == 64 ? many<64>(a, items, st) : a.D == 128 ? many<128>(a, items, st) : many<256>(a, items, st);

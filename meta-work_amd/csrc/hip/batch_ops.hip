@@ -124,6 +124,7 @@ static bool packed_batch_ok(int type, int T, int H, int Hkv, int D, int n_seq) {
 static void batch_args(BatchAttnArgs &a, int type, int n_req, int T, int H, int Hkv, int D, int window, int n_sink) {
     a.type = row_type(type);
     a.n_req = n_req; a.T = T; a.H = H; a.Hkv = Hkv; a.D = D; a.G = H / Hkv;
+    a.inv_g = UINT32_MAX / (uint32_t)a.G;
     a.window = window < (1 << 30) ? window : 0;   // positions are below 2^30
     a.sinks = n_sink;
 }

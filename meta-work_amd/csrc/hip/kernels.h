@@ -450,6 +450,7 @@ struct BatchAttnArgs {
     const int32_t *cu;
     int32_t lg, n_pages, max_blocks;
     int32_t n_req, T, max_new, H, Hkv, D, G;
+    uint32_t inv_g;                               // (2^32 - 1) / G
     int32_t type, kv_type;                        // RowType of q, gate, out, and of k, v
     int32_t window, sinks;
     float scale;
