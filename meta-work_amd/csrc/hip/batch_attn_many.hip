@@ -38,17 +38,25 @@ __device__ __forceinline__ u32x2 lds_read_turned(uint32_t at, uint32_t off) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(at + off)));
 }
+// The lane's number, anew: what is made of it is not kept in registers from one use to the next.
+__device__ __forceinline__ int fresh_lane() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+}
 // What a wavefront holds of its M rows, 32 or 16, on the instruction of M by M by 512 / M. Lane l: row l % M, part h = l / M of the keys.
 // With 32 rows every operand read from LDS feeds one instruction of 32 clocks, which is as fast as LDS can be; it needs D / 2 registers for the sums and
-// D / 4 for the queries, and with 256 dims the compiler does not keep both in the 256 that two wavefronts a SIMD leave it. With 16 rows it is half of
-// each, LDS the bound for 16-bit rows, but not for float ones, whose planes use an operand two or three times.
+// D / 4 for the queries, with 256 dims just within the 256 that two wavefronts a SIMD leave it (a register that lies in memory instead is waited for
+// behind the tiles on their way). With 16 rows it is half of each: for float rows, whose planes use an operand two or three times.
 template <int D, class E, int NP, int NK, class R, int M>
 struct WaveRows {
     static constexpr int BN = many_keys(D), NS = D * M / 512, ND = D / M, CH = D / 8, KI = 512 / M;   // KI: keys a step of the second product
     static constexpr int PER = M * M / 64, NB = BN / M, NE = NB * PER;                                  // scores a block, blocks, scores a lane
     static constexpr int PLANE = BN * D * 2, TENSOR = NK * PLANE;
+    static constexpr int QL = D == 256 && M == 32 ? 3 : 0;   // steps whose queries lie in LDS: what two work-groups a CU leave of it
     typedef float F __attribute__((ext_vector_type(PER)));
-    V8<E> q[NS][NP];
+    V8<E> q[NS - QL][NP];
+    uint32_t q_lds;   // where the wavefront's first QL steps lie
     F o[ND];
     float m, l, c;   // the reference in powers of two (a whole number, so that every rescaling is exact), the weights' sum, the scale
     int lane, h;
@@ -71,9 +79,10 @@ struct WaveRows {
     }
 
     // Queries, with the scale's sign; float ones over f16 scaled to 2^14 .. 2^15 before they become planes.
-    __device__ __forceinline__ void start(const R *qp, float scale) {
+    __device__ __forceinline__ void start(const R *qp, float scale, uint32_t q_area) {
         lane = threadIdx.x & 63;
         h = lane / M;
+        q_lds = q_area + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 * QL;
         c = fabsf(scale) * 1.44269504088896340736f;
         float up = scale < 0.f ? -1.f : 1.f;
         Rows<R, 8> x[NS];
@@ -97,7 +106,13 @@ struct WaveRows {
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] = (float)x[s][i] * up;
-            planes<E, NP>(f, q[s]);
+            if (s < QL) {
+                V8<E> y[NP];
+                planes<E, NP>(f, y);
+                *(__attribute__((address_space(3))) V8<E> *)(uintptr_t)(q_lds + 1024 * s + 16 * lane) = y[0];
+            } else {
+                planes<E, NP>(f, q[s - QL]);
+            }
         }
 #pragma unroll
         for (int d = 0; d < ND; d++)
@@ -108,7 +123,7 @@ struct WaveRows {
     }
     // Scores of a tile whose keys begin at LDS address kb.
     __device__ __forceinline__ void scores(uint32_t kb, F (&s)[NB]) const {
-        const int kr = lane % M;
+        const int lane = QL ? fresh_lane() : this->lane, kr = lane % M, h = lane / M;
         const uint32_t at = (kb + kr * 2 * D) | (16 * (h ^ key_swz(kr)));   // chunk KI / 8 * st + h: exclusive or with 2 KI st
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -120,7 +135,8 @@ struct WaveRows {
                 for (int k = NK - 1; k >= 0; k--) {
                     const V8<E> kf = lds_read<V8<E>>(at ^ (2 * KI * st), k * PLANE + 2 * M * b * D);
 #pragma unroll
-                    for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--) s[b] = mfma(kf, q[st][n], s[b]);
+                    for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--)
+                        s[b] = mfma(kf, st < QL ? lds_read<V8<E>>(q_lds + 16 * lane, 1024 * st) : q[st - QL < 0 ? 0 : st - QL][n], s[b]);
                 }
         }
     }
@@ -147,7 +163,7 @@ struct WaveRows {
     __device__ __forceinline__ void weigh(uint32_t vb, const F (&s)[NB], uint32_t vis) {
         const float lift = Op<E>::kLift - m;
         // the lane fetches 4 dims of one key of a step's first (second) half for the others
-        const int key = 4 * h + (lane >> 2 & 3), low = (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (lane & 3);
+        const int lane = QL ? fresh_lane() : this->lane, h = lane / M, key = 4 * h + (lane >> 2 & 3), low = (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (lane & 3);
         const uint32_t at = (vb + key * 2 * D) | (low ^ 16 * val_swz(key));
         constexpr int DX = 128 / M;   // dims within which chunks are permuted, over M
 #pragma unroll
@@ -272,7 +288,6 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     constexpr int BN = X::BN, NB = X::NB, CH = X::CH, TENSOR = X::TENSOR;
     constexpr int W = kManyRows / M, COPIES = BN * CH / (64 * W);   // wavefronts; copies of 16 bytes a lane and tensor
     extern __shared__ __align__(1024) char lds[];   // keys, keys, values, values, marks, flag
-    char *const vals = lds + 2 * TENSOR;
     uint8_t *const marks = (uint8_t *)lds + 4 * TENSOR;
     int *const flag = (int *)(marks + many_marks(D));
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -280,42 +295,47 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     if (!find_item<kManyRows, BN, false>(a, blockIdx.x, it)) return;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     const int R0 = it.tile * kManyRows, n_rows = it.s.rows * a.G;
-    const int row = R0 + M * w + lane % M, rq = min(row, n_rows - 1), tok = token_of(a, rq), p = it.s.pos0 + tok;
+    const int row = R0 + M * w + (X::QL ? fresh_lane() : lane) % M, rq = min(row, n_rows - 1), tok = token_of(a, rq);
     const int pf = it.s.pos0 + token_of(a, R0), pl = it.s.pos0 + token_of(a, min(R0 + kManyRows, n_rows) - 1);
-    const int wf = it.s.pos0 + token_of(a, min(R0 + M * w, n_rows - 1)), wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
+    const int wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
     const Range g = range_of<BN>(a, pf, pl);
     const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
     const int32_t *tab = SRC == kPages ? a.table + (int64_t)it.s.r * a.max_blocks : nullptr;
 
     // ---- a tile's keys or values into LDS: chunk (row, x ^ swizzle). A wavefront's copy is of 64 chunks, in rows r0 .. of one page;
     // its lanes' offsets are of two kinds at most (the keys' with D = 256: odd copies)
-    const int64_t k_row = SRC == kPages ? D : a.k_tok, v_row = SRC == kPages ? D : a.v_tok;
-    uint32_t k_off[2], v_off;
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-        const int c = (n * W + w) * 64 + lane, r = c / CH, x = c % CH;
-        k_off[n] = (uint32_t)(lane / CH) * (uint32_t)k_row * 2 + 16 * (x ^ X::key_swz(r));
-        if (n == 0) v_off = (uint32_t)(lane / CH) * (uint32_t)v_row * 2 + 16 * (x ^ X::val_swz(r));
-    }
-    auto whole_tile = [&](int f, int l, int j0) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
-    auto copy = [&](auto values, int t) {
+    const uint32_t k_row = 2 * (SRC == kPages ? D : (uint32_t)a.k_tok), v_row = 2 * (SRC == kPages ? D : (uint32_t)a.v_tok);   // bytes
+    const int64_t first = SRC == kPages ? ((int64_t)it.head << a.lg) * D : 0;
+    const char *const k_base = (const char *)((const E *)a.k + (SRC == kPages ? first : it.s.start * a.k_tok + it.head * a.k_head));
+    const char *const v_base = (const char *)((const E *)a.v + (SRC == kPages ? first : it.s.start * a.v_tok + it.head * a.v_head));
+    const int64_t page_bytes = ((int64_t)a.Hkv << a.lg) * (2 * D);
+    const int page_mask = (1 << a.lg) - 1;
+    auto whole_tile = [&](int f, int l, int j0) __attribute__((always_inline)) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
+    auto copy = [&](auto values, int t) __attribute__((always_inline)) {
         constexpr bool V = decltype(values)::value;
         const int j0 = g.tile(i0 + t) * BN;
         const bool every = whole_tile(pl, pf, j0);   // some row sees each of its keys
+        const int ln = X::QL ? fresh_lane() : lane;
+        uint32_t offs[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const int c = (n * W + w) * 64 + ln, r = c / CH, x = c % CH;
+            offs[n] = (uint32_t)(ln / CH) * (V ? v_row : k_row) + 16 * (x ^ (V ? X::val_swz(r) : X::key_swz(r)));
+        }
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c0 = (n * W + w) * 64, r0 = c0 / CH;
             const int page = SRC == kPages ? page_at(a, tab, j0 + r0) : 0;
-            const uint32_t off = V ? v_off : k_off[n & 1], to = base + (V ? 2 + (t & 1) : t & 1) * TENSOR + 16 * c0;
-            const E *from = (const E *)(V ? a.v : a.k);
-            if (SRC == kPages) from += (((((int64_t)max(page, 0) * a.Hkv + it.head) << a.lg) + ((j0 + r0) & ((1 << a.lg) - 1)))) * D;
-            else from += (it.s.start + j0 + r0) * (V ? v_row : k_row) + it.head * (V ? a.v_head : a.k_head);
+            const uint32_t off = offs[V ? 0 : n & 1], to = base + (V ? 2 + (t & 1) : t & 1) * TENSOR + 16 * c0;
+            const char *from;
+            if (SRC == kPages) from = (V ? v_base : k_base) + (int64_t)max(page, 0) * page_bytes + ((j0 + r0) & page_mask) * (2 * D);
+            else from = (V ? v_base : k_base) + (int64_t)(j0 + r0) * (V ? v_row : k_row);
             if (every && page >= 0) {
                 dma16(from, off, to);
             } else {   // what no row sees counts for nothing, whatever lies there
-                const int j = j0 + r0 + lane / CH;
+                const int j = j0 + r0 + ln / CH;
                 const bool use = page >= 0 && j <= pl && (!a.window || j > pf - a.window || j < a.sinks);
-                dma16(use ? (const char *)from + off : (const char *)kZeros, to);
+                dma16(use ? from + off : (const char *)kZeros, to);
             }
         }
     };
@@ -327,39 +347,44 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     }
     if (n_tiles > 1) copy(keys, 1);
     if (tid == 0) *flag = 0;
+    const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
-    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale);
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
     wait_vm<0>();
     lds_barrier();
     typename X::F s[NB];
-    auto has_keys = [&](int t) { return R0 + M * w < n_rows && t < n_tiles && g.tile(i0 + t) * BN <= wl; };
+    auto has_keys = [&](int t) __attribute__((always_inline)) { return R0 + M * w < n_rows && t < n_tiles && g.tile(i0 + t) * BN <= wl; };
     if (has_keys(0)) x.scores(base, s);
 
-    for (int t = 0; t < n_tiles; t++) {
-        const int j0 = g.tile(i0 + t) * BN;
-        if (t) wait_vm<0>();
+    auto vals_at = [&](int t) __attribute__((always_inline)) { return base + (2 + (t & 1)) * TENSOR; };
+    auto keys_at = [&](int t) __attribute__((always_inline)) { return base + (t & 1) * TENSOR; };
+    // Tile t's values and the next one's keys are there; what lies behind them is requested.
+    auto turn = [&](int t) __attribute__((always_inline)) {
+        wait_vm<0>();
         lds_barrier();
         if (t + 2 < n_tiles) copy(keys, t + 2);
         if (t + 1 < n_tiles) copy(values, t + 1);
-        uint32_t page_ok = 0xFFFFFFFFu;   // a bit for 16 keys
+    };
+    auto pages_at = [&](int j0) __attribute__((always_inline)) {   // a bit for 16 keys
+        uint32_t ok = 0xFFFFFFFFu;
         if (SRC == kPages)
 #pragma unroll
             for (int u = 0; u < BN / 16; u++)
-                if (page_at(a, tab, j0 + 16 * u) < 0) page_ok &= ~(1u << u);
-        const bool pages = page_ok == 0xFFFFFFFFu, all_whole = pages && whole_tile(pf, pl, j0);
-        char *const vt = vals + (t & 1) * TENSOR;
-        const uint32_t kb = base + ((t + 1) & 1) * TENSOR, vb = base + (2 + (t & 1)) * TENSOR;
-        if (pages && whole_tile(wf, wl, j0) && all_whole && has_keys(t + 1)) {
-            x.template raise<false>(s, 0, true);
-            typename X::F s2[NB];
-            x.scores(kb, s2);
-            x.template weigh<false>(vb, s, 0);
-#pragma unroll
-            for (int b = 0; b < NB; b++) s[b] = s2[b];
-            continue;
-        }
+                if (page_at(a, tab, j0 + 16 * u) < 0) ok &= ~(1u << u);
+        return ok;
+    };
+    // Every row of the work-group sees all of tile t, and this wavefront some of the next.
+    auto plain = [&](int t) __attribute__((always_inline)) {
+        const int j0 = g.tile(i0 + t) * BN;
+        return has_keys(t + 1) && whole_tile(pf, pl, j0) && pages_at(j0) == 0xFFFFFFFFu;
+    };
+    auto any_tile = [&](int t) __attribute__((always_inline)) {
+        const int j0 = g.tile(i0 + t) * BN;
+        turn(t);
+        const uint32_t page_ok = pages_at(j0);
         bool spoilt = false;
-        if (!all_whole) {
+        if (page_ok != 0xFFFFFFFFu || !whole_tile(pf, pl, j0)) {
+            char *const vt = lds + (2 + (t & 1)) * TENSOR;
             if (X::find_spoilt(vt)) *flag = 1;
             lds_barrier();
             spoilt = *flag != 0;
@@ -371,15 +396,27 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
             }
         }
         if (has_keys(t)) {
+            const int p = it.s.pos0 + token_of(a, min(R0 + M * w + (X::QL ? fresh_lane() : lane) % M, n_rows - 1));
             uint32_t vis;
             const bool seen = x.look(a, p, j0, page_ok, vis);
             x.template raise<true>(s, vis, seen);
-            x.template weigh<true>(vb, s, vis);
+            x.template weigh<true>(vals_at(t), s, vis);
             if (spoilt) x.take_spoilt(a, p, j0, page_ok, marks);
         }
-        if (has_keys(t + 1)) x.scores(kb, s);
+        if (has_keys(t + 1)) x.scores(keys_at(t + 1), s);
+    };
+    // (Three loops, not one with two paths: the sums would be moved between the paths' registers at every tile.)
+    int t = 0;
+    for (; t < n_tiles && !plain(t); t++) any_tile(t);
+    for (; t < n_tiles && plain(t); t++) {
+        turn(t);
+        x.template raise<false>(s, 0, true);
+        x.template weigh<false>(vals_at(t), s, 0);
+        x.scores(keys_at(t + 1), s);
     }
-    x.finish(a, it, row, tok);
+    for (; t < n_tiles; t++) any_tile(t);
+    const int last_row = R0 + M * w + (X::QL ? fresh_lane() : lane) % M;
+    x.finish(a, it, last_row, token_of(a, min(last_row, n_rows - 1)));
 }
 
 // The same with keys and values that pass through registers: rows of any alignment, and floats in NK planes. A tile at a time; the next one
@@ -405,7 +442,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     const Range g = range_of<BN>(a, pf, pl);
     const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
     Rows<R, 8> kx[COPIES], vx[COPIES];
-    auto request = [&](int t) {
+    auto request = [&](int t) __attribute__((always_inline)) {
         const int j0 = g.tile(i0 + t) * BN;
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
@@ -417,7 +454,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
             }
         }
     };
-    auto put = [&]() {
+    auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c = n * 64 * W + tid, r = c / CH, e = c % CH;
@@ -443,17 +480,22 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     };
     if (n_tiles > 0) request(0);
     if (tid == 0) *flag = 0;
+    const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
-    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale);
-    for (int t = 0; t < n_tiles; t++) {
-        const int j0 = g.tile(i0 + t) * BN;
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
+    auto turn = [&](int t) __attribute__((always_inline)) {
         if (t) lds_barrier();
         put();
         lds_barrier();
         if (t + 1 < n_tiles) request(t + 1);
-        auto whole_tile = [&](int f, int l) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
+    };
+    auto whole_tile = [&](int f, int l, int j0) __attribute__((always_inline)) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
+    auto plain = [&](int t) __attribute__((always_inline)) { return R0 + M * w < n_rows && whole_tile(pf, pl, g.tile(i0 + t) * BN); };
+    auto any_tile = [&](int t) __attribute__((always_inline)) {
+        const int j0 = g.tile(i0 + t) * BN;
+        turn(t);
         bool spoilt = false;
-        if (!whole_tile(pf, pl)) {
+        if (!whole_tile(pf, pl, j0)) {
             if (X::find_spoilt(vb)) *flag = 1;
             lds_barrier();
             spoilt = *flag != 0;
@@ -464,21 +506,25 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
                 lds_barrier();
             }
         }
-        if (R0 + M * w < n_rows && j0 <= wl) {
-            typename X::F s[NB];
-            x.scores(base, s);
-            if (whole_tile(wf, wl)) {
-                x.template raise<false>(s, 0, true);
-                x.template weigh<false>(base + TENSOR, s, 0);
-            } else {
-                uint32_t vis;
-                const bool seen = x.look(a, p, j0, 0xFFFFFFFFu, vis);
-                x.template raise<true>(s, vis, seen);
-                x.template weigh<true>(base + TENSOR, s, vis);
-            }
-            if (spoilt) x.take_spoilt(a, p, j0, 0xFFFFFFFFu, marks);
-        }
+        if (R0 + M * w >= n_rows || j0 > wl) return;
+        typename X::F s[NB];
+        x.scores(base, s);
+        uint32_t vis;
+        const bool seen = x.look(a, p, j0, 0xFFFFFFFFu, vis);
+        x.template raise<true>(s, vis, seen);
+        x.template weigh<true>(base + TENSOR, s, vis);
+        if (spoilt) x.take_spoilt(a, p, j0, 0xFFFFFFFFu, marks);
+    };
+    int t = 0;
+    for (; t < n_tiles && !plain(t); t++) any_tile(t);
+    for (; t < n_tiles && plain(t); t++) {
+        turn(t);
+        typename X::F s[NB];
+        x.scores(base, s);
+        x.template raise<false>(s, 0, true);
+        x.template weigh<false>(base + TENSOR, s, 0);
     }
+    for (; t < n_tiles; t++) any_tile(t);
     x.finish(a, it, row, tok);
 }
 
@@ -488,17 +534,17 @@ static int many_run(F *f, int threads, int bytes, const BatchAttnArgs &a, int64_
     f<<<dim3((unsigned)items), threads, bytes, st>>>(a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
-// Rows a wavefront: 32 where their registers allow it (WaveRows).
-constexpr int many_wave(int D, int NP) { return D <= 128 && NP == 1 ? 32 : 16; }
 template <int D, class E, int NP, int RT, int SRC>
 static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
-    constexpr int M = many_wave(D, NP);
-    return many_run(attn_many_kernel<D, E, NP, RT, SRC, M>, 8192 / M, 4 * many_keys(D) * D * 2 + many_marks(D) + 16, a, items, st);
+    constexpr int M = NP == 1 ? 32 : 16;   // rows a wavefront (WaveRows)
+    typedef WaveRows<D, E, NP, 1, typename Row<RT>::t, M> X;
+    return many_run(attn_many_kernel<D, E, NP, RT, SRC, M>, 8192 / M, 4 * X::TENSOR + many_marks(D) + 16 + X::QL * 1024 * (kManyRows / M), a, items, st);
 }
 template <int D, class E, int NP, int NK, int RT>
 static int many_any(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
-    constexpr int M = many_wave(D, NP);
-    return many_run(attn_many_any_kernel<D, E, NP, NK, RT, M>, 8192 / M, 2 * NK * many_keys(D) * D * 2 + many_marks(D) + 16, a, items, st);
+    constexpr int M = NP == 1 && D <= 128 ? 32 : 16;
+    typedef WaveRows<D, E, NP, NK, typename Row<RT>::t, M> X;
+    return many_run(attn_many_any_kernel<D, E, NP, NK, RT, M>, 8192 / M, 2 * X::TENSOR + many_marks(D) + 16, a, items, st);
 }
 template <int D>
 static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
