@@ -93,6 +93,9 @@ __device__ __forceinline__ int token_of(const BatchAttnArgs &a, int x) {
     const int q = (int)__umulhi((uint32_t)x, a.inv_g);   // or one less
     return q + (x - q * a.G >= a.G);
 }
+constexpr int kFewRows = 16, kFewKeys = 32, kFewLimit = 2 * kFewRows;   // requests of up to kFewLimit rows a kv head are few
+constexpr int kManyRows = 128;
+constexpr int many_keys(int D) { return D == 256 ? 32 : 64; }
 // The rows of one request.
 struct Seq {
     int r, start, rows, pos0;   // its rows of q, the first one's position
@@ -124,6 +127,7 @@ __device__ __forceinline__ Seq seq_of(const BatchAttnArgs &a, int r) {
     s.rows = min(max(c1, s.start), a.T) - s.start;
     if (a.kv_len) s.pos0 = (int)max((int64_t)min(max(a.kv_len[r], 0), a.max_blocks << a.lg) - ((int64_t)c1 - c0), (int64_t)(-1 << 30));
     s.tiles = (s.rows * a.G + BM - 1) / BM;
+    if (a.only && (a.only == 1) != (s.rows * a.G <= kFewLimit)) s.tiles = 0;
     if (s.tiles) s.len = range_of<BN>(a, s.pos0 + token_of(a, (s.tiles - 1) * BM), s.pos0 + s.rows - 1).n;
     return s;
 }
@@ -154,7 +158,9 @@ struct Item {
 // Work item `item` (with MERGE: row tile and head `item` of those in more than one piece); false beyond the last. Every
 // wavefront finds its own, from the lengths, 64 requests at a time: with U key tiles over all row tiles and heads, a piece is about U / a.target
 // of them and no fewer than a.least, so that the pieces are alike whatever the lengths. At most a.target + (row tiles * heads) items,
-// 2 a.target of them in pieces: a request is cut only if it has more than a piece's tiles.
+// 2 a.target of them in pieces: a request is cut only if it has more than a piece's tiles. Where the uncut items are at most half of a.target, what
+// the GPU holds at once, longer pieces that it holds at once are better than the last of more (5 rows of 8 requests behind a window of
+// 2048, 16 heads on 4 of 256: 256 items 30 us, 512 47).
 template <int BM, int BN, bool MERGE>
 __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item &it) {
     const int lane = threadIdx.x & 63;
@@ -168,6 +174,14 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
         }
         u = wave_sum(u);
         per = max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1);
+        if (a.n_req <= 64) {
+            const float uncut = wave_sum((float)s.tiles) * a.Hkv;
+            for (int k = 0; k < 8 && 2.f * uncut <= (float)a.target; k++) {
+                const float n = wave_sum((float)(s.tiles * (s.len > per ? (int)((uint32_t)(s.len + per - 1) / (uint32_t)per) : 1))) * a.Hkv;
+                if (n <= (float)a.target) break;
+                per += max(1, per / 16);
+            }
+        }
     }
     int items = 0, slots = 0;
     for (int r0 = 0; r0 < a.n_req; r0 += 64) {
@@ -259,8 +273,5 @@ constexpr float kLowest = -1e38f;
 int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st);
 int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
 int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
-constexpr int kFewRows = 16, kFewKeys = 32;
-constexpr int kManyRows = 128;
-constexpr int many_keys(int D) { return D == 256 ? 32 : 64; }
 
 }  // namespace xjk

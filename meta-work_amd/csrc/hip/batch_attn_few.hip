@@ -260,40 +260,49 @@ int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
 
 // ----------------------------------------------------------------- merge --
 
-// Rows in more than one piece: a work-group joins a row's pieces, D / 4 threads taking one piece at a time, the others the next ones.
+// Rows in more than one piece, joined by D / 4 threads each. Of few rows there are many pieces: the work-group takes one row, its threads'
+// other runs the next pieces (128 pieces of a row of 256 dims 6 us, 23 by a wavefront a row). Of many rows there are few: the runs take the next rows.
 template <int D, int BM, int BN, int RT>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
     constexpr int TD = D / 4, TP = 256 / TD;
-    __shared__ __align__(16) float so[TP][D];
+    constexpr bool FEW = BM == kFewRows;
+    __shared__ __align__(16) float so[FEW ? TP : 1][D];
     __shared__ float sl[TP];
     const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % TD), tp = tid / TD;
     Item it;
     if (!find_item<BM, BN, true>(a, blockIdx.x, it)) return;
-    const int i = blockIdx.y;
-    if (i >= it.s.rows * a.G - it.tile * BM) return;
+    const int n_rows = it.s.rows * a.G - it.tile * BM, i = FEW ? blockIdx.y : blockIdx.y * TP + tp;
+    if (i >= n_rows) return;   // FEW: the whole work-group
     const int64_t at = (int64_t)it.slot * BM + i, step = (int64_t)a.Hkv * BM;
     float M = -INFINITY, L = 0.f;
-    for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
-    M = xjd::wave_max(M);
+    if (FEW) {
+        for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
+        M = xjd::wave_max(M);
+    } else {
+#pragma unroll 4
+        for (int p = 0; p < it.pieces; p++) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
+    }
     f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
     if (M != -INFINITY)
 #pragma unroll 4
-        for (int p = tp; p < it.pieces; p += TP) {
+        for (int p = FEW ? tp : 0; p < it.pieces; p += FEW ? TP : 1) {
             const float2 s = *part_stat(a, at + p * step, BM, D);
             const f32x4 x = *(const f32x4 *)(part_sums(a, at + p * step, D) + d);
             const float f = __builtin_amdgcn_exp2f(s.x - M);
             L += f * s.y;
             y += f * x;
         }
-    *(f32x4 *)&so[tp][d] = y;
-    if (d == 0) sl[tp] = L;
-    __syncthreads();
-    if (tp) return;
+    if constexpr (FEW) {
+        *(f32x4 *)&so[tp][d] = y;
+        if (d == 0) sl[tp] = L;
+        __syncthreads();
+        if (tp) return;
 #pragma unroll
-    for (int k = 1; k < TP; k++) {
-        y += *(const f32x4 *)&so[k][d];
-        L += sl[k];
+        for (int k = 1; k < TP; k++) {
+            y += *(const f32x4 *)&so[k][d];
+            L += sl[k];
+        }
     }
     const int row = it.tile * BM + i, t = token_of(a, row), h = it.head * a.G + row - t * a.G;
     finish4(y, M == -INFINITY ? 0.f : 1.f / L, a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr,
@@ -311,7 +320,7 @@ static void merge(const BatchAttnArgs &a, dim3 grid, hipStream_t st) {
     else merge<D, BM, many_keys(D)>(a, grid, st);
 }
 int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st) {
-    const dim3 grid((unsigned)groups, BM);
+    const dim3 grid((unsigned)groups, BM == kFewRows ? BM : BM * a.D / 1024);
     if (BM == kFewRows) {
         if (a.D == 64) merge<kFewRows, 64>(a, grid, st);
         else if (a.D == 128) merge<kFewRows, 128>(a, grid, st);

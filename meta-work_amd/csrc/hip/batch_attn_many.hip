@@ -311,7 +311,28 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     const int64_t page_bytes = ((int64_t)a.Hkv << a.lg) * (2 * D);
     const int page_mask = (1 << a.lg) - 1;
     auto whole_tile = [&](int f, int l, int j0) __attribute__((always_inline)) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
-    auto copy = [&](auto values, int t) __attribute__((always_inline)) {
+    // the pages of a tile, one for 16 positions (no array: indexed, it would lie in memory), asked for three tiles ahead
+    struct Pages {
+        int a, b, c, d;
+        __device__ __forceinline__ int at(int u) const { return u == 0 ? a : u == 1 ? b : u == 2 ? c : d; }
+        __device__ __forceinline__ uint32_t ok() const {   // a bit for each
+            if (SRC != kPages) return 0xFFFFFFFFu;
+            return 0xFFFFFFF0u | (uint32_t)(a >= 0) | (uint32_t)(b >= 0) << 1 | (uint32_t)(c >= 0) << 2 | (uint32_t)(d >= 0) << 3;
+        }
+    };
+    auto pages_of = [&](int t) __attribute__((always_inline)) {
+        Pages x{0, 0, 0, 0};
+        if (SRC != kPages) return x;
+        const int j0 = g.tile(i0 + max(min(t, n_tiles - 1), 0)) * BN;
+        x.a = page_at(a, tab, j0);
+        x.b = page_at(a, tab, j0 + 16);
+        if (BN == 64) {
+            x.c = page_at(a, tab, j0 + 32);
+            x.d = page_at(a, tab, j0 + 48);
+        }
+        return x;
+    };
+    auto copy = [&](auto values, int t, const Pages &pages) __attribute__((always_inline)) {
         constexpr bool V = decltype(values)::value;
         const int j0 = g.tile(i0 + t) * BN;
         const bool every = whole_tile(pl, pf, j0);   // some row sees each of its keys
@@ -325,7 +346,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c0 = (n * W + w) * 64, r0 = c0 / CH;
-            const int page = SRC == kPages ? page_at(a, tab, j0 + r0) : 0;
+            const int page = pages.at(r0 / 16);
             const uint32_t off = offs[V ? 0 : n & 1], to = base + (V ? 2 + (t & 1) : t & 1) * TENSOR + 16 * c0;
             const char *from;
             if (SRC == kPages) from = (V ? v_base : k_base) + (int64_t)max(page, 0) * page_bytes + ((j0 + r0) & page_mask) * (2 * D);
@@ -341,11 +362,12 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     };
     const std::false_type keys;
     const std::true_type values;
+    Pages now = pages_of(0), next = pages_of(1), after = pages_of(2), last;   // of tiles t .. t + 3
     if (n_tiles > 0) {
-        copy(keys, 0);
-        copy(values, 0);
+        copy(keys, 0, now);
+        copy(values, 0, now);
     }
-    if (n_tiles > 1) copy(keys, 1);
+    if (n_tiles > 1) copy(keys, 1, next);
     if (tid == 0) *flag = 0;
     const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
@@ -360,34 +382,32 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     auto keys_at = [&](int t) __attribute__((always_inline)) { return base + (t & 1) * TENSOR; };
     // Tile t's values and the next one's keys are there; what lies behind them is requested.
     auto turn = [&](int t) __attribute__((always_inline)) {
+        last = pages_of(t + 3);
         wait_vm<0>();
         lds_barrier();
-        if (t + 2 < n_tiles) copy(keys, t + 2);
-        if (t + 1 < n_tiles) copy(values, t + 1);
+        if (t + 2 < n_tiles) copy(keys, t + 2, after);
+        if (t + 1 < n_tiles) copy(values, t + 1, next);
     };
-    auto pages_at = [&](int j0) __attribute__((always_inline)) {   // a bit for 16 keys
-        uint32_t ok = 0xFFFFFFFFu;
-        if (SRC == kPages)
-#pragma unroll
-            for (int u = 0; u < BN / 16; u++)
-                if (page_at(a, tab, j0 + 16 * u) < 0) ok &= ~(1u << u);
-        return ok;
+    auto advance = [&]() __attribute__((always_inline)) {
+        now = next;
+        next = after;
+        after = last;
     };
     // Every row of the work-group sees all of tile t, and this wavefront some of the next.
     auto plain = [&](int t) __attribute__((always_inline)) {
         const int j0 = g.tile(i0 + t) * BN;
-        return has_keys(t + 1) && whole_tile(pf, pl, j0) && pages_at(j0) == 0xFFFFFFFFu;
+        return has_keys(t + 1) && whole_tile(pf, pl, j0) && now.ok() == 0xFFFFFFFFu;
     };
     auto any_tile = [&](int t) __attribute__((always_inline)) {
         const int j0 = g.tile(i0 + t) * BN;
         turn(t);
-        const uint32_t page_ok = pages_at(j0);
+        const uint32_t page_ok = now.ok();
         bool spoilt = false;
         if (page_ok != 0xFFFFFFFFu || !whole_tile(pf, pl, j0)) {
             char *const vt = lds + (2 + (t & 1)) * TENSOR;
             if (X::find_spoilt(vt)) *flag = 1;
             lds_barrier();
-            spoilt = *flag != 0;
+            spoilt = __builtin_amdgcn_readfirstlane(*flag) != 0;
             if (spoilt) {
                 lds_barrier();
                 if (tid == 0) *flag = 0;
@@ -404,6 +424,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
             if (spoilt) x.take_spoilt(a, p, j0, page_ok, marks);
         }
         if (has_keys(t + 1)) x.scores(keys_at(t + 1), s);
+        advance();
     };
     // (Three loops, not one with two paths: the sums would be moved between the paths' registers at every tile.)
     int t = 0;
@@ -413,6 +434,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
         x.template raise<false>(s, 0, true);
         x.template weigh<false>(vals_at(t), s, 0);
         x.scores(keys_at(t + 1), s);
+        advance();
     }
     for (; t < n_tiles; t++) any_tile(t);
     const int last_row = R0 + M * w + (X::QL ? fresh_lane() : lane) % M;
@@ -498,7 +520,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
         if (!whole_tile(pf, pl, j0)) {
             if (X::find_spoilt(vb)) *flag = 1;
             lds_barrier();
-            spoilt = *flag != 0;
+            spoilt = __builtin_amdgcn_readfirstlane(*flag) != 0;
             if (spoilt) {
                 lds_barrier();
                 if (tid == 0) *flag = 0;
@@ -569,47 +591,66 @@ int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
 
 // ---------------------------------------------------------------- launch --
 
-// Few rows: the kernel that reads keys straight into registers takes requests whose new tokens fill at most two of its tiles.
-static bool few_rows(const BatchAttnArgs &a) {
-    return a.table && a.max_new > 0 && (int64_t)a.max_new * a.G <= 2 * kFewRows;
-}
-// Row tiles times heads, at most.
-static int64_t tiles_bound(const BatchAttnArgs &a, int BM) {
-    return ((int64_t)a.T * a.G / BM + std::min(a.n_req, a.T)) * a.Hkv;
-}
-struct Split {
-    int BM, target, least;
-    int64_t tiles, items;
+// How a batch is run: in one launch of the kernel for few rows or of that for many (only = 0), or in one of each, for the requests of up to
+// kFewLimit rows a kv head (1) and for the others (2).
+struct Run {
+    int BM, only, target, least;
+    int64_t tiles, items;   // row tiles times heads, and work items, at most
 };
-// Pieces aimed at: enough for every CU.
-static Split split_of(const BatchAttnArgs &a) {
-    Split s;
-    const bool few = few_rows(a);
-    s.BM = few ? kFewRows : kManyRows;
-    s.tiles = tiles_bound(a, s.BM);
+static Run run_of(const BatchAttnArgs &a, bool few, int only) {
+    Run r;
+    r.BM = few ? kFewRows : kManyRows;
+    r.only = only;
+    const int64_t rows = (int64_t)a.T * a.G, n = std::min<int64_t>(only == 2 ? std::min<int64_t>(a.n_req, rows / (kFewLimit + 1)) : a.n_req, a.T);
+    r.tiles = rows / r.BM + n;
+    if (only == 1) r.tiles = std::min(r.tiles, 2 * n);
+    r.tiles *= a.Hkv;
+    r.least = 8;
+    // pieces aimed at: the work-groups that the GPU holds of the kernel
+    const int held = few ? (a.D == 64 ? 3 : a.D == 128 && a.type != kRowF32 ? 2 : 1) : a.type == kRowF32 ? 1 : 2;
     const int BN = few ? kFewKeys : many_keys(a.D);
-    s.least = few ? 8 : 8;
     const int64_t longest = ((a.table ? (int64_t)a.max_blocks << a.lg : a.T) + BN - 1) / BN;
-    s.target = longest <= s.least || s.tiles > 1024 ? 0 : 512;
-    s.items = s.target ? std::min(s.tiles * ((longest + s.least - 1) / s.least), s.tiles + s.target) : s.tiles;
-    return s;
+    r.target = longest <= r.least || r.tiles > 1024 ? 0 : 256 * held;
+    r.items = r.target ? std::min(r.tiles * ((longest + r.least - 1) / r.least), r.tiles + r.target) : r.tiles;
+    return r;
+}
+static int runs_of(const BatchAttnArgs &a, Run (&r)[2]) {
+    const bool few = a.table && (int64_t)(a.max_new > 0 ? a.max_new : a.T) * a.G <= kFewLimit;
+    if (few || !a.table || a.n_req == 1) {
+        r[0] = run_of(a, few, 0);
+        return 1;
+    }
+    r[0] = run_of(a, true, 1);
+    r[1] = run_of(a, false, 2);
+    return 2;
 }
 static int64_t slot_floats(const BatchAttnArgs &a, int BM) { return (int64_t)BM * (a.D + 2); }
 
 int64_t batch_attn_part_floats(const BatchAttnArgs &a) {
-    const Split s = split_of(a);
-    return s.target ? std::min<int64_t>(s.items, 2 * s.target) * slot_floats(a, s.BM) : 0;
+    Run r[2];
+    int64_t most = 0;
+    for (int i = 0, n = runs_of(a, r); i < n; i++)
+        if (r[i].target) most = std::max(most, std::min<int64_t>(r[i].items, 2 * r[i].target) * slot_floats(a, r[i].BM));
+    return most;
 }
 
 int batch_attn_launch(const BatchAttnArgs &args, int64_t part_floats, hipStream_t st) {
-    BatchAttnArgs a = args;
-    Split s = split_of(a);
-    a.slots = (int)std::min<int64_t>(part_floats / slot_floats(a, s.BM), 1 << 20);
-    a.target = std::min(s.target, a.slots / 2);   // at most 2 a.target items in pieces
-    a.least = s.least;
-    const int64_t items = a.target ? std::min(s.items, s.tiles + a.target) : s.tiles;
-    if (s.BM == kFewRows ? attn_few_launch(a, items, st) : attn_many_launch(a, items, st)) return -1;
-    return a.target ? attn_merge_launch(a, s.BM, std::min<int64_t>(s.tiles, a.target), st) : 0;
+    Run runs[2];
+    const int n = runs_of(args, runs);
+    for (int i = 0; i < n; i++) {
+        const Run &r = runs[i];
+        if (!r.tiles) continue;
+        BatchAttnArgs a = args;
+        a.only = r.only;
+        a.slots = (int)std::min<int64_t>(part_floats / slot_floats(a, r.BM), 1 << 20);
+        // at most 2 a.target items are in pieces
+        a.target = a.slots >= std::min<int64_t>(r.items, 2 * r.target) ? r.target : std::min(r.target, a.slots / 2);
+        a.least = r.least;
+        const int64_t items = a.target ? std::min(r.items, r.tiles + a.target) : r.tiles;
+        if (r.BM == kFewRows ? attn_few_launch(a, items, st) : attn_many_launch(a, items, st)) return -1;
+        if (a.target && attn_merge_launch(a, r.BM, std::min<int64_t>(r.tiles, a.target), st)) return -1;
+    }
+    return 0;
 }
 
 }  // namespace xjk

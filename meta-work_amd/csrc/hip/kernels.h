@@ -456,6 +456,7 @@ struct BatchAttnArgs {
     float scale;
     float *part;                                  // split partials
     int32_t target, least, slots;                 // set by batch_attn_launch: pieces aimed at, key tiles a piece at least, the partials' room
+    int32_t only;                                 // and: requests of few rows (1), of many (2), all (0)
 };
 int batch_attn_launch(const BatchAttnArgs &a, int64_t part_floats, hipStream_t st);
 int64_t batch_attn_part_floats(const BatchAttnArgs &a);      // beyond this nothing is gained
