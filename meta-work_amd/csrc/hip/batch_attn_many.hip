@@ -53,9 +53,9 @@ struct WaveRows {
     static constexpr int BN = many_keys(D), NS = D * M / 512, ND = D / M, CH = D / 8, KI = 512 / M;   // KI: keys a step of the second product
     static constexpr int PER = M * M / 64, NB = BN / M, NE = NB * PER;                                  // scores a block, blocks, scores a lane
     static constexpr int PLANE = BN * D * 2, TENSOR = NK * PLANE;
-    static constexpr int QL = D == 256 && M == 32 ? 3 : 0;   // steps whose queries lie in LDS: what two work-groups a CU leave of it
+    static constexpr int QL = D < 256 ? 0 : M == 32 ? 3 : NK == 3 ? 4 : 0;   // steps whose queries' last plane lies in LDS, as far as that is free
     typedef float F __attribute__((ext_vector_type(PER)));
-    V8<E> q[NS - QL][NP];
+    V8<E> q[NS][NP];
     uint32_t q_lds;   // where the wavefront's first QL steps lie
     F o[ND];
     float m, l, c;   // the reference in powers of two (a whole number, so that every rescaling is exact), the weights' sum, the scale
@@ -106,13 +106,8 @@ struct WaveRows {
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] = (float)x[s][i] * up;
-            if (s < QL) {
-                V8<E> y[NP];
-                planes<E, NP>(f, y);
-                *(__attribute__((address_space(3))) V8<E> *)(uintptr_t)(q_lds + 1024 * s + 16 * lane) = y[0];
-            } else {
-                planes<E, NP>(f, q[s - QL]);
-            }
+            planes<E, NP>(f, q[s]);
+            if (s < QL) *(__attribute__((address_space(3))) V8<E> *)(uintptr_t)(q_lds + 1024 * s + 16 * lane) = q[s][NP - 1];
         }
 #pragma unroll
         for (int d = 0; d < ND; d++)
@@ -136,7 +131,7 @@ struct WaveRows {
                     const V8<E> kf = lds_read<V8<E>>(at ^ (2 * KI * st), k * PLANE + 2 * M * b * D);
 #pragma unroll
                     for (int n = (NK == 1 ? NP : NP - k) - 1; n >= 0; n--)
-                        s[b] = mfma(kf, st < QL ? lds_read<V8<E>>(q_lds + 16 * lane, 1024 * st) : q[st - QL < 0 ? 0 : st - QL][n], s[b]);
+                        s[b] = mfma(kf, st < QL && n == NP - 1 ? lds_read<V8<E>>(q_lds + 16 * lane, 1024 * st) : q[st][n], s[b]);
                 }
         }
     }
@@ -441,8 +436,8 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     x.finish(a, it, last_row, token_of(a, min(last_row, n_rows - 1)));
 }
 
-// The same with keys and values that pass through registers: rows of any alignment, and floats in NK planes. A tile at a time; the next one
-// is requested before this one's products.
+// The same with keys and values that pass through registers: rows of any alignment, and floats in NK planes. A tile's values are put into LDS beside
+// its scores, the next one's keys beside its sums, so that what makes planes of them runs beside the matrix cores; two barriers a tile.
 template <int D, class E, int NP, int NK, int RT, int M>
 __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
@@ -464,58 +459,70 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     const Range g = range_of<BN>(a, pf, pl);
     const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
     Rows<R, 8> kx[COPIES], vx[COPIES];
-    auto request = [&](int t) __attribute__((always_inline)) {
+    auto request = [&](auto values, int t) __attribute__((always_inline)) {
+        constexpr bool V = decltype(values)::value;
         const int j0 = g.tile(i0 + t) * BN;
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c = n * 64 * W + tid, r = c / CH, e = c % CH, j = j0 + r;
-            kx[n] = vx[n] = R(0);
+            Rows<R, 8> &x = V ? vx[n] : kx[n];
+            x = R(0);
             if (j <= pl && (!a.window || j > pf - a.window || j < a.sinks)) {   // what no row sees counts for nothing, whatever lies there
-                kx[n] = *(const Rows<R, 8> *)((const R *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * e);
-                vx[n] = *(const Rows<R, 8> *)((const R *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * e);
+                if (V) x = *(const Rows<R, 8> *)((const R *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * e);
+                else x = *(const Rows<R, 8> *)((const R *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * e);
             }
         }
     };
-    auto put = [&]() __attribute__((always_inline)) {
+    auto put = [&](auto values) __attribute__((always_inline)) {
+        constexpr bool V = decltype(values)::value;
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c = n * 64 * W + tid, r = c / CH, e = c % CH;
-            V8<E> kp[NK], vp[NK];
+            const Rows<R, 8> &x = V ? vx[n] : kx[n];
+            V8<E> p[NK];
             if constexpr (NK == 1) {
-                kp[0] = __builtin_bit_cast(V8<E>, kx[n]);
-                vp[0] = __builtin_bit_cast(V8<E>, vx[n]);
+                p[0] = __builtin_bit_cast(V8<E>, x);
             } else {
                 float f[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) f[i] = (float)kx[n][i];
-                planes<E, NK>(f, kp);
-#pragma unroll
-                for (int i = 0; i < 8; i++) f[i] = (float)vx[n][i];
-                planes<E, NK>(f, vp);
+                for (int i = 0; i < 8; i++) f[i] = (float)x[i];
+                planes<E, NK>(f, p);
             }
+            char *const to = (V ? vb : lds) + 16 * (r * CH + (e ^ (V ? X::val_swz(r) : X::key_swz(r))));
 #pragma unroll
-            for (int k = 0; k < NK; k++) {
-                *(V8<E> *)(lds + k * PLANE + 16 * (r * CH + (e ^ X::key_swz(r)))) = kp[k];
-                *(V8<E> *)(vb + k * PLANE + 16 * (r * CH + (e ^ X::val_swz(r)))) = vp[k];
-            }
+            for (int k = 0; k < NK; k++) *(V8<E> *)(to + k * PLANE) = p[k];
         }
     };
-    if (n_tiles > 0) request(0);
+    const std::false_type keys;
+    const std::true_type values;
+    if (n_tiles > 0) {
+        request(keys, 0);
+        request(values, 0);
+    }
     if (tid == 0) *flag = 0;
     const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
     x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
-    auto turn = [&](int t) __attribute__((always_inline)) {
-        if (t) lds_barrier();
-        put();
-        lds_barrier();
-        if (t + 1 < n_tiles) request(t + 1);
+    if (n_tiles > 0) put(keys);
+    if (n_tiles > 1) request(keys, 1);
+    auto put_values = [&](int t) __attribute__((always_inline)) {
+        put(values);
+        if (t + 1 < n_tiles) request(values, t + 1);
+    };
+    auto put_keys = [&](int t) __attribute__((always_inline)) {   // the next tile's
+        if (t + 1 < n_tiles) put(keys);
+        if (t + 2 < n_tiles) request(keys, t + 2);
     };
     auto whole_tile = [&](int f, int l, int j0) __attribute__((always_inline)) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
     auto plain = [&](int t) __attribute__((always_inline)) { return R0 + M * w < n_rows && whole_tile(pf, pl, g.tile(i0 + t) * BN); };
     auto any_tile = [&](int t) __attribute__((always_inline)) {
         const int j0 = g.tile(i0 + t) * BN;
-        turn(t);
+        const bool here = R0 + M * w < n_rows && j0 <= wl;
+        typename X::F s[NB];
+        lds_barrier();
+        if (here) x.scores(base, s);
+        put_values(t);
+        lds_barrier();
         bool spoilt = false;
         if (!whole_tile(pf, pl, j0)) {
             if (X::find_spoilt(vb)) *flag = 1;
@@ -528,23 +535,26 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
                 lds_barrier();
             }
         }
-        if (R0 + M * w >= n_rows || j0 > wl) return;
-        typename X::F s[NB];
-        x.scores(base, s);
-        uint32_t vis;
-        const bool seen = x.look(a, p, j0, 0xFFFFFFFFu, vis);
-        x.template raise<true>(s, vis, seen);
-        x.template weigh<true>(base + TENSOR, s, vis);
-        if (spoilt) x.take_spoilt(a, p, j0, 0xFFFFFFFFu, marks);
+        if (here) {
+            uint32_t vis;
+            const bool seen = x.look(a, p, j0, 0xFFFFFFFFu, vis);
+            x.template raise<true>(s, vis, seen);
+            x.template weigh<true>(base + TENSOR, s, vis);
+            if (spoilt) x.take_spoilt(a, p, j0, 0xFFFFFFFFu, marks);
+        }
+        put_keys(t);
     };
     int t = 0;
     for (; t < n_tiles && !plain(t); t++) any_tile(t);
     for (; t < n_tiles && plain(t); t++) {
-        turn(t);
         typename X::F s[NB];
+        lds_barrier();
         x.scores(base, s);
+        put_values(t);
+        lds_barrier();
         x.template raise<false>(s, 0, true);
         x.template weigh<false>(base + TENSOR, s, 0);
+        put_keys(t);
     }
     for (; t < n_tiles; t++) any_tile(t);
     x.finish(a, it, row, tok);
@@ -566,7 +576,7 @@ template <int D, class E, int NP, int NK, int RT>
 static int many_any(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
     constexpr int M = NP == 1 && D <= 128 ? 32 : 16;
     typedef WaveRows<D, E, NP, NK, typename Row<RT>::t, M> X;
-    return many_run(attn_many_any_kernel<D, E, NP, NK, RT, M>, 8192 / M, 2 * X::TENSOR + many_marks(D) + 16, a, items, st);
+    return many_run(attn_many_any_kernel<D, E, NP, NK, RT, M>, 8192 / M, 2 * X::TENSOR + many_marks(D) + 16 + X::QL * 1024 * (kManyRows / M), a, items, st);
 }
 template <int D>
 static int many(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
