@@ -131,16 +131,6 @@ __device__ __forceinline__ Seq seq_of(const BatchAttnArgs &a, int r) {
     if (s.tiles) s.len = range_of<BN>(a, s.pos0 + token_of(a, (s.tiles - 1) * BM), s.pos0 + s.rows - 1).n;
     return s;
 }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
-__device__ __forceinline__ int wave_scan(int v) {   // sums up to and with this lane
-    v = dpp_add<0x111, 0xF>(v);   // the lane 1, 2, 4, 8 below in its row of 16
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);   // lane 15 to row 1, lane 47 to row 3
-    return dpp_add<0x143, 0xC>(v);   // lane 31 to rows 2 and 3
-}
 __device__ __forceinline__ float wave_sum(float v) {   // the same for every lane and in the same order
     v = xjd::row16_sum(v);
     auto at = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
@@ -183,12 +173,24 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
             }
         }
     }
+    const bool once = a.n_req <= 64;
+    if (once && !a.target) s = seq_of<BM, BN>(a, lane);
+    if (BM == kManyRows && once && a.n_req > 1) {   // the requests that see most first: the last items are then short ones
+        const int key = s.tiles ? s.len : -1;
+        int rank = 0;
+        for (int j = 0; j < a.n_req; j++) {
+            const int other = __builtin_amdgcn_readlane(key, j);
+            rank += other > key || (other == key && j < lane);
+        }
+        auto move = [&](int v) { return __builtin_amdgcn_ds_permute(4 * (lane < a.n_req ? rank : lane), v); };
+        s = Seq{move(s.r), move(s.start), move(s.rows), move(s.pos0), move(s.tiles), move(s.len)};
+    }
     int items = 0, slots = 0;
     for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-        if (a.n_req > 64 || !a.target) s = seq_of<BM, BN>(a, r0 + lane);
+        if (!once) s = seq_of<BM, BN>(a, r0 + lane);
         const int pieces = s.len > per ? (int)((uint32_t)(s.len + per - 1) / (uint32_t)per) : 1, heads = s.tiles * a.Hkv;
         const int n_slot = pieces > 1 ? heads * pieces : 0, n = MERGE ? (pieces > 1 ? heads : 0) : heads * pieces;
-        const int to = items + wave_scan(n), slot_to = slots + wave_scan(n_slot);
+        const int to = items + xjd::wave_scan(n), slot_to = slots + xjd::wave_scan(n_slot);
         const unsigned long long m = __ballot(to > item);
         if (m) {
             const int l = __builtin_ctzll(m);

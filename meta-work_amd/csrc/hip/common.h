@@ -73,6 +73,20 @@ __device__ __forceinline__ double readlane_d(double v, int l) {
     return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
 }
 
+// Sums over the lanes up to and with this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int row16_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);   // the lane 1, 2, 4, 8 below in its row of 16
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    return dpp_add<0x118, 0xF>(v);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x142, 0xA>(row16_scan(v));   // lane 15 to row 1, lane 47 to row 3
+    return dpp_add<0x143, 0xC>(v);            // lane 31 to rows 2 and 3
+}
+
 // Sum over the 64 lanes of a wavefront in double, in a fixed order: DPP
 // butterflies inside each row of 16 lanes, then the four row sums (read into
 // scalar registers) as (r0 + r1) + (r2 + r3). Every lane gets the total; all

@@ -38,66 +38,65 @@ __device__ __forceinline__ int run_of(const int32_t *cu, int n, int x) {
 
 constexpr int kPlanThreads = 1024;
 
-// Sums over the requests before each: rows, pages given back, pages taken. One work-group, the requests in runs of its threads.
+// Sums over the requests before each: rows, pages given back, pages taken. One work-group, the requests in runs of its threads. (Rows in
+// two halves of 16 bits: their sum may pass 32.)
 __device__ __forceinline__ void plan_scan(const PlanArgs &a) {
-    __shared__ int64_t red[3][kPlanThreads / 64];
+    constexpr int W = kPlanThreads / 64;
+    __shared__ int red[4][W];
+    __shared__ int64_t over[W];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int64_t base[3] = {0, 0, 0}, beyond = 0;
+    int64_t rows = 0, beyond = 0;
+    int base[2] = {0, 0};
     for (int r0 = 0; r0 < a.n_req; r0 += kPlanThreads) {
         const int r = r0 + tid;
         Req q{};
         if (r < a.n_req) q = request(a, r);
         beyond += q.beyond;
-        const int64_t own[3] = {q.fresh, max(q.have - q.need, 0), max(q.need - q.have, 0)};
-        int64_t x[3];
+        int x[4] = {q.fresh & 0xFFFF, q.fresh >> 16, max(q.have - q.need, 0), max(q.need - q.have, 0)}, all[4];
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            x[i] = own[i];
-            for (int o = 1; o < 64; o <<= 1) {
-                const int64_t y = __shfl_up(x[i], o, 64);
-                if (lane >= o) x[i] += y;
-            }
+        for (int i = 0; i < 4; i++) {
+            x[i] = xjd::wave_scan(x[i]);
             if (lane == 63) red[i][w] = x[i];
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            int64_t all = 0, before = 0;
-            for (int k = 0; k < kPlanThreads / 64; k++) {
-                if (k == w) before = all;
-                all += red[i][k];
-            }
-            x[i] += base[i] + before;
-            base[i] += all;
+        for (int i = 0; i < 4; i++) {
+            const int own = red[i][lane % W], to = xjd::row16_scan(own);
+            x[i] += __builtin_amdgcn_readlane(to - own, w);
+            all[i] = __builtin_amdgcn_readlane(to, W - 1);
         }
         if (r < a.n_req) {
-            a.cu[r + 1] = (int)min(x[0], (int64_t)INT32_MAX);
-            a.rel_cu[r + 1] = (int)min(x[1], (int64_t)INT32_MAX);
-            a.take_cu[r + 1] = (int)min(x[2], (int64_t)INT32_MAX);
+            a.cu[r + 1] = (int)min(rows + x[0] + ((int64_t)x[1] << 16), (int64_t)INT32_MAX);
+            a.rel_cu[r + 1] = base[0] + x[2];
+            a.take_cu[r + 1] = base[1] + x[3];
             a.kv_len[r] = q.kv;
         }
+        rows += all[0] + ((int64_t)all[1] << 16);
+        base[0] += all[2];
+        base[1] += all[3];
         __syncthreads();
     }
-    for (int o = 32; o; o >>= 1) beyond += __shfl_xor(beyond, o, 64);
-    if (lane == 0) red[0][w] = beyond;
+    if (__any(beyond != 0))
+        for (int o = 32; o; o >>= 1) beyond += __shfl_xor(beyond, o, 64);
+    if (lane == 0) over[w] = beyond;
     __syncthreads();
     if (tid == 0) {
         beyond = 0;
-        for (int k = 0; k < kPlanThreads / 64; k++) beyond += red[0][k];
+        for (int k = 0; k < W; k++) beyond += over[k];
         const int n_free = min(max(*a.n_free, 0), a.n_pages);
-        const int all = (int)min(n_free + base[1], (int64_t)a.n_pages);
-        const int64_t left = base[2] > all ? all : all - base[2];   // pages missing: none is taken
+        const int all = (int)min((int64_t)n_free + base[0], (int64_t)a.n_pages), takes = base[1];
+        const int left = takes > all ? all : all - takes;   // pages missing: none is taken
         const int64_t big = INT32_MAX;
         a.cu[0] = a.rel_cu[0] = a.take_cu[0] = 0;
         a.sum[0] = n_free;
         a.sum[1] = all;
-        a.sum[2] = (int)left;
-        a.sum[3] = (int)min(base[2], big);
-        *a.n_free_out = (int)left;
-        a.status[0] = (int)min(max(base[2] - all, (int64_t)0), big);
+        a.sum[2] = left;
+        a.sum[3] = takes;
+        *a.n_free_out = left;
+        a.status[0] = max(takes - all, 0);
         a.status[1] = (int)min(beyond, big);
-        a.status[2] = (int)min(max(base[0] - a.T, (int64_t)0), big);
-        a.status[3] = (int)min(base[0], big);
+        a.status[2] = (int)min(max(rows - a.T, (int64_t)0), big);
+        a.status[3] = (int)min(rows, big);
     }
 }
 // Entry i of the free pages with those given back behind them.
@@ -106,41 +105,71 @@ __device__ __forceinline__ int stack_at(const PlanArgs &a, int n_free, int i) {
     const int k = i - n_free, r = run_of(a.rel_cu, a.n_req, k);
     return a.table[(int64_t)r * a.max_blocks + request(a, r).need + k - a.rel_cu[r]];
 }
-// The pages that move, and the rows' positions and slots, each by a thread of its own. (What is read here of the table and of the
-// free list is not what is written: rows give or take, and pages are taken from `left` on, put back below it.)
-__device__ __forceinline__ void plan_expand(const PlanArgs &a) {
+// The pages that move (what 1: taken, 2: given back), and the rows' positions and slots (4), each by a thread of its own. What is read here of the
+// table and of the free list is not what is written: rows give or take, and pages are taken from `left` on, put back below it. cu: the requests'
+// first rows, the array or a copy in LDS.
+__device__ __forceinline__ void plan_expand(const PlanArgs &a, int what, const int32_t *cu) {
     const int n_free = a.sum[0], all = a.sum[1], left = a.sum[2], takes = a.sum[3];
     const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
     auto taken = [&](int i) { return takes <= all ? stack_at(a, n_free, all - 1 - i) : -1; };
-    for (int64_t i = first; i < takes; i += step) {
-        const int r = run_of(a.take_cu, a.n_req, (int)i);
-        a.table[(int64_t)r * a.max_blocks + request(a, r).have + (int)i - a.take_cu[r]] = taken((int)i);
-    }
-    for (int64_t i = n_free + first; i < left; i += step) a.free_list[i] = stack_at(a, n_free, (int)i);
-    const int rows = a.n_req ? a.cu[a.n_req] : 0;
-    for (int64_t t = first; t < a.T; t += step) {
-        int pos = 0, slot = -1;
-        if (t < rows) {
-            const int r = run_of(a.cu, a.n_req, (int)t);
-            const Req q = request(a, r);
-            const int64_t p = (int64_t)q.past + (t - a.cu[r]);
-            pos = (int)min(p, (int64_t)INT32_MAX);
-            if (p < q.kv) {
-                const int b = (int)(p >> a.lg);
-                const int page = b < q.have ? a.table[(int64_t)r * a.max_blocks + b] : taken(a.take_cu[r] + b - q.have);
-                if (page >= 0 && page < a.n_pages) slot = (page << a.lg) + (int)(p & ((1 << a.lg) - 1));
-            }
+    if (what & 1)
+        for (int64_t i = first; i < takes; i += step) {
+            const int r = run_of(a.take_cu, a.n_req, (int)i);
+            a.table[(int64_t)r * a.max_blocks + request(a, r).have + (int)i - a.take_cu[r]] = taken((int)i);
         }
-        if (a.pos) a.pos[t] = pos;
-        if (a.slot) a.slot[t] = slot;
+    if (what & 2)
+        for (int64_t i = n_free + first; i < left; i += step) a.free_list[i] = stack_at(a, n_free, (int)i);
+    if (what & 4) {
+        const int rows = a.n_req ? cu[a.n_req] : 0;
+        for (int64_t t = first; t < a.T; t += step) {
+            int pos = 0, slot = -1;
+            if (t < rows) {
+                const int r = run_of(cu, a.n_req, (int)t);
+                const Req q = request(a, r);
+                const int64_t p = (int64_t)q.past + (t - cu[r]);
+                pos = (int)min(p, (int64_t)INT32_MAX);
+                if (p < q.kv) {
+                    const int b = (int)(p >> a.lg);
+                    const int page = b < q.have ? a.table[(int64_t)r * a.max_blocks + b] : taken(a.take_cu[r] + b - q.have);
+                    if (page >= 0 && page < a.n_pages) slot = (page << a.lg) + (int)(p & ((1 << a.lg) - 1));
+                }
+            }
+            if (a.pos) a.pos[t] = pos;
+            if (a.slot) a.slot[t] = slot;
+        }
     }
 }
 __global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(const PlanArgs a) { plan_scan(a); }
-__global__ __launch_bounds__(256) void plan_expand_kernel(const PlanArgs a) { plan_expand(a); }
+// Work-groups of one kind each, so that no thread waits for one chain of loads after the other.
+constexpr int kPlanLds = 4096;
+__global__ __launch_bounds__(256) void plan_expand_kernel(const PlanArgs a) {
+    __shared__ int32_t cu[kPlanLds + 1];
+    const int what = 1 << blockIdx.y;
+    if (what == 4 && a.n_req <= kPlanLds) {
+        for (int i = threadIdx.x; i <= a.n_req; i += 256) cu[i] = a.cu[i];
+        __syncthreads();
+        plan_expand(a, what, cu);
+    } else {
+        plan_expand(a, what, a.cu);
+    }
+}
+// All of it in one work-group: what it wrote it reads back behind a barrier.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs a) {
+    plan_scan(a);
+    __threadfence_block();
+    __syncthreads();
+    plan_expand(a, 7, a.cu);
+}
 
 int page_plan_launch(const PlanArgs &a, hipStream_t st) {
-    plan_scan_kernel<<<1, kPlanThreads, 0, st>>>(a);
-    plan_expand_kernel<<<std::min(1024, std::max(16, (a.T + 255) / 256)), 256, 0, st>>>(a);
+    // A second launch costs what a thread's four rows do. The pages that move are not known here: of few requests
+    // and rows they are few, or long prompts', whose rows are many.
+    if (a.n_req <= 256 && a.T <= 4 * kPlanThreads) {
+        plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+    } else {
+        plan_scan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+        plan_expand_kernel<<<dim3(std::min(1024, std::max(64, (a.T + 255) / 256)), 3), 256, 0, st>>>(a);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
