@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 
 import xjpipe as xp
-from test_long_context import Hip
+from test_long_context import Hip, rope64
 
 
 # ------------------------------------------------------------ plain forms --
@@ -619,3 +619,217 @@ def test_attention_refusals():
     # enough for any smaller batch
     n = [L.xjh_attn_paged_work_bytes(C.byref(c), xp.F16, T, 4, T, 1, 4096) for T in (1, 2, 8, 64)]
     assert n[0] > 0 and n == sorted(n)
+
+
+# --------------------------------------------------------------- together --
+
+def _call(name, *args):
+    err = C.create_string_buffer(512)
+    assert getattr(xp.lib(), name)(*args, err, 512) == 0, err.value
+
+
+class _Step:
+    """A layer step of several requests on a stream, every length on the device: plan, rope of queries and keys at the plan's
+    positions, store into the plan's slots, attention over the plan's table."""
+
+    def __init__(self, n_req, T, H, Hkv, D, page, n_pages, blocks, rows="f32", cache="f16", max_new=0, window=0, n_sink=0):
+        self.n_req, self.T, self.H, self.max_new, self.window, self.n_sink, self.blocks, self.rows = n_req, T, H, max_new, window, n_sink, blocks, rows
+        self.pool = xp.PagePool(page, n_pages, n_req, blocks)
+        self.kv = xp.PagedKv(Hkv, D, page, n_pages, type=IDS[cache])
+        nan = np.full(self.kv.c.bytes // 2, 0x7FC0 if cache == "bf16" else 0x7E00, np.uint16)
+        self.kv.k.put(nan), self.kv.v.put(nan)
+        i32 = {"held": n_req, "past": n_req, "new": n_req, "cu": n_req + 1, "kv": n_req, "pos": T, "slot": T, "status": 4}
+        self.d = {k: xp.Dev(np.zeros(n, np.int32)) for k, n in i32.items()}
+        self.q, self.qr, self.k, self.kr, self.v, self.out = (xp.Dev(nbytes=4 * T * h * D) for h in (H, H, Hkv, Hkv, Hkv, H))
+        self.cfg = xp.XjhRopeCfg(pairs=0, n_rot=D, base=1e4, scaling=0, factor=1.0)
+        self.plan_bytes = xp.lib().xjh_page_plan_work_bytes(n_req)
+        self.bytes = xp.lib().xjh_attn_paged_work_bytes(C.byref(self.kv.c), IDS[rows], T, H, n_req, max_new, blocks)
+        self.plan_work, self.work = xp.Dev(nbytes=max(16, self.plan_bytes)), xp.Dev(nbytes=max(16, self.bytes))
+        self.seen = [(np.zeros((0, Hkv, D)), np.zeros((0, Hkv, D))) for _ in range(n_req)]   # what every request's cache holds
+
+    def run(self, st):
+        d, c, T, H = {k: x.ptr for k, x in self.d.items()}, self.kv.c, self.T, self.H
+        D, row, free = c.D, c.Hkv * c.D, self.pool._n_free.ptr
+        _call("xjh_page_plan", C.byref(self.pool.p), d["held"], d["past"], d["new"], self.n_req, free, free, T, d["cu"], d["kv"], d["pos"], d["slot"],
+              d["status"], self.plan_work.ptr, self.plan_bytes, st)
+        for x, y, h in ((self.q, self.qr, H), (self.k, self.kr, c.Hkv)):
+            _call("xjh_rope_scaled", x.ptr, h * D, D, y.ptr, h * D, D, T, h, D, C.byref(self.cfg), d["pos"], 0, st)
+        _call("xjh_paged_store", C.byref(c), xp.F32, self.kr.ptr, row, self.v.ptr, row, T, d["slot"], st)
+        _call("xjh_attn_paged", C.byref(c), xp.F32, self.qr.ptr, H * D, D, None, 0, 0, self.pool._table.ptr, self.blocks, d["cu"], d["kv"], self.n_req, T,
+              self.max_new, H, self.window, self.n_sink, D ** -0.5, self.out.ptr, H * D, self.work.ptr, self.bytes, st)
+
+    def feed(self, rng, held, past, new):
+        for k, x in (("held", held), ("past", past), ("new", new)):
+            self.d[k].put(np.asarray(x, np.int32))
+        D, Hkv = self.kv.c.D, self.kv.c.Hkv
+        self.x = [rng.standard_normal((self.T, h, D)).astype(np.float32) for h in (self.H, Hkv, Hkv)]
+        for d, x in zip((self.q, self.k, self.v), self.x):
+            d.put(x)
+        self.out.put(np.full((self.T, self.H, D), 7, np.float32))
+
+    def check(self, past, new):
+        got, t = self.out.get(np.float32, (self.T, self.H, self.kv.c.D)), 0
+        assert self.d["status"].get(np.int32, (4,)).tolist() == [0, 0, 0, sum(new)]
+        for r, (p, n) in enumerate(zip(past, new)):
+            pos = p + np.arange(n)
+            q, k = (rope64(x[t:t + n], self.cfg, pos)[0].astype(np.float32) for x in self.x[:2])
+            k, v = (np.concatenate([old[:p], value(to_type(x, "f16"))]) for old, x in zip(self.seen[r], (k, self.x[2][t:t + n])))
+            self.seen[r] = k, v
+            want, mag = attend64(q.astype(np.float64), k, v, p, window=self.window, n_sink=self.n_sink)
+            # a key within half a bit of a border may round to the other side after the rotation: half a step of f16 in a few of a key's elements, each
+            # 2^-11 of one of D products of a score of size 1, is below 2^-11 |q| / sqrt(D) in a score; as much of a weight
+            err = np.abs(got[t:t + n] - want)
+            assert np.all(err <= (1e-5 + 2.0 ** -11) * mag), (r, p, n, float((err / np.maximum(mag, 1e-30)).max()))
+            assert np.linalg.norm(err) <= 2e-5 * max(np.linalg.norm(mag), 1e-30)
+            t += n
+        assert np.all(got[t:] == 7)   # the padding's rows
+
+
+def _lengths(rng, n_req, T, limit, steps, most=None):
+    """held, past, new of the steps of a batch: prompts, pieces of them, single tokens, rejected drafts, requests that end."""
+    past, new = np.zeros(n_req, int), np.zeros(n_req, int)
+    for _ in range(steps):
+        held = past + new
+        past = held - rng.integers(0, 3, n_req) * (rng.random(n_req) < 0.3)
+        past[rng.random(n_req) < 0.1] = 0
+        past = np.maximum(past, 0)
+        new = np.where(rng.random(n_req) < 0.3, rng.integers(0, T // 2, n_req), rng.integers(0, 4, n_req))
+        new = np.minimum(new, limit - past if most is None else most)
+        while new.sum() > T:
+            new[new.argmax()] //= 2
+        yield held.tolist(), past.tolist(), new.tolist()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hkv,page,max_new,window,n_sink", [(128, 2, 16, 0, 0, 0), (64, 1, 32, 0, 40, 3), (256, 2, 64, 0, 0, 0), (128, 2, 16, 3, 0, 0)])
+def test_captured_steps_of_a_batch(D, Hkv, page, max_new, window, n_sink):
+    """Two steps captured once each, with work areas of their own, and replayed by turns over a batch's life, eager work between."""
+    rng, hip = np.random.default_rng(D + page), Hip()
+    steps = [_Step(5, 40, 2 * Hkv, Hkv, D, page, 5 * up(320, page), up(320, page), max_new=max_new, window=window, n_sink=n_sink) for _ in range(2)]
+    streams = [hip.stream() for _ in steps]
+    graphs = [hip.capture(st, s.run) for s, st in zip(steps, streams)]
+    for i, (held, past, new) in enumerate(_lengths(rng, 5, 40, 320, 10, max_new or None)):
+        for s in steps:
+            s.feed(rng, held, past, new)
+        hip.sync()
+        for g, st in zip(graphs, streams):
+            hip("hipGraphLaunch", g, st)
+        xp.norm(rng.standard_normal((3, 64)).astype(np.float32), None, 1, 1e-6)
+        hip.sync()
+        for s in steps:
+            s.check(past, new)
+    for g in graphs:
+        hip("hipGraphExecDestroy", g)
+    for st in streams:
+        hip("hipStreamDestroy", st)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("handle", [None, 1, 2])
+def test_eager_steps_on_predefined_streams(handle):
+    rng = np.random.default_rng(3)
+    s = _Step(3, 24, 4, 2, 64, 16, 60, 20)
+    for held, past, new in _lengths(rng, 3, 24, 320, 5):
+        s.feed(rng, held, past, new)
+        s.run(handle)
+        xp.lib().xjh_sync()
+        s.check(past, new)
+
+
+@pytest.mark.gpu
+def test_batch_calls_follow_their_stream():
+    """Inputs that a side stream copies in behind half a gigabyte of other copies are there when the calls run."""
+    rng, hip = np.random.default_rng(5), Hip()
+    s = _Step(3, 24, 4, 2, 128, 16, 60, 20)
+    s.feed(rng, [0, 0, 0], [0, 0, 0], [9, 1, 14])
+    src, to = [xp.Dev(x) for x in s.x], (s.q, s.k, s.v)
+    for d, x in zip(to, s.x):
+        d.put(x * 0)
+    big, st = [xp.Dev(nbytes=1 << 26) for _ in range(2)], hip.stream()
+    hip.sync()
+    for _ in range(8):
+        hip("hipMemcpyAsync", C.c_void_p(big[0].ptr), C.c_void_p(big[1].ptr), C.c_size_t(1 << 26), C.c_int(3), st)
+    for d, y in zip(to, src):
+        hip("hipMemcpyAsync", C.c_void_p(d.ptr), C.c_void_p(y.ptr), C.c_size_t(y.nbytes), C.c_int(3), st)
+    s.run(st)
+    hip.sync()
+    hip("hipStreamDestroy", st)
+    s.check([0, 0, 0], [9, 1, 14])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [1, 0])
+def test_pages_beyond_four_gigabytes(max_new):
+    """Requests in the last pages of caches of 5 GB each."""
+    rng, Hkv, D, page, n_pages = np.random.default_rng(6), 8, 256, 256, 5000
+    c = xp.XjhPaged(xp.BF16, Hkv, D, page, n_pages, 16, 16, 0)
+    c.bytes = xp.lib().xjh_paged_bytes(C.byref(c))
+    assert c.bytes > 1 << 32
+    pool = [xp.Dev(nbytes=c.bytes) for _ in range(2)]
+    c.k, c.v = pool[0].ptr, pool[1].ptr
+    n, table = 700, np.array([[n_pages - 1, n_pages - 3, n_pages - 2]], np.int32)
+    k, v = (to_type(kv_rows(rng, n, Hkv, D), "bf16") for _ in range(2))
+    q = to_type(rng.standard_normal((40, Hkv, D)).astype(np.float32), "bf16")
+    j = np.arange(n)
+    slot = (table[0, j // page] * page + j % page).astype(np.int32)
+    dk, dv, ds, dq, dt, dc, dl = (xp.Dev(x) for x in (k, v, slot, q, table, np.array([0, 40], np.int32), np.array([n], np.int32)))
+    out, row = xp.Dev(nbytes=q.nbytes), Hkv * D
+    nb = xp.lib().xjh_attn_paged_work_bytes(C.byref(c), xp.BF16, 40, Hkv, 1, max_new, 3)
+    work = xp.Dev(nbytes=max(16, nb))
+    _call("xjh_paged_store", C.byref(c), xp.BF16, dk.ptr, row, dv.ptr, row, n, ds.ptr, None)
+    _call("xjh_attn_paged", C.byref(c), xp.BF16, dq.ptr, row, D, None, 0, 0, dt.ptr, 3, dc.ptr, dl.ptr, 1, 40, max_new, Hkv, 0, 0, D ** -0.5, out.ptr, row,
+          work.ptr, nb, None)
+    xp.lib().xjh_sync()
+    check(out.get(np.uint16, q.shape), *attend64(value(q), value(k), value(v), n - 40), "bf16")
+    for b in pool:
+        b.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+def test_packed_of_very_many_short_prompts(rows):
+    rng = np.random.default_rng(9)
+    lens = rng.integers(0, 4, 3000)
+    lens[[0, 1700]] = 70, 150
+    T, cu = int(lens.sum()), np.cumsum(np.concatenate([[0], lens]))
+    q, k, v = (to_type(rng.standard_normal((T, h, 64)).astype(np.float32), rows) for h in (4, 2, 2))
+    got = xp.attn_packed(q, k, v, cu)
+    w = [attend64(*(value(x[a:b]) for x in (q, k, v)), 0) for a, b in zip(cu, cu[1:])]
+    check(got, *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("max_new", [1, 0])
+def test_paged_rising_scores(rows, cache, max_new):
+    """Scores that rise by some powers of two from tile to tile, and fall: the running maximum changes at every one, up to weights that vanish."""
+    D, n = 64, 900
+    for sign in (1, -1):
+        def kv(r, m):
+            rng = np.random.default_rng(4)
+            k = np.zeros((m, 1, D))
+            k[:, 0, 0] = sign * np.arange(m) / 4
+            return (k + 0.1 * rng.standard_normal(k.shape)).astype(np.float32), rng.standard_normal((m, 1, D)).astype(np.float32)
+
+        b = Batch(np.random.default_rng(4), [(n, 2), (n, 60)], 2, 1, D, 16, rows, cache, kv=kv)
+        b.q = to_type(np.concatenate([np.ones((62, 2, 1)), 0.1 * np.random.default_rng(1).standard_normal((62, 2, D - 1))], -1).astype(np.float32), rows)
+        # scores up to 225 of sums of that size: 225 * 1.44 * 4 * 2^-24 = 8e-5 in a weight beside what `check` allows
+        got, (want, mag) = value(b.attend(scale=1.0, max_new=max_new)).reshape(-1, 2, D), b.want(scale=1.0)
+        u = HALF[rows]
+        assert np.all(np.abs(got - want) <= u * np.abs(want) + (u + 1e-4) * mag + 2.0 ** -24)
+
+
+def test_batch_wrappers_refuse_arrays_of_other_shapes():
+    x, kv = np.zeros((3, 2, 64), np.float32), xp.PagedKv.__new__(xp.PagedKv)   # (without memory: nothing is launched)
+    kv.c = xp.XjhPaged(xp.F16, 2, 64, 16, 4, None, None, 0)
+    tab = np.zeros((2, 3), np.int32)
+    for call in (lambda: kv.store(x, x[:2], [0, 1, 2]), lambda: kv.store(x, x, [0, 1]), lambda: kv.store(x, x, [0, 1, 1]), lambda: kv.store(x, x.astype(np.float16), [0, 1, 2]),
+                 lambda: kv.store(x.astype(np.float64), x, [0, 1, 2]), lambda: kv.store(x, x, [0, 1, 1 << 31]),
+                 lambda: kv.attend(x[..., :32], tab, [0, 1, 3], [5, 5]), lambda: kv.attend(x, tab[0], [0, 1, 3], [5, 5]), lambda: kv.attend(x, tab, [0, 3], [5, 5]),
+                 lambda: kv.attend(x, tab, [0, 1, 3], [5]), lambda: kv.attend(x, tab, [0, 1, 3], [5, 5], gate=x[:1]),
+                 lambda: kv.attend(x, tab, [0, 1, 3], [5, 5], window=1 << 32), lambda: kv.attend(x, tab, [0, 1, 3], [5, 1 << 31]),
+                 lambda: xp.attn_packed(x, x, x[:2], [0, 3]), lambda: xp.attn_packed(x, x.astype(np.float16), x, [0, 3]), lambda: xp.attn_packed(x, x, x, []),
+                 lambda: xp.attn_packed(x, x, x, [0, 3], gate=x.astype(np.float16)), lambda: xp.attn_packed(x, x, x, [0, 3], n_sink=1 << 31),
+                 lambda: xp.PagedKv(2, 60, 16, 4), lambda: xp.PagedKv(2, 64, 16, 4, type=xp.F32), lambda: xp.PagedKv(2, 64, 16, 1 << 31)):
+        with pytest.raises(xp.XjError):
+            call()
