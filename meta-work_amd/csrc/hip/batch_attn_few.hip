@@ -1,4 +1,4 @@
-// Attention over pages for requests of few rows (gfx950): single tokens and short drafts. See batch_attn.h.
+// Attention for requests of few rows (gfx950): single tokens and short drafts over pages, short prompts. See batch_attn.h.
 #include "batch_attn.h"
 
 namespace xjk {
@@ -8,7 +8,7 @@ namespace xjk {
 // the lane's VW dims of the eight keys whose weights it holds and turned in registers. A tile's keys are requested as soon as the scores of
 // the one before are there, its values behind that one's sums. Weights enter in two planes at least: the
 // matrix cores wait for memory here.
-template <int D, class E, int NP, int RT>
+template <int D, class E, int NP, int RT, bool PAGES>
 __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
     constexpr int NS = D / 32, VW = D >= 128 ? 8 : 4, NB = D / (16 * VW), PAD = D + 4, NW = NP > 2 ? NP : 2;
@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     const int i0 = part_from(g.n, it.piece, it.pieces) + w, i1 = part_from(g.n, it.piece + 1, it.pieces);
 
     // ---- a tile: its pages, keys and values
-    const int32_t *tab = a.table + (int64_t)it.s.r * a.max_blocks;
+    const int32_t *tab = PAGES ? a.table + (int64_t)it.s.r * a.max_blocks : nullptr;
     struct Pages {
         int j0, page[2];
     };
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
         Pages x;
         x.j0 = g.tile(min(i, i1 - 1)) * kFewKeys;
 #pragma unroll
-        for (int u = 0; u < 2; u++) x.page[u] = page_at(a, tab, x.j0 + 16 * u);
+        for (int u = 0; u < 2; u++) x.page[u] = PAGES ? page_at(a, tab, x.j0 + 16 * u) : 0;
         return x;
     };
     auto at = [&](const Pages &x, int u) {   // of a page that is none, page 0's, which counts for nothing
@@ -44,19 +44,37 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     auto load_keys = [&](const Pages &x) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const E *kp = (const E *)a.k + at(x, u) + li * D + 8 * kq;
+            if constexpr (PAGES) {
+                const E *kp = (const E *)a.k + at(x, u) + li * D + 8 * kq;
 #pragma unroll
-            for (int s = 0; s < NS; s++) kf[u][s] = *(const V8<E> *)(kp + 32 * s);
+                for (int s = 0; s < NS; s++) kf[u][s] = *(const V8<E> *)(kp + 32 * s);
+            } else {   // behind the last row, the last one, which counts for nothing there
+                const E *kp = (const E *)a.k + (it.s.start + min(x.j0 + 16 * u + li, it.s.rows - 1)) * a.k_tok + it.head * a.k_head + 8 * kq;
+#pragma unroll
+                for (int s = 0; s < NS; s++) kf[u][s] = __builtin_bit_cast(V8<E>, *(const Rows<E, 8> *)(kp + 32 * s));
+            }
         }
     };
     auto load_values = [&](const Pages &x) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const E *vp = (const E *)a.v + at(x, u) + 4 * kq * D + VW * li;
+            if constexpr (PAGES) {
+                const E *vp = (const E *)a.v + at(x, u) + 4 * kq * D + VW * li;
 #pragma unroll
-            for (int r = 0; r < 4; r++)
+                for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int b = 0; b < NB; b++) __builtin_memcpy(vv[4 * u + r][b], __builtin_assume_aligned(vp + r * D + 16 * VW * b, 2 * VW), 2 * VW);
+                    for (int b = 0; b < NB; b++) __builtin_memcpy(vv[4 * u + r][b], __builtin_assume_aligned(vp + r * D + 16 * VW * b, 2 * VW), 2 * VW);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const E *vp = (const E *)a.v + (it.s.start + min(x.j0 + 16 * u + 4 * kq + r, it.s.rows - 1)) * a.v_tok + it.head * a.v_head + VW * li;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const Rows<E, VW> y = *(const Rows<E, VW> *)(vp + 16 * VW * b);
+                        __builtin_memcpy(vv[4 * u + r][b], &y, 2 * VW);
+                    }
+                }
+            }
         }
     };
     // ---- queries, with the scale's sign; float ones scaled to 2^14 .. 2^15 before they become f16 planes
@@ -246,10 +264,13 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
 template <int D>
 static void few(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
     const dim3 grid((unsigned)items);
-    if (a.type == kRowF16) attn_few_kernel<D, _Float16, 1, kRowF16><<<grid, 256, 0, st>>>(a);
-    else if (a.type == kRowBf16) attn_few_kernel<D, __bf16, 1, kRowBf16><<<grid, 256, 0, st>>>(a);
-    else if (a.kv_type == kRowF16) attn_few_kernel<D, _Float16, 2, kRowF32><<<grid, 256, 0, st>>>(a);
-    else attn_few_kernel<D, __bf16, 3, kRowF32><<<grid, 256, 0, st>>>(a);
+    if (!a.table) {
+        if (a.type == kRowF16) attn_few_kernel<D, _Float16, 1, kRowF16, false><<<grid, 256, 0, st>>>(a);
+        else attn_few_kernel<D, __bf16, 1, kRowBf16, false><<<grid, 256, 0, st>>>(a);
+    } else if (a.type == kRowF16) attn_few_kernel<D, _Float16, 1, kRowF16, true><<<grid, 256, 0, st>>>(a);
+    else if (a.type == kRowBf16) attn_few_kernel<D, __bf16, 1, kRowBf16, true><<<grid, 256, 0, st>>>(a);
+    else if (a.kv_type == kRowF16) attn_few_kernel<D, _Float16, 2, kRowF32, true><<<grid, 256, 0, st>>>(a);
+    else attn_few_kernel<D, __bf16, 3, kRowF32, true><<<grid, 256, 0, st>>>(a);
 }
 int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
     if (a.D == 64) few<64>(a, items, st);

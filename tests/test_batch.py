@@ -541,10 +541,11 @@ def test_packed_long(rows, work_bytes):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("D,shift,tok,head", [(64, 0, 0, 0), (64, 8, 16, 8), (128, 1, 3, 1), (128, 2, 8, 8), (256, 4, 8, 0), (64, 8, 1, 8)])
-def test_packed_strides_and_alignment(D, shift, tok, head, rows):
+@pytest.mark.parametrize("lens", [(40, 1, 49), (1030, 3, 70)])
+def test_packed_strides_and_alignment(lens, D, shift, tok, head, rows):
     """Rows that begin at any element, heads and tokens apart, q k v and gate in one buffer; what lies between is left alone."""
     rng, err = np.random.default_rng(5), C.create_string_buffer(512)
-    H, Hkv, cu, T = 4, 2, np.array([0, 40, 41, 90], np.int32), 93
+    H, Hkv, cu, T, n = 4, 2, np.cumsum((0,) + lens).astype(np.int32), sum(lens) + 3, sum(lens)
     hs = D + head
     ts = 2 * H * hs + 2 * Hkv * hs + tok
     buf = to_type(rng.standard_normal(shift + T * ts + 8 * D).astype(np.float32), rows)
@@ -560,21 +561,22 @@ def test_packed_strides_and_alignment(D, shift, tok, head, rows):
                                     D ** -0.5, do.ptr, o_tok, work.ptr, wb, None, err, 512) == 0, err.value
     xp.lib().xjh_sync()
     got = do.get(buf.dtype, out.shape).reshape(T, o_tok)
-    assert np.all(got[:, H * D:] == 9) and np.all(got[90:] == 9)
+    assert np.all(got[:, H * D:] == 9) and np.all(got[n:] == 9)
     def take(x, n):
         return value(np.stack([[buf[x + t * ts + h * hs:x + t * ts + h * hs + D] for h in range(n)] for t in range(T)]))
 
     q, k, v, g = take(at[0], H), take(at[1], Hkv), take(at[2], Hkv), take(at[3], H)
     w = [attend64(q[a:b], k[a:b], v[a:b], 0, gate=g[a:b]) for a, b in zip(cu, cu[1:])]
-    check(np.ascontiguousarray(got[:90, :H * D]), *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+    check(np.ascontiguousarray(got[:n, :H * D]), *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
-def test_packed_values_that_are_not_finite(rows):
+@pytest.mark.parametrize("T", [120, 1200])
+def test_packed_values_that_are_not_finite(T, rows):
     """One prompt's do not reach another's rows, nor earlier ones of its own."""
     rng = np.random.default_rng(2)
-    T, D, cu = 120, 64, [0, 70, 120]
+    D, cu = 64, [0, 70, T]
     q = to_type(rng.standard_normal((T, 2, D)).astype(np.float32), rows)
     k, v = (kv_rows(rng, T, 1, D) for _ in range(2))
     want = value(xp.attn_packed(q, to_type(k, rows), to_type(v, rows), cu))
