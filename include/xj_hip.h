@@ -587,8 +587,9 @@ typedef struct {
  *              -1, what was given back stays given back, and the step can be tried again with less (held as
  *              it was for requests that wanted pages, n_past for those that gave some).
  * Negative lengths count as 0, n_past and held beyond the rows as the whole row; the sum of n_new is
- * below 2^31. n_req is at most 65536, n_req * max_blocks 2^30. Calls on the same pages are ordered. work: xjh_page_plan_work_bytes
- * bytes, 16-byte aligned. */
+ * below 2^31. n_req is at most 65536, n_req * max_blocks 2^30. The lengths lie in no buffer that is written (held is not
+ * kv_len's array). A page is in one row of the table only: one that rows share would be given back by each. Calls on
+ * the same pages are ordered. work: xjh_page_plan_work_bytes bytes, 16-byte aligned. */
 int xjh_page_plan(const xjh_pages *p, const int32_t *held, const int32_t *n_past, const int32_t *n_new, int n_req,
                   const int32_t *n_free, int32_t *n_free_out, int T, int32_t *cu, int32_t *kv_len, int32_t *pos,
                   int32_t *slot, int32_t *status, void *work, size_t work_bytes, void *stream, char *err, size_t errlen);
@@ -606,7 +607,7 @@ typedef struct {
 uint64_t xjh_paged_bytes(const xjh_paged *c);
 /* Rows k, v [T][Hkv*D] (token strides k_tok, v_tok) of `type` (XJ_F32 or the cache's) into their
  * slots: row t goes to offset slot[t] % page of page slot[t] / page, rounded to nearest (beyond the type's
- * range: infinity). A slot outside [0, n_pages * page) skips its row. The slots of a call differ. */
+ * range: infinity). A slot outside [0, n_pages * page) skips its row. The slots of a call differ. T * Hkv is at most 2^26. */
 int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, const void *v, int64_t v_tok, int T,
                     const int32_t *slot, void *stream, char *err, size_t errlen);
 /* Attention of every request's new tokens over its pages: request r's are the rows cu[r] .. cu[r+1]-1
@@ -625,7 +626,8 @@ int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, 
  * weights to 2^-33 of the row's largest) and 24 over bf16.
  * max_new: the largest n, as far as the program knows (0: it does not); it decides which kernel runs, and a
  * larger n is right too. The result does not depend on it, or on the work area, beyond the rounding of sums.
- * T * H is at most 2^28, n_req 65536. */
+ * Scores (scale q.K^T) are below 2^22 in magnitude: beyond, where float scores have no fractions, rows may be 0 or not finite.
+ * T * H is at most 2^27, n_req 65536, min(n_req, T) * Hkv 2^22. */
 int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, int64_t q_head, const void *gate, int64_t g_tok,
                    int64_t g_head, const int32_t *table, int max_blocks, const int32_t *cu, const int32_t *kv_len, int n_req,
                    int T, int max_new, int H, int window, int n_sink, float scale, void *out, int64_t o_tok, void *work,

@@ -153,6 +153,7 @@ struct Item {
 // 2048, 16 heads on 4 of 256: 256 items 30 us, 512 47).
 template <int BM, int BN, bool MERGE>
 __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item &it) {
+#pragma clang fp contract(off)   // the kernels of a call cut alike
     const int lane = threadIdx.x & 63;
     int per = INT32_MAX;
     Seq s{};

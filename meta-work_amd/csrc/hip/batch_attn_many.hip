@@ -458,7 +458,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     const int R0 = it.tile * kManyRows, n_rows = it.s.rows * a.G;
     const int row = R0 + M * w + lane % M, rq = min(row, n_rows - 1), tok = token_of(a, rq), p = it.s.pos0 + tok;
     const int pf = it.s.pos0 + token_of(a, R0), pl = it.s.pos0 + token_of(a, min(R0 + kManyRows, n_rows) - 1);
-    const int wf = it.s.pos0 + token_of(a, min(R0 + M * w, n_rows - 1)), wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
+    const int wl = it.s.pos0 + token_of(a, min(R0 + M * w + M, n_rows) - 1);
     const Range g = range_of<BN>(a, pf, pl);
     const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
     Rows<R, 8> kx[COPIES], vx[COPIES];

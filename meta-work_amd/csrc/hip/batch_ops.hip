@@ -4,7 +4,9 @@
 #include "kernels.h"
 #include "xj_hip.h"
 
+#include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 using namespace xjk;
 
@@ -46,6 +48,15 @@ int row_type(int type) { return type == XJ_F32 ? kRowF32 : type == XJ_F16 ? kRow
 
 constexpr int kMaxReq = 65536;
 
+struct Span {
+    const void *p;
+    uint64_t bytes;
+};
+bool overlap(Span x, Span y) {
+    const uint64_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return a && b && a < b + y.bytes && b < a + x.bytes;
+}
+
 }  // namespace
 
 extern "C" size_t xjh_page_plan_work_bytes(int n_req) {
@@ -71,6 +82,15 @@ extern "C" int xjh_page_plan(const xjh_pages *p, const int32_t *held, const int3
                  (unsigned long long)xjh_page_plan_work_bytes(n_req));
         return -1;
     }
+    // the lengths are read again after the first results are written
+    const uint64_t row = 4 * (uint64_t)n_req, rows = 4 * (uint64_t)T;
+    for (const Span in : {Span{held, row}, Span{n_past, row}, Span{n_new, row}})
+        for (const Span to : {Span{n_free_out, 4}, Span{cu, row + 4}, Span{kv_len, row}, Span{pos, rows}, Span{slot, rows}, Span{status, 16},
+                              Span{work, work_bytes}, Span{p->table, row * p->max_blocks}, Span{p->free_list, 4 * (uint64_t)p->n_pages}})
+            if (overlap(in, to)) {
+                snprintf(err, errlen, "page_plan: the requests' lengths lie in a buffer that is written");
+                return -1;
+            }
     hipStream_t st;
     if (!stream_of(stream, st, "page_plan", err, errlen)) return -1;
     PlanArgs a{};
@@ -96,7 +116,7 @@ extern "C" int xjh_paged_store(const xjh_paged *c, int type, const void *k, int6
                                const int32_t *slot, void *stream, char *err, size_t errlen) {
     PagedStoreArgs a{};
     if (!cache_ok(c, "paged_store", a.c, err, errlen)) return -1;
-    if (T < 0 || (int64_t)T * c->Hkv > (1 << 28) || (type != XJ_F32 && type != c->type)) {
+    if (T < 0 || (int64_t)T * c->Hkv > (1 << 26) || (type != XJ_F32 && type != c->type)) {
         snprintf(err, errlen, "paged_store: bad rows (T=%d, type=%d into a cache of type %d)", T, type, c->type);
         return -1;
     }
@@ -111,7 +131,8 @@ extern "C" int xjh_paged_store(const xjh_paged *c, int type, const void *k, int6
 }
 
 static bool batch_ok(int n_req, int T, int H, int Hkv, int window, int n_sink) {
-    return n_req >= 0 && n_req <= kMaxReq && T >= 0 && Hkv >= 1 && Hkv <= 1024 && H >= Hkv && H % Hkv == 0 && (int64_t)T * H <= (1 << 28) &&
+    return n_req >= 0 && n_req <= kMaxReq && T >= 0 && Hkv >= 1 && Hkv <= 1024 && H >= Hkv && H % Hkv == 0 && (int64_t)T * H <= (1 << 27) &&
+           (int64_t)std::min(n_req, T) * Hkv <= (1 << 22) &&   // a launch has fewer than 2^32 threads
            window >= 0 && n_sink >= 0;
 }
 static bool paged_batch_ok(const xjh_paged *c, int type, int T, int H, int n_req, int max_blocks) {

@@ -1006,7 +1006,8 @@ class PagedKv:
         k, t = _typed(k, (None, self.c.Hkv, self.c.D), "paged_store: k")
         v, tv = _typed(v, k.shape, "paged_store: v")
         slot = _ints(slot, k.shape[0], "paged_store: slot")
-        if t != tv or np.unique(slot[slot >= 0]).size != np.count_nonzero(slot >= 0):
+        there = slot[(slot >= 0) & (slot < self.c.n_pages * self.c.page)]
+        if t != tv or np.unique(there).size != there.size:
             raise XjError("paged_store: k and v of two types, or a slot twice")
         (dk, kp), (dv, vp), (ds, sp), row, err = _opt(k), _opt(v), _opt(slot), self.c.Hkv * self.c.D, _err()
         _check(lib().xjh_paged_store(C.byref(self.c), t, kp, row, vp, row, k.shape[0], sp, None, err, ERR), err, "paged_store")

@@ -154,6 +154,23 @@ def test_plan_refusals():
             xp.PagePool(*bad)
 
 
+def test_plan_refuses_lengths_where_it_writes():
+    L, err = xp.lib(), C.create_string_buffer(512)
+    at = {k: 4096 * (i + 1) for i, k in enumerate(("table", "free", "held", "past", "new", "n_free", "out", "cu", "kv", "pos", "slot", "status", "work"))}
+
+    def plan(**to):
+        b = {k: C.c_void_p(to.get(k, v)) for k, v in at.items()}
+        p = xp.XjhPages(16, 8, 4, b["table"], b["free"])
+        return L.xjh_page_plan(C.byref(p), b["held"], b["past"], b["new"], 5, b["n_free"], b["out"], 7, b["cu"], b["kv"], b["pos"], b["slot"], b["status"],
+                               b["work"], 256, None, err, 512)
+
+    sizes = {"out": 4, "cu": 24, "kv": 20, "pos": 28, "slot": 28, "status": 16, "work": 256, "table": 80, "free": 32}
+    for n in ("held", "past", "new"):
+        for k, size in sizes.items():
+            for where in (at[k], at[k] + size - 4, at[k] - 16):
+                assert plan(**{n: where}) == -1 and b"a buffer that is written" in err.value, (n, k)
+
+
 # ------------------------------------------------------------------ store --
 
 @pytest.mark.gpu
@@ -214,6 +231,7 @@ def test_store_refusals():
         assert store(**bad) == -1 and b"memory" in err.value, bad
     for bad in ({"rows": xp.BF16}, {"rows": xp.Q4_K}, {"T": -1}, {"T": (1 << 28) + 1}):
         assert store(**bad) == -1 and b"bad rows" in err.value, bad
+    assert store(T=(1 << 26) + 1) == -1 and b"bad rows" in err.value
     for bad in ({"x": None}, {"slot": None}):
         assert store(**bad) == -1 and b"no rows" in err.value, bad
     assert store(T=0, x=None, slot=None) == 0
@@ -605,6 +623,8 @@ def test_attention_refusals():
     for bad in ({"q": None}, {"out": None}, {"table": None}, {"cu": None}, {"kv": None}, {"work": C.c_void_p(8)}):
         assert paged(**bad) == -1 and b"buffer is missing" in err.value, bad
     assert paged(T=0, q=None) == 0 and paged(n_req=0, table=None) == 0
+    for bad in ({"T": (1 << 25) + 1}, {"T": 65536, "n_req": 65536, "Hkv": 128, "H": 128, "bytes": 1 << 23}):   # more rows than a launch has room for
+        assert paged(**bad) == -1 and b"bad shape" in err.value, bad
 
     def packed(type=xp.F32, q=one, k=one, v=one, out=one, cu=one, n=1, T=1, H=4, Hkv=2, D=64, window=0, n_sink=0, scale=1.0, work=None):
         return L.xjh_attn_packed(type, q, 256, 64, k, 128, 64, v, 128, 64, None, 0, 0, cu, n, T, H, Hkv, D, window, n_sink, scale, out, 256, work, 0, None,
