@@ -5,7 +5,7 @@
 
 namespace xjk {
 
-__device__ const u32x4 kZeros[1] = {};
+__device__ const u32x4 kZeros[2] = {};
 
 // Lane l: 16 bytes at p to LDS offset off + 16 l; off is uniform over the wavefront.
 __device__ __forceinline__ void dma16(const void *p, uint32_t off) {
@@ -53,7 +53,7 @@ struct WaveRows {
     static constexpr int BN = many_keys(D), NS = D * M / 512, ND = D / M, CH = D / 8, KI = 512 / M;   // KI: keys a step of the second product
     static constexpr int PER = M * M / 64, NB = BN / M, NE = NB * PER;                                  // scores a block, blocks, scores a lane
     static constexpr int PLANE = BN * D * 2, TENSOR = NK * PLANE;
-    static constexpr int QL = D < 256 ? 0 : M == 32 ? 3 : NK == 3 ? 4 : 0;   // steps whose queries' last plane lies in LDS, as far as that is free
+    static constexpr int QL = D < 256 ? 0 : M == 32 ? 3 : NK == 3 ? 7 : 0;   // steps whose queries' last plane lies in LDS, as far as that is free
     typedef float F __attribute__((ext_vector_type(PER)));
     V8<E> q[NS][NP];
     uint32_t q_lds;   // where the wavefront's first QL steps lie
@@ -462,18 +462,17 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     const Range g = range_of<BN>(a, pf, pl);
     const int i0 = part_from(g.n, it.piece, it.pieces), n_tiles = part_from(g.n, it.piece + 1, it.pieces) - i0;
     Rows<R, 8> kx[COPIES], vx[COPIES];
+    // (no branch about a load, and behind the last tile that one again: so it is known how many are on their way)
     auto request = [&](auto values, int t) __attribute__((always_inline)) {
         constexpr bool V = decltype(values)::value;
-        const int j0 = g.tile(i0 + t) * BN;
+        const int j0 = g.tile(i0 + min(t, n_tiles - 1)) * BN;
 #pragma unroll
         for (int n = 0; n < COPIES; n++) {
             const int c = n * 64 * W + tid, r = c / CH, e = c % CH, j = j0 + r;
-            Rows<R, 8> &x = V ? vx[n] : kx[n];
-            x = R(0);
-            if (j <= pl && (!a.window || j > pf - a.window || j < a.sinks)) {   // what no row sees counts for nothing, whatever lies there
-                if (V) x = *(const Rows<R, 8> *)((const R *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * e);
-                else x = *(const Rows<R, 8> *)((const R *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * e);
-            }
+            const R *const from = V ? (const R *)a.v + (it.s.start + j) * a.v_tok + it.head * a.v_head + 8 * e
+                                    : (const R *)a.k + (it.s.start + j) * a.k_tok + it.head * a.k_head + 8 * e;
+            const bool use = j <= pl && (!a.window || j > pf - a.window || j < a.sinks);   // what no row sees counts for nothing, whatever lies there
+            (V ? vx[n] : kx[n]) = *(const __attribute__((address_space(1))) Rows<R, 8> *)(uintptr_t)(use ? from : (const R *)kZeros);
         }
     };
     auto put = [&](auto values) __attribute__((always_inline)) {
@@ -506,15 +505,17 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
     x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
-    if (n_tiles > 0) put(keys);
-    if (n_tiles > 1) request(keys, 1);
+    if (n_tiles > 0) {
+        put(keys);
+        request(keys, 1);
+    }
     auto put_values = [&](int t) __attribute__((always_inline)) {
         put(values);
-        if (t + 1 < n_tiles) request(values, t + 1);
+        request(values, t + 1);
     };
     auto put_keys = [&](int t) __attribute__((always_inline)) {   // the next tile's
-        if (t + 1 < n_tiles) put(keys);
-        if (t + 2 < n_tiles) request(keys, t + 2);
+        put(keys);
+        request(keys, t + 2);
     };
     auto whole_tile = [&](int f, int l, int j0) __attribute__((always_inline)) { return j0 + BN - 1 <= f && (!a.window || j0 > l - a.window || j0 + BN - 1 < a.sinks); };
     auto plain = [&](int t) __attribute__((always_inline)) { return R0 + M * w < n_rows && whole_tile(pf, pl, g.tile(i0 + t) * BN); };
