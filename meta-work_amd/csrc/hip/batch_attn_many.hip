@@ -548,17 +548,20 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
         }
         put_keys(t);
     };
+    const bool early = w >= W / 2;   // of a SIMD's two wavefronts one makes planes while the other has the matrix cores
     int t = 0;
     for (; t < n_tiles && !plain(t); t++) any_tile(t);
     for (; t < n_tiles && plain(t); t++) {
         typename X::F s[NB];
         lds_barrier();
+        if (early) put_values(t);
         x.scores(base, s);
-        put_values(t);
+        if (!early) put_values(t);
         lds_barrier();
+        if (early) put_keys(t);
         x.template raise<false>(s, 0, true);
         x.template weigh<false>(base + TENSOR, s, 0);
-        put_keys(t);
+        if (!early) put_keys(t);
     }
     for (; t < n_tiles; t++) any_tile(t);
     x.finish(a, it, row, tok);
