@@ -440,7 +440,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
 
 // The same with keys and values that pass through registers: rows of any alignment, and floats in NK planes. A tile's values are put into LDS beside
 // its scores, the next one's keys beside its sums, so that what makes planes of them runs beside the matrix cores; two barriers a tile. 2000 float rows of 16 heads on 4 of
-// 256 in five prompts 155 us: 24 operand reads of 1 KB for 48 products of 16 clocks, and a work-group a CU.
+// 256 in five prompts 147 us: 24 operand reads of 1 KB for 48 products of 16 clocks and about as many clocks of vector instructions, a work-group a CU.
 template <int D, class E, int NP, int NK, int RT, int M>
 __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
