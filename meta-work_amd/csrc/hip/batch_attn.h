@@ -168,7 +168,7 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
         if (a.n_req <= 64) {
             const float uncut = wave_sum((float)s.tiles) * a.Hkv;
             for (int k = 0; k < 8 && 2.f * uncut <= (float)a.target; k++) {
-                const float n = wave_sum((float)(s.tiles * (s.len > per ? (int)((uint32_t)(s.len + per - 1) / (uint32_t)per) : 1))) * a.Hkv;
+                const float n = wave_sum((float)s.tiles * fmaxf(ceilf((float)s.len * __builtin_amdgcn_rcpf((float)per)), 1.f)) * a.Hkv;   // about
                 if (n <= (float)a.target) break;
                 per += max(1, per / 16);
             }

@@ -1,5 +1,6 @@
 // Attention for requests of few rows (gfx950): single tokens and short drafts over pages, short prompts. See batch_attn.h.
 #include "batch_attn.h"
+#include <algorithm>
 
 namespace xjk {
 
@@ -294,41 +295,45 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const BatchAttnArgs a) 
     const int tid = threadIdx.x, lane = tid & 63, d = 4 * (tid % TD), tp = tid / TD;
     Item it;
     if (!find_item<BM, BN, true>(a, blockIdx.x, it)) return;
-    const int n_rows = it.s.rows * a.G - it.tile * BM, i = FEW ? blockIdx.y : blockIdx.y * TP + tp;
-    if (i >= n_rows) return;   // FEW: the whole work-group
-    const int64_t at = (int64_t)it.slot * BM + i, step = (int64_t)a.Hkv * BM;
-    float M = -INFINITY, L = 0.f;
-    if (FEW) {
-        for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
-        M = xjd::wave_max(M);
-    } else {
+    const int n_rows = min(it.s.rows * a.G - it.tile * BM, BM);
+    const int64_t step = (int64_t)a.Hkv * BM;
+    for (int i = FEW ? blockIdx.y : blockIdx.y * TP + tp; i < n_rows; i += FEW ? (int)gridDim.y : BM) {   // FEW: the same for the whole work-group
+        const int64_t at = (int64_t)it.slot * BM + i;
+        float M = -INFINITY, L = 0.f;
+        if (FEW) {
+            for (int p = lane; p < it.pieces; p += 64) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
+            M = xjd::wave_max(M);
+        } else {
 #pragma unroll 4
-        for (int p = 0; p < it.pieces; p++) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
-    }
-    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (M != -INFINITY)
-#pragma unroll 4
-        for (int p = FEW ? tp : 0; p < it.pieces; p += FEW ? TP : 1) {
-            const float2 s = *part_stat(a, at + p * step, BM, D);
-            const f32x4 x = *(const f32x4 *)(part_sums(a, at + p * step, D) + d);
-            const float f = __builtin_amdgcn_exp2f(s.x - M);
-            L += f * s.y;
-            y += f * x;
+            for (int p = 0; p < it.pieces; p++) M = fmaxf(M, part_stat(a, at + p * step, BM, D)->x);
         }
-    if constexpr (FEW) {
-        *(f32x4 *)&so[tp][d] = y;
-        if (d == 0) sl[tp] = L;
-        __syncthreads();
-        if (tp) return;
+        f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (M != -INFINITY)
+#pragma unroll 4
+            for (int p = FEW ? tp : 0; p < it.pieces; p += FEW ? TP : 1) {
+                const float2 s = *part_stat(a, at + p * step, BM, D);
+                const f32x4 x = *(const f32x4 *)(part_sums(a, at + p * step, D) + d);
+                const float f = __builtin_amdgcn_exp2f(s.x - M);
+                L += f * s.y;
+                y += f * x;
+            }
+        if constexpr (FEW) {
+            *(f32x4 *)&so[tp][d] = y;
+            if (d == 0) sl[tp] = L;
+            __syncthreads();
+            if (tp == 0)
 #pragma unroll
-        for (int k = 1; k < TP; k++) {
-            y += *(const f32x4 *)&so[k][d];
-            L += sl[k];
+                for (int k = 1; k < TP; k++) {
+                    y += *(const f32x4 *)&so[k][d];
+                    L += sl[k];
+                }
+            __syncthreads();
+            if (tp) continue;
         }
+        const int row = it.tile * BM + i, t = token_of(a, row), h = it.head * a.G + row - t * a.G;
+        finish4(y, M == -INFINITY ? 0.f : 1.f / L, a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr,
+                (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d);
     }
-    const int row = it.tile * BM + i, t = token_of(a, row), h = it.head * a.G + row - t * a.G;
-    finish4(y, M == -INFINITY ? 0.f : 1.f / L, a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr,
-            (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d);
 }
 template <int D, int BM, int BN>
 static void merge(const BatchAttnArgs &a, dim3 grid, hipStream_t st) {
@@ -342,7 +347,9 @@ static void merge(const BatchAttnArgs &a, dim3 grid, hipStream_t st) {
     else merge<D, BM, many_keys(D)>(a, grid, st);
 }
 int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st) {
-    const dim3 grid((unsigned)groups, BM == kFewRows ? BM : BM * a.D / 1024);
+    // Of few rows as many work-groups a tile as it has rows, as far as that is known: each has to find its tile.
+    const int known = a.max_new > 0 ? a.max_new : 2;
+    const dim3 grid((unsigned)groups, BM == kFewRows ? (int)std::min<int64_t>(BM, (int64_t)known * a.G) : BM * a.D / 1024);
     if (BM == kFewRows) {
         if (a.D == 64) merge<kFewRows, 64>(a, grid, st);
         else if (a.D == 128) merge<kFewRows, 128>(a, grid, st);
