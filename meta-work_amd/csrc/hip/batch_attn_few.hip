@@ -283,7 +283,7 @@ int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
 
 // ----------------------------------------------------------------- merge --
 
-// Rows in more than one piece, joined by D / 4 threads each. Of few rows there are many pieces: the work-group takes one row, its threads'
+// Rows in more than one piece, joined by D / 4 threads each. Of few rows there are many pieces: the work-group takes a row at a time, its threads'
 // other runs the next pieces (128 pieces of a row of 256 dims 6 us, 23 by a wavefront a row). Of many rows there are few: the runs take the next rows.
 template <int D, int BM, int BN, int RT>
 __global__ __launch_bounds__(256) void attn_merge_kernel(const BatchAttnArgs a) {
