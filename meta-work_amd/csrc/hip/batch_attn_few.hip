@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     const int t = token_of(a, R0), h = it.head * a.G + R0 - t * a.G, d0 = 4 * (tid & 15);
     const int64_t to = (int64_t)it.slot * 16 + rt;
     if (!whole && d0 == 0) *part_stat(a, to, 16, D) = float2{M, L};
-    R *out = (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d0;
+    R *out = (R *)a.out + (it.s.start + t) * a.o_tok + (int64_t)h * D + d0;
     const R *gate = a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d0 : nullptr;
 #pragma unroll
     for (int d = 0; d < D; d += 64) {
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(const BatchAttnArgs a) 
         }
         const int row = it.tile * BM + i, t = token_of(a, row), h = it.head * a.G + row - t * a.G;
         finish4(y, M == -INFINITY ? 0.f : 1.f / L, a.gate ? (const R *)a.gate + (it.s.start + t) * a.g_tok + h * a.g_head + d : nullptr,
-                (R *)a.out + (it.s.start + t) * a.o_tok + h * D + d);
+                (R *)a.out + (it.s.start + t) * a.o_tok + (int64_t)h * D + d);
     }
 }
 template <int D, int BM, int BN>

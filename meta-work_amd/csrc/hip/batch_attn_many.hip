@@ -260,7 +260,7 @@ struct WaveRows {
             return;
         }
         const int head = it.head * a.G + row - tok * a.G;
-        R *out = (R *)a.out + (it.s.start + tok) * a.o_tok + head * D + 4 * h;
+        R *out = (R *)a.out + (it.s.start + tok) * a.o_tok + (int64_t)head * D + 4 * h;
         const R *gate = a.gate ? (const R *)a.gate + (it.s.start + tok) * a.g_tok + head * a.g_head + 4 * h : nullptr;
         const float inv = m == -INFINITY ? 0.f : 1.f / l;   // a row that has seen nothing is 0
 #pragma unroll

@@ -808,6 +808,33 @@ def test_pages_beyond_four_gigabytes(max_new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_rows_of_more_than_two_billion_elements(packed):
+    """A token of 2^23 heads of 256 and five more, all of one query: the same result in each, the last ones' too."""
+    rng, hip, D, H, n = np.random.default_rng(7), Hip(), 256, (1 << 23) + 5, 20
+    kv = xp.PagedKv(1, D, 32, 1)
+    k, v = (kv_rows(rng, n, 1, D).astype(np.float16) for _ in range(2))
+    q = rng.standard_normal((1, 1, D)).astype(np.float16)
+    if packed:
+        k, v, n = k[:1], v[:1], 1
+    kv.store(k, v, np.arange(n))
+    dq, dk, dv, dt, dc, dl = (xp.Dev(x) for x in (q, k, v, np.zeros((1, 1), np.int32), np.array([0, 1], np.int32), np.array([n], np.int32)))
+    out = xp.Dev(nbytes=2 * H * D)
+    hip("hipMemset", C.c_void_p(out.ptr), C.c_int(0xFF), C.c_size_t(out.nbytes))
+    if packed:
+        _call("xjh_attn_packed", xp.F16, dq.ptr, D, 0, dk.ptr, D, D, dv.ptr, D, D, None, 0, 0, dc.ptr, 1, 1, H, 1, D, 0, 0, D ** -0.5, out.ptr, H * D,
+              None, 0, None)
+    else:
+        _call("xjh_attn_paged", C.byref(kv.c), xp.F16, dq.ptr, D, 0, None, 0, 0, dt.ptr, 1, dc.ptr, dl.ptr, 1, 1, 1, H, 0, 0, D ** -0.5, out.ptr, H * D,
+              None, 0, None)
+    xp.lib().xjh_sync()
+    got = out.get(np.float16, (H, D))
+    check(got[:1], *attend64(value(q), value(k), value(v), n - 1), "f16")
+    for i in range(0, H, 1 << 20):
+        assert np.all(got[i:i + (1 << 20)].view(np.uint16) == got[0].view(np.uint16)), i
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
 def test_packed_of_very_many_short_prompts(rows):
     rng = np.random.default_rng(9)
