@@ -27,9 +27,9 @@ template <>
 struct Op<_Float16> {
     typedef hf8 v8;
     static constexpr uint32_t kExp = 0x7C00, kOne = 0x3C00;
-    // Weights are 2^kLift p to a reference that the running maximum may exceed by kTol before the sums are rescaled to it (on random
+    // Weights are 2^lift p (lift_of) to a reference that the running maximum may exceed by kTol before the sums are rescaled to it (on random
     // scores nearly every tile raises some row's maximum a little), 2^15 at most: bits are lost from 2^-22 of the largest on only.
-    static constexpr float kLift = 8.f, kTol = 7.f;
+    static constexpr float kTol = 7.f;
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -37,7 +37,7 @@ template <>
 struct Op<__bf16> {
     typedef bf8 v8;
     static constexpr uint32_t kExp = 0x7F80, kOne = 0x3F80;
-    static constexpr float kLift = -8.f, kTol = 8.f;   // 1 at most: no sum of theirs is beyond the largest value
+    static constexpr float kTol = 8.f;
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -222,6 +222,15 @@ __device__ __forceinline__ int page_at(const BatchAttnArgs &a, const int32_t *ro
 }
 __device__ __forceinline__ bool sees(const BatchAttnArgs &a, int p, int j) {
     return j <= p && (!a.window || j > p - a.window || j < a.sinks);
+}
+
+// The power of two by which a request's weights are raised. Over f16 values no sum leaves fp32's range. bf16's range is fp32's: a weight is
+// 2^-n at most, where the request sees up to 2^n positions, so that no sum of weighted values is beyond the largest of them. (Small values pay for it: a
+// sum has 24 bits from 2^(n - 93) on, of 16000 positions from 2^-79.)
+template <class E, int BN>
+__device__ __forceinline__ float lift_of(const Seq &s) {
+    if constexpr (__is_same(E, _Float16)) return 8.f;
+    return -(Op<E>::kTol + (32 - __builtin_clz(max(s.len * BN, 2) - 1)));
 }
 
 // State of the splits in the work area: [slots][BM][D] unscaled sums, then [slots][BM] of (the largest score in powers of two,

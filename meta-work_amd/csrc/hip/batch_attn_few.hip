@@ -119,6 +119,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
 #pragma unroll
     for (int d = 0; d < D / 16; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;   // m: a whole number, so that every rescaling is exact
+    const float lift = lift_of<E, kFewKeys>(it.s), raised = __builtin_amdgcn_exp2f(lift);
 
     for (int i = i0; i < i1; i += 4) {
         f32x4 s[2];
@@ -185,7 +186,8 @@ __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
         float pr[8];
 #pragma unroll
         for (int n = 0; n < 8; n++) {
-            pr[n] = __builtin_amdgcn_exp2f(fmaf(s[n >> 2][n & 3], c, Op<E>::kLift - m));
+            // (with 24 bits behind the exponential: a far exponent would round its argument)
+            pr[n] = NP == 3 ? __builtin_amdgcn_exp2f(fmaf(s[n >> 2][n & 3], c, -m)) * raised : __builtin_amdgcn_exp2f(fmaf(s[n >> 2][n & 3], c, lift - m));
             if (!full && !(vis >> n & 1)) pr[n] = 0.f;
             l += pr[n];
         }

@@ -59,6 +59,7 @@ struct WaveRows {
     uint32_t q_lds;   // where the wavefront's first QL steps lie
     F o[ND];
     float m, l, c;   // the reference in powers of two (a whole number, so that every rescaling is exact), the weights' sum, the scale
+    float lift;      // with NP = 3 as a factor behind the exponential: a far exponent would round its argument
     int lane, h;
 
     static __device__ __forceinline__ F mfma(V8<E> a, V8<E> b, F x) {
@@ -79,7 +80,7 @@ struct WaveRows {
     }
 
     // Queries, with the scale's sign; float ones over f16 scaled to 2^14 .. 2^15 before they become planes.
-    __device__ __forceinline__ void start(const R *qp, float scale, uint32_t q_area) {
+    __device__ __forceinline__ void start(const R *qp, float scale, uint32_t q_area, const Seq &seq) {
         lane = threadIdx.x & 63;
         h = lane / M;
         q_lds = q_area + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 * QL;
@@ -115,6 +116,8 @@ struct WaveRows {
             for (int r = 0; r < PER; r++) o[d][r] = 0.f;
         m = -INFINITY;
         l = 0.f;
+        lift = lift_of<E, BN>(seq);
+        if (NP == 3) lift = __builtin_amdgcn_exp2f(lift);
     }
     // Scores of a tile whose keys begin at LDS address kb.
     __device__ __forceinline__ void scores(uint32_t kb, F (&s)[NB]) const {
@@ -156,7 +159,7 @@ struct WaveRows {
     // Weights and sums.
     template <bool MASKED>
     __device__ __forceinline__ void weigh(uint32_t vb, const F (&s)[NB], uint32_t vis) {
-        const float lift = Op<E>::kLift - m;
+        const float zero = NP == 3 ? -m : lift - m;
         // the lane fetches 4 dims of one key of a step's first (second) half for the others
         const int lane = QL ? fresh_lane() : this->lane, h = lane / M, key = 4 * h + (lane >> 2 & 3), low = (M == 32 ? 32 * (lane >> 4 & 1) : 0) + 8 * (lane & 3);
         const uint32_t at = (vb + key * 2 * D) | (low ^ 16 * val_swz(key));
@@ -167,7 +170,8 @@ struct WaveRows {
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 const int e = 8 * u + n;
-                pr[n] = __builtin_amdgcn_exp2f(fmaf(s[e / PER][e % PER], c, lift));
+                pr[n] = __builtin_amdgcn_exp2f(fmaf(s[e / PER][e % PER], c, zero));
+                if (NP == 3) pr[n] *= lift;
                 if (MASKED && !(vis >> e & 1)) pr[n] = 0.f;
                 l += pr[n];
             }
@@ -368,7 +372,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnA
     if (tid == 0) *flag = 0;
     const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
-    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds, it.s);
     wait_vm<0>();
     lds_barrier();
     typename X::F s[NB];
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(8192 / M, 2) void attn_many_any_kernel(const BatchA
     if (tid == 0) *flag = 0;
     const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(marks + many_marks(D) + 16);
     X x;
-    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds);
+    x.start((const R *)a.q + (it.s.start + tok) * a.q_tok + (it.head * a.G + rq - tok * a.G) * a.q_head, a.scale, q_lds, it.s);
     if (n_tiles > 0) {
         put(keys);
         request(keys, 1);

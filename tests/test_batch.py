@@ -868,6 +868,59 @@ def test_paged_rising_scores(rows, cache, max_new):
         assert np.all(np.abs(got - want) <= u * np.abs(want) + (u + 1e-4) * mag + 2.0 ** -24)
 
 
+def _sized(rng, n, Hkv, D, size, scores):
+    """Keys whose scores with queries of 1 in the first dim (0 elsewhere) are `scores` at scale 1, and values of that size, of one sign in the first half."""
+    k = np.zeros((n, Hkv, D), np.float32)
+    k[:, :, 0] = scores[:, None]
+    v = (size * rng.uniform(0.5, 1, (n, Hkv, D))).astype(np.float32)
+    v[:, :, D // 2:] *= np.where(rng.random((n, Hkv, D - D // 2)) < 0.5, -1, 1)
+    return k, v
+
+
+SCORES = {"equal": lambda n: np.zeros(n), "within the reference's tolerance": lambda n: np.where(np.arange(n) < 64, 0, 5.375)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("scores", SCORES)
+@pytest.mark.parametrize("size", [2e38, 1e-30])
+@pytest.mark.parametrize("max_new,work_bytes", [(1, None), (1, 0), (0, None), (0, 0)])
+def test_paged_finite_values_of_any_size(max_new, work_bytes, size, scores, rows):
+    """A mean of finite values is finite, and as near as that of ordinary ones. (1e-30 = 2^-100: what is lost below the smallest number, 2^-126, of
+    900 products with weights of 2^-18 at least is 2^-26 of the result each, and they have the result's size together.)"""
+    def kv(r, n):
+        return _sized(np.random.default_rng(r), n, 2, 64, size, SCORES[scores](n))
+
+    b = Batch(np.random.default_rng(1), [(900, 1), (900, 40), (3, 2)], 4, 2, 64, 16, rows, "bf16", kv=kv, spare=60)
+    b.q = to_type(np.eye(1, 64, dtype=np.float32)[None].repeat(43, 0).repeat(4, 1), rows)
+    b.check(scale=1.0, max_new=max_new, work_bytes=work_bytes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,shift", [("f32", 0), ("bf16", 0), ("bf16", 1)])
+@pytest.mark.parametrize("scores", SCORES)
+@pytest.mark.parametrize("size", [2e38, 1e-30])
+@pytest.mark.parametrize("lens,work", [((50, 14), True), ((900, 1100), True), ((900, 1100), False)])
+def test_packed_finite_values_of_any_size(lens, work, size, scores, rows, shift):
+    rng, T, H, Hkv, D = np.random.default_rng(2), sum(lens), 2, 1, 128
+    q = to_type(np.eye(1, D, dtype=np.float32)[None].repeat(T, 0).repeat(H, 1), rows)
+    kv = [_sized(rng, n, Hkv, D, size, SCORES[scores](n)) for n in lens]
+    k, v = (to_type(np.concatenate([x[i] for x in kv]), rows) for i in range(2))
+    pad = np.zeros(shift, q.dtype)
+    dq, dk, dv, dc = (xp.Dev(x) for x in (q, np.concatenate([pad, k.ravel()]), np.concatenate([pad, v.ravel()]), np.cumsum((0,) + lens).astype(np.int32)))
+    out, t = xp.Dev(nbytes=q.nbytes), IDS[rows]
+    nb = xp.lib().xjh_attn_packed_work_bytes(t, T, H, Hkv, D, 2) if work else 0
+    area, at = xp.Dev(nbytes=max(16, nb)), shift * q.itemsize
+    _call("xjh_attn_packed", t, dq.ptr, H * D, D, dk.ptr + at, D, D, dv.ptr + at, D, D, None, 0, 0, dc.ptr, 2, T, H, Hkv, D, 0, 0, 1.0, out.ptr, H * D,
+          area.ptr, nb, None)
+    xp.lib().xjh_sync()
+    w, lo = [], 0
+    for n in lens:
+        w.append(attend64(*(value(x[lo:lo + n]) for x in (q, k, v)), 0, scale=1.0))
+        lo += n
+    check(out.get(q.dtype, q.shape), *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
 def test_batch_wrappers_refuse_arrays_of_other_shapes():
     x, kv = np.zeros((3, 2, 64), np.float32), xp.PagedKv.__new__(xp.PagedKv)   # (without memory: nothing is launched)
     kv.c = xp.XjhPaged(xp.F16, 2, 64, 16, 4, None, None, 0)
