@@ -632,7 +632,7 @@ int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, i
                    int64_t g_head, const int32_t *table, int max_blocks, const int32_t *cu, const int32_t *kv_len, int n_req,
                    int T, int max_new, int H, int window, int n_sink, float scale, void *out, int64_t o_tok, void *work,
                    size_t work_bytes, void *stream, char *err, size_t errlen);
-/* The work area beyond which nothing is gained for these; 0 when they are not supported. */
+/* The work area beyond which nothing is gained for these and any smaller T and n_req; 0 when they are not supported. */
 size_t xjh_attn_paged_work_bytes(const xjh_paged *c, int type, int T, int H, int n_req, int max_new, int max_blocks);
 /* The same for whole sequences that lie packed in rows: sequence s is the rows cu[s] .. cu[s+1]-1 of q, k, v, gate and
  * out (all of `type`, XJ_F32, XJ_F16 or XJ_BF16), the first at position 0; kv head g of a row at k + row*k_tok +

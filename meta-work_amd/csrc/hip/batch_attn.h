@@ -145,10 +145,13 @@ struct Item {
     Seq s;
     int tile, head, piece, pieces, slot;
 };
+// With U key tiles over all row tiles and heads, u * a.Hkv, a piece is about U / a.target of them and no fewer than a.least, so that the pieces are
+// alike whatever the lengths. At most a.target + (row tiles * heads) items, 2 a.target of them in pieces: a request is cut only if it has
+// more than a piece's tiles.
+__device__ __forceinline__ int piece_of(const BatchAttnArgs &a, float u) { return max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1); }
 // Work item `item` (with MERGE: row tile and head `item` of those in more than one piece); false beyond the last. Every
-// wavefront finds its own, from the lengths, 64 requests at a time: with U key tiles over all row tiles and heads, a piece is about U / a.target
-// of them and no fewer than a.least, so that the pieces are alike whatever the lengths. At most a.target + (row tiles * heads) items,
-// 2 a.target of them in pieces: a request is cut only if it has more than a piece's tiles. Where the uncut items are at most half of a.target, what
+// wavefront finds its own, from the lengths, 64 requests at a time, and of up to 64 requests the tiles of a piece too; of more, they are in a.per.
+// Where the uncut items are at most half of a.target, what
 // the GPU holds at once, longer pieces that it holds at once are better than the last of more (5 rows of 8 requests behind a window of
 // 2048, 16 heads on 4 of 256: 256 items 30 us, 512 47).
 template <int BM, int BN, bool MERGE>
@@ -156,26 +159,22 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
 #pragma clang fp contract(off)   // the kernels of a call cut alike
     const int lane = threadIdx.x & 63;
     int per = INT32_MAX;
-    Seq s{};
-    if (a.target) {
-        float u = 0.f;
-        for (int r0 = 0; r0 < a.n_req; r0 += 64) {
-            s = seq_of<BM, BN>(a, r0 + lane);
-            u += (float)s.tiles * (float)s.len;
-        }
-        u = wave_sum(u);
-        per = max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1);
-        if (a.n_req <= 64) {
-            const float uncut = wave_sum((float)s.tiles) * a.Hkv;
-            for (int k = 0; k < 8 && 2.f * uncut <= (float)a.target; k++) {
-                const float n = wave_sum((float)s.tiles * fmaxf(ceilf((float)s.len * __builtin_amdgcn_rcpf((float)per)), 1.f)) * a.Hkv;   // about
-                if (n <= (float)a.target) break;
-                per += max(1, per / 16);
-            }
-        }
-    }
     const bool once = a.n_req <= 64;
-    if (once && !a.target) s = seq_of<BM, BN>(a, lane);
+    Seq s{};
+    if (once) s = seq_of<BM, BN>(a, lane);
+    if (a.target && once) {
+        per = piece_of(a, wave_sum((float)s.tiles * (float)s.len));
+        const float uncut = wave_sum((float)s.tiles) * a.Hkv;
+        for (int k = 0; k < 8 && 2.f * uncut <= (float)a.target; k++) {
+            const float n = wave_sum((float)s.tiles * fmaxf(ceilf((float)s.len * __builtin_amdgcn_rcpf((float)per)), 1.f)) * a.Hkv;   // about
+            if (n <= (float)a.target) break;
+            per += max(1, per / 16);
+        }
+        if (MERGE && !__any(s.len > per)) return false;   // nothing is cut
+    } else if (a.target) {
+        per = __builtin_amdgcn_readfirstlane(*a.per);
+        if (MERGE && per == INT32_MAX) return false;
+    }
     if (BM == kManyRows && once && a.n_req > 1) {   // the requests that see most first: the last items are then short ones
         const int key = s.tiles ? s.len : -1;
         int rank = 0;
@@ -282,6 +281,7 @@ __device__ __forceinline__ void finish4(f32x4 y, float inv, const R *gate, R *ou
 // Scores that underflow every weight still count as seen: the running maximum (in powers of two, rounded up) stays finite.
 constexpr float kLowest = -1e38f;
 
+int attn_cut_launch(const BatchAttnArgs &a, int BM, hipStream_t st);
 int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st);
 int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
 int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);

@@ -634,7 +634,7 @@ static Run run_of(const BatchAttnArgs &a, bool few, int only) {
     const int held = held_of(a, few);
     const int BN = few ? kFewKeys : many_keys(a.D);
     const int64_t longest = ((a.table ? (int64_t)a.max_blocks << a.lg : a.T) + BN - 1) / BN;
-    r.target = longest <= r.least || r.tiles > 1024 ? 0 : held;   // pieces aimed at
+    r.target = longest <= r.least ? 0 : held;   // pieces aimed at
     r.items = r.target ? std::min(r.tiles * ((longest + r.least - 1) / r.least), r.tiles + r.target) : r.tiles;
     return r;
 }
@@ -651,13 +651,21 @@ static int runs_of(const BatchAttnArgs &a, Run (&r)[2]) {
     r[1] = run_of(a, false, 2);
     return 2;
 }
+// Whether requests may be cut. Packed, a tile of rows sees its own prompt only, whose other tiles are as many: from 1024 tiles on the GPU is full without
+// (8200 rows of 32 heads on 8 of 128 564 us, 573 with the joins that find nothing). Over pages one row may see more than all the others do (100000
+// positions beside 103 requests of 100, 32 heads on 8 of 128: 101 us, 1298 uncut), and a join that finds nothing costs 2 to 8 us (8192 rows in one request 733
+for 724, 32 single tokens of 32 kv heads at 1000 positions 98 for 96).
+static bool may_cut(const BatchAttnArgs &a, const Run &r) { return a.table || r.tiles <= 1024; }
+constexpr int kPer = 64;   // floats in front of the partials, whose rows begin at cache lines then: a.per
 static int64_t slot_floats(const BatchAttnArgs &a, int BM) { return (int64_t)BM * (a.D + 2); }
 
 int64_t batch_attn_part_floats(const BatchAttnArgs &a) {
-    Run r[2];
     int64_t most = 0;
-    for (int i = 0, n = runs_of(a, r); i < n; i++)
-        if (r[i].target) most = std::max(most, std::min<int64_t>(r[i].items, 2 * r[i].target) * slot_floats(a, r[i].BM));
+    for (const bool few : {true, false}) {   // a smaller batch may run in the other tiles
+        if (few ? !a.table && a.type == kRowF32 : a.table && (int64_t)(a.max_new > 0 ? a.max_new : a.T) * a.G <= kFewLimit) continue;
+        const Run r = run_of(a, few, 0);
+        if (r.target) most = std::max(most, kPer + std::min<int64_t>(r.items, 2 * r.target) * slot_floats(a, r.BM));
+    }
     return most;
 }
 
@@ -669,10 +677,13 @@ int batch_attn_launch(const BatchAttnArgs &args, int64_t part_floats, hipStream_
         if (!r.tiles) continue;
         BatchAttnArgs a = args;
         a.only = r.only;
-        a.slots = (int)std::min<int64_t>(part_floats / slot_floats(a, r.BM), 1 << 20);
+        a.slots = may_cut(a, r) ? (int)std::min<int64_t>(std::max<int64_t>(part_floats - kPer, 0) / slot_floats(a, r.BM), 1 << 20) : 0;
+        a.per = (int32_t *)args.part;
+        a.part = args.part + kPer;
         // at most 2 a.target items are in pieces
         a.target = a.slots >= std::min<int64_t>(r.items, 2 * r.target) ? r.target : std::min(r.target, a.slots / 2);
         a.least = r.least;
+        if (a.target && a.n_req > 64 && attn_cut_launch(a, r.BM, st)) return -1;
         const int64_t items = a.target ? std::min(r.items, r.tiles + a.target) : r.tiles;
         if (r.BM == kFewRows ? attn_few_launch(a, items, st) : attn_many_launch(a, items, st)) return -1;
         if (a.target && attn_merge_launch(a, r.BM, std::min<int64_t>(r.tiles, a.target), st)) return -1;

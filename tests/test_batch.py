@@ -389,6 +389,35 @@ def test_paged_many_requests(n_req, max_new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("work_bytes", [None, 0, 16, 200000])
+@pytest.mark.parametrize("max_new", [1, 0])
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("n_req,H,Hkv,D", [(250, 32, 8, 64), (40, 32, 32, 128), (70, 16, 4, 256)])
+def test_paged_long_request_among_many_short_ones(n_req, H, Hkv, D, rows, cache, max_new, work_bytes):
+    """More rows than the GPU holds at once, or than a wavefront looks at together; one of the requests is cut, in a mixed batch another of many rows too."""
+    rng = np.random.default_rng(n_req)
+    lens = [(int(n), 1) for n in rng.integers(1, 60, n_req)]
+    lens[n_req // 3] = (6000, 1)
+    if max_new == 0:
+        lens[n_req // 2] = (1500, 40)
+    Batch(rng, lens, H, Hkv, D, 32, rows, cache, spare=9).check(max_new=max_new, work_bytes=work_bytes)
+
+
+def test_work_areas_serve_smaller_batches():
+    """A work area asked for the largest step is as much as any smaller one's. A batch past the size at which the GPU is full without cutting has one too."""
+    L, sizes = xp.lib(), [1, 2, 3, 8, 9, 30, 63, 64, 65, 103, 104, 105, 250, 505, 511, 512, 513, 1000, 1024, 1025, 3000, 9000]
+    for t, H, Hkv, D in ((xp.BF16, 32, 8, 128), (xp.F32, 16, 4, 256), (xp.F16, 2, 1, 64), (xp.BF16, 16, 8, 128), (xp.F16, 32, 32, 64)):
+        c = xp.XjhPaged(xp.F16 if t == xp.F32 else t, Hkv, D, 32, 1000, None, None, 0)
+        paged = {}
+        for most in (0, 1, 5, 100):
+            n = paged[most] = [[L.xjh_attn_paged_work_bytes(C.byref(c), t, T, H, r, most, 4096) for T in sizes] for r in sizes]
+            n = np.array(n, np.int64)
+            assert n.min() > 0 and np.all(np.diff(n, axis=0) >= 0) and np.all(np.diff(n, axis=1) >= 0), (t, H, Hkv, D, most)
+        n = np.array([[L.xjh_attn_packed_work_bytes(t, T, H, Hkv, D, r) for T in sizes] for r in sizes], np.int64)
+        assert n[-1, -1] > 0 and np.all(np.diff(n, axis=0) >= 0) and np.all(np.diff(n, axis=1) >= 0), (t, H, Hkv, D)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("max_new", [1, 0])
 def test_paged_rows_before_the_first_position_and_of_no_request(max_new):
     """More new rows than positions: those before position 0 see nothing and are 0; rows past the last request keep their values."""
@@ -744,6 +773,51 @@ def test_captured_steps_of_a_batch(D, Hkv, page, max_new, window, n_sink):
         hip("hipGraphExecDestroy", g)
     for st in streams:
         hip("hipStreamDestroy", st)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [60, 1, 0])   # 1: told wrongly
+def test_captured_step_of_many_slots(max_new):
+    """A step of 70 slots, most of them idle: one request grows until it is cut, shrinks, ends and begins anew; replayed beside eager work. The attention is
+    compared over the keys and values that lie in the pages: a key that the rotation's own rounding takes over a border of f16 moves the
+    scores of a request of two or three positions by more than all else does. Those keys are their rotated rows', rounded once: half a step of f16, and
+    the rotation's four roundings in fp32 of elements up to 6."""
+    rng, hip = np.random.default_rng(70), Hip()
+    s = _Step(70, 90, 4, 2, 64, 16, 70 * 40, 40, max_new=max_new)
+    st = hip.stream()
+    graph = hip.capture(st, s.run)
+    past = np.zeros(70, int)
+    for i, grow in enumerate((60, 60, 60, 60, 1, 60, 60, 1, 1, 60, 1, 1, 0, 1, 50)):
+        held = past.copy()
+        if i == 8:
+            past[17] -= 170
+        if i == 12:
+            past[17] = 0
+        new = np.zeros(70, int)
+        new[rng.integers(0, 70, 25)] += 1
+        new[17] = grow
+        s.feed(rng, held.tolist(), past.tolist(), new.tolist())
+        hip.sync()
+        hip("hipGraphLaunch", graph, st)
+        xp.norm(rng.standard_normal((3, 64)).astype(np.float32), None, 1, 1e-6)
+        hip.sync()
+        assert s.d["status"].get(np.int32, (4,)).tolist() == [0, 0, 0, new.sum()]
+        got, q, table, pages = s.out.get(np.float32, (90, 4, 64)), s.qr.get(np.float32, (90, 4, 64)), s.pool.table, s.kv.pages()
+        want, t = [], 0
+        for r in np.flatnonzero(new):
+            n, m = past[r] + new[r], new[r]
+            k, v = (x[table[r, :up(n, 16)]].transpose(0, 2, 1, 3).reshape(-1, 2, 64)[:n].astype(np.float64) for x in pages)
+            turned = rope64(s.x[1][t:t + m], s.cfg, past[r] + np.arange(m))[0]
+            assert np.all(np.abs(k[past[r]:] - turned) <= 2.0 ** -11 * np.abs(turned) + 4 * 6 * 2.0 ** -24 + 2.0 ** -25)
+            assert np.array_equal(v[past[r]:], s.x[2][t:t + m].astype(np.float16))
+            assert np.all(np.abs(q[t:t + m] - rope64(s.x[0][t:t + m], s.cfg, past[r] + np.arange(m))[0]) <= 4 * 6 * 2.0 ** -24)
+            want.append(attend64(q[t:t + m].astype(np.float64), k, v, past[r]))
+            t += m
+        check(got[:t], *(np.concatenate([x[i] for x in want]) for i in range(2)), "f32")
+        assert np.all(got[t:] == 7)
+        past = past + new
+    hip("hipGraphExecDestroy", graph)
+    hip("hipStreamDestroy", st)
 
 
 @pytest.mark.gpu
