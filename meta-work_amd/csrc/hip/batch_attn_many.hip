@@ -654,7 +654,7 @@ static int runs_of(const BatchAttnArgs &a, Run (&r)[2]) {
 // Whether requests may be cut. Packed, a tile of rows sees its own prompt only, whose other tiles are as many: from 1024 tiles on the GPU is full without
 // (8200 rows of 32 heads on 8 of 128 564 us, 573 with the joins that find nothing). Over pages one row may see more than all the others do (100000
 // positions beside 103 requests of 100, 32 heads on 8 of 128: 101 us, 1298 uncut), and a join that finds nothing costs 2 to 8 us (8192 rows in one request 733
-for 724, 32 single tokens of 32 kv heads at 1000 positions 98 for 96).
+// for 724, 32 single tokens of 32 kv heads at 1000 positions 98 for 96).
 static bool may_cut(const BatchAttnArgs &a, const Run &r) { return a.table || r.tiles <= 1024; }
 constexpr int kPer = 64;   // floats in front of the partials, whose rows begin at cache lines then: a.per
 static int64_t slot_floats(const BatchAttnArgs &a, int BM) { return (int64_t)BM * (a.D + 2); }
