@@ -621,11 +621,15 @@ int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, 
  * xjh_pages (max_blocks * page <= 2^30; kv_len beyond that counts as it); requests may share pages.
  * A table entry outside [0, n_pages) stands for positions that are not seen. What lies at positions
  * that a row does not see, NaN too, counts for nothing in it; a value that it sees and is not finite leaves it not finite.
- * Products of 16-bit elements are exact and sums are fp32. Weights enter with the cache's bits; with float rows the
+ * Products of 16-bit elements are exact and sums are fp32. With 16-bit rows the weights are rounded to the cache's bits
+ * by the kernel for many rows and kept to twice as many by that for few. With float rows the
  * queries and the weights enter with 22 bits over f16 (queries to 2^-40 of the row's largest element,
  * weights to 2^-33 of the row's largest) and 24 over bf16.
  * max_new: the largest n, as far as the program knows (0: it does not); it decides which kernel runs, and a
- * larger n is right too. The result does not depend on it, or on the work area, beyond the rounding of sums.
+ * larger n is right too. With max_new * H/Hkv up to 32, or T * H/Hkv where it is 0, that for few rows runs for all requests, otherwise for those of
+ * at most 32 rows a kv head, if there is more than one request. By that, by the other requests and by the work area the result changes with the rounding
+ * of sums, and with 16-bit rows, where the kernel changes, with that of the weights: by half a step of the type (f16 2^-11, bf16 2^-8) of
+ * sum_j p_j |v_j| at most, before the result is rounded.
  * Scores (scale q.K^T) are below 2^22 in magnitude: beyond, where float scores have no fractions, rows may be 0 or not finite.
  * T * H is at most 2^27, n_req 65536, min(n_req, T) * Hkv 2^22. */
 int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, int64_t q_head, const void *gate, int64_t g_tok,
@@ -636,7 +640,8 @@ int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, i
 size_t xjh_attn_paged_work_bytes(const xjh_paged *c, int type, int T, int H, int n_req, int max_new, int max_blocks);
 /* The same for whole sequences that lie packed in rows: sequence s is the rows cu[s] .. cu[s+1]-1 of q, k, v, gate and
  * out (all of `type`, XJ_F32, XJ_F16 or XJ_BF16), the first at position 0; kv head g of a row at k + row*k_tok +
- * g*k_head, D elements (64, 128 or 256). Float queries, keys, values and weights enter with 24 bits. Rows of k and v
+ * g*k_head, D elements (64, 128 or 256). Float queries, keys, values and weights enter with 24 bits; the weights of 16-bit rows as
+ * there, T, n_seq and the heads deciding which kernel runs (that for few rows up to some hundred rows). Rows of k and v
  * whose addresses are multiples of 16 bytes are read faster. */
 int xjh_attn_packed(int type, const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
                     const void *v, int64_t v_tok, int64_t v_head, const void *gate, int64_t g_tok, int64_t g_head,

@@ -555,6 +555,28 @@ def test_paged_same_bits_again_and_in_any_batch(max_new, work_bytes):
         assert np.array_equal(one, b.attend(max_new=max_new, work_bytes=work_bytes))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("others", [2, 80])
+@pytest.mark.parametrize("rows,cache", PAIRS)
+def test_paged_request_alone_and_in_any_batch(rows, cache, others):
+    """A request's rows by themselves, in a batch, and with other kernels and work areas: each result is rounded once (u of it), weights are rounded to u in
+    one kernel and not in the other (u of sum p |v|), and fp32 sums are 1e-5 of that apart from the exact ones, as above."""
+    lens = [(3000, 1), (900, 60), (17, 3), (2500, 9)] + [(40, 1)] * others
+    b = Batch(np.random.default_rng(2), lens, 8, 2, 128, 16, rows, cache)   # (60 tokens: 240 rows a kv head; 9: 36)
+    want, mag = b.want()
+    batches = [value(b.attend(max_new=m, work_bytes=w)).reshape(want.shape) for m, w in ((None, None), (0, None), (1, None), (None, 0), (1, 100000))]
+    u, t = HALF[rows], 0
+    for r, (n, m) in enumerate(lens[:5]):
+        rs = slice(t, t + m)
+        for most in (m, 0, 1):
+            one = value(b.cache.attend(b.q[rs], b.table[r:r + 1], [0, m], [n], max_new=most)).reshape(m, 8, 128)
+            for got in batches:
+                assert np.all(np.abs(one - got[rs]) <= 2 * u * np.abs(want[rs]) + (u + 2e-5) * mag[rs] + (2.0 ** -24 if rows == "f16" else 0)), (r, most)
+            if m * 4 <= 32 or most == 1:   # the kernel for few rows in both: no weights' rounding
+                assert np.all(np.abs(one - batches[2][rs]) <= 2 * u * np.abs(want[rs]) + (u * u + 2e-5) * mag[rs] + (2.0 ** -24 if rows == "f16" else 0)), (r, most)
+        t += m
+
+
 PROMPTS = [300, 1, 0, 33, 128, 5, 129, 64, 0]
 
 
