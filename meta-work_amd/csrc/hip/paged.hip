@@ -163,9 +163,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs a) {
 }
 
 int page_plan_launch(const PlanArgs &a, hipStream_t st) {
-    // A second launch costs what a thread's four rows do (8 requests of a token each 5.2 + 2.9 us in two, 4.2 in one). The pages that move are not known here: of few requests
-    // and rows they are few, or long prompts', whose rows are many.
-    if (a.n_req <= 256 && a.T <= 4 * kPlanThreads) {
+    // A second launch costs what a thread's four rows do (8 requests of a token each 5.2 + 2.9 us in two, 4.2 in one). The pages that move are not known here:
+    // those taken are few where the rows are, but requests that end give back all of theirs, a thread some 0.7 us each (8 of 131000 positions in pages
+    // of 16: 52 us a call, 10.5 in two launches; 64 of 4000 20 and 10.5). So one launch only where there are no more pages than cost some 50 us.
+    const int64_t pages = std::min<int64_t>(a.n_pages, (int64_t)a.n_req * a.max_blocks);
+    if (a.n_req <= 256 && a.T <= 4 * kPlanThreads && pages <= 64 * kPlanThreads) {
         plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
     } else {
         plan_scan_kernel<<<1, kPlanThreads, 0, st>>>(a);

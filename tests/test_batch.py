@@ -131,6 +131,20 @@ def test_plan_many_requests(n_req):
     same_plan(pool, ref, n_past=past.tolist(), n_new=[1] * n_req, held=new.tolist())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_req,blocks", [(8, 8192), (8, 8193), (200, 500)])
+def test_plan_small_steps_that_give_many_pages_back(n_req, blocks):
+    """Long requests end while others take a token or a prompt, on both sides of 65536 pages."""
+    L = blocks * 16
+    pool, ref = xp.PagePool(16, n_req * blocks, n_req, blocks), RefPool(16, n_req * blocks, n_req, blocks)
+    full = [L - 5 * r for r in range(n_req)]
+    same_plan(pool, ref, n_past=[0] * n_req, n_new=full, T=50)
+    end = [r % 4 != 1 for r in range(n_req)]
+    past = [0 if e else n for e, n in zip(end, full)]
+    got = same_plan(pool, ref, n_past=past, n_new=[17 if r == 2 else not e for r, e in enumerate(end)], held=full)
+    assert got["status"][0] == 0 and pool.free.size > n_req * blocks // 2
+
+
 def test_plan_refusals():
     L, err, one = xp.lib(), C.create_string_buffer(512), C.c_void_p(16)
 
