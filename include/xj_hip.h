@@ -624,7 +624,7 @@ int xjh_paged_store(const xjh_paged *c, int type, const void *k, int64_t k_tok, 
  * Products of 16-bit elements are exact and sums are fp32. With 16-bit rows the weights are rounded to the cache's bits
  * by the kernel for many rows and kept to twice as many by that for few. With float rows the
  * queries and the weights enter with 22 bits over f16 (queries to 2^-40 of the row's largest element,
- * weights to 2^-33 of the row's largest) and 24 over bf16.
+ * weights to 2^-33 of the row's largest) and 24 over bf16. A sum over 2^n positions of bf16 values keeps its bits down to 2^(n - 93).
  * max_new: the largest n, as far as the program knows (0: it does not); it decides which kernel runs, and a
  * larger n is right too. With max_new * H/Hkv up to 32, or T * H/Hkv where it is 0, that for few rows runs for all requests, otherwise for those of
  * at most 32 rows a kv head, if there is more than one request. By that, by the other requests and by the work area the result changes with the rounding
@@ -640,8 +640,8 @@ int xjh_attn_paged(const xjh_paged *c, int type, const void *q, int64_t q_tok, i
 size_t xjh_attn_paged_work_bytes(const xjh_paged *c, int type, int T, int H, int n_req, int max_new, int max_blocks);
 /* The same for whole sequences that lie packed in rows: sequence s is the rows cu[s] .. cu[s+1]-1 of q, k, v, gate and
  * out (all of `type`, XJ_F32, XJ_F16 or XJ_BF16), the first at position 0; kv head g of a row at k + row*k_tok +
- * g*k_head, D elements (64, 128 or 256). Float queries, keys, values and weights enter with 24 bits; the weights of 16-bit rows as
- * there, T, n_seq and the heads deciding which kernel runs (that for few rows up to some hundred rows). Rows of k and v
+ * g*k_head, D elements (64, 128 or 256). Float queries, keys, values and weights enter with 24 bits, and their sums keep as many as those
+ * over bf16 pages; the weights of 16-bit rows are rounded as there, by the kernel that T, n_seq and the heads select (that for few rows up to some hundred rows). Rows of k and v
  * whose addresses are multiples of 16 bytes are read faster. */
 int xjh_attn_packed(int type, const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
                     const void *v, int64_t v_tok, int64_t v_head, const void *gate, int64_t g_tok, int64_t g_head,

@@ -8,8 +8,8 @@ namespace xjk {
 // Keys come straight into the operand's registers (key li, dims 32 s + 8 kq ..); values are read as
 // the lane's VW dims of the eight keys whose weights it holds and turned in registers. A tile's keys are requested as soon as the scores of
 // the one before are there, its values behind that one's sums. Weights enter in two planes at least (in the kernel for
-// many rows in one, of 16 bits): the matrix cores wait for memory here. A token at 131000 positions of 4 heads of 256 in f16, 537 MB: 95 us (5.6 TB/s); 64 tokens at 1 to 16000 positions of
-// 8 heads of 128 in bf16, 502 MB: 107 us.
+// many rows those of 16-bit rows in one): the matrix cores wait for memory here. By the trace a token at 131000 positions of 4 heads of 256 in f16, 537 MB,
+// takes 96 us (5.6 TB/s), 64 tokens at 1 to 16000 positions of 8 heads of 128 in bf16, 502 MB, 110 us.
 template <int D, class E, int NP, int RT, bool PAGES>
 __global__ __launch_bounds__(256) void attn_few_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
