@@ -150,8 +150,8 @@ struct Item {
 // more than a piece's tiles.
 __device__ __forceinline__ int piece_of(const BatchAttnArgs &a, float u) { return max(a.least, (int)fminf(u * a.Hkv * 1.0001f / a.target, 1e9f) + 1); }
 // Work item `item` (with MERGE: row tile and head `item` of those in more than one piece); false beyond the last. Every
-// wavefront finds its own, from the lengths, 64 requests at a time, and of up to 64 requests the tiles of a piece too; of more, they are in a.per.
-// Where the uncut items are at most half of a.target, what
+// wavefront finds its own, from the lengths, 64 requests at a time, and the tiles of a piece too, if they are not in a.per. (Of more than 64 requests those of less
+// than two pieces are not worth a cut: 5 rows of 200 requests of up to 2000 positions, 32 heads on 8 of 128: 103 us, 117 where some are cut.) Where the uncut items are at most half of a.target, what
 // the GPU holds at once, longer pieces that it holds at once are better than the last of more (5 rows of 8 requests behind a window of
 // 2048, 16 heads on 4 of 256: 256 items 30 us, 512 47).
 template <int BM, int BN, bool MERGE>
@@ -162,7 +162,23 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
     const bool once = a.n_req <= 64;
     Seq s{};
     if (once) s = seq_of<BM, BN>(a, lane);
-    if (a.target && once) {
+    if (a.target && a.per) {
+        per = __builtin_amdgcn_readfirstlane(*a.per);
+        if (MERGE && per == INT32_MAX) return false;   // nothing is cut
+    } else if (a.target && !once) {
+        float u = 0.f;
+        int most = 0;
+        for (int r0 = 0; r0 < a.n_req; r0 += 64) {
+            s = seq_of<BM, BN>(a, r0 + lane);
+            u += (float)s.tiles * (float)s.len;
+            most = max(most, s.len);
+        }
+        per = piece_of(a, wave_sum(u));
+        if (!__any(most > 2 * per)) {
+            if (MERGE) return false;
+            per = INT32_MAX;
+        }
+    } else if (a.target) {
         per = piece_of(a, wave_sum((float)s.tiles * (float)s.len));
         const float uncut = wave_sum((float)s.tiles) * a.Hkv;
         for (int k = 0; k < 8 && 2.f * uncut <= (float)a.target; k++) {
@@ -170,10 +186,7 @@ __device__ __forceinline__ bool find_item(const BatchAttnArgs &a, int item, Item
             if (n <= (float)a.target) break;
             per += max(1, per / 16);
         }
-        if (MERGE && !__any(s.len > per)) return false;   // nothing is cut
-    } else if (a.target) {
-        per = __builtin_amdgcn_readfirstlane(*a.per);
-        if (MERGE && per == INT32_MAX) return false;
+        if (MERGE && !__any(s.len > per)) return false;
     }
     if (BM == kManyRows && once && a.n_req > 1) {   // the requests that see most first: the last items are then short ones
         const int key = s.tiles ? s.len : -1;

@@ -285,9 +285,8 @@ int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st) {
 
 // ------------------------------------------------------------------- cut --
 
-// The tiles of a piece (piece_of) of more than 64 requests, or that none is cut. Where every wavefront of the other kernels sums the requests
-// for itself, 104 to 1000 requests of 100 positions take 7 to 126 us more; this launch and that of a join that finds nothing take 4 to 13. Requests of less
-// than two pieces are not worth it (5 rows of 200 requests of up to 2000 positions, 32 heads on 8 of 128: 103 us, 117 where some are cut).
+// The tiles of a piece (piece_of) of more than 64 requests, or that none is cut, as find_item finds them. Where every wavefront of the other kernels sums the
+// requests for itself, 104 to 1000 requests of 100 positions take 7 to 126 us more; this launch and that of a join that finds nothing take 4 to 13.
 template <int BM, int BN>
 __global__ __launch_bounds__(1024) void attn_cut_kernel(const BatchAttnArgs a) {
     __shared__ float su[16];

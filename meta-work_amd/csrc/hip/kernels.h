@@ -455,7 +455,7 @@ struct BatchAttnArgs {
     int32_t window, sinks;
     float scale;
     float *part;                                  // split partials
-    int32_t *per;                                 // set by batch_attn_launch: where attn_cut_kernel leaves the key tiles of a piece, of more than 64 requests
+    int32_t *per;                                 // set by batch_attn_launch: where attn_cut_kernel leaves the key tiles of a piece, or none
     int32_t target, least, slots;                 // set by batch_attn_launch: pieces aimed at, key tiles a piece at least, the partials' room
     int32_t only;                                 // and: requests of few rows (1), of many (2), all (0)
 };

@@ -813,24 +813,25 @@ def test_captured_steps_of_a_batch(D, Hkv, page, max_new, window, n_sink):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_new", [60, 1, 0])   # 1: told wrongly
-def test_captured_step_of_many_slots(max_new):
-    """A step of 70 slots, most of them idle: one request grows until it is cut, shrinks, ends and begins anew; replayed beside eager work. The attention is
+@pytest.mark.parametrize("slots", [70, 140])
+def test_captured_step_of_many_slots(slots, max_new):
+    """A step of 70 and of 140 slots, most of them idle: one request grows until it is cut, shrinks, ends and begins anew; replayed beside eager work. The attention is
     compared over the keys and values that lie in the pages: a key that the rotation's own rounding takes over a border of f16 moves the
     scores of a request of two or three positions by more than all else does. Those keys are their rotated rows', rounded once: half a step of f16, and
     the rotation's four roundings in fp32 of elements up to 6."""
     rng, hip = np.random.default_rng(70), Hip()
-    s = _Step(70, 90, 4, 2, 64, 16, 70 * 40, 40, max_new=max_new)
+    s = _Step(slots, 90, 4, 2, 64, 16, slots * 40, 40, max_new=max_new)
     st = hip.stream()
     graph = hip.capture(st, s.run)
-    past = np.zeros(70, int)
+    past = np.zeros(slots, int)
     for i, grow in enumerate((60, 60, 60, 60, 1, 60, 60, 1, 1, 60, 1, 1, 0, 1, 50)):
         held = past.copy()
         if i == 8:
             past[17] -= 170
         if i == 12:
             past[17] = 0
-        new = np.zeros(70, int)
-        new[rng.integers(0, 70, 25)] += 1
+        new = np.zeros(slots, int)
+        new[rng.integers(0, slots, 25)] += 1
         new[17] = grow
         s.feed(rng, held.tolist(), past.tolist(), new.tolist())
         hip.sync()
