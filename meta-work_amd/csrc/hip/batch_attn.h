@@ -295,7 +295,7 @@ __device__ __forceinline__ void finish4(f32x4 y, float inv, const R *gate, R *ou
 constexpr float kLowest = -1e38f;
 
 int attn_cut_launch(const BatchAttnArgs &a, int BM, hipStream_t st);
-int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, hipStream_t st);
+int attn_merge_launch(const BatchAttnArgs &a, int BM, int64_t groups, bool rare, hipStream_t st);
 int attn_few_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
 int attn_many_launch(const BatchAttnArgs &a, int64_t items, hipStream_t st);
 

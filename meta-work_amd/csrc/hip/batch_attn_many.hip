@@ -653,11 +653,9 @@ static int runs_of(const BatchAttnArgs &a, Run (&r)[2]) {
     r[1] = run_of(a, false, 2);
     return 2;
 }
-// Whether requests may be cut. Packed, a tile of rows sees its own prompt only, whose other tiles are as many: from 1024 tiles on the GPU is full without
-// (8200 rows of 32 heads on 8 of 128 564 us, 573 with the joins that find nothing). Over pages one row may see more than all the others do (100000
-// positions beside 103 requests of 100, 32 heads on 8 of 128: 101 us, 1298 uncut), and a join that finds nothing costs 2 to 8 us (8192 rows in one request 733
-// for 724, 32 single tokens of 32 kv heads at 1000 positions 98 for 96).
-static bool may_cut(const BatchAttnArgs &a, const Run &r) { return a.table || r.tiles <= 1024; }
+// (Requests may be cut whatever the bounds of the call say: a batch of 8200 rows may be one prompt among a thousand empty ones, 2 heads on 1 of 128: 97 us, 204
+// uncut; over pages one row may see more than all the others do, 100000 positions beside 103 requests of 100, 32 heads on 8 of 128: 101 us, 1298 uncut. A join that
+// finds nothing costs 2 to 6 us.)
 constexpr int kPer = 64;   // floats in front of the partials, whose rows begin at cache lines then: a.per
 static int64_t slot_floats(const BatchAttnArgs &a, int BM) { return (int64_t)BM * (a.D + 2); }
 
@@ -679,7 +677,7 @@ int batch_attn_launch(const BatchAttnArgs &args, int64_t part_floats, hipStream_
         if (!r.tiles) continue;
         BatchAttnArgs a = args;
         a.only = r.only;
-        a.slots = may_cut(a, r) ? (int)std::min<int64_t>(std::max<int64_t>(part_floats - kPer, 0) / slot_floats(a, r.BM), 1 << 20) : 0;
+        a.slots = (int)std::min<int64_t>(std::max<int64_t>(part_floats - kPer, 0) / slot_floats(a, r.BM), 1 << 20);
         // 65 to 128 requests whose tiles the GPU holds at once sum for themselves side by side (66 to 100 of 2 heads on 1 of 128 12 to 20 us, 13.5 to 21.5 with the
         // launch; 200 prompts of 20 tokens 27 without, 19 with it).
         a.per = a.n_req > 128 || (a.n_req > 64 && r.tiles > 256) ? (int32_t *)args.part : nullptr;
@@ -690,7 +688,7 @@ int batch_attn_launch(const BatchAttnArgs &args, int64_t part_floats, hipStream_
         if (a.target && a.per && attn_cut_launch(a, r.BM, st)) return -1;
         const int64_t items = a.target ? std::min(r.items, r.tiles + a.target) : r.tiles;
         if (r.BM == kFewRows ? attn_few_launch(a, items, st) : attn_many_launch(a, items, st)) return -1;
-        if (a.target && attn_merge_launch(a, r.BM, std::min<int64_t>(r.tiles, a.target), st)) return -1;
+        if (a.target && attn_merge_launch(a, r.BM, std::min<int64_t>(r.tiles, a.target), r.tiles > 1024, st)) return -1;
     }
     return 0;
 }

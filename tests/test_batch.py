@@ -947,6 +947,23 @@ def test_rows_of_more_than_two_billion_elements(packed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("D,at", [(64, 0), (128, 900), (256, 1199)])
+def test_packed_long_prompt_among_empty_ones(D, at, rows):
+    """A batch that may have more row tiles than the GPU holds and has a dozen: it is cut."""
+    rng = np.random.default_rng(D)
+    lens = np.zeros(1200, int)
+    lens[[at, 500]] = 1500, 60
+    T, cu = int(lens.sum()), np.cumsum(np.concatenate([[0], lens]))
+    q = to_type((rng.standard_normal((T, 2, D)) * 1.5).astype(np.float32), rows)
+    k, v = (to_type(kv_rows(rng, T, 1, D), rows) for _ in range(2))
+    w = [attend64(*(value(x[a:b]) for x in (q, k, v)), 0) for a, b in zip(cu, cu[1:]) if b > a]
+    for work_bytes in (None, 0, 500000):
+        got = xp.attn_packed(q, k, v, cu, work_bytes=work_bytes)
+        check(got, *(np.concatenate([x[i] for x in w]) for i in range(2)), rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["f16", "bf16", "f32"])
 def test_packed_of_very_many_short_prompts(rows):
     rng = np.random.default_rng(9)
     lens = rng.integers(0, 4, 3000)
