@@ -283,7 +283,7 @@ constexpr int many_marks(int D) { return many_keys(D) * D / 8; }
 // A tile of 128 rows, M a wavefront; tiles of BN keys and values pass through LDS. Each tile's sums are followed by the next one's scores, whose keys are
 // there already, and the keys behind it and its values are on their way: a barrier a tile. Two work-groups a CU: while one's wavefront has the vector
 // units for its softmax, the other's has the matrix cores. Bound by a wavefront's chain of operand reads, products and softmax: 8200 rows of 32 heads on 8
-// of 128 in bf16 554 us (947 TFLOP/s), 512 rows behind 32000 of 16 on 4 of 256 369 with the join (733), calls back to back.
+// of 128 in bf16 568 us (924 TFLOP/s), 512 rows behind 32000 of 16 on 4 of 256 369 with the join (733), calls back to back.
 template <int D, class E, int NP, int RT, int SRC, int M>
 __global__ __launch_bounds__(8192 / M, 2) void attn_many_kernel(const BatchAttnArgs a) {
     typedef typename Row<RT>::t R;
